@@ -46,6 +46,8 @@ GGK_MOE_STATUS = 12
 GGK_MOE_NEGATIVE = 1
 GGK_MOE_CLAMPED = 2
 GG_MOE_NOALLOC_SCRATCH_BYTES = 99840
+GGK_TYPE_F32, GGK_TYPE_F16, GGK_TYPE_BF16 = 0, 1, 2
+GGK_ROUTE_MAX_SLOTS = 64
 
 c_int_p = ctypes.POINTER(ctypes.c_int)
 c_ll_p = ctypes.POINTER(ctypes.c_longlong)
@@ -134,6 +136,42 @@ class GGKMoeLayout(ctypes.Structure):
     ]
 
 
+class GGKRouteArgs(ctypes.Structure):
+    """ggk_route_args (grouped_gemm_amd_kernels.h)"""
+    _fields_ = [
+        ("tokens", ctypes.c_int), ("experts", ctypes.c_int), ("slots", ctypes.c_int), ("type", ctypes.c_int),
+        ("logits", ctypes.c_void_p), ("ld", ctypes.c_longlong), ("token_mask", ctypes.c_void_p),
+        ("given_ids", ctypes.c_void_p), ("normalize", ctypes.c_int), ("scale", ctypes.c_float),
+        ("weights", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+        ("order", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("slope", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class GGKRouteGradientArgs(ctypes.Structure):
+    """ggk_route_gradient_args (grouped_gemm_amd_kernels.h)"""
+    _fields_ = [
+        ("tokens", ctypes.c_int), ("experts", ctypes.c_int), ("slots", ctypes.c_int), ("type", ctypes.c_int),
+        ("logits", ctypes.c_void_p), ("ld", ctypes.c_longlong), ("ids", ctypes.c_void_p),
+        ("slope", ctypes.c_void_p), ("normalize", ctypes.c_int), ("scale", ctypes.c_float),
+        ("d_weights", ctypes.c_void_p), ("d_loss", ctypes.c_void_p), ("d_logits", ctypes.c_void_p),
+    ]
+
+
+class GGKW4Args(ctypes.Structure):
+    """ggk_w4_args (grouped_gemm_amd_kernels.h)"""
+    _fields_ = [
+        ("rows", ctypes.c_int), ("x_rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int),
+        ("group", ctypes.c_int), ("experts", ctypes.c_int),
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong),
+        ("q", ctypes.c_void_p), ("ldq", ctypes.c_longlong), ("stride_q", ctypes.c_longlong),
+        ("scales", ctypes.c_void_p), ("lds", ctypes.c_longlong), ("stride_s", ctypes.c_longlong),
+        ("zeros", ctypes.c_void_p), ("ldz", ctypes.c_longlong), ("stride_z", ctypes.c_longlong),
+        ("counts", ctypes.c_void_p), ("order", ctypes.c_void_p), ("row_weights", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong), ("y_type", ctypes.c_int),
+    ]
+
+
 _P = ctypes.POINTER
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -197,6 +235,13 @@ SIGNATURES = {
     "ggk_launch_single": (_i, [_i, _i, _P(GGDeviceProblemDesc), _vp]),
     "ggk_moe_prepare": (_i, [_i, _i, _P(GGKMoeLayout), _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ggk_moe_layout_check": (_i, [_i, _i, _P(GGKMoeLayout)]),
+    "ggk_route_workspace": (ctypes.c_size_t, [_i, _i]),
+    "ggk_route_check": (_i, [_P(GGKRouteArgs)]),
+    "ggk_route": (_i, [_P(GGKRouteArgs), _vp]),
+    "ggk_route_gradient_check": (_i, [_P(GGKRouteGradientArgs)]),
+    "ggk_route_gradient": (_i, [_P(GGKRouteGradientArgs), _vp]),
+    "ggk_w4_check": (_i, [_P(GGKW4Args)]),
+    "ggk_w4_multiply": (_i, [_P(GGKW4Args), _vp]),
     "ggk_launch_grouped_device": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp]),
     "ggk_launch_grouped_device_done": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, c_int_p, _vp]),
     "ggk_kernel_resources_get": (_i, [_i, _i, _i, _P(GGKKernelResources)]),

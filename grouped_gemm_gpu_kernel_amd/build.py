@@ -27,6 +27,7 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC_DIR = PKG / "csrc"
 BUILD = PKG / "_build"
+DEVICE_SOURCES = ["gg_moe.hip", "gg_route.hip", "gg_w4.hip"]  # beside gg_kernels.hip, whose resources are reported
 LIB_DIR = PKG / "lib"
 LIB_NAME = "libgrouped_gemm_amd.so"
 FORMS_NAME = "gg_kernel_forms.json"  # resources of every compiled kernel form, beside the objects
@@ -107,15 +108,16 @@ def build_library(out_path: Path | None = None, defines: tuple[str, ...] = (), c
     build_dir.mkdir(parents=True, exist_ok=True)
     out.parent.mkdir(parents=True, exist_ok=True)
     kernels_o = build_dir / "gg_kernels.o"
-    moe_o = build_dir / "gg_moe.o"
     extra = [f"-D{d}" for d in defines]
 
     def compile_kernels() -> str:
         return _run([HIPCC, *HIP_FLAGS, *extra, "-Rpass-analysis=kernel-resource-usage", "-c",
                      str(CSRC / "gg_kernels.hip"), "-o", str(kernels_o)], capture_stderr=True)
 
-    def compile_moe() -> None:
-        _run([HIPCC, *HIP_FLAGS, "-c", str(CSRC / "gg_moe.hip"), "-o", str(moe_o)])
+    def compile_device(name: str) -> Path:
+        obj = build_dir / (Path(name).stem + ".o")
+        _run([HIPCC, *HIP_FLAGS, "-c", str(CSRC / name), "-o", str(obj)])
+        return obj
 
     def compile_host(name: str) -> Path:
         obj = build_dir / (Path(name).stem + ".o")
@@ -124,10 +126,10 @@ def build_library(out_path: Path | None = None, defines: tuple[str, ...] = (), c
 
     with ThreadPoolExecutor(max_workers=4) as pool:
         fut_k = pool.submit(compile_kernels)
-        fut_moe = pool.submit(compile_moe)
+        futs = [pool.submit(compile_device, name) for name in DEVICE_SOURCES]
         host_objs = list(pool.map(compile_host, ["grouped_gemm.cpp", "c_api.cpp"]))
         report = fut_k.result()
-        fut_moe.result()
+        device_objs = [f.result() for f in futs]
 
     rows = parse_resource_report(report)
     if len(rows) != 24:
@@ -139,8 +141,8 @@ def build_library(out_path: Path | None = None, defines: tuple[str, ...] = (), c
     _run([*CXX_FLAGS, f"-I{build_dir}", "-c", str(CSRC / "gg_resources.cpp"), "-o", str(res_o)])
 
     tmp = out.parent / (out.name + ".tmp")
-    _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), str(kernels_o), str(moe_o),
-          *map(str, host_objs), str(res_o)])
+    _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), str(kernels_o),
+          *map(str, device_objs), *map(str, host_objs), str(res_o)])
     os.replace(tmp, out)
     return out
 
@@ -158,7 +160,8 @@ def build_host_sanitized(out_path: Path) -> Path:
         _run([*CXX_FLAGS, "-O1", "-g", "-fno-omit-frame-pointer", "-fsanitize=address,undefined",
               f"-I{CSRC_DIR}", "-c", str(CSRC_DIR / name), "-o", str(obj)])
         objs.append(str(obj))
-    kernel_objs = [str(BUILD / n) for n in ("gg_kernels.o", "gg_moe.o", "gg_resources.o")]
+    kernel_objs = [str(BUILD / n) for n in ("gg_kernels.o", *(Path(d).stem + ".o" for d in DEVICE_SOURCES),
+                                              "gg_resources.o")]
     _run(["g++", "-shared", "-fsanitize=address,undefined", "-o", str(out), *kernel_objs, *objs,
           f"-L{ROCM / 'lib'}", "-lamdhip64", f"-Wl,-rpath,{ROCM / 'lib'}"])
     return out

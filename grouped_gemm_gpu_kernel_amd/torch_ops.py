@@ -17,12 +17,18 @@ Two forms:
   (include/grouped_gemm/grouped_gemm.cuh:94-115).  The plan holds its tensors; refill them in place
   between runs.
 
+Around the products of a mixture-of-experts layer: moe_route (choice of experts, their weights, the counts
+and the order by expert, the balance loss, with gradients), MoeGroupedGemmPlan (float16 expert
+weights) and moe_w4_matmul / w4_matmul (4-bit weights, for a few rows).
+
 All work runs in the HIP library (lib/libgrouped_gemm_amd.so); there is no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
-from typing import Optional, Sequence, Union
+import operator
+from typing import NamedTuple, Optional, Sequence, Union
 
 import numpy as np
 import torch
@@ -331,6 +337,277 @@ class MoeGroupedGemmPlan:
 
     def close(self) -> None:
         self.moe.close()
+
+
+# ---------------------------------------------------------------- routing
+
+_TYPES = {torch.float32: _lib.GGK_TYPE_F32, torch.float16: _lib.GGK_TYPE_F16, torch.bfloat16: _lib.GGK_TYPE_BF16}
+
+
+class Routing(NamedTuple):
+    """What moe_route returns; T tokens, k slots each, E experts, all on the logits' device."""
+    weights: torch.Tensor  # float32 [T, k]
+    ids: torch.Tensor  # int32 [T, k], -1 where a slot has no expert
+    counts: torch.Tensor  # int32 [E], slots on each expert: what MoeGroupedGemmPlan.run takes
+    order: torch.Tensor  # int32 [T * k], slot indices t * k + s grouped by expert
+    balance_loss: Optional[torch.Tensor]  # float32 scalar, None unless asked for
+
+
+def _on_device(device: torch.device):
+    """The device made current, at no cost where it is already."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _launch(name: str, args, device: torch.device) -> None:
+    """A library entry point on the device's current stream."""
+    with _on_device(device):
+        status = getattr(_lib.lib(), name)(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream or None)
+    _lib.check(status, name)
+
+
+def _check_vector(t: torch.Tensor, name: str, dtype: torch.dtype, count: int, device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.numel() != count:
+        raise ValueError(f"{name} has {t.numel()} entries, expected {count}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _route(logits, ids, token_mask, slots, normalize, scale, balance):
+    """The launch behind moe_route: weights, ids, counts, order, loss, slope."""
+    tokens, experts = logits.shape
+    device = logits.device
+    dummy = _placeholder(device)
+    weights = torch.empty((tokens, slots), dtype=torch.float32, device=device)
+    chosen = torch.empty((tokens, slots), dtype=torch.int32, device=device)
+    counts = torch.empty(experts, dtype=torch.int32, device=device)
+    order = torch.empty(tokens * slots, dtype=torch.int32, device=device)
+    loss = torch.empty((), dtype=torch.float32, device=device) if balance else None
+    slope = torch.empty(experts, dtype=torch.float32, device=device) if balance else None
+    size = _lib.lib().ggk_route_workspace(tokens, experts)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    _launch("ggk_route", _lib.GGKRouteArgs(
+        tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr() or dummy, _row_stride(logits),
+        token_mask.data_ptr() or dummy if token_mask is not None else None,
+        ids.data_ptr() or dummy if ids is not None else None, normalize, scale, weights.data_ptr() or dummy,
+        chosen.data_ptr() or dummy, counts.data_ptr(), order.data_ptr() or dummy, loss.data_ptr() if balance else None,
+        slope.data_ptr() if balance else None, workspace.data_ptr(), size), device)
+    return weights, chosen, counts, order, loss, slope
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, token_mask, slots, normalize, scale, balance):
+        weights, chosen, counts, order, loss, slope = _route(logits, ids, token_mask, slots, normalize, scale, balance)
+        ctx.save_for_backward(logits, chosen, slope)
+        ctx.how = (slots, normalize, scale)
+        ctx.mark_non_differentiable(chosen, counts, order)
+        ctx.set_materialize_grads(False)
+        return weights, chosen, counts, order, loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_weights, _ids, _counts, _order, d_loss):
+        logits, chosen, slope = ctx.saved_tensors
+        if d_weights is None and d_loss is None:
+            return (None,) * 7
+        slots, normalize, scale = ctx.how
+        tokens, experts = logits.shape
+        dummy = _placeholder(logits.device)
+        # Gradients may come expanded (a sum's) or in any strides.
+        d_weights = d_weights.contiguous() if d_weights is not None else None
+        d_logits = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
+        _launch("ggk_route_gradient", _lib.GGKRouteGradientArgs(
+            tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr() or dummy, _row_stride(logits),
+            chosen.data_ptr() or dummy, slope.data_ptr() if slope is not None else None, normalize, scale,
+            d_weights.data_ptr() or dummy if d_weights is not None else None,
+            d_loss.data_ptr() if d_loss is not None else None, d_logits.data_ptr() or dummy), logits.device)
+        return (d_logits,) + (None,) * 6
+
+
+def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optional[torch.Tensor] = None,
+              token_mask: Optional[torch.Tensor] = None, normalize: bool = True, scale: float = 1.0,
+              balance: bool = False) -> Routing:
+    """The routing of a mixture-of-experts layer from its router's logits [T, E] (float32, float16 or
+    bfloat16; rows may be padded).
+
+    Each token takes its top_k experts of the largest logits, in descending order, ties to the lower
+    expert, NaN above everything; an expert with logit -inf is closed to the token.  Instead of
+    top_k, ids (int32 [T, k]) gives the experts: they are taken as they stand, the same one twice
+    included.  token_mask (bool [T]) is False for padding.  A slot with no expert -- too few open
+    ones, an id outside [0, E) or of a closed expert, a padding token -- gets id -1 and weight 0 and is
+    not counted.
+
+    weights: scale * softmax over the token's chosen logits (normalize) or scale * the chosen entries
+    of the softmax over all experts.  counts and order are what the experts' products take: a token's
+    row for slot o is o // k, `order` lists the slots by expert (ascending within one, those without an
+    expert last), so MoeGroupedGemmPlan runs on tokens[order // k] with counts, and moe_w4_matmul takes
+    both as they are.  balance_loss (with balance): E * sum_e f_e P_e, f_e expert e's share of all
+    counted slots and P_e the mean of softmax(logits)[:, e] over the tokens with an expert; 0 if there
+    is none.
+
+    weights and balance_loss carry gradients to logits (f_e counts as a constant).  Everything runs on the
+    current stream of the logits' device without waiting for it, and can be captured in a graph; the
+    same call gives the same bits.  E at most 1024, k at most 64."""
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits must be a torch.Tensor")
+    if logits.device.type != "cuda":
+        raise ValueError(f"tensors must be on a GPU, got {logits.device}")
+    if logits.dtype not in _TYPES:
+        raise TypeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    _check_matrix(logits, "logits", logits.dtype, None, logits.device)
+    tokens, experts = logits.shape
+    if not 1 <= experts <= _lib.GGK_MOE_MAX_EXPERTS:
+        raise ValueError(f"logits has {experts} experts, expected 1 to {_lib.GGK_MOE_MAX_EXPERTS}")
+    if (top_k is None) == (ids is None):
+        raise ValueError("give one of top_k and ids")
+    if ids is not None:
+        if not isinstance(ids, torch.Tensor):
+            raise TypeError("ids must be a torch.Tensor")
+        if ids.dim() != 2 or ids.shape[0] != tokens:
+            raise ValueError(f"ids must be [{tokens}, k], got shape {tuple(ids.shape)}")
+        _check_vector(ids, "ids", torch.int32, ids.numel(), logits.device)
+        slots = ids.shape[1]
+        if not 1 <= slots <= _lib.GGK_ROUTE_MAX_SLOTS:
+            raise ValueError(f"ids has {slots} slots, expected 1 to {_lib.GGK_ROUTE_MAX_SLOTS}")
+    else:
+        slots = operator.index(top_k)
+        if not 1 <= slots <= min(experts, _lib.GGK_ROUTE_MAX_SLOTS):
+            raise ValueError(f"top_k is {slots}, expected 1 to {min(experts, _lib.GGK_ROUTE_MAX_SLOTS)}")
+    if tokens * slots > 0x7fffffff:
+        raise ValueError(f"{tokens} tokens with {slots} slots each: 2^31 slots or more")
+    if token_mask is not None:
+        _check_vector(token_mask, "token_mask", torch.bool, tokens, logits.device)
+    args = (logits, ids, token_mask, slots, bool(normalize), float(scale), bool(balance))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return Routing(*_Route.apply(*args))
+    return Routing(*_route(*args)[:5])
+
+
+# ---------------------------------------------------------------- 4-bit weights
+
+def _check_w4(x, q, scales, zeros, row_weights, lead, out_dtype):
+    """Checks shared by the two products: lead is the number of dimensions ahead of a matrix's two."""
+    if row_weights is not None and not isinstance(row_weights, torch.Tensor):
+        raise TypeError("row_weights must be a torch.Tensor")
+    if not isinstance(x, torch.Tensor) or not isinstance(q, torch.Tensor) or not isinstance(scales, torch.Tensor):
+        raise TypeError("x, q and scales must be torch.Tensors")
+    device = x.device
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a GPU, got {device}")
+    _check_matrix(x, "x", torch.float16, None, device)
+    if out_dtype not in (torch.float32, torch.float16):
+        raise TypeError(f"out_dtype must be float32 or float16, got {out_dtype}")
+    shape = "[N, K / 2]" if lead == 0 else "[experts, N, K / 2]"
+    for t, name, dtype in ((q, "q", torch.uint8), (scales, "scales", torch.float16), (zeros, "zeros", torch.uint8)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+        if t.dim() != 2 + lead:
+            raise ValueError(f"{name} must have {2 + lead} dimensions (q is {shape}), got shape {tuple(t.shape)}")
+        if t.shape[:-1] != q.shape[:-1]:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, q has {tuple(q.shape)}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name} must have contiguous rows")
+        if t.shape[-2] > 1 and t.stride(-2) < t.shape[-1]:
+            raise ValueError(f"{name} rows overlap")
+    if zeros is not None and zeros.shape != scales.shape:
+        raise ValueError(f"zeros has shape {tuple(zeros.shape)}, scales has {tuple(scales.shape)}")
+    k = 2 * q.shape[-1]
+    if x.shape[1] != k:
+        raise ValueError(f"x has {x.shape[1]} columns, q has K = {k}")
+    groups = scales.shape[-1]
+    if groups < 1 or k % groups != 0 or (k // groups) % 32 != 0 or k == 0:
+        raise ValueError(f"scales has {groups} groups for K = {k}: a group is a multiple of 32 values that divides K")
+    if q.data_ptr() % 16 != 0 or any(n > 1 and s % 16 != 0 for n, s in zip(q.shape[:-1], q.stride()[:-1])):
+        raise ValueError("q must start on a multiple of 16 bytes, and so must its rows and matrices")
+    if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or
+                                    (row_weights is not None and row_weights.requires_grad)):
+        raise RuntimeError("the products with 4-bit weights have no gradient: detach x, scales and row_weights")
+
+
+def _w4(x, q, scales, zeros, rows, experts, counts, order, row_weights, out_dtype):
+    n, k, groups = q.shape[-2], 2 * q.shape[-1], scales.shape[-1]
+    device = x.device
+    y = torch.empty((rows, n), dtype=out_dtype, device=device)
+    if y.numel() == 0:
+        return y
+
+    def strides(t):  # of rows and of matrices
+        if t is None:
+            return 0, 0
+        return (t.stride(-2) if n > 1 else t.shape[-1]), (t.stride(0) if experts > 1 else 0)
+
+    (ldq, stride_q), (lds, stride_s), (ldz, stride_z) = strides(q), strides(scales), strides(zeros)
+    _launch("ggk_w4_multiply", _lib.GGKW4Args(
+        rows, x.shape[0], n, k, k // groups, experts, x.data_ptr(), _row_stride(x), q.data_ptr(), ldq, stride_q,
+        scales.data_ptr(), lds, stride_s, zeros.data_ptr() if zeros is not None else None, ldz, stride_z,
+        counts.data_ptr() if counts is not None else None, order.data_ptr() if order is not None else None,
+        row_weights.data_ptr() if row_weights is not None else None, y.data_ptr(), n, _TYPES[out_dtype]), device)
+    return y
+
+
+def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
+              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """y = x @ w.T for a few rows x (float16 [M, K]) and a matrix w [N, K] of 4-bit weights:
+
+        w[j, k] = scales[j, k // G] * (q[j, k] - zeros[j, k // G])
+
+    q: uint8 [N, K / 2], two values a byte along K, the low half the even k; scales: float16 [N, K / G];
+    zeros: uint8 [N, K / G], 8 everywhere if not given.  The group G is a multiple of 32 that divides
+    K.  Rows of x, scales and zeros may be padded, those of q by multiples of 16 bytes.  Weights are
+    never rounded: products and sums are float32, y is float32 or float16, rounded once.
+
+    Runs on the current stream of x's device, without waiting; no gradient (inputs that require one are
+    refused).  Any number of rows is right; it is made for up to 64 or so."""
+    _check_w4(x, q, scales, zeros, None, 0, out_dtype)
+    return _w4(x, q, scales, zeros, x.shape[0], 0, None, None, None, out_dtype)
+
+
+def moe_w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, counts: torch.Tensor, order: torch.Tensor,
+                  zeros: Optional[torch.Tensor] = None, *, row_weights: Optional[torch.Tensor] = None,
+                  out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """w4_matmul for the expert matrices of a mixture-of-experts layer, q uint8 [E, N, K / 2], scales (and zeros)
+    [E, N, K / G], each slot with its expert's:
+
+        y[o] = row_weights[o] * x[o // fan] @ w[expert of o].T       o = 0 .. R - 1, fan = R // x.shape[0]
+
+    counts (int32 [E]) and order (int32 [R]) as moe_route returns them: with x [T, K] the tokens, R = T * k
+    and y [T * k, N] holds token t's slots at rows t * k ...; with x already one row a slot, fan is 1.
+    Slots without an expert (the end of order, past the counts' sum) get zeros.  row_weights: float32, R
+    entries (e.g. the routing's weights), 1 if not given.  Counts and order stay on the GPU and
+    are not trusted: a negative count is taken as 0, counts past R and entries outside [0, R) are dropped;
+    rows that order does not name are left unwritten."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise ValueError("q must be [experts, N, K / 2]")
+    _check_w4(x, q, scales, zeros, row_weights, 1, out_dtype)
+    experts = q.shape[0]
+    if not 1 <= experts <= _lib.GGK_MOE_MAX_EXPERTS:
+        raise ValueError(f"q has {experts} experts, expected 1 to {_lib.GGK_MOE_MAX_EXPERTS}")
+    _check_vector(counts, "counts", torch.int32, experts, x.device)
+    if not isinstance(order, torch.Tensor):
+        raise TypeError("order must be a torch.Tensor")
+    rows = order.numel()
+    _check_vector(order, "order", torch.int32, rows, x.device)
+    if rows > 0x7fffffff:
+        raise ValueError(f"order has {rows} entries: 2^31 or more")
+    if rows and (x.shape[0] == 0 or rows % x.shape[0] != 0):
+        raise ValueError(f"order has {rows} entries, not a multiple of x's {x.shape[0]} rows")
+    if row_weights is not None:
+        _check_vector(row_weights, "row_weights", torch.float32, rows, x.device)
+    return _w4(x, q, scales, zeros, rows, experts, counts, order, row_weights, out_dtype)
 
 
 # ---------------------------------------------------------------- custom op

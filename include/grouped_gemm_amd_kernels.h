@@ -356,6 +356,126 @@ hipError_t ggk_launch_grouped_device_done(int variant, int path, int addressing,
                                           const int* d_order, int problem_count, const int* d_header, int* d_state,
                                           int grid, hipEvent_t done, int* recorded, hipStream_t stream);
 
+/* Routing of a mixture-of-experts layer (no reference counterpart: it makes
+ * the token counts that the grouped launch of a device-prepared set takes).
+ * Row t of logits (tokens x experts, `type`, ld elements between rows) gives
+ * token t's slots: the `slots` largest logits in descending order, ties to the
+ * lower expert, NaN above everything, -inf (an expert closed to the token)
+ * never; or, with given_ids [tokens][slots], those experts as they stand,
+ * duplicates included.  A slot with no expert (too few open ones, a given id
+ * outside [0, experts) or of a closed expert, token_mask[t] == 0) has id -1
+ * and weight 0 and is not counted.
+ *   weights[t][s] = scale * exp(z_s) / sum of exp(z): over the token's slots
+ *                   that have an expert (normalize) or over all experts;
+ *   counts[e]     = slots on expert e;
+ *   order         = the slot indices t * slots + s by expert, ascending within
+ *                   one, the slots with no expert last;
+ *   loss          = experts * sum over e of (counts[e] / all counts) * (mean of
+ *                   softmax(z_t)[e] over the tokens with an expert), 0 with no
+ *                   such token; slope[e] = d loss / d (sum of softmax(z_t)[e]).
+ * loss and slope may be NULL, both or neither.  Sums are made in a fixed
+ * order: the same call gives the same bits.  workspace holds
+ * ggk_route_workspace(tokens, experts) bytes, written before they are read;
+ * calls that may overlap need one each.  1 <= experts <=
+ * GGK_MOE_MAX_EXPERTS, 1 <= slots <= GGK_ROUTE_MAX_SLOTS and, without
+ * given_ids, slots <= experts; tokens * slots < 2^31. */
+enum { GGK_TYPE_F32 = 0, GGK_TYPE_F16 = 1, GGK_TYPE_BF16 = 2 };
+#define GGK_ROUTE_MAX_SLOTS 64
+
+typedef struct ggk_route_args {
+  int tokens;
+  int experts;
+  int slots;
+  int type; /* of logits: GGK_TYPE_* */
+  const void* logits;
+  long long ld;
+  const unsigned char* token_mask; /* NULL: every token */
+  const int* given_ids;            /* NULL: the largest logits */
+  int normalize;
+  float scale;
+  float* weights; /* [tokens][slots] */
+  int* ids;       /* [tokens][slots] */
+  int* counts;    /* [experts] */
+  int* order;     /* [tokens * slots] */
+  float* loss;
+  float* slope; /* [experts] */
+  void* workspace;
+  size_t workspace_bytes;
+} ggk_route_args;
+
+size_t ggk_route_workspace(int tokens, int experts);
+/* The host-side checks ggk_route makes before it launches anything. */
+hipError_t ggk_route_check(const ggk_route_args* args);
+hipError_t ggk_route(const ggk_route_args* args, hipStream_t stream);
+
+/* The gradient of ggk_route: d_logits (tokens x experts, dense, `type`) from
+ * d_weights [tokens][slots] (NULL: none) and *d_loss (device memory; NULL:
+ * none), with the forward call's logits, ids, slope (may be NULL without
+ * d_loss), normalize and scale.  Counts and order have no gradient. */
+typedef struct ggk_route_gradient_args {
+  int tokens;
+  int experts;
+  int slots;
+  int type;
+  const void* logits;
+  long long ld;
+  const int* ids;
+  const float* slope;
+  int normalize;
+  float scale;
+  const float* d_weights;
+  const float* d_loss;
+  void* d_logits;
+} ggk_route_gradient_args;
+
+hipError_t ggk_route_gradient_check(const ggk_route_gradient_args* args);
+hipError_t ggk_route_gradient(const ggk_route_gradient_args* args, hipStream_t stream);
+
+/* Products of a few rows with 4-bit weights (no reference counterpart: its
+ * operands are binary16):
+ *   y[i][j] = sum over groups g of scales[j][g] * sum over k in g of
+ *             x[i][k] * (q[j][k] - zeros[j][g])
+ * x binary16 (x_rows x k, ldx elements between rows); q two values a byte along
+ * k, the low half the even k (n x k / 2 bytes, ldq bytes between rows); scales
+ * binary16 and zeros bytes (NULL: 8), one per row and group of `group` values
+ * of k; y float or binary16 (y_type).  Products and sums are held in float;
+ * y is rounded once.  group is a multiple of 32 that divides k; q and its
+ * strides are multiples of 16 bytes.
+ * experts == 0: one matrix, y row i from x row i, rows == x_rows.
+ * experts > 0: matrix e at q + e * stride_q (bytes), scales + e * stride_s,
+ * zeros + e * stride_z.  order[rows] lists the slots grouped by expert, counts
+ * [experts] how many each has (device memory, as ggk_route writes them): slot
+ * o = order[r] reads x row o / (rows / x_rows) and writes y row o, times
+ * row_weights[o] if given; slots past the counts' sum are set to 0.  Counts
+ * are not trusted: a negative one is taken as 0, what goes past `rows` is
+ * dropped, and an order entry outside [0, rows) is passed over. */
+typedef struct ggk_w4_args {
+  int rows; /* of y */
+  int x_rows;
+  int n;
+  int k;
+  int group;
+  int experts;
+  const void* x;
+  long long ldx;
+  const unsigned char* q;
+  long long ldq, stride_q;
+  const void* scales;
+  long long lds, stride_s;
+  const unsigned char* zeros;
+  long long ldz, stride_z;
+  const int* counts;
+  const int* order;
+  const float* row_weights;
+  void* y;
+  long long ldy;
+  int y_type; /* GGK_TYPE_F32 or GGK_TYPE_F16 */
+} ggk_w4_args;
+
+/* The host-side checks ggk_w4_multiply makes before it launches anything. */
+hipError_t ggk_w4_check(const ggk_w4_args* args);
+hipError_t ggk_w4_multiply(const ggk_w4_args* args, hipStream_t stream);
+
 /* One problem, one workgroup per work tile, row-major work-tile order
  * (single_problem_gemm_kernel + launch_single_problem_variant,
  * src/grouped_gemm.cu:677-688, 753-769).  *problem is read on the host and
