@@ -22,402 +22,820 @@
 namespace {
 
 constexpr int kWave = 64;
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxExperts = GGK_MOE_MAX_EXPERTS;
-constexpr int kMaxBlocks = 1024;  // blocks of tokens, each with one partial sum per expert
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
-__device__ __forceinline__ float to_float(__hip_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void from_float(float v, float* out) { *out = v; }
-__device__ __forceinline__ void from_float(float v, _Float16* out) { *out = (_Float16)v; }
-__device__ __forceinline__ void from_float(float v, __hip_bfloat16* out) { *out = __float2bfloat16(v); }
+typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
 
-// A logit as an unsigned key of the same order: NaN above everything, -0 equal to 0.
-__device__ __forceinline__ uint32_t order_key(float z) {
-  if (z != z) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(z + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+// ---------------------------------------------------------------- logits
+
+// A logit as an unsigned key of the same order: NaN above everything, -0 equal to 0.  A float's key has 32
+// bits; a 16-bit type's leaves room for the expert below it, lower experts larger, which makes keys of a
+// token distinct and their maximum the choice itself.
+template <class T>
+struct Logit;
+
+template <>
+struct Logit<float> {
+  static constexpr bool kDistinct = false;
+  static constexpr uint32_t kClosed = 0x007fffffu;  // key of -inf: no expert is chosen at or below it
+  static __device__ __forceinline__ float value(float v) { return v; }
+  static __device__ __forceinline__ uint32_t key(float v, int) {
+    if (v != v) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  }
+  // The logit of a key (NaN of NaN's).
+  static __device__ __forceinline__ float of_key(uint32_t k) {
+    return __uint_as_float(k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u));
+  }
+  static __device__ __forceinline__ float store(float v) { return v; }
+};
+
+template <class T, uint32_t NAN_BITS, uint32_t INF_BITS>
+struct Logit16 {
+  static constexpr bool kDistinct = true;
+  static constexpr uint32_t kClosed = ((~INF_BITS & 0x7fffu) << 16) | 0xffffu;
+  static __device__ __forceinline__ uint32_t key(T v, int expert) {
+    uint32_t b = __builtin_bit_cast(uint16_t, v);
+    if ((b & 0x7fffu) > INF_BITS) {
+      b = 0xffffu;
+    } else {
+      b = b == 0x8000u ? 0u : b;
+      b = b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+    }
+    return b << 16 | (0xffffu - (uint32_t)expert);
+  }
+  static __device__ __forceinline__ T bits_of_key(uint32_t k) {
+    uint32_t b = k >> 16;
+    b = b == 0xffffu ? NAN_BITS : (b & 0x8000u ? b & 0x7fffu : ~b & 0xffffu);
+    return __builtin_bit_cast(T, (uint16_t)b);
+  }
+};
+
+template <>
+struct Logit<_Float16> : Logit16<_Float16, 0x7e00u, 0x7c00u> {
+  static __device__ __forceinline__ float value(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ float of_key(uint32_t k) { return (float)bits_of_key(k); }
+  static __device__ __forceinline__ _Float16 store(float v) { return (_Float16)v; }
+};
+
+template <>
+struct Logit<__hip_bfloat16> : Logit16<__hip_bfloat16, 0x7fc0u, 0x7f80u> {
+  static __device__ __forceinline__ float value(__hip_bfloat16 v) {
+    return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, v) << 16);
+  }
+  static __device__ __forceinline__ float of_key(uint32_t k) { return value(bits_of_key(k)); }
+  static __device__ __forceinline__ __hip_bfloat16 store(float v) { return __float2bfloat16(v); }
+};
+
+// exp(x) for x <= 0 on the hardware's exp2: x is rounded once more by the product, which a softmax over
+// logits of spread d bears as it bears the rounding of z - max (d half steps of float).
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+
+// ---------------------------------------------------------------- groups of lanes
+
+// A token's logits are held by L lanes: 16 (one DPP row, four tokens a wave) or the whole wave.  Reductions
+// exchange within the row by DPP -- neighbours, pairs, halves mirrored, the row mirrored, so that every
+// lane adds the same pairs and ends with the same bits -- and across rows by the lane swaps of gfx950.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
 }
-constexpr uint32_t kClosedKey = 0x007fffffu;  // order_key(-inf): no expert is chosen at or below it
 
-__device__ __forceinline__ float wave_sum(float v) {
-  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d, kWave);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-  for (int d = 1; d < kWave; d *= 2) v = fmaxf(v, __shfl_xor(v, d, kWave));
-  return v;
+template <int L, class Op>
+__device__ __forceinline__ uint32_t group_reduce(uint32_t x, Op op) {
+  x = op(x, dpp<0xb1>(x));   // quad_perm [1, 0, 3, 2]
+  x = op(x, dpp<0x4e>(x));   // quad_perm [2, 3, 0, 1]
+  x = op(x, dpp<0x141>(x));  // row_half_mirror
+  x = op(x, dpp<0x140>(x));  // row_mirror
+  if constexpr (L == kWave) {
+    uint2v r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = op(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = op(r[0], r[1]);
+  }
+  return x;
 }
 
+template <int L>
+__device__ __forceinline__ uint32_t group_max(uint32_t x) {
+  return group_reduce<L>(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+template <int L>
+__device__ __forceinline__ uint32_t group_min(uint32_t x) {
+  return group_reduce<L>(x, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+template <int L>
+__device__ __forceinline__ float group_max(float x) {
+  return __uint_as_float(group_reduce<L>(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+template <int L>
+__device__ __forceinline__ float group_sum(float x) {
+  return __uint_as_float(group_reduce<L>(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+
+// Does the predicate hold for any lane of this lane's group?
+template <int L>
+__device__ __forceinline__ bool group_any(bool v) {
+  const unsigned long long b = __ballot(v);
+  if constexpr (L == kWave) return b != 0;
+  return ((b >> (threadIdx.x & 48)) & 0xffffu) != 0;
+}
+
+// Expert of value j of a lane: V values in vectors of W, so that a vector's load is 4 to 16 bytes.
+template <int L, int V>
+struct Columns {
+  static constexpr int W = V < 4 ? V : 4;
+  static __device__ __forceinline__ int expert(int lane, int j) { return (j / W * L + lane) * W + j % W; }
+};
+
+// The lane's values of a row, `fill` past the experts.  vectors: every row's start and length are whole vectors.
+template <class T, int L, int V>
+__device__ __forceinline__ void load_row(const T* row, int lane, int experts, bool vectors, T fill, T* out) {
+  constexpr int W = Columns<L, V>::W;
+  typedef struct alignas(sizeof(T) * W) {
+    T v[W];
+  } Vector;
+#pragma unroll
+  for (int j = 0; j < V; j += W) {
+    const int e = Columns<L, V>::expert(lane, j);
+    if (vectors) {
+      if (e < experts) {
+        const Vector x = *reinterpret_cast<const Vector*>(row + e);
+#pragma unroll
+        for (int i = 0; i < W; ++i) out[j + i] = x.v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) out[j + i] = fill;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) out[j + i] = e + i < experts ? row[e + i] : fill;
+    }
+  }
+}
+
+template <class T, int V>
+bool whole_vectors(const void* base, long long ld, int experts) {
+  constexpr long long kBytes = sizeof(T) * (V < 4 ? V : 4);
+  return reinterpret_cast<uintptr_t>(base) % kBytes == 0 && ld * (long long)sizeof(T) % kBytes == 0 &&
+         experts * (long long)sizeof(T) % kBytes == 0;
+}
+
+// ---------------------------------------------------------------- forward
+
+// Tokens are dealt to blocks in runs of `rows`.
 struct Plan {
-  int blocks, rows_per_block;
+  int blocks, rows;
+  bool columns;  // the columns kernel runs between the rows and the order
+  bool vectors;
 };
 
-Plan plan_blocks(int tokens) {
+// Workspace, written by the rows kernel: per block and expert the sum of p and the slots taken (one more
+// column: slots without an expert), then per block the routed tokens.  The columns kernel turns the
+// counts into sums over the blocks before, and the first block's sums of p into those over all.
+struct Workspace {
+  float* p;     // [blocks][experts]
+  int* count;   // [blocks][experts + 1]
+  int* routed;  // [blocks]
+};
+
+// At most this many entries of `count` are summed by every block of the order kernel itself.
+constexpr int kMaxOwnSums = 20 * 1024;
+constexpr int kMaxBlocks = 512;
+
+Plan plan_blocks(int tokens, int experts) {
+  const int least = kThreads / 16;  // one token a group
   int rows = (tokens + kMaxBlocks - 1) / kMaxBlocks;
-  rows = rows < 16 ? 16 : rows;
+  rows = rows < least ? least : (rows + least - 1) / least * least;
   const int blocks = tokens > 0 ? (tokens + rows - 1) / rows : 1;
-  return {blocks, rows};
+  return {blocks, rows, (long long)blocks * experts > kMaxOwnSums, false};
 }
 
-// Workspace: partial sums of p [experts][blocks], then slot counts [experts + 1][blocks] (the last row: slots
-// without an expert), then per expert the sum of p and the number of routed tokens.
-struct Workspace {
-  float* p;
-  int* count;
-  int* routed;
-};
+size_t workspace_ints(int experts, int blocks) {
+  return (size_t)experts * blocks + (size_t)(experts + 1) * blocks + (size_t)blocks;
+}
 
 Workspace carve(void* base, int experts, int blocks) {
-  char* b = static_cast<char*>(base);
   Workspace w;
-  w.p = reinterpret_cast<float*>(b);
-  w.count = reinterpret_cast<int*>(b + sizeof(float) * (size_t)experts * blocks);
+  w.p = static_cast<float*>(base);
+  w.count = reinterpret_cast<int*>(w.p + (size_t)experts * blocks);
   w.routed = w.count + (size_t)(experts + 1) * blocks;
   return w;
 }
 
-size_t workspace_bytes(int experts, int blocks) {
-  return sizeof(int) * ((size_t)experts * blocks + (size_t)(experts + 1) * blocks + (size_t)blocks);
+// One token by its group: ids and weights to memory, slots counted in s_count, p added to sums.  Every lane
+// of the wave calls it; `t` at or past `last` does nothing.  Returns whether the token was routed.
+template <class T, int L, int V>
+__device__ __forceinline__ bool route_token(const ggk_route_args& a, bool vectors, int t, int last, int* s_count,
+                                            float (&sums)[V]) {
+  using Z = Logit<T>;
+  using C = Columns<L, V>;
+  const int lane = threadIdx.x % L;
+  const bool in = t < last;
+  const bool live = in && (a.token_mask == nullptr || a.token_mask[t] != 0);
+  const T* row = static_cast<const T*>(a.logits) + (long long)(in ? t : 0) * a.ld;
+  const long long slot0 = (long long)t * a.slots;
+  const T closed = Z::store(-__builtin_inff());
+  const bool all = a.given_ids == nullptr || !a.normalize || a.loss != nullptr;  // every logit is needed
+  uint32_t key[V], best = 0;
+  T z[V];
+  if (all) {
+    load_row<T, L, V>(row, lane, live ? a.experts : 0, vectors, closed, z);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      key[j] = Z::key(z[j], C::expert(lane, j));
+      best = key[j] > best ? key[j] : best;
+    }
+    best = group_max<L>(best);
+  }
+  int my_id = -1;
+  float my_z = -__builtin_inff();
+  const float top = Z::of_key(best);  // NaN where the row holds one; what follows is NaN then, as it should be
+  float inv = 0.0f;
+  bool routed = best > Z::kClosed;
+  if (a.given_ids != nullptr) {
+    if (live && lane < a.slots) {
+      const int id = a.given_ids[slot0 + lane];
+      if (id >= 0 && id < a.experts) {
+        const T v = row[id];
+        if (Z::key(v, id) > Z::kClosed) {
+          my_id = id;
+          my_z = Z::value(v);
+        }
+      }
+    }
+    routed = group_any<L>(my_id >= 0);
+  }
+  // The softmax over all experts, before the choice takes its keys away.
+  if (!a.normalize || a.loss != nullptr) {
+    float p[V], total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      p[j] = routed ? exp_of(Z::value(z[j]) - top) : 0.0f;
+      total += p[j];
+    }
+    total = group_sum<L>(total);
+    inv = routed ? 1.0f / total : 0.0f;
+    if (a.loss != nullptr) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) sums[j] = fmaf(p[j], inv, sums[j]);
+    }
+  }
+  if (a.given_ids == nullptr) {
+    for (int s = 0;; ++s) {
+      const bool open = best > Z::kClosed;
+      uint32_t at;
+      bool first[V];
+      if constexpr (Z::kDistinct) {
+        at = 0xffffu - (best & 0xffffu);
+      } else {
+        // The lowest expert among those with the best key: a lane's first, then the least over lanes.
+        at = 0xffffffffu;
+        bool none = true;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          first[j] = none && key[j] == best;
+          none = none && key[j] != best;
+          at = first[j] ? (uint32_t)C::expert(lane, j) : at;
+        }
+        const uint32_t mine = at;
+        at = group_min<L>(at);
+        const bool owner = mine == at;
+#pragma unroll
+        for (int j = 0; j < V; ++j) first[j] = first[j] && owner;
+      }
+      if (lane == s && open) {
+        my_id = (int)at;
+        my_z = Z::of_key(best);
+      }
+      if (s + 1 == a.slots || __ballot(open) == 0) break;
+      uint32_t next = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if constexpr (Z::kDistinct) {
+          key[j] = key[j] == best ? 0u : key[j];
+        } else {
+          key[j] = first[j] ? 0u : key[j];
+        }
+        next = key[j] > next ? key[j] : next;
+      }
+      best = group_max<L>(next);
+    }
+  }
+  const bool has = my_id >= 0;
+  float w;
+  if (a.normalize) {
+    const float peak = a.given_ids != nullptr ? group_max<L>(my_z) : top;
+    const float e = has ? exp_of(my_z - peak) : 0.0f;
+    w = e / group_sum<L>(e);
+  } else {
+    w = exp_of(my_z - top) * inv;
+  }
+  if (in && lane < a.slots) {
+    a.weights[slot0 + lane] = has ? a.scale * w : 0.0f;
+    a.ids[slot0 + lane] = my_id;
+    atomicAdd(&s_count[has ? my_id : a.experts], 1);
+  }
+  return routed;
 }
 
-// One wave a token: lane holds experts lane + 64 j.
-template <class T, int V>
+// The block's sums of p (balance) over its groups, to out[e].  s_part: kWaves * experts floats.
+template <int L, int V>
+__device__ __forceinline__ void block_sums(float (&sums)[V], int experts, float* s_part, float* out) {
+  using C = Columns<L, V>;
+  const int tid = threadIdx.x, lane = tid % L, wave = tid / kWave;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if constexpr (L < kWave) {
+      uint2v r = __builtin_amdgcn_permlane16_swap(__float_as_uint(sums[j]), __float_as_uint(sums[j]), false, false);
+      float x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+      r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      sums[j] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    const int e = C::expert(lane, j);
+    if (tid % kWave < L && e < experts) s_part[wave * experts + e] = sums[j];
+  }
+  __syncthreads();
+  for (int e = tid; e < experts; e += kThreads) {
+    float x = 0.0f;
+    for (int w = 0; w < kWaves; ++w) x += s_part[w * experts + e];
+    out[e] = x;
+  }
+}
+
+template <class T, int L, int V>
 __global__ __launch_bounds__(kThreads) void route_rows_kernel(ggk_route_args a, Workspace ws, Plan plan) {
-  __shared__ int s_count[kMaxExperts + 1];
-  __shared__ float s_p[kWaves][kMaxExperts];
-  __shared__ int s_routed;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  for (int e = tid; e <= a.experts; e += kThreads) s_count[e] = 0;
-  if (tid == 0) s_routed = 0;
+  extern __shared__ int shared[];  // counts [experts + 1], routed, then (balance) kWaves * experts floats
+  int* s_count = shared;
+  int* s_routed = shared + a.experts + 1;
+  const int tid = threadIdx.x;
+  for (int e = tid; e < a.experts + 2; e += kThreads) shared[e] = 0;
   __syncthreads();
   float sums[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) sums[j] = 0.0f;
-  const int first = blockIdx.x * plan.rows_per_block;
-  const int last = min(a.tokens, first + plan.rows_per_block);
-  for (int t = first + wave; t < last; t += kWaves) {
-    const T* row = static_cast<const T*>(a.logits) + (long long)t * a.ld;
-    const bool live = a.token_mask == nullptr || a.token_mask[t] != 0;
-    float z[V];
-    uint32_t key[V];
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = lane + kWave * j;
-      z[j] = live && e < a.experts ? to_float(row[e]) : -__builtin_inff();
-      key[j] = order_key(z[j]);
-      top = fmaxf(top, z[j]);
-    }
-    top = wave_max(top);
-    float my_z = 0.0f;
-    int my_id = -1;
-    const long long slot0 = (long long)t * a.slots;
-    if (a.given_ids != nullptr) {
-      if (lane < a.slots && live) {
-        const int id = a.given_ids[slot0 + lane];
-        if (id >= 0 && id < a.experts) {
-          my_z = to_float(row[id]);
-          if (order_key(my_z) > kClosedKey) my_id = id;
-        }
-      }
-    } else {
-      for (int s = 0; s < a.slots; ++s) {
-        uint32_t best = 0;
-        int at = 0x7fffffff;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if (key[j] > best) {
-            best = key[j];
-            at = lane + kWave * j;
-          }
-        }
-        for (int d = 1; d < kWave; d *= 2) {
-          const uint32_t other = __shfl_xor(best, d, kWave);
-          const int other_at = __shfl_xor(at, d, kWave);
-          if (other > best || (other == best && other_at < at)) {
-            best = other;
-            at = other_at;
-          }
-        }
-        if (best <= kClosedKey) break;
-        float chosen_z = 0.0f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if (at == lane + kWave * j) {
-            key[j] = 0;
-            chosen_z = z[j];
-          }
-        }
-        chosen_z = __shfl(chosen_z, at % kWave, kWave);
-        if (lane == s) {
-          my_id = at;
-          my_z = chosen_z;
-        }
-      }
-    }
-    const bool routed = __ballot(my_id >= 0) != 0;
-    const bool has = my_id >= 0;
-    float total = 0.0f, p[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) p[j] = 0.0f;
-    if (routed) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        p[j] = expf(z[j] - top);
-        total += p[j];
-      }
-      total = wave_sum(total);
-      const float inv = 1.0f / total;
-#pragma unroll
-      for (int j = 0; j < V; ++j) sums[j] += p[j] * inv;
-    }
-    // A NaN logit is the largest of its row for the choice, and makes the row's weights NaN.
-    float w = 0.0f;
-    if (a.normalize) {
-      const float peak = wave_max(has ? my_z : -__builtin_inff());
-      const float e = has ? expf(my_z - peak) : 0.0f;
-      const float sum = wave_sum(e);
-      w = has ? a.scale * (e / sum) : 0.0f;
-    } else if (has) {
-      w = a.scale * (expf(my_z - top) / total);
-    }
-    if (lane < a.slots) {
-      a.weights[slot0 + lane] = w;
-      a.ids[slot0 + lane] = my_id;
-      atomicAdd(&s_count[has ? my_id : a.experts], 1);
-    }
-    if (lane == 0 && routed) atomicAdd(&s_routed, 1);
+  const int first = blockIdx.x * plan.rows;
+  const int last = min(a.tokens, first + plan.rows);
+  int routed = 0;
+  for (int t0 = first; t0 < last; t0 += kThreads / L) {
+    routed += route_token<T, L, V>(a, plan.vectors, t0 + tid / L, last, s_count, sums) ? 1 : 0;
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (lane + kWave * j < a.experts) s_p[wave][lane + kWave * j] = sums[j];
+  if (tid % L == 0 && routed > 0) atomicAdd(s_routed, routed);
+  if (a.loss != nullptr) {
+    block_sums<L, V>(sums, a.experts, reinterpret_cast<float*>(shared + a.experts + 2),
+                     ws.p + (size_t)blockIdx.x * a.experts);
   }
   __syncthreads();
-  for (int e = tid; e <= a.experts; e += kThreads) {
-    ws.count[(size_t)e * plan.blocks + blockIdx.x] = s_count[e];
-    if (e < a.experts) {
-      float p = 0.0f;
-      for (int w = 0; w < kWaves; ++w) p += s_p[w][e];
-      ws.p[(size_t)e * plan.blocks + blockIdx.x] = p;
-    }
-  }
-  if (tid == 0) ws.routed[blockIdx.x] = s_routed;
+  for (int e = tid; e <= a.experts; e += kThreads) ws.count[(size_t)blockIdx.x * (a.experts + 1) + e] = s_count[e];
+  if (tid == 0) ws.routed[blockIdx.x] = *s_routed;
 }
 
-// One block an expert (and one for the slots without any): its slot counts over the blocks of tokens become their
-// exclusive prefix sums, its count the total; p's sum goes to the front of its row.
+// Sums over the blocks, kColumns columns a workgroup: each column's slices of blocks are added up, then the
+// counts become the sums over the blocks before, the totals go to a.counts, and the sums of p to block 0's.
+constexpr int kColumns = 16;
+constexpr int kSlices = kThreads / kColumns;
+
 __global__ __launch_bounds__(kThreads) void route_columns_kernel(ggk_route_args a, Workspace ws, int blocks) {
-  __shared__ int s_total[kWaves];
-  __shared__ float s_sum[kWaves];
-  const int e = blockIdx.x, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  int* count = ws.count + (size_t)e * blocks;
-  constexpr int kPer = kMaxBlocks / kThreads;
-  int mine[kPer], sum = 0;
+  __shared__ int s_count[kSlices][kColumns];
+  __shared__ float s_p[kSlices][kColumns];
+  const int tid = threadIdx.x, c = tid % kColumns, slice = tid / kColumns;
+  const int e = blockIdx.x * kColumns + c, width = a.experts + 1;
+  constexpr int kPer = kMaxBlocks / kSlices;
+  const int each = (blocks + kSlices - 1) / kSlices;
+  const int b0 = slice * each, rows = max(0, min(each, blocks - b0));
+  int count[kPer], sum = 0;
   float p = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int b = tid * kPer + i;
-    mine[i] = b < blocks ? count[b] : 0;
-    sum += mine[i];
-    if (b < blocks && e < a.experts) p += ws.p[(size_t)e * blocks + b];
+    count[i] = i < rows && e < width ? ws.count[(size_t)(b0 + i) * width + e] : 0;
+    sum += count[i];
   }
-  int x = sum;
+  if (a.loss != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) p += i < rows && e < a.experts ? ws.p[(size_t)(b0 + i) * a.experts + e] : 0.0f;
+  }
+  s_count[slice][c] = sum;
+  s_p[slice][c] = p;
+  __syncthreads();
+  int before = 0, total = 0;
+  p = 0.0f;
+#pragma unroll
+  for (int s = 0; s < kSlices; ++s) {
+    before += s < slice ? s_count[s][c] : 0;
+    total += s_count[s][c];
+    p += s_p[s][c];
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (i < rows && e < width) ws.count[(size_t)(b0 + i) * width + e] = before;
+    before += count[i];
+  }
+  if (slice == 0 && e < a.experts) {
+    a.counts[e] = total;
+    if (a.loss != nullptr) ws.p[e] = p;  // block 0's row, read above by this column's threads alone
+  }
+}
+
+// Exclusive prefix sum of one value per thread in thread order; ends with a barrier.
+__device__ __forceinline__ int block_before(int v, int* s_waves) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int x = v;
+#pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
     const int y = __shfl_up(x, d, kWave);
     if (lane >= d) x += y;
   }
-  p = wave_sum(p);
-  if (lane == kWave - 1) s_total[wave] = x;
-  if (lane == 0) s_sum[wave] = p;
+  if (lane == kWave - 1) s_waves[wave] = x;
   __syncthreads();
-  int before = x - sum, total = 0;
-  p = 0.0f;
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? s_total[w] : 0;
-    total += s_total[w];
-    p += s_sum[w];
-  }
+  int before = x - v;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int b = tid * kPer + i;
-    if (b < blocks) count[b] = before;
-    before += mine[i];
-  }
-  if (tid == 0 && e < a.experts) {
-    a.counts[e] = total;
-    ws.p[(size_t)e * blocks] = p;
-  }
+  for (int w = 0; w < kWaves; ++w) before += w < wave ? s_waves[w] : 0;
+  __syncthreads();
+  return before;
 }
 
-// Places each slot at its expert's part of the order, slots of a block in their own order; block 0 also
-// computes the loss.
-__global__ __launch_bounds__(kThreads) void route_order_kernel(ggk_route_args a, Workspace ws, Plan plan) {
-  __shared__ int s_at[kMaxExperts + 1];
-  __shared__ int s_totals[kThreads];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  constexpr int kPer = (kMaxExperts + kThreads) / kThreads;
+// Turns s_at[e], the places taken before this block's slots of each expert, into places in the order, adding the
+// experts before (total[e]: all slots of e; the slots without an expert come last).
+__device__ __forceinline__ void add_experts_before(int* s_at, const int* total, int experts, int* s_waves) {
+  const int tid = threadIdx.x;
+  constexpr int kPer = (kMaxExperts + 1 + kThreads - 1) / kThreads;
   int mine[kPer], sum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = tid * kPer + i;
-    mine[i] = e < a.experts ? a.counts[e] : 0;
+    mine[i] = e < experts ? total[e] : 0;
     sum += mine[i];
   }
-  s_totals[tid] = sum;
-  __syncthreads();
-  int before = 0;
-  for (int i = 0; i < tid; ++i) before += s_totals[i];
+  int before = block_before(sum, s_waves);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = tid * kPer + i;
-    if (e <= a.experts) s_at[e] = before + ws.count[(size_t)e * plan.blocks + blockIdx.x];
+    if (e <= experts) s_at[e] += before;
     before += mine[i];
   }
   __syncthreads();
-  if (wave == 0) {
-    const long long first = (long long)blockIdx.x * plan.rows_per_block * a.slots;
-    long long last = first + (long long)plan.rows_per_block * a.slots;
-    const long long all = (long long)a.tokens * a.slots;
-    last = last < all ? last : all;
-    for (long long i0 = first; i0 < last; i0 += kWave) {
-      const bool in = i0 + lane < last;
-      int id = in ? a.ids[i0 + lane] : -1;
-      id = id < 0 ? a.experts : id;
-      unsigned long long same = __ballot(in);
-      for (int bit = 0; bit < 11; ++bit) {
-        const unsigned long long set = __ballot((id >> bit) & 1);
-        same &= ((id >> bit) & 1) ? set : ~set;
-      }
-      if (in) {
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        const int at = s_at[id];
-        __builtin_amdgcn_wave_barrier();
-        a.order[at + rank] = (int)(i0 + lane);
-        if (rank == 0) s_at[id] = at + __popcll(same);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// Places slots [first, last) by expert, in their own order within one.  s_at: the next place of each expert;
+// s_wave: kWaves * (experts + 1) ints.  Every wave takes a run of slots, 64 at a time: it counts its slots of
+// each expert, the waves' counts become their first places, and a slot goes to its wave's next place plus the number of
+// lanes below with the same expert.  Waves write only their own row of s_wave.
+__device__ __forceinline__ void place_slots(const ggk_route_args& a, long long first, long long last, const int* s_at,
+                                            int* s_wave) {
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, width = a.experts + 1;
+  for (int i = tid; i < kWaves * width; i += kThreads) s_wave[i] = 0;
+  __syncthreads();
+  const long long each = ((last - first + kWaves - 1) / kWaves + kWave - 1) / kWave * kWave;
+  const long long mine = first + wave * each, end = min(last, mine + each);
+  int* my = s_wave + wave * width;
+  const int bits = 32 - __builtin_clz(a.experts);
+  for (long long i = mine + lane; i < end; i += kWave) {
+    const int id = a.ids[i];
+    atomicAdd(&my[id < 0 ? a.experts : id], 1);
+  }
+  __syncthreads();
+  for (int e = tid; e < width; e += kThreads) {
+    int at = s_at[e];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const int n = s_wave[w * width + e];
+      s_wave[w * width + e] = at;
+      at += n;
     }
-  } else if (wave == 1 && blockIdx.x == 0 && a.loss != nullptr) {
-    int routed = 0;
-    for (int b = lane; b < plan.blocks; b += kWave) routed += ws.routed[b];
-    float used = 0.0f, part = 0.0f;
-    for (int d = 1; d < kWave; d *= 2) routed += __shfl_xor(routed, d, kWave);
-    for (int e = lane; e < a.experts; e += kWave) used += (float)a.counts[e];
-    used = wave_sum(used);
-    const float inv_used = used > 0.0f ? 1.0f / used : 0.0f;
-    const float inv_routed = routed > 0 ? 1.0f / (float)routed : 0.0f;
-    for (int e = lane; e < a.experts; e += kWave) {
-      const float f = (float)a.counts[e] * inv_used;
-      part += f * (ws.p[(size_t)e * plan.blocks] * inv_routed);
-      a.slope[e] = (float)a.experts * f * inv_routed;
+  }
+  __syncthreads();
+  for (long long i0 = mine; i0 < end; i0 += kWave) {
+    const bool in = i0 + lane < end;
+    int id = in ? a.ids[i0 + lane] : -1;
+    id = id < 0 ? a.experts : id;
+    unsigned long long same = __ballot(in);
+    for (int bit = 0; bit < bits; ++bit) {
+      const bool set = (id >> bit) & 1;
+      const unsigned long long other = __ballot(set);
+      same &= set ? other : ~other;
     }
-    part = wave_sum(part);
-    if (lane == 0) *a.loss = (float)a.experts * part;
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    const int at = my[id];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // every lane has read before the first lane of each expert writes
+    if (in) {
+      a.order[at + rank] = (int)(i0 + lane);
+      if (rank == 0) my[id] = at + __popcll(same);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
-// dz of one token a wave.
-template <class T, int V>
-__global__ __launch_bounds__(kThreads) void route_gradient_kernel(ggk_route_gradient_args a) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+// The loss and its slopes, by one wave: p[e] sums over all tokens, counts as in a.counts.
+__device__ __forceinline__ void balance_loss(const ggk_route_args& a, const float* p, const int* counts, int routed) {
+  const int lane = threadIdx.x % kWave;
+  int used = 0;
+  for (int e = lane; e < a.experts; e += kWave) used += counts[e];
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) used += __shfl_xor(used, d, kWave);
+  const float inv_used = used > 0 ? 1.0f / (float)used : 0.0f;
+  const float inv_routed = routed > 0 ? 1.0f / (float)routed : 0.0f;
+  float part = 0.0f;
+  for (int e = lane; e < a.experts; e += kWave) {
+    const float f = (float)counts[e] * inv_used;
+    part += f * (p[e] * inv_routed);
+    a.slope[e] = (float)a.experts * f * inv_routed;
+  }
+  part = group_sum<kWave>(part);
+  if (lane == 0) *a.loss = (float)a.experts * part;
+}
+
+__device__ __forceinline__ int all_routed(const Workspace& ws, int blocks) {
+  int routed = 0;
+  for (int b = threadIdx.x % kWave; b < blocks; b += kWave) routed += ws.routed[b];
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) routed += __shfl_xor(routed, d, kWave);
+  return routed;
+}
+
+// The order of one block's slots; the last block also computes the loss.  Without the columns kernel every block
+// adds up the counts of all blocks itself, and the last one the sums of p.
+__global__ __launch_bounds__(kThreads) void route_order_kernel(ggk_route_args a, Workspace ws, Plan plan) {
+  extern __shared__ int shared[];  // s_at, s_total [experts + 1] each, then s_wave
+  __shared__ int s_waves[kWaves];
+  const int tid = threadIdx.x, width = a.experts + 1, block = blockIdx.x;
+  int* s_at = shared;
+  int* s_total = shared + width;
+  int* s_wave = shared + 2 * width;
+  const bool last_block = block == (int)gridDim.x - 1;
+  if (plan.columns) {
+    for (int e = tid; e < width; e += kThreads) s_at[e] = ws.count[(size_t)block * width + e];
+    __syncthreads();
+    add_experts_before(s_at, a.counts, a.experts, s_waves);
+  } else {
+    // Threads take (slice of blocks, expert): slices of the columns are added up in LDS.
+    for (int e = tid; e < 2 * width; e += kThreads) shared[e] = 0;
+    __syncthreads();
+    const int slices = max(1, kThreads / width), each = (plan.blocks + slices - 1) / slices;
+    for (int i = tid; i < slices * width; i += kThreads) {
+      const int e = i % width, b0 = i / width * each, b1 = min(plan.blocks, b0 + each);
+      int before = 0, total = 0;
+#pragma unroll 8
+      for (int b = b0; b < b1; ++b) {
+        const int n = ws.count[(size_t)b * width + e];
+        before += b < block ? n : 0;
+        total += n;
+      }
+      atomicAdd(&s_at[e], before);
+      atomicAdd(&s_total[e], total);
+    }
+    __syncthreads();
+    add_experts_before(s_at, s_total, a.experts, s_waves);
+    if (last_block) {
+      for (int e = tid; e < a.experts; e += kThreads) a.counts[e] = s_total[e];
+    }
+  }
+  const long long all = (long long)a.tokens * a.slots;
+  const long long first = (long long)block * plan.rows * a.slots;
+  place_slots(a, first, min(all, first + (long long)plan.rows * a.slots), s_at, s_wave);
+  if (last_block && a.loss != nullptr) {
+    __syncthreads();
+    if (plan.columns) {
+      if (tid < kWave) balance_loss(a, ws.p, a.counts, all_routed(ws, plan.blocks));
+      return;
+    }
+    // Sums of p: slices of the blocks per expert, then the slices in their order.
+    float* s_p = reinterpret_cast<float*>(s_wave);
+    const int slices = min(kWaves, max(1, kThreads / a.experts)), each = (plan.blocks + slices - 1) / slices;
+    for (int i = tid; i < slices * a.experts; i += kThreads) {
+      const int e = i % a.experts, b0 = i / a.experts * each, b1 = min(plan.blocks, b0 + each);
+      float p = 0.0f;
+#pragma unroll 8
+      for (int b = b0; b < b1; ++b) p += ws.p[(size_t)b * a.experts + e];
+      s_p[i] = p;
+    }
+    __syncthreads();
+    for (int e = tid; e < a.experts; e += kThreads) {
+      float p = s_p[e];
+      for (int s = 1; s < slices; ++s) p += s_p[s * a.experts + e];
+      s_p[e] = p;
+    }
+    __syncthreads();
+    if (tid < kWave) balance_loss(a, s_p, s_total, all_routed(ws, plan.blocks));
+  }
+}
+
+// All of it for a few tokens, in one workgroup.
+template <class T, int L, int V>
+__global__ __launch_bounds__(kThreads) void route_small_kernel(ggk_route_args a, bool vectors) {
+  extern __shared__ int shared[];  // counts [experts + 1], routed, s_at [experts + 1], then s_part / s_wave
+  __shared__ int s_waves[kWaves];
+  const int tid = threadIdx.x, width = a.experts + 1;
+  int* s_count = shared;
+  int* s_routed = shared + width;
+  int* s_at = shared + width + 1;
+  int* s_rest = shared + 2 * width + 1;
+  for (int e = tid; e < 2 * width + 1; e += kThreads) shared[e] = 0;
+  __syncthreads();
+  float sums[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sums[j] = 0.0f;
+  int routed = 0;
+  for (int t0 = 0; t0 < a.tokens; t0 += kThreads / L) {
+    routed += route_token<T, L, V>(a, vectors, t0 + tid / L, a.tokens, s_count, sums) ? 1 : 0;
+  }
+  if (tid % L == 0 && routed > 0) atomicAdd(s_routed, routed);
+  __syncthreads();  // ids are read back below by other threads of this workgroup
+  if (a.loss != nullptr) {
+    float* s_part = reinterpret_cast<float*>(s_rest);
+    block_sums<L, V>(sums, a.experts, s_part, s_part);
+    __syncthreads();
+    if (tid < kWave) balance_loss(a, s_part, s_count, *s_routed);
+    __syncthreads();
+  }
+  for (int e = tid; e < a.experts; e += kThreads) a.counts[e] = s_count[e];
+  add_experts_before(s_at, s_count, a.experts, s_waves);
+  place_slots(a, 0, (long long)a.tokens * a.slots, s_at, s_rest);
+}
+
+// ---------------------------------------------------------------- backward
+
+template <class T, int L, int V>
+__global__ __launch_bounds__(kThreads) void route_gradient_kernel(ggk_route_gradient_args a, bool vectors) {
+  using Z = Logit<T>;
+  using C = Columns<L, V>;
+  constexpr int W = C::W;
+  constexpr int kGroups = kThreads / L;
+  const int lane = threadIdx.x % L;
   const float d_loss = a.d_loss != nullptr ? *a.d_loss : 0.0f;
-  for (int t = blockIdx.x * kWaves + wave; t < a.tokens; t += gridDim.x * kWaves) {
-    const T* row = static_cast<const T*>(a.logits) + (long long)t * a.ld;
-    T* out = static_cast<T*>(a.d_logits) + (long long)t * a.experts;
+  // Without a loss, normalized weights depend on the chosen logits alone.
+  const bool softmax = a.d_loss != nullptr || !a.normalize;
+  float c[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int e = C::expert(lane, j);
+    c[j] = a.d_loss != nullptr && e < a.experts ? d_loss * a.slope[e] : 0.0f;
+  }
+  for (long long t0 = (long long)blockIdx.x * kGroups; t0 < a.tokens; t0 += (long long)gridDim.x * kGroups) {
+    const int t = (int)t0 + threadIdx.x / L;
+    const bool in = t < a.tokens;
+    const T* row = static_cast<const T*>(a.logits) + (long long)(in ? t : 0) * a.ld;
     const long long slot0 = (long long)t * a.slots;
-    const int my_id = lane < a.slots ? a.ids[slot0 + lane] : -1;
+    const int my_id = in && lane < a.slots ? a.ids[slot0 + lane] : -1;
     const bool has = my_id >= 0 && my_id < a.experts;
-    float d[V];
+    const bool routed = group_any<L>(has);
+    const float g = has && a.d_weights != nullptr ? a.scale * a.d_weights[slot0 + lane] : 0.0f;
+    const float my_z = has ? Z::value(row[my_id]) : -__builtin_inff();
+    float d[V], top = 0.0f, inv = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = 0.0f;
-    if (__ballot(has) != 0) {
-      float z[V], top = -__builtin_inff(), total = 0.0f;
+    if (softmax) {
+      T z[V];
+      load_row<T, L, V>(row, lane, in ? a.experts : 0, vectors, Z::store(-__builtin_inff()), z);
+      top = -__builtin_inff();
+      float total = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) top = fmaxf(top, Z::value(z[j]));
+      top = group_max<L>(top);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int e = lane + kWave * j;
-        z[j] = e < a.experts ? to_float(row[e]) : -__builtin_inff();
-        top = fmaxf(top, z[j]);
+        d[j] = routed ? exp_of(Z::value(z[j]) - top) : 0.0f;
+        total += d[j];
       }
-      top = wave_max(top);
-      float p[V];
+      total = group_sum<L>(total);
+      inv = routed ? 1.0f / total : 0.0f;
+    }
+    float my_a;
+    if (a.normalize) {
+      const float peak = group_max<L>(my_z);  // by every lane: exchanges are not made under a lane's condition
+      const float e = has ? exp_of(my_z - peak) : 0.0f;
+      my_a = e / group_sum<L>(e);
+    } else {
+      my_a = exp_of(my_z - top) * inv;
+    }
+    const float mean = group_sum<L>(has ? my_a * g : 0.0f);
+    const float my_d = has ? my_a * (a.normalize ? g - mean : g) : 0.0f;
+    if (softmax) {
+      float dot = 0.0f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        p[j] = expf(z[j] - top);
-        total += p[j];
+        d[j] *= inv;
+        dot = fmaf(d[j], c[j], dot);
       }
-      total = wave_sum(total);
-      const float my_z = has ? to_float(row[my_id]) : -__builtin_inff();
-      float my_a = 0.0f;
-      if (a.normalize) {
-        const float peak = wave_max(my_z);
-        const float e = has ? expf(my_z - peak) : 0.0f;
-        my_a = e / wave_sum(e);
-      } else {
-        my_a = has ? expf(my_z - top) / total : 0.0f;
-      }
-      const float g = has && a.d_weights != nullptr ? a.scale * a.d_weights[slot0 + lane] : 0.0f;
-      const float mean = wave_sum(has ? my_a * g : 0.0f);
-      const float my_d = has ? (a.normalize ? my_a * (g - mean) : my_a * g) : 0.0f;
-      float c[V], dot = 0.0f;
+      dot = group_sum<L>(dot) + (a.normalize ? 0.0f : mean);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = lane + kWave * j;
-        p[j] = p[j] / total;
-        c[j] = e < a.experts && a.slope != nullptr ? d_loss * a.slope[e] : 0.0f;
-        dot += p[j] * c[j];
-      }
-      dot = wave_sum(dot) + (a.normalize ? 0.0f : mean);
-#pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = p[j] * (c[j] - dot);
+      for (int j = 0; j < V; ++j) d[j] = routed ? d[j] * (c[j] - dot) : 0.0f;
+    }
+    if (a.d_weights != nullptr) {
+      // Slot by slot, so that an expert named twice is added in the slots' order.
       for (int s = 0; s < a.slots; ++s) {
-        const int id = __shfl(has ? my_id : -1, s, kWave);
-        const float part = __shfl(my_d, s, kWave);
+        const int id = __shfl(has ? my_id : -1, s, L);
+        const float part = __shfl(my_d, s, L);
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] += id == lane + kWave * j ? part : 0.0f;
+        for (int j = 0; j < V; ++j) d[j] += id == C::expert(lane, j) ? part : 0.0f;
       }
     }
+    T* out = static_cast<T*>(a.d_logits) + (long long)t * a.experts;
+    typedef struct alignas(sizeof(T) * W) {
+      T v[W];
+    } Vector;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (lane + kWave * j < a.experts) from_float(d[j], &out[lane + kWave * j]);
+    for (int j = 0; j < V; j += W) {
+      const int e = C::expert(lane, j);
+      if (vectors) {
+        if (in && e < a.experts) {
+          Vector x;
+#pragma unroll
+          for (int i = 0; i < W; ++i) x.v[i] = Z::store(d[j + i]);
+          *reinterpret_cast<Vector*>(out + e) = x;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          if (in && e + i < a.experts) out[e + i] = Z::store(d[j + i]);
+        }
+      }
     }
   }
 }
 
-template <class T>
-hipError_t launch_rows(const ggk_route_args& a, const Workspace& ws, const Plan& plan, hipStream_t stream) {
-  auto kernel = a.experts <= 64 ? route_rows_kernel<T, 1>
-                : a.experts <= 128 ? route_rows_kernel<T, 2>
-                : a.experts <= 256 ? route_rows_kernel<T, 4>
-                : a.experts <= 512 ? route_rows_kernel<T, 8> : route_rows_kernel<T, 16>;
-  hipLaunchKernelGGL(kernel, dim3(plan.blocks), dim3(kThreads), 0, stream, a, ws, plan);
+// ---------------------------------------------------------------- launches
+
+// At most this many tokens are routed by one workgroup.
+constexpr int kSmallTokens = 128;
+
+template <class T, int L, int V>
+hipError_t launch_route(const ggk_route_args& a, Plan plan, hipStream_t stream) {
+  const size_t width = a.experts + 1;
+  const size_t waves = sizeof(int) * kWaves * width;
+  plan.vectors = whole_vectors<T, V>(a.logits, a.tokens > 1 ? a.ld : 0, a.experts);
+  if (a.tokens <= kSmallTokens) {
+    hipLaunchKernelGGL((route_small_kernel<T, L, V>), dim3(1), dim3(kThreads), sizeof(int) * (2 * width + 1) + waves,
+                       stream, a, plan.vectors);
+    return hipGetLastError();
+  }
+  const Workspace ws = carve(a.workspace, a.experts, plan.blocks);
+  hipLaunchKernelGGL((route_rows_kernel<T, L, V>), dim3(plan.blocks), dim3(kThreads),
+                     sizeof(int) * (width + 1) + (a.loss != nullptr ? waves : 0), stream, a, ws, plan);
+  hipError_t st = hipGetLastError();
+  if (st != hipSuccess) return st;
+  if (plan.columns) {
+    hipLaunchKernelGGL(route_columns_kernel, dim3((a.experts + kColumns) / kColumns), dim3(kThreads), 0, stream, a, ws,
+                       plan.blocks);
+    st = hipGetLastError();
+    if (st != hipSuccess) return st;
+  }
+  hipLaunchKernelGGL(route_order_kernel, dim3(plan.blocks), dim3(kThreads), sizeof(int) * 2 * width + waves, stream, a,
+                     ws, plan);
   return hipGetLastError();
 }
 
-template <class T>
+template <class T, int L, int V>
 hipError_t launch_gradient(const ggk_route_gradient_args& a, hipStream_t stream) {
-  auto kernel = a.experts <= 64 ? route_gradient_kernel<T, 1>
-                : a.experts <= 128 ? route_gradient_kernel<T, 2>
-                : a.experts <= 256 ? route_gradient_kernel<T, 4>
-                : a.experts <= 512 ? route_gradient_kernel<T, 8> : route_gradient_kernel<T, 16>;
-  const int blocks = min((a.tokens + kWaves - 1) / kWaves, 8192);
-  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, stream, a);
+  const int groups = kThreads / L;
+  const int blocks = (int)(((long long)a.tokens + groups - 1) / groups);
+  const bool vectors = whole_vectors<T, V>(a.logits, a.tokens > 1 ? a.ld : 0, a.experts) &&
+                       whole_vectors<T, V>(a.d_logits, a.experts, a.experts);
+  hipLaunchKernelGGL((route_gradient_kernel<T, L, V>), dim3(blocks < 1024 ? blocks : 1024), dim3(kThreads), 0, stream, a,
+                     vectors);
   return hipGetLastError();
+}
+
+// Lanes a token and values a lane: 16 lanes while a token's experts fit them at 16 values each and its slots
+// fit one a lane, else the wave.
+#define GG_ROUTE_FORMS(T, CALL)                                      \
+  if (a.experts <= 256 && a.slots <= 16) {                           \
+    return a.experts <= 16 ? CALL(T, 16, 1) : a.experts <= 32 ? CALL(T, 16, 2) : a.experts <= 64 ? CALL(T, 16, 4) \
+           : a.experts <= 128 ? CALL(T, 16, 8) : CALL(T, 16, 16);    \
+  }                                                                  \
+  return a.experts <= 256 ? CALL(T, 64, 4) : a.experts <= 512 ? CALL(T, 64, 8) : CALL(T, 64, 16);
+
+template <class T>
+hipError_t route_of_type(const ggk_route_args& a, const Plan& plan, hipStream_t stream) {
+#define GG_CALL(T, L, V) launch_route<T, L, V>(a, plan, stream)
+  GG_ROUTE_FORMS(T, GG_CALL)
+#undef GG_CALL
+}
+
+template <class T>
+hipError_t gradient_of_type(const ggk_route_gradient_args& a, hipStream_t stream) {
+#define GG_CALL(T, L, V) launch_gradient<T, L, V>(a, stream)
+  GG_ROUTE_FORMS(T, GG_CALL)
+#undef GG_CALL
 }
 
 bool bad_sizes(int tokens, int experts, int slots, int type, long long ld) {
   return tokens < 0 || experts < 1 || experts > kMaxExperts || slots < 1 || slots > GGK_ROUTE_MAX_SLOTS ||
          (type != GGK_TYPE_F32 && type != GGK_TYPE_F16 && type != GGK_TYPE_BF16) || (tokens > 1 && ld < experts) ||
-         (long long)tokens * slots > 0x7fffffffLL;
+         (long long)tokens * slots > GGK_ROUTE_MAX_TOTAL_SLOTS;
 }
 
 }  // namespace
 
 extern "C" size_t ggk_route_workspace(int tokens, int experts) {
-  if (tokens < 0 || experts < 1 || experts > kMaxExperts) return 0;
-  return workspace_bytes(experts, plan_blocks(tokens).blocks);
+  if (tokens <= kSmallTokens || experts < 1 || experts > kMaxExperts) return 0;
+  return sizeof(int) * workspace_ints(experts, plan_blocks(tokens, experts).blocks);
 }
 
 extern "C" hipError_t ggk_route_check(const ggk_route_args* args) {
@@ -426,7 +844,7 @@ extern "C" hipError_t ggk_route_check(const ggk_route_args* args) {
   if (bad_sizes(a.tokens, a.experts, a.slots, a.type, a.ld)) return hipErrorInvalidValue;
   if (a.given_ids == nullptr && a.slots > a.experts) return hipErrorInvalidValue;
   if (a.workspace_bytes < ggk_route_workspace(a.tokens, a.experts)) return hipErrorInvalidValue;
-  if (a.counts == nullptr || a.workspace == nullptr || (a.loss == nullptr) != (a.slope == nullptr) ||
+  if (a.counts == nullptr || (a.workspace == nullptr && a.tokens > kSmallTokens) || (a.loss == nullptr) != (a.slope == nullptr) ||
       (a.tokens > 0 && (a.logits == nullptr || a.weights == nullptr || a.ids == nullptr || a.order == nullptr))) {
     return hipErrorInvalidDevicePointer;
   }
@@ -434,20 +852,13 @@ extern "C" hipError_t ggk_route_check(const ggk_route_args* args) {
 }
 
 extern "C" hipError_t ggk_route(const ggk_route_args* args, hipStream_t stream) {
-  hipError_t st = ggk_route_check(args);
+  const hipError_t st = ggk_route_check(args);
   if (st != hipSuccess) return st;
   const ggk_route_args& a = *args;
-  const Plan plan = plan_blocks(a.tokens);
-  const Workspace ws = carve(a.workspace, a.experts, plan.blocks);
-  st = a.type == GGK_TYPE_F32 ? launch_rows<float>(a, ws, plan, stream)
-       : a.type == GGK_TYPE_F16 ? launch_rows<_Float16>(a, ws, plan, stream)
-                                : launch_rows<__hip_bfloat16>(a, ws, plan, stream);
-  if (st != hipSuccess) return st;
-  hipLaunchKernelGGL(route_columns_kernel, dim3(a.experts + 1), dim3(kThreads), 0, stream, a, ws, plan.blocks);
-  st = hipGetLastError();
-  if (st != hipSuccess) return st;
-  hipLaunchKernelGGL(route_order_kernel, dim3(plan.blocks), dim3(kThreads), 0, stream, a, ws, plan);
-  return hipGetLastError();
+  const Plan plan = plan_blocks(a.tokens, a.experts);
+  return a.type == GGK_TYPE_F32 ? route_of_type<float>(a, plan, stream)
+         : a.type == GGK_TYPE_F16 ? route_of_type<_Float16>(a, plan, stream)
+                                  : route_of_type<__hip_bfloat16>(a, plan, stream);
 }
 
 extern "C" hipError_t ggk_route_gradient_check(const ggk_route_gradient_args* args) {
@@ -464,7 +875,7 @@ extern "C" hipError_t ggk_route_gradient_check(const ggk_route_gradient_args* ar
 extern "C" hipError_t ggk_route_gradient(const ggk_route_gradient_args* args, hipStream_t stream) {
   const hipError_t st = ggk_route_gradient_check(args);
   if (st != hipSuccess || args->tokens == 0) return st;
-  return args->type == GGK_TYPE_F32 ? launch_gradient<float>(*args, stream)
-         : args->type == GGK_TYPE_F16 ? launch_gradient<_Float16>(*args, stream)
-                                      : launch_gradient<__hip_bfloat16>(*args, stream);
+  return args->type == GGK_TYPE_F32 ? gradient_of_type<float>(*args, stream)
+         : args->type == GGK_TYPE_F16 ? gradient_of_type<_Float16>(*args, stream)
+                                      : gradient_of_type<__hip_bfloat16>(*args, stream);
 }

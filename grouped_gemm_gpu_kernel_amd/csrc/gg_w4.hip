@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kThreads) void w4_kernel(ggk_w4_args a) {
 extern "C" hipError_t ggk_w4_check(const ggk_w4_args* args) {
   if (args == nullptr) return hipErrorInvalidValue;
   const ggk_w4_args& a = *args;
-  if (a.rows < 0 || a.x_rows < 0 || a.n < 0 || a.k < 0 || a.experts < 0 || a.experts > GGK_MOE_MAX_EXPERTS ||
+  if (a.rows < 0 || a.rows > GGK_ROUTE_MAX_TOTAL_SLOTS || a.x_rows < 0 || a.n < 0 || a.k < 0 || a.experts < 0 || a.experts > GGK_MOE_MAX_EXPERTS ||
       a.group < 32 || a.group % 32 != 0 || a.k % a.group != 0 || (a.y_type != GGK_TYPE_F32 && a.y_type != GGK_TYPE_F16)) {
     return hipErrorInvalidValue;
   }

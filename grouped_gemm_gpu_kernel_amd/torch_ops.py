@@ -25,7 +25,6 @@ All work runs in the HIP library (lib/libgrouped_gemm_amd.so); there is no CPU f
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import operator
 from typing import NamedTuple, Optional, Sequence, Union
@@ -353,18 +352,19 @@ class Routing(NamedTuple):
     balance_loss: Optional[torch.Tensor]  # float32 scalar, None unless asked for
 
 
-def _on_device(device: torch.device):
-    """The device made current, at no cost where it is already."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
 def _launch(name: str, args, device: torch.device) -> None:
-    """A library entry point on the device's current stream."""
-    with _on_device(device):
-        status = getattr(_lib.lib(), name)(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream or None)
-    _lib.check(status, name)
+    """A library entry point on the device's current stream (its handle as it is: the Stream object that
+    torch.cuda.current_stream makes costs 2 us)."""
+    index = device.index
+    entry = getattr(_lib.lib(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index) or None
+    if index == torch.cuda.current_device():
+        status = entry(ctypes.byref(args), stream)
+    else:
+        with torch.cuda.device(device):
+            status = entry(ctypes.byref(args), stream)
+    if status:
+        _lib.check(status, name)
 
 
 def _check_vector(t: torch.Tensor, name: str, dtype: torch.dtype, count: int, device) -> None:
@@ -392,13 +392,13 @@ def _route(logits, ids, token_mask, slots, normalize, scale, balance):
     loss = torch.empty((), dtype=torch.float32, device=device) if balance else None
     slope = torch.empty(experts, dtype=torch.float32, device=device) if balance else None
     size = _lib.lib().ggk_route_workspace(tokens, experts)
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _launch("ggk_route", _lib.GGKRouteArgs(
         tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr() or dummy, _row_stride(logits),
         token_mask.data_ptr() or dummy if token_mask is not None else None,
         ids.data_ptr() or dummy if ids is not None else None, normalize, scale, weights.data_ptr() or dummy,
         chosen.data_ptr() or dummy, counts.data_ptr(), order.data_ptr() or dummy, loss.data_ptr() if balance else None,
-        slope.data_ptr() if balance else None, workspace.data_ptr(), size), device)
+        slope.data_ptr() if balance else None, workspace.data_ptr() if size else None, size), device)
     return weights, chosen, counts, order, loss, slope
 
 
@@ -481,8 +481,8 @@ def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optiona
         slots = operator.index(top_k)
         if not 1 <= slots <= min(experts, _lib.GGK_ROUTE_MAX_SLOTS):
             raise ValueError(f"top_k is {slots}, expected 1 to {min(experts, _lib.GGK_ROUTE_MAX_SLOTS)}")
-    if tokens * slots > 0x7fffffff:
-        raise ValueError(f"{tokens} tokens with {slots} slots each: 2^31 slots or more")
+    if tokens * slots > _lib.GGK_ROUTE_MAX_TOTAL_SLOTS:
+        raise ValueError(f"{tokens} tokens with {slots} slots each: more than 2^30 slots")
     if token_mask is not None:
         _check_vector(token_mask, "token_mask", torch.bool, tokens, logits.device)
     args = (logits, ids, token_mask, slots, bool(normalize), float(scale), bool(balance))
@@ -601,8 +601,8 @@ def moe_w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, counts
         raise TypeError("order must be a torch.Tensor")
     rows = order.numel()
     _check_vector(order, "order", torch.int32, rows, x.device)
-    if rows > 0x7fffffff:
-        raise ValueError(f"order has {rows} entries: 2^31 or more")
+    if rows > _lib.GGK_ROUTE_MAX_TOTAL_SLOTS:
+        raise ValueError(f"order has {rows} entries: more than 2^30")
     if rows and (x.shape[0] == 0 or rows % x.shape[0] != 0):
         raise ValueError(f"order has {rows} entries, not a multiple of x's {x.shape[0]} rows")
     if row_weights is not None:

@@ -375,12 +375,13 @@ hipError_t ggk_launch_grouped_device_done(int variant, int path, int addressing,
  *                   such token; slope[e] = d loss / d (sum of softmax(z_t)[e]).
  * loss and slope may be NULL, both or neither.  Sums are made in a fixed
  * order: the same call gives the same bits.  workspace holds
- * ggk_route_workspace(tokens, experts) bytes, written before they are read;
- * calls that may overlap need one each.  1 <= experts <=
+ * ggk_route_workspace(tokens, experts) bytes (0 for a few tokens), written
+ * before they are read; calls that may overlap need one each.  1 <= experts <=
  * GGK_MOE_MAX_EXPERTS, 1 <= slots <= GGK_ROUTE_MAX_SLOTS and, without
- * given_ids, slots <= experts; tokens * slots < 2^31. */
+ * given_ids, slots <= experts; tokens * slots <= GGK_ROUTE_MAX_TOTAL_SLOTS. */
 enum { GGK_TYPE_F32 = 0, GGK_TYPE_F16 = 1, GGK_TYPE_BF16 = 2 };
 #define GGK_ROUTE_MAX_SLOTS 64
+#define GGK_ROUTE_MAX_TOTAL_SLOTS (1 << 30)
 
 typedef struct ggk_route_args {
   int tokens;
@@ -448,7 +449,8 @@ hipError_t ggk_route_gradient(const ggk_route_gradient_args* args, hipStream_t s
  * o = order[r] reads x row o / (rows / x_rows) and writes y row o, times
  * row_weights[o] if given; slots past the counts' sum are set to 0.  Counts
  * are not trusted: a negative one is taken as 0, what goes past `rows` is
- * dropped, and an order entry outside [0, rows) is passed over. */
+ * dropped, and an order entry outside [0, rows) is passed over.  rows <=
+ * GGK_ROUTE_MAX_TOTAL_SLOTS. */
 typedef struct ggk_w4_args {
   int rows; /* of y */
   int x_rows;

@@ -132,9 +132,10 @@ def _route_args(**over):
 @pytest.mark.parametrize("over,status", [
     ({}, 0), ({"tokens": -1}, 1), ({"experts": 0}, 1), ({"experts": 1025, "ld": 1025}, 1), ({"slots": 0}, 1),
     ({"slots": 9}, 1), ({"slots": 9, "given_ids": 0x1000}, 0), ({"slots": 65, "given_ids": 0x1000}, 1),
-    ({"type": 3}, 1), ({"ld": 7}, 1), ({"tokens": 1, "ld": 0}, 0), ({"workspace_bytes": 0}, 1), ({"logits": None}, 17),
+    ({"type": 3}, 1), ({"ld": 7}, 1), ({"tokens": 1, "ld": 0}, 0), ({"workspace": None, "workspace_bytes": 0}, 0), ({"logits": None}, 17),
     ({"counts": None}, 17), ({"order": None}, 17), ({"loss": 0x1000}, 17), ({"slope": 0x1000}, 17),
-    ({"loss": 0x1000, "slope": 0x1000}, 0), ({"tokens": 1 << 30}, 1),
+    ({"loss": 0x1000, "slope": 0x1000}, 0), ({"tokens": (1 << 29) + 1}, 1), ({"tokens": 1 << 29}, 0),
+    ({"tokens": 1000, "workspace_bytes": 0}, 1), ({"tokens": 1000, "workspace": None}, 17),
     ({"tokens": 0, "logits": None, "weights": None, "ids": None, "order": None}, 0)])
 def test_route_arguments_are_checked_on_the_host(over, status):
     assert _lib.lib().ggk_route_check(ctypes.byref(_route_args(**over))) == status
@@ -189,8 +190,8 @@ def test_refusals_of_the_torch_call():
                  "contiguous")]:
             with pytest.raises(error, match=text):
                 torch_ops.moe_route(z, **bad)
-        with pytest.raises(ValueError, match="2\\^31"):
-            torch_ops.moe_route(logits(1 << 28, 8), 8)
+        with pytest.raises(ValueError, match="2\\^30"):
+            torch_ops.moe_route(logits((1 << 27) + 1, 8), 8)
 
 
 # ---------------------------------------------------------------- GPU
