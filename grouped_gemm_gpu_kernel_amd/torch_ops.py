@@ -356,13 +356,12 @@ def _launch(name: str, args, device: torch.device) -> None:
     """A library entry point on the device's current stream (its handle as it is: the Stream object that
     torch.cuda.current_stream makes costs 2 us)."""
     index = device.index
-    entry = getattr(_lib.lib(), name)
     stream = torch._C._cuda_getCurrentRawStream(index) or None
     if index == torch.cuda.current_device():
-        status = entry(ctypes.byref(args), stream)
+        status = getattr(_lib.lib(), name)(ctypes.byref(args), stream)
     else:
         with torch.cuda.device(device):
-            status = entry(ctypes.byref(args), stream)
+            status = getattr(_lib.lib(), name)(ctypes.byref(args), stream)
     if status:
         _lib.check(status, name)
 
@@ -384,22 +383,49 @@ def _route(logits, ids, token_mask, slots, normalize, scale, balance):
     """The launch behind moe_route: weights, ids, counts, order, loss, slope."""
     tokens, experts = logits.shape
     device = logits.device
-    dummy = _placeholder(device)
     weights = torch.empty((tokens, slots), dtype=torch.float32, device=device)
     chosen = torch.empty((tokens, slots), dtype=torch.int32, device=device)
     counts = torch.empty(experts, dtype=torch.int32, device=device)
     order = torch.empty(tokens * slots, dtype=torch.int32, device=device)
-    loss = torch.empty((), dtype=torch.float32, device=device) if balance else None
-    slope = torch.empty(experts, dtype=torch.float32, device=device) if balance else None
+    loss = slope = workspace = None
+    if balance:
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        slope = torch.empty(experts, dtype=torch.float32, device=device)
+    if tokens == 0:
+        counts.zero_()
+        return weights, chosen, counts, order, loss.zero_() if balance else None, slope
     size = _lib.lib().ggk_route_workspace(tokens, experts)
-    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    if size:
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
     _launch("ggk_route", _lib.GGKRouteArgs(
-        tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr() or dummy, _row_stride(logits),
-        token_mask.data_ptr() or dummy if token_mask is not None else None,
-        ids.data_ptr() or dummy if ids is not None else None, normalize, scale, weights.data_ptr() or dummy,
-        chosen.data_ptr() or dummy, counts.data_ptr(), order.data_ptr() or dummy, loss.data_ptr() if balance else None,
-        slope.data_ptr() if balance else None, workspace.data_ptr() if size else None, size), device)
+        tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr(), _row_stride(logits),
+        None if token_mask is None else token_mask.data_ptr(), None if ids is None else ids.data_ptr(), normalize, scale,
+        weights.data_ptr(), chosen.data_ptr(), counts.data_ptr(), order.data_ptr(),
+        loss.data_ptr() if balance else None, slope.data_ptr() if balance else None,
+        workspace.data_ptr() if size else None, size), device)
     return weights, chosen, counts, order, loss, slope
+
+
+def _route_gradient(ctx, d_weights, _ids, _counts, _order, d_loss):
+    logits, chosen, slope = ctx.saved_tensors
+    if d_weights is None and d_loss is None:
+        return (None,) * 7
+    slots, normalize, scale = ctx.how
+    tokens, experts = logits.shape
+    d_logits = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
+    if tokens:
+        if d_weights is not None:
+            d_weights = d_weights.contiguous()  # it may come expanded (a sum's) or in any strides
+        _launch("ggk_route_gradient", _lib.GGKRouteGradientArgs(
+            tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr(), _row_stride(logits), chosen.data_ptr(),
+            None if slope is None else slope.data_ptr(), normalize, scale,
+            None if d_weights is None else d_weights.data_ptr(), None if d_loss is None else d_loss.data_ptr(),
+            d_logits.data_ptr()), logits.device)
+    return d_logits, None, None, None, None, None, None
+
+
+# For a backward pass that builds a graph: a second derivative through it is refused.
+_route_gradient_once = torch.autograd.function.once_differentiable(_route_gradient)
 
 
 class _Route(torch.autograd.Function):
@@ -413,23 +439,8 @@ class _Route(torch.autograd.Function):
         return weights, chosen, counts, order, loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_weights, _ids, _counts, _order, d_loss):
-        logits, chosen, slope = ctx.saved_tensors
-        if d_weights is None and d_loss is None:
-            return (None,) * 7
-        slots, normalize, scale = ctx.how
-        tokens, experts = logits.shape
-        dummy = _placeholder(logits.device)
-        # Gradients may come expanded (a sum's) or in any strides.
-        d_weights = d_weights.contiguous() if d_weights is not None else None
-        d_logits = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
-        _launch("ggk_route_gradient", _lib.GGKRouteGradientArgs(
-            tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr() or dummy, _row_stride(logits),
-            chosen.data_ptr() or dummy, slope.data_ptr() if slope is not None else None, normalize, scale,
-            d_weights.data_ptr() or dummy if d_weights is not None else None,
-            d_loss.data_ptr() if d_loss is not None else None, d_logits.data_ptr() or dummy), logits.device)
-        return (d_logits,) + (None,) * 6
+    def backward(ctx, *grads):
+        return _route_gradient_once(ctx, *grads) if torch.is_grad_enabled() else _route_gradient(ctx, *grads)
 
 
 def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optional[torch.Tensor] = None,

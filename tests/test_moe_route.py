@@ -403,6 +403,29 @@ def test_gradient_against_differences(torch_cuda):
 
 
 @pytest.mark.gpu
+def test_a_second_derivative_is_refused(torch_cuda):
+    z = _logits(20, 8, "f32", 2).requires_grad_(True)
+    r = torch_ops.moe_route(z, 2, balance=True)
+    d, = torch.autograd.grad((r.weights.square().sum() + r.balance_loss,), z, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        d.sum().backward()
+
+
+@pytest.mark.gpu
+def test_saved_tensors_changed_in_place_are_noticed(torch_cuda):
+    """ids changed before the backward pass raise; counts and order, which it does not read, may be."""
+    z = _logits(200, 8, "f32", 2).requires_grad_(True)
+    r = torch_ops.moe_route(z, 2, balance=True)
+    r.counts.add_(1)
+    r.order.zero_()
+    r.weights.sum().backward()
+    r = torch_ops.moe_route(z, 2, balance=True)
+    r.ids.zero_()
+    with pytest.raises(RuntimeError, match="inplace"):
+        r.weights.sum().backward()
+
+
+@pytest.mark.gpu
 def test_no_tokens(torch_cuda):
     z = torch.empty(0, 12, device="cuda", requires_grad=True)
     r = torch_ops.moe_route(z, 3, balance=True)

@@ -53,7 +53,7 @@ MOE = dict(experts=3, counts=0x1000, order=0x1000, stride_q=512, stride_s=16)
 
 @pytest.mark.parametrize("over,status", [
     ({}, 0), ({"rows": -1}, 1), ({"rows": 5}, 1), ({"n": -1}, 1), ({"group": 16}, 1), ({"group": 48}, 1),
-    ({"group": 96}, 1), ({"group": 0}, 1), ({"k": 96}, 1), ({"ldx": 127}, 1), ({"ldq": 48}, 1), ({"ldq": 72}, 1),
+    ({"group": 96}, 1), ({"group": 0}, 1), ({"k": 96}, 1), ({"k": 0}, 1), ({"ldx": 127}, 1), ({"ldq": 48}, 1), ({"ldq": 72}, 1),
     ({"q": 0x1008}, 1), ({"lds": 1}, 1), ({"zeros": 0x1000, "ldz": 1}, 1), ({"zeros": 0x1000, "ldz": 2}, 0),
     ({"ldy": 7}, 1), ({"y_type": _lib.GGK_TYPE_BF16}, 1), ({"x": None}, 17), ({"q": None}, 17), ({"scales": None}, 17),
     ({"y": None}, 17), ({"rows": 0, "x_rows": 0, "x": None, "y": None}, 0), ({"n": 0, "q": None}, 0), (MOE, 0),
@@ -192,17 +192,16 @@ def test_odd_values(torch_cuda, rows):
     s[11, 3] = math.inf
     x[rows - 1, 5] = math.inf
     y = torch_ops.w4_matmul(x, q, s, z)
-    want = x.double() @ values(q, s, z).t()
     fine = torch.ones_like(y, dtype=torch.bool)
     fine[rows - 1] = False
     fine[:, 10:12] = False
     assert torch.isfinite(y[fine]).all()
+    # an infinite scale gives infinity or NaN, by whether it multiplies a group's sum or each weight of it
     assert torch.isnan(y[:, 10]).all() and not torch.isfinite(y[:, 11]).any()
     assert not torch.isfinite(y[rows - 1]).any()
     if rows > 1:
         keep = [j for j in range(70) if j not in (10, 11)]
         check(y[: rows - 1, keep], x[: rows - 1].double(), w[keep])
-        assert torch.equal(torch.isnan(y[:-1, 11]), torch.isnan(want[:-1, 11]))
 
 
 @pytest.mark.gpu
