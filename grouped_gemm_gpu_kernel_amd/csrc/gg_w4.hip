@@ -3,21 +3,23 @@
 //
 //   y[i][j] = sum_g scales[j][g] * sum_{k in g} x[i][k] * (q[j][k] - zeros[j][g])
 //
-// With few rows the weights' bytes are what counts: they are read once, 16
-// bytes a lane, straight into registers, and turned into binary16 there.
-// q - zero is an integer of at most 9 bits, so binary16 holds it exactly, the
-// matrix instructions (v_mfma_f32_16x16x32_f16: 16 rows of x by 16 columns j)
-// sum exact products in float, and a group's scale multiplies its sum: no weight
-// is ever rounded.
+// With few rows the weights' bytes are what counts: they are read once, into registers, and turned into binary16
+// there.  q - zero is an integer of at most 9 bits, which binary16 holds exactly; the matrix instructions
+// (v_mfma_f32_16x16x32_f16: 16 rows of x by 16 columns j) sum exact products in float, and a group's scale
+// multiplies its sum: no weight is ever rounded.
 //
-// A workgroup of 8 waves computes 16 NT (8 / WK) columns of up to 16 MAXT rows: WK waves split K among them, step
-// by step, so that a narrow matrix still gives every CU loads to wait for, and their sums are joined in LDS in the
-// waves' order.  x goes through LDS, a chunk of K at a time (all of it if the rows are few): read by every wave
-// from memory it would take the vector memory path for longer than the weights do (four 16-byte loads a lane
-// for each 16 bytes of weights).
+// Both operands go through LDS.  A load is coalesced among 16 neighbouring lanes, which in the instruction's order
+// hold 16 rows: straight to registers each would take 64 cache accesses instead of 16, and that bounded the kernel (55
+// accesses a load, three quarters of its cycles).  Weights are loaded 64 bytes of each of 16 rows of q at a time into
+// registers, four steps ahead, then written to the wave's own LDS and read back in the instruction's order.  x is
+// loaded by the workgroup straight into LDS, a chunk of K ahead.
+//
+// A workgroup of 8 waves computes 16 (8 / WK) columns of up to R rows: WK waves split K among them, step by step, so
+// that a narrow matrix still gives every CU loads to wait for, and their sums are joined in LDS in the waves' order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "gg_common.h"
 #include "grouped_gemm_amd_kernels.h"
 
 namespace {
@@ -27,53 +29,39 @@ typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
-// A row of x may start on any element.
-typedef half8v half8_any __attribute__((aligned(2)));
 
 constexpr int kWave = 64;
 constexpr int kCus = 256;
 constexpr int kStep = 128;  // values of k a wave takes at once: 16 bytes of each of 16 rows of q in 4 lanes
 constexpr int kMaxExperts = GGK_MOE_MAX_EXPERTS;
 
-// The 8 weights of a dword less `zero`, in the order k0 k4 k1 k5 k2 k6 k3 k7.  1024 + q and 1024 + 16 q are
-// what the nibbles are as the low mantissa bits of 0x6400; both differences are exact.
-__device__ __forceinline__ half8v unpack(uint32_t w, half2v low, half2v high) {
-  const half2v sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-  const uint32_t v = w >> 8;
-  const half2v a = __builtin_bit_cast(half2v, (w & 0x000f000fu) | 0x64006400u) - low;
-  const half2v b = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w & 0x00f000f0u) | 0x64006400u), sixteenth, -high);
-  const half2v c = __builtin_bit_cast(half2v, (v & 0x000f000fu) | 0x64006400u) - low;
-  const half2v d = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (v & 0x00f000f0u) | 0x64006400u), sixteenth, -high);
-  return half8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+// The 8 weights of a dword (nibble i: k + i) less a zero point, times 2^-9; minus_zero: the zero point times -2^-9.  An
+// integer up to 15 as the bits of a binary16 is a subnormal, that many times 2^-24: the nibbles become halves by two
+// masks and a byte permutation a pair, and the fused multiply-add that brings them to normal numbers and subtracts the
+// zero point is exact.  (Subnormal operands themselves cost the matrix instruction bits: the sums' error
+// was 5e-6 instead of 1e-7.)  The sums are multiplied by 2^9 at the end.
+constexpr float kWeightUnit = 0.001953125f;  // 2^-9
+
+__device__ __forceinline__ half8v unpack(uint32_t w, half2v minus_zero) {
+  const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+  const half2v up = {(_Float16)32768.0f, (_Float16)32768.0f};
+  uint4v r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = __builtin_amdgcn_perm(odd, even, 0x0c040c00u + i * 0x00010001u);  // 0x0c: a byte of zeros
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, pair), up, minus_zero));
+  }
+  return __builtin_bit_cast(half8v, r);
 }
 
-// x in the same order.
-__device__ __forceinline__ half8v like_weights(half8v x) { return __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7); }
-
-// Register j of lane row r to register r of lane row j (rows of 16 lanes).
-__device__ __forceinline__ void transpose_rows(uint4v& w) {
-  uint2v r = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-  const uint32_t a0 = r[0], a2 = r[1];
-  r = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-  const uint32_t a1 = r[0], a3 = r[1];
-  r = __builtin_amdgcn_permlane16_swap(a0, a1, false, false);
-  w[0] = r[0];
-  w[1] = r[1];
-  r = __builtin_amdgcn_permlane16_swap(a2, a3, false, false);
-  w[2] = r[0];
-  w[3] = r[1];
-}
-
-// The values of all four lane rows, in every lane.
-__device__ __forceinline__ void gather_rows(uint32_t v, uint32_t (&out)[4]) {
-  const uint2v even_odd = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  const uint2v e = __builtin_amdgcn_permlane32_swap(even_odd[0], even_odd[0], false, false);
-  const uint2v o = __builtin_amdgcn_permlane32_swap(even_odd[1], even_odd[1], false, false);
-  out[0] = e[0];
-  out[1] = o[0];
-  out[2] = e[1];
-  out[3] = o[1];
-}
+// A launch: the call's arguments and what the host divides for the kernel.
+struct Launch {
+  ggk_w4_args a;
+  int stride_groups, stride_rest;  // the groups from one load of a lane's scales to the next, and the rest in values
+  uint32_t group_inverse;          // ceil(2^32 / group)
+  int blocks;                      // of columns
+  int stride_tiles, stride_blocks; // experts: from one item of a workgroup to the next
+};
 
 // The rows of one tile: the expert, its first place in the order, how many.
 struct RowTile {
@@ -161,149 +149,188 @@ __device__ RowTile expert_tile(const ggk_w4_args& a, const Experts& s, int tile)
 
 constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kDepth = 4;  // steps a wave has in flight
+constexpr int kDepth = 4;  // steps of weights a wave has in flight
 
-template <int MAXT>
+// Steps of every wave that a chunk of x holds: four, less where two chunks of R rows would not fit 64 KB (32 KB beside
+// the experts' table), so that a CU holds two workgroups.  A load instruction takes 512 values of one row.
+template <int R, int WK, bool EXPERTS>
+constexpr int kChunk = R * WK <= (EXPERTS ? 16 : 32) ? 4 : (EXPERTS ? 64 : 128) / (R * WK);
+
+// Length in values of a row of x in LDS: 16 bytes more than its chunk, so that the 16 rows of an instruction's
+// operand lie in distinct banks.
+template <int R, int WK, bool EXPERTS>
+constexpr int kRowLength = kChunk<R, WK, EXPERTS> * WK * kStep + 8;
+
+// Bytes of two chunks of x, or of the waves' sums at the end.
+template <int R, int WK, bool EXPERTS>
+constexpr int kXBytes = 4 * R * kRowLength<R, WK, EXPERTS> > kWaves * (R < 16 ? 16 : R) * 64
+                            ? 4 * R * kRowLength<R, WK, EXPERTS>
+                            : kWaves * (R < 16 ? 16 : R) * 64;
+
+// What a workgroup keeps in LDS: pointers to arrays of their own, so that accesses to one may pass those to another.
 struct Shared {
-  // Rows of x, each 16 bytes longer than its chunk so that the 16 rows of an instruction's operand lie in
-  // distinct banks; at the end the waves' sums.
-  static constexpr int kXBytes = MAXT == 1 ? 32 * 1024 + 16 * 16 : 64 * 1024 + 64 * 16;
-  alignas(16) unsigned char x[kXBytes];
-  int slot[16 * MAXT];
-  Experts experts;
+  unsigned char* x;
+  // A step's weights per wave: 64 bytes a column, the four pieces of 16 in an order that depends on the column
+  // (piece), so that neither the write nor the read meets a bank twice.
+  unsigned char (*w)[16 * 64];
+  uint32_t (*sz)[16][4];  // scales and zero points, per wave and column
+  int* slot;              // of the tile's rows, -1 for none
+  int* x_row;
 };
 
-// One item's rows and columns: sums over the wave's steps of K.  M row tiles of 16.
-// FINE: groups that are not whole steps; each instruction's 32 values then lie in one group, for which a step's
-// dwords are exchanged between the lanes of a column.
-template <int M, int NT, int WK, int MAXT, bool FINE, bool ZEROS>
-__device__ __forceinline__ void multiply_item(const ggk_w4_args& a, const RowTile& t, int column0, Shared<MAXT>& s,
-                                              float4v (&sum)[M][NT]) {
+// Place of piece p (32 values of k) of a column in Shared::w.
+__device__ __forceinline__ int piece(int column, int p) { return column * 64 + ((p ^ (column >> 2)) & 3) * 16; }
+
+// One item's sums over the wave's steps of K, of up to R rows, times kWeightUnit.  FINE: groups that are not whole steps,
+// each instruction's 32 values lie in one; else a step lies in one group.  Every load of weights is made without a
+// condition, past K too (there it reads the row's last values, with a scale of 0): the waits before a load's use
+// are counted in the loads made since, and a load that may not have been made does not count.
+template <int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
+__device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t, int column0, const Shared& s,
+                                              float4v (&sum)[(R + 15) / 16]) {
+  const ggk_w4_args& a = l.a;
+  constexpr int M = (R + 15) / 16, kTurns = kChunk<R, WK, EXPERTS>, kLength = kRowLength<R, WK, EXPERTS>;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int column = lane % 16, row = lane / 16;  // of the lane in an instruction's operands; lane row
   const int wk = wave % WK;
+  const int column = lane % 16, row = lane / 16;        // of the lane in an instruction's operands; lane row
+  const int my_column = lane / 4, my_piece = lane % 4;  // of the lane in a load
   const int steps = (a.k + kStep - 1) / kStep;
   const int turns = (steps + WK - 1) / WK;  // steps of a wave, at most
-  // Turns that a chunk of x holds, and its row length in values.
-  const int rows = max(1, t.rows);
-  const int chunk_turns = min(turns, (Shared<MAXT>::kXBytes / rows - 16) / (2 * kStep * WK));
-  const int chunk_k = chunk_turns * WK * kStep;
-  const int ld = chunk_k + 8;
 
-  const unsigned char* q[NT];
-  const _Float16* scales[NT];
-  const unsigned char* zeros[NT];
+  // A chunk of x into its half of s.x, 512 values of a row an instruction; zeros past K by the resource's range check.
+  auto stage = [&](int chunk) {
+    constexpr int kLoads = kTurns * WK / 4;  // of a row
+    static_assert(kTurns * WK % 4 == 0, "whole instructions a row");
+    const int k0 = chunk * kTurns * WK * kStep;
 #pragma unroll
-  for (int c = 0; c < NT; ++c) {
-    const long long j = min(column0 + 16 * c + column, a.n - 1);
-    q[c] = a.q + t.expert * a.stride_q + j * a.ldq;
-    scales[c] = static_cast<const _Float16*>(a.scales) + t.expert * a.stride_s + j * a.lds;
-    zeros[c] = ZEROS ? a.zeros + t.expert * a.stride_z + j * a.ldz : nullptr;
-  }
-  auto scale_of = [&](int c, int k) {  // scale and zero point of the group of k
-    const int g = k / a.group;
-    uint32_t v = *reinterpret_cast<const uint16_t*>(scales[c] + g);
-    if constexpr (ZEROS) v |= (uint32_t)zeros[c][g] << 16;
+    for (int i = 0; i < (R * kLoads + kWaves - 1) / kWaves; ++i) {
+      const int at = wave + i * kWaves, r = at / kLoads, k = k0 + at % kLoads * 512;
+      if (r < t.rows && k < a.k) {
+        const _Float16* x = static_cast<const _Float16*>(a.x) + (EXPERTS ? __builtin_amdgcn_readfirstlane(s.x_row[r]) : t.first + r) * a.ldx + k;
+        gg::load_to_lds16(x, 2 * (a.k - k < 512 ? a.k - k : 512),
+                          gg::lds_address(s.x) + 2 * ((chunk % 2 * R + r) * kLength + at % kLoads * 512), 16 * lane, 0);
+      } else if (r < t.rows) {  // a chunk that K does not reach the end of
+        *reinterpret_cast<uint4v*>(s.x + 2 * ((chunk % 2 * R + r) * kLength + at % kLoads * 512) + 16 * lane) = uint4v{0, 0, 0, 0};
+      }
+    }
+  };
+  stage(0);
+
+  const long long j = min(column0 + my_column, a.n - 1);
+  const unsigned char* q = a.q + t.expert * a.stride_q + j * a.ldq;
+  const _Float16* scales = static_cast<const _Float16*>(a.scales) + t.expert * a.stride_s + j * a.lds;
+  const unsigned char* zeros = ZEROS ? a.zeros + t.expert * a.stride_z + j * a.ldz : nullptr;
+  // Scale (low half) and zero point of the group that holds the lane's k, which goes from load to load in equal
+  // strides: the group goes on by the whole groups of a stride, and one more where the rest has come to one.
+  constexpr int kStride = (FINE ? 1 : kDepth) * WK * kStep;
+  int scale_k = FINE ? wk * kStep + 32 * my_piece : (my_piece * WK + wk) * kStep;  // below 2^12: the product below is exact
+  int group = (int)__umulhi((uint32_t)scale_k, l.group_inverse), rest = scale_k - group * a.group;
+  const int last_group = a.k / a.group - 1;
+  auto next_scale = [&]() {
+    const int g = min(group, last_group);
+    uint32_t v = *reinterpret_cast<const uint16_t*>(scales + g);
+    if constexpr (ZEROS) v |= (uint32_t)zeros[g] << 16;
+    v = scale_k < a.k ? v : 0;
+    scale_k += kStride;
+    group += l.stride_groups;
+    rest += l.stride_rest;
+    if (rest >= a.group) {
+      rest -= a.group;
+      ++group;
+    }
     return v;
   };
-  uint4v w[kDepth][NT];
-  uint32_t sz[FINE ? kDepth : 1][NT];  // FINE: the lane row's 32 values of a step; else: the lane row's step of the next four
+  uint4v w[kDepth];
+  uint32_t sz[FINE ? kDepth : 1];  // FINE: of the lane's 32 values of each step; else: of the lane's step of the next four
   auto load = [&](int turn, int d) {
-    const int mine = (turn * WK + wk) * kStep + 32 * row;  // the lane's 32 values of k
-    const bool in = mine < a.k;
+    const int k = min((turn * WK + wk) * kStep + 32 * my_piece, a.k - 32);
+    w[d] = *reinterpret_cast<const uint4v*>(q + k / 2);
+    if constexpr (FINE) sz[d] = next_scale();
+  };
+  auto write = [&](int d) {
+    *reinterpret_cast<uint4v*>(&s.w[wave][piece(my_column, my_piece)]) = w[d];
+    if constexpr (FINE) s.sz[wave][my_column][my_piece] = sz[d];
+  };
+  // The next step's weights go through LDS while a step is multiplied: a wave's LDS operations keep their order, so
+  // that what is written after a read does not change it.
+  auto read = [&](uint4v& v, uint4v& g) {
+    if constexpr (FINE) {
 #pragma unroll
-    for (int c = 0; c < NT; ++c) {
-      w[d][c] = uint4v{0, 0, 0, 0};
-      if (in) w[d][c] = *reinterpret_cast<const uint4v*>(q[c] + mine / 2);
-      if constexpr (FINE) sz[d][c] = in ? scale_of(c, mine) : 0;
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint32_t*>(&s.w[wave][piece(column, i) + 4 * row]);
+      g = *reinterpret_cast<const uint4v*>(s.sz[wave][column]);
+    } else {
+      v = *reinterpret_cast<const uint4v*>(&s.w[wave][piece(column, row)]);
     }
   };
-  auto load_scales = [&](int turn) {
-#pragma unroll
-    for (int c = 0; c < NT; ++c) sz[0][c] = scale_of(c, min(((turn + row) * WK + wk) * kStep, a.k - kStep));
-  };
+  if constexpr (!FINE) sz[0] = next_scale();
 #pragma unroll
   for (int d = 0; d < kDepth; ++d) load(d, d);
-  if constexpr (!FINE) load_scales(0);
+#pragma unroll
+  for (int m = 0; m < M; ++m) sum[m] = float4v{};
+  const unsigned char* x[M];  // the lane's rows in LDS
 #pragma unroll
   for (int m = 0; m < M; ++m) {
-#pragma unroll
-    for (int c = 0; c < NT; ++c) sum[m][c] = float4v{};
+    x[m] = s.x + 2 * (min(16 * m + column, R - 1) * kLength + wk * kStep + (FINE ? 8 : 32) * row);
   }
-
-  // x of one chunk, in the order of the weights' halves, zeros past K and for slots that name no row.
-  const int fan = a.rows / a.x_rows;
-  auto stage = [&](int chunk) {
-    const int pieces = chunk_k / 8;
-    for (int i = tid; i < t.rows * pieces; i += kThreads) {
-      const int r = i / pieces, p = i % pieces, k = chunk * chunk_k + 8 * p;
-      const int slot = s.slot[r];
-      half8v x = half8v{};
-      if (slot >= 0 && k < a.k) x = *reinterpret_cast<const half8_any*>(static_cast<const _Float16*>(a.x) + slot / fan * a.ldx + k);
-      *reinterpret_cast<half8v*>(s.x + 2 * (r * ld + 8 * p)) = like_weights(x);
-    }
-  };
-  // The lane's rows of x in LDS; rows past the tile's are read as its last (their sums are not used).
-  const unsigned char* x[M];
-#pragma unroll
-  for (int m = 0; m < M; ++m) x[m] = s.x + 2 * (min(16 * m + column, rows - 1) * ld + (FINE ? 8 : 32) * row);
-
-  uint32_t four[NT][4];
-  int in_chunk = chunk_turns;
+  uint4v v, g, four;
+  write(0);
+  load(kDepth, 0);
+  read(v, g);
   for (int turn0 = 0; turn0 < turns; turn0 += kDepth) {
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       const int turn = turn0 + d;
       if (turn >= turns) break;
-      if (in_chunk == chunk_turns) {
-        if (turn > 0) __syncthreads();
-        stage(turn / chunk_turns);
-        __syncthreads();
-        in_chunk = 0;
+      if (d % kTurns == 0) {
+        // This chunk's loads are older than the weights' of the last kTurns steps; behind the barrier every wave's have
+        // landed, and every wave is done with the chunk before, whose place the next one takes.
+        const int chunk = turn / kTurns;
+        asm volatile("" ::: "memory");
+        gg::wait_vmcnt<kTurns>();
+        gg::stage_barrier();
+        if (turn + kTurns < turns) stage(chunk + 1);
+        if constexpr (FINE) asm volatile("" ::: "memory");
       }
       if constexpr (!FINE) {
         if (d == 0) {
-#pragma unroll
-          for (int c = 0; c < NT; ++c) gather_rows(sz[0][c], four[c]);
-          load_scales(turn + kDepth);
+          s.sz[wave][my_column][my_piece] = sz[0];
+          four = *reinterpret_cast<const uint4v*>(s.sz[wave][column]);
+          sz[0] = next_scale();
         }
       }
-      const int at = 2 * (in_chunk * WK + wk) * kStep;
+      uint4v next_v, next_g;
+      write((d + 1) % kDepth);
+      load(turn + 1 + kDepth, (d + 1) % kDepth);
+      read(next_v, next_g);
+      if constexpr (!FINE) g = uint4v{four[d], four[d], four[d], four[d]};
+      half8v b[4];
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        uint32_t g[4];
-        if constexpr (FINE) {
-          transpose_rows(w[d][c]);
-          gather_rows(sz[d][c], g);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) g[j] = turn * WK + wk < steps ? four[c][d] : 0;  // no step: zero times zero
+      for (int i = 0; i < 4; ++i) {
+        half2v minus_zero = {(_Float16)(-8.0f * kWeightUnit), (_Float16)(-8.0f * kWeightUnit)};
+        if constexpr (ZEROS) {  // the zero point's bits are that many times 2^-24
+          const half2v down = {(_Float16)-32768.0f, (_Float16)-32768.0f};
+          minus_zero = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(g[i], g[i], 0x03020302u)) * down;
         }
-        half8v v[4];
+        b[i] = unpack(v[i], minus_zero);
+      }
+      const int at = 2 * ((turn / kTurns % 2) * R * kLength + turn % kTurns * WK * kStep);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const _Float16 zero = ZEROS ? (_Float16)(float)(g[j] >> 16) : (_Float16)8.0f;
-          const _Float16 low = (_Float16)1024.0f + zero, high = (_Float16)64.0f + zero;
-          v[j] = unpack(w[d][c][j], half2v{low, low}, half2v{high, high});
-        }
+      for (int m = 0; m < M; ++m) {
+        float4v part = float4v{};
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-          float4v part = float4v{};
+        for (int i = 0; i < 4; ++i) {
+          const half8v xs = *reinterpret_cast<const half8v*>(x[m] + at + (FINE ? 64 : 16) * i);
+          part = __builtin_amdgcn_mfma_f32_16x16x32_f16(xs, b[i], part, 0, 0, 0);
+          if (FINE || i == 3) {
+            const float scale = (float)__builtin_bit_cast(_Float16, (uint16_t)g[i]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const half8v xs = *reinterpret_cast<const half8v*>(x[m] + at + (FINE ? 64 : 16) * j);
-            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(xs, v[j], part, 0, 0, 0);
-            if (FINE || j == 3) {
-              const float scale = (float)__builtin_bit_cast(_Float16, (uint16_t)g[j]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) sum[m][c][i] = fmaf(scale, part[i], sum[m][c][i]);
-              part = float4v{};
-            }
+            for (int e = 0; e < 4; ++e) sum[m][e] = fmaf(scale, part[e], sum[m][e]);
+            part = float4v{};
           }
         }
       }
-      load(turn + kDepth, d);
-      ++in_chunk;
+      v = next_v;
+      g = next_g;
     }
   }
 }
@@ -317,100 +344,115 @@ __device__ __forceinline__ void store_y(const ggk_w4_args& a, int slot, int j, f
   }
 }
 
-// Joins the waves' sums and writes y.
-template <int M, int NT, int WK, int MAXT>
-__device__ __forceinline__ void finish_item(const ggk_w4_args& a, const RowTile& t, int block0, Shared<MAXT>& s,
-                                            const float4v (&sum)[M][NT]) {
-  constexpr int kColumns = 16 * NT * (kWaves / WK);  // of the workgroup
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+// One tile of rows by the workgroup's columns from block0 on: sums, their join over the waves that split K, y.
+template <int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
+__device__ __forceinline__ void run_item(const Launch& l, const RowTile& t, int block0, const Shared& s) {
+  const ggk_w4_args& a = l.a;
+  constexpr int M = (R + 15) / 16, kColumns = 16 * (kWaves / WK);
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int column = lane % 16, row = lane / 16, wn = wave / WK, wk = wave % WK;
+  float4v sum[M];
+  multiply_item<R, WK, EXPERTS, FINE, ZEROS>(l, t, block0 + wn * 16, s, sum);
   float* s_sum = reinterpret_cast<float*>(s.x);  // [WK][16 M][kColumns]
-  static_assert(WK * 16 * MAXT * kColumns * 4 <= Shared<MAXT>::kXBytes, "the sums fit x's place");
-  __syncthreads();
+  gg::stage_barrier();
 #pragma unroll
   for (int m = 0; m < M; ++m) {
 #pragma unroll
-    for (int c = 0; c < NT; ++c) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s_sum[(wk * 16 * M + 16 * m + 4 * row + i) * kColumns + 16 * (wn * NT + c) + column] = sum[m][c][i];
-      }
-    }
+    for (int i = 0; i < 4; ++i) s_sum[(wk * 16 * M + 16 * m + 4 * row + i) * kColumns + 16 * wn + column] = sum[m][i];
   }
-  __syncthreads();
+  gg::stage_barrier();
   for (int i = tid; i < t.rows * kColumns; i += kThreads) {
-    const int r = i / kColumns, c = i % kColumns, j = block0 + c, slot = s.slot[r];
+    const int r = i / kColumns, c = i % kColumns, j = block0 + c, slot = EXPERTS ? s.slot[r] : t.first + r;
     if (j < a.n && slot >= 0) {
       float y = 0.0f;
 #pragma unroll
       for (int w = 0; w < WK; ++w) y += s_sum[(w * 16 * M + r) * kColumns + c];
+      y *= 1.0f / kWeightUnit;
       if (a.row_weights != nullptr) y *= a.row_weights[slot];
       store_y(a, slot, j, y);
     }
   }
 }
 
-template <int M, int NT, int WK, int MAXT, bool FINE, bool ZEROS>
-__device__ __forceinline__ void run_item(const ggk_w4_args& a, const RowTile& t, int block0, Shared<MAXT>& s) {
-  float4v sum[M][NT];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  multiply_item<M, NT, WK, MAXT, FINE, ZEROS>(a, t, block0 + wave / WK * 16 * NT, s, sum);
-  finish_item<M, NT, WK, MAXT>(a, t, block0, s, sum);
-}
-
-template <int NT, int WK, int MAXT, bool FINE, bool ZEROS>
-__global__ __launch_bounds__(kThreads, 4) void w4_kernel(ggk_w4_args a) {
-  constexpr int kRows = 16 * MAXT, kColumns = 16 * NT * (kWaves / WK);
-  __shared__ Shared<MAXT> s;
+// R: rows of an item, at most.
+template <int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
+__global__ __launch_bounds__(kThreads, 4) void w4_kernel(Launch l) {
+  const ggk_w4_args& a = l.a;
+  constexpr int kColumns = 16 * (kWaves / WK);
+  __shared__ alignas(16) unsigned char s_x[kXBytes<R, WK, EXPERTS>];
+  __shared__ alignas(16) unsigned char s_w[kWaves][16 * 64];
+  __shared__ alignas(16) uint32_t s_sz[kWaves][16][4];
   const int tid = threadIdx.x;
-  const int blocks = (a.n + kColumns - 1) / kColumns;
-  int tiles = (a.rows + kRows - 1) / kRows;
-  if (a.experts > 0) {
-    list_experts<kThreads, kRows>(a, s.experts);
-    tiles = s.experts.tile[a.experts + 1];
-  }
-  for (long long item = blockIdx.x; item < (long long)tiles * blocks; item += gridDim.x) {
-    const int tile = (int)(item / blocks), block0 = (int)(item % blocks) * kColumns;
-    RowTile t{0, tile * kRows, 0};
-    t.rows = min(kRows, a.rows - t.first);
-    if (a.experts > 0) t = expert_tile<kRows>(a, s.experts, tile);
-    for (int i = tid; i < t.rows; i += kThreads) {
-      int slot = t.first + i;
-      if (a.experts > 0) {
-        slot = a.order[slot];
+  if constexpr (!EXPERTS) {
+    const Shared s{s_x, s_w, s_sz, nullptr, nullptr};
+    const int tiles = (a.rows + R - 1) / R;
+    for (int tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
+      const RowTile t{0, tile * R, min(R, a.rows - tile * R)};
+      run_item<R, WK, false, FINE, ZEROS>(l, t, blockIdx.x * kColumns, s);
+      gg::stage_barrier();
+    }
+  } else {
+    __shared__ int s_slot[R], s_x_row[R];
+    __shared__ Experts s_experts;
+    const Shared s{s_x, s_w, s_sz, s_slot, s_x_row};
+    const int fan = a.rows / a.x_rows;
+    list_experts<kThreads, R>(a, s_experts);
+    const int tiles = s_experts.tile[a.experts + 1];
+    int tile = blockIdx.x / l.blocks, block = blockIdx.x % l.blocks;
+    while (tile < tiles) {
+      const RowTile t = expert_tile<R>(a, s_experts, tile);
+      for (int i = tid; i < t.rows; i += kThreads) {
+        int slot = a.order[t.first + i];
         if (slot >= a.rows) slot = -1;
+        s.slot[i] = slot;
+        s.x_row[i] = max(slot, 0) / fan;  // where a slot names no row, row 0: its sums are not used
       }
-      s.slot[i] = slot;
-    }
-    __syncthreads();
-    if (a.experts > 0 && t.expert == a.experts) {
-      for (int i = tid; i < t.rows * kColumns; i += kThreads) {
-        const int slot = s.slot[i / kColumns], j = block0 + i % kColumns;
-        if (j < a.n && slot >= 0) store_y(a, slot, j, 0.0f);
+      gg::stage_barrier();
+      if (t.expert == a.experts) {
+        for (int i = tid; i < t.rows * kColumns; i += kThreads) {
+          const int slot = s.slot[i / kColumns], j = block * kColumns + i % kColumns;
+          if (j < a.n && slot >= 0) store_y(a, slot, j, 0.0f);
+        }
+      } else if (R > 4 && t.rows <= 4) {
+        // The rows are a constant of the whole loop over K: the compiler leaves out the wait between a matrix
+        // instruction and the use of its result when a branch on them lies between.
+        run_item<4, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
+      } else {
+        run_item<R, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
       }
-    } else if (MAXT == 1 || t.rows <= 16) {
-      // Row tiles are a constant of the whole loop over K: the compiler leaves out the wait between a matrix
-      // instruction and the use of its result when a branch on them lies between.
-      run_item<1, NT, WK, MAXT, FINE, ZEROS>(a, t, block0, s);
-    } else if (t.rows <= 32) {
-      run_item<2, NT, WK, MAXT, FINE, ZEROS>(a, t, block0, s);
-    } else {
-      run_item<MAXT, NT, WK, MAXT, FINE, ZEROS>(a, t, block0, s);
+      gg::stage_barrier();
+      tile += l.stride_tiles;
+      block += l.stride_blocks;
+      if (block >= l.blocks) {
+        block -= l.blocks;
+        ++tile;
+      }
     }
-    __syncthreads();
   }
 }
 
-template <int NT, int WK, int MAXT>
+template <int R, int WK, bool EXPERTS>
 hipError_t launch(const ggk_w4_args& a, hipStream_t stream) {
   const bool fine = a.group % kStep != 0;
-  auto kernel = fine ? (a.zeros != nullptr ? w4_kernel<NT, WK, MAXT, true, true> : w4_kernel<NT, WK, MAXT, true, false>)
-                     : (a.zeros != nullptr ? w4_kernel<NT, WK, MAXT, false, true> : w4_kernel<NT, WK, MAXT, false, false>);
-  const int columns = 16 * NT * (kWaves / WK), rows = 16 * MAXT;
-  const long long tiles = (a.rows + rows - 1) / rows + (a.experts > 0 ? min(a.rows, a.experts + 1) : 0);
-  const long long items = tiles * ((a.n + columns - 1) / columns);
-  const long long most = a.experts > 0 ? kCus * 2 : 0x7fffffff;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(items < most ? items : most)), dim3(kThreads), 0, stream, a);
+  auto kernel = fine ? (a.zeros != nullptr ? w4_kernel<R, WK, EXPERTS, true, true> : w4_kernel<R, WK, EXPERTS, true, false>)
+                     : (a.zeros != nullptr ? w4_kernel<R, WK, EXPERTS, false, true> : w4_kernel<R, WK, EXPERTS, false, false>);
+  constexpr int kColumns = 16 * (kWaves / WK);
+  const int stride = (fine ? 1 : kDepth) * WK * kStep;
+  Launch l{};
+  l.a = a;
+  l.stride_groups = stride / a.group;
+  l.stride_rest = stride % a.group;
+  l.group_inverse = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
+  l.blocks = (a.n + kColumns - 1) / kColumns;
+  const long long tiles = (a.rows + R - 1) / R + (EXPERTS ? min(a.rows, a.experts + 1) : 0);
+  dim3 grid(l.blocks, (unsigned)(tiles < 65535 ? tiles : 65535));
+  if (EXPERTS) {
+    const long long items = tiles * l.blocks;
+    grid = dim3((unsigned)(items < kCus * 2 ? items : kCus * 2));
+    l.stride_tiles = (int)grid.x / l.blocks;
+    l.stride_blocks = (int)grid.x % l.blocks;
+  }
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, l);
   return hipGetLastError();
 }
 
@@ -448,14 +490,19 @@ extern "C" hipError_t ggk_w4_multiply(const ggk_w4_args* args, hipStream_t strea
   const hipError_t st = ggk_w4_check(args);
   if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
   const ggk_w4_args& a = *args;
-  // Waves that split K: as many as it takes for 4096 waves in all, half of what the GPU holds.
-  const int row_tiles = a.experts > 0 ? min(a.rows, a.experts) : (a.rows + 63) / 64;
-  const long long waves = (long long)((a.n + 15) / 16) * row_tiles;
-  if (a.experts > 0 || a.rows > 16) {
-    return waves >= 4096 ? launch<1, 1, 4>(a, stream) : waves >= 2048 ? launch<1, 2, 4>(a, stream) : launch<1, 4, 4>(a, stream);
+  // Waves that split K, by the waves there would be without: 8192 fill the GPU, and more than about 3000 only add the
+  // fixed cost of a workgroup (3.2 us for 224 of them, 6.5 for 896) to a launch of a few microseconds.
+  const long long columns = (a.n + 15) / 16;
+  if (a.experts > 0) {
+    const long long waves = columns * min(a.rows, a.experts);
+    return waves >= 1024 ? launch<16, 1, true>(a, stream) : waves >= 512 ? launch<16, 2, true>(a, stream) : launch<16, 4, true>(a, stream);
   }
-  return waves >= 4096   ? launch<1, 1, 1>(a, stream)
-         : waves >= 2048 ? launch<1, 2, 1>(a, stream)
-         : waves >= 1024 ? launch<1, 4, 1>(a, stream)
-                         : launch<1, 8, 1>(a, stream);
+  if (a.rows > 16) {
+    const long long waves = columns * ((a.rows + 31) / 32);
+    return waves > 1344 ? launch<32, 2, false>(a, stream) : launch<32, 4, false>(a, stream);
+  }
+  const bool few = a.rows <= 4;
+  if (columns <= 384) return few ? launch<4, 8, false>(a, stream) : launch<16, 8, false>(a, stream);
+  if (columns <= 1344) return few ? launch<4, 4, false>(a, stream) : launch<16, 4, false>(a, stream);
+  return few ? launch<4, 2, false>(a, stream) : launch<16, 2, false>(a, stream);
 }

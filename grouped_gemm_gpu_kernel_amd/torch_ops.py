@@ -504,6 +504,30 @@ def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optiona
 
 # ---------------------------------------------------------------- 4-bit weights
 
+def _w4_in_order(x, q, scales, zeros, row_weights, lead, out_dtype) -> bool:
+    """Whether _check_w4 finds nothing: the same checks, each tensor's metadata read once."""
+    try:
+        qs, qt, ss, st = q.shape, q.stride(), scales.shape, scales.stride()
+        rows, k = x.shape
+        groups, device = ss[-1], x.device
+        ok = (x.dtype is torch.float16 and q.dtype is torch.uint8 and scales.dtype is torch.float16 and
+              (out_dtype is torch.float32 or out_dtype is torch.float16) and device.type == "cuda" and
+              q.device == device and scales.device == device and len(qs) == 2 + lead and ss[:-1] == qs[:-1] and
+              k == 2 * qs[-1] and groups > 0 and k > 0 and k % (32 * groups) == 0 and
+              qt[-1] == 1 and (qs[-2] <= 1 or (qt[-2] >= qs[-1] and qt[-2] % 16 == 0)) and
+              (lead == 0 or qs[0] <= 1 or qt[0] % 16 == 0) and q.data_ptr() % 16 == 0 and
+              (groups == 1 or st[-1] == 1) and (qs[-2] <= 1 or st[-2] >= groups) and
+              (x.is_contiguous() or (x.stride(1) == 1 and (rows <= 1 or x.stride(0) >= k))))
+        if ok and zeros is not None:
+            zt = zeros.stride()
+            ok = (zeros.dtype is torch.uint8 and zeros.shape == ss and zeros.device == device and
+                  (groups == 1 or zt[-1] == 1) and (qs[-2] <= 1 or zt[-2] >= groups))
+        return ok and not (torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or (
+            row_weights is not None and row_weights.requires_grad)))
+    except (AttributeError, TypeError, ValueError, IndexError):
+        return False
+
+
 def _check_w4(x, q, scales, zeros, row_weights, lead, out_dtype):
     """Checks shared by the two products: lead is the number of dimensions ahead of a matrix's two."""
     if row_weights is not None and not isinstance(row_weights, torch.Tensor):
@@ -550,23 +574,22 @@ def _check_w4(x, q, scales, zeros, row_weights, lead, out_dtype):
 
 
 def _w4(x, q, scales, zeros, rows, experts, counts, order, row_weights, out_dtype):
-    n, k, groups = q.shape[-2], 2 * q.shape[-1], scales.shape[-1]
+    n, half = q.shape[-2:]
+    groups = scales.shape[-1]
     device = x.device
     y = torch.empty((rows, n), dtype=out_dtype, device=device)
-    if y.numel() == 0:
+    if rows == 0 or n == 0:
         return y
-
-    def strides(t):  # of rows and of matrices
-        if t is None:
-            return 0, 0
-        return (t.stride(-2) if n > 1 else t.shape[-1]), (t.stride(0) if experts > 1 else 0)
-
-    (ldq, stride_q), (lds, stride_s), (ldz, stride_z) = strides(q), strides(scales), strides(zeros)
+    qt, st = q.stride(), scales.stride()
+    zt = zeros.stride() if zeros is not None else st
+    several = experts > 1
     _launch("ggk_w4_multiply", _lib.GGKW4Args(
-        rows, x.shape[0], n, k, k // groups, experts, x.data_ptr(), _row_stride(x), q.data_ptr(), ldq, stride_q,
-        scales.data_ptr(), lds, stride_s, zeros.data_ptr() if zeros is not None else None, ldz, stride_z,
-        counts.data_ptr() if counts is not None else None, order.data_ptr() if order is not None else None,
-        row_weights.data_ptr() if row_weights is not None else None, y.data_ptr(), n, _TYPES[out_dtype]), device)
+        rows, x.shape[0], n, 2 * half, 2 * half // groups, experts, x.data_ptr(), _row_stride(x),
+        q.data_ptr(), qt[-2] if n > 1 else half, qt[0] if several else 0,
+        scales.data_ptr(), st[-2] if n > 1 else groups, st[0] if several else 0,
+        None if zeros is None else zeros.data_ptr(), zt[-2] if n > 1 else groups, zt[0] if several else 0,
+        None if counts is None else counts.data_ptr(), None if order is None else order.data_ptr(),
+        None if row_weights is None else row_weights.data_ptr(), y.data_ptr(), n, _TYPES[out_dtype]), device)
     return y
 
 
@@ -583,7 +606,8 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
 
     Runs on the current stream of x's device, without waiting; no gradient (inputs that require one are
     refused).  Any number of rows is right; it is made for up to 64 or so."""
-    _check_w4(x, q, scales, zeros, None, 0, out_dtype)
+    if not _w4_in_order(x, q, scales, zeros, None, 0, out_dtype):
+        _check_w4(x, q, scales, zeros, None, 0, out_dtype)
     return _w4(x, q, scales, zeros, x.shape[0], 0, None, None, None, out_dtype)
 
 
@@ -603,7 +627,8 @@ def moe_w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, counts
     rows that order does not name are left unwritten."""
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise ValueError("q must be [experts, N, K / 2]")
-    _check_w4(x, q, scales, zeros, row_weights, 1, out_dtype)
+    if not _w4_in_order(x, q, scales, zeros, row_weights, 1, out_dtype):
+        _check_w4(x, q, scales, zeros, row_weights, 1, out_dtype)
     experts = q.shape[0]
     if not 1 <= experts <= _lib.GGK_MOE_MAX_EXPERTS:
         raise ValueError(f"q has {experts} experts, expected 1 to {_lib.GGK_MOE_MAX_EXPERTS}")

@@ -205,6 +205,23 @@ def test_odd_values(torch_cuda, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3, 16, 33])
+@pytest.mark.parametrize("group", [32, 128])
+def test_sums_of_integers_are_exact(torch_cuda, rows, group):
+    """Whole x and scales of 1: every partial sum is a whole number below 2^24, which float32 holds, in any order.  One
+    term a row of x is 2^11 times the others, so that bits lost in an instruction's alignment show."""
+    q, s, z = _weights((), 333, 4096, group, True, 17)
+    s.fill_(1.0)
+    g = torch.Generator().manual_seed(18)
+    x = torch.randint(-1, 2, (rows, 4096), generator=g).half().cuda()
+    x[:, 7::512] = 2048.0  # 8 terms of at most 15 * 2048, 4088 of at most 15: below 2^19
+    want = x.double() @ values(q, s, z).t()
+    assert torch.equal(torch_ops.w4_matmul(x, q, s, z).double(), want)
+    want = x.double() @ values(q, s).t()
+    assert torch.equal(torch_ops.w4_matmul(x, q, s).double(), want)
+
+
+@pytest.mark.gpu
 def test_half_output_overflows_to_infinity(torch_cuda):
     q = torch.full((2, 64), 255, dtype=torch.uint8, device="cuda")
     s = torch.ones(2, 1, dtype=torch.float16, device="cuda")
