@@ -12,6 +12,7 @@ import os
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libgrouped_gemm_amd.so"
+TORCH_PATH = LIB_PATH.parent / "gg_torch.so"  # the C++ part of torch_ops
 
 # hipError_t values used by the API (hip_runtime_api.h).
 HIP_SUCCESS = 0

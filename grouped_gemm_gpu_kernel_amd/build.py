@@ -5,6 +5,7 @@ Produces, in-tree:
   grouped_gemm_gpu_kernel_amd/_build/bin/test_correctness   C++ drop-in test driver
   grouped_gemm_gpu_kernel_amd/_build/bin/benchmark_grouped_gemm   benchmark harness (reference CLI)
   grouped_gemm_gpu_kernel_amd/_build/bin/vendor_hipblaslt   hipBLASLt comparison program (bench only)
+  grouped_gemm_gpu_kernel_amd/lib/gg_torch.so               C++ part of the PyTorch binding
   oracle/liboracle.so                                       CPU oracle (test infrastructure)
 
 Steps: hipcc compiles the kernels for gfx950 with the compiler's resource
@@ -14,12 +15,14 @@ Usage: python -m grouped_gemm_gpu_kernel_amd.build [--no-tests] [--no-oracle]
 """
 from __future__ import annotations
 
+import importlib.util
 import json
 import os
 import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -167,6 +170,22 @@ def build_host_sanitized(out_path: Path) -> Path:
     return out
 
 
+def build_torch_binding() -> Path:
+    """The C++ part of torch_ops (csrc/torch_binding.cpp), a Python module linked against the library beside it; torch's
+    own libraries are those that `import torch` has loaded."""
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    out = LIB_DIR / "gg_torch.so"
+    tmp = out.parent / (out.name + ".tmp")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+          f"-I{ROOT / 'include'}", "-isystem", str(torch / "include"),
+          "-isystem", str(torch / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(ROCM / "include"),
+          "-isystem", sysconfig.get_paths()["include"], str(CSRC_DIR / "torch_binding.cpp"), "-o", str(tmp),
+          f"-L{LIB_DIR}", "-lgrouped_gemm_amd", f"-L{torch / 'lib'}", "-ltorch_cpu", "-lc10", "-lc10_hip",
+          "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, out)
+    return out
+
+
 def build_cpp_tests() -> Path:
     """The C++ drop-in test driver (tests/cpp/test_correctness.cpp), linked
     against the library with an rpath to it."""
@@ -213,6 +232,7 @@ def build_oracle() -> Path:
 
 def main(argv: list[str]) -> int:
     build_library()
+    build_torch_binding()
     if "--no-oracle" not in argv:
         build_oracle()
     if "--no-tests" not in argv:

@@ -26,6 +26,7 @@ All work runs in the HIP library (lib/libgrouped_gemm_amd.so); there is no CPU f
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import operator
 from typing import NamedTuple, Optional, Sequence, Union
 
@@ -39,6 +40,7 @@ Scalars = Union[float, Sequence[float]]
 
 _OP_NAME = "grouped_gemm_amd::grouped_gemm"
 _placeholders: dict = {}
+_gg_torch = None
 
 
 def _placeholder(device: torch.device) -> int:
@@ -352,18 +354,19 @@ class Routing(NamedTuple):
     balance_loss: Optional[torch.Tensor]  # float32 scalar, None unless asked for
 
 
-def _launch(name: str, args, device: torch.device) -> None:
-    """A library entry point on the device's current stream (its handle as it is: the Stream object that
-    torch.cuda.current_stream makes costs 2 us)."""
-    index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index) or None
-    if index == torch.cuda.current_device():
-        status = getattr(_lib.lib(), name)(ctypes.byref(args), stream)
-    else:
-        with torch.cuda.device(device):
-            status = getattr(_lib.lib(), name)(ctypes.byref(args), stream)
-    if status:
-        _lib.check(status, name)
+def _binding():
+    """The C++ binding of the calls below (csrc/torch_binding.cpp); raises if it has not been built."""
+    global _gg_torch
+    if _gg_torch is None:
+        if not _lib.TORCH_PATH.exists():
+            raise RuntimeError(f"{_lib.TORCH_PATH} is missing: build it with `python -m grouped_gemm_gpu_kernel_amd.build` "
+                               "(or __graft_entry__.build()); there is no fallback implementation")
+        _lib.lib()
+        spec = importlib.util.spec_from_file_location("gg_torch", _lib.TORCH_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _gg_torch = module
+    return _gg_torch
 
 
 def _check_vector(t: torch.Tensor, name: str, dtype: torch.dtype, count: int, device) -> None:
@@ -377,70 +380,6 @@ def _check_vector(t: torch.Tensor, name: str, dtype: torch.dtype, count: int, de
         raise ValueError(f"{name} has {t.numel()} entries, expected {count}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-
-
-def _route(logits, ids, token_mask, slots, normalize, scale, balance):
-    """The launch behind moe_route: weights, ids, counts, order, loss, slope."""
-    tokens, experts = logits.shape
-    device = logits.device
-    weights = torch.empty((tokens, slots), dtype=torch.float32, device=device)
-    chosen = torch.empty((tokens, slots), dtype=torch.int32, device=device)
-    counts = torch.empty(experts, dtype=torch.int32, device=device)
-    order = torch.empty(tokens * slots, dtype=torch.int32, device=device)
-    loss = slope = workspace = None
-    if balance:
-        loss = torch.empty((), dtype=torch.float32, device=device)
-        slope = torch.empty(experts, dtype=torch.float32, device=device)
-    if tokens == 0:
-        counts.zero_()
-        return weights, chosen, counts, order, loss.zero_() if balance else None, slope
-    size = _lib.lib().ggk_route_workspace(tokens, experts)
-    if size:
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    _launch("ggk_route", _lib.GGKRouteArgs(
-        tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr(), _row_stride(logits),
-        None if token_mask is None else token_mask.data_ptr(), None if ids is None else ids.data_ptr(), normalize, scale,
-        weights.data_ptr(), chosen.data_ptr(), counts.data_ptr(), order.data_ptr(),
-        loss.data_ptr() if balance else None, slope.data_ptr() if balance else None,
-        workspace.data_ptr() if size else None, size), device)
-    return weights, chosen, counts, order, loss, slope
-
-
-def _route_gradient(ctx, d_weights, _ids, _counts, _order, d_loss):
-    logits, chosen, slope = ctx.saved_tensors
-    if d_weights is None and d_loss is None:
-        return (None,) * 7
-    slots, normalize, scale = ctx.how
-    tokens, experts = logits.shape
-    d_logits = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
-    if tokens:
-        if d_weights is not None:
-            d_weights = d_weights.contiguous()  # it may come expanded (a sum's) or in any strides
-        _launch("ggk_route_gradient", _lib.GGKRouteGradientArgs(
-            tokens, experts, slots, _TYPES[logits.dtype], logits.data_ptr(), _row_stride(logits), chosen.data_ptr(),
-            None if slope is None else slope.data_ptr(), normalize, scale,
-            None if d_weights is None else d_weights.data_ptr(), None if d_loss is None else d_loss.data_ptr(),
-            d_logits.data_ptr()), logits.device)
-    return d_logits, None, None, None, None, None, None
-
-
-# For a backward pass that builds a graph: a second derivative through it is refused.
-_route_gradient_once = torch.autograd.function.once_differentiable(_route_gradient)
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, token_mask, slots, normalize, scale, balance):
-        weights, chosen, counts, order, loss, slope = _route(logits, ids, token_mask, slots, normalize, scale, balance)
-        ctx.save_for_backward(logits, chosen, slope)
-        ctx.how = (slots, normalize, scale)
-        ctx.mark_non_differentiable(chosen, counts, order)
-        ctx.set_materialize_grads(False)
-        return weights, chosen, counts, order, loss
-
-    @staticmethod
-    def backward(ctx, *grads):
-        return _route_gradient_once(ctx, *grads) if torch.is_grad_enabled() else _route_gradient(ctx, *grads)
 
 
 def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optional[torch.Tensor] = None,
@@ -467,6 +406,21 @@ def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optiona
     weights and balance_loss carry gradients to logits (f_e counts as a constant).  Everything runs on the
     current stream of the logits' device without waiting for it, and can be captured in a graph; the
     same call gives the same bits.  E at most 1024, k at most 64."""
+    try:
+        out = _binding().route(logits, top_k, ids, token_mask, normalize, scale, balance)
+    except TypeError:  # an argument of another kind
+        _check_route(logits, top_k, ids, token_mask)
+        raise
+    if out.__class__ is tuple:
+        return Routing._make(out)
+    if out is None:
+        _check_route(logits, top_k, ids, token_mask)
+        raise ValueError("moe_route: arguments not in order")
+    raise _lib.HipError(out, "ggk_route")
+
+
+def _check_route(logits, top_k, ids, token_mask) -> None:
+    """Says what is wrong with moe_route's arguments (the binding has the same checks)."""
     if not isinstance(logits, torch.Tensor):
         raise TypeError("logits must be a torch.Tensor")
     if logits.device.type != "cuda":
@@ -496,40 +450,13 @@ def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optiona
         raise ValueError(f"{tokens} tokens with {slots} slots each: more than 2^30 slots")
     if token_mask is not None:
         _check_vector(token_mask, "token_mask", torch.bool, tokens, logits.device)
-    args = (logits, ids, token_mask, slots, bool(normalize), float(scale), bool(balance))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return Routing(*_Route.apply(*args))
-    return Routing(*_route(*args)[:5])
 
 
 # ---------------------------------------------------------------- 4-bit weights
 
-def _w4_in_order(x, q, scales, zeros, row_weights, lead, out_dtype) -> bool:
-    """Whether _check_w4 finds nothing: the same checks, each tensor's metadata read once."""
-    try:
-        qs, qt, ss, st = q.shape, q.stride(), scales.shape, scales.stride()
-        rows, k = x.shape
-        groups, device = ss[-1], x.device
-        ok = (x.dtype is torch.float16 and q.dtype is torch.uint8 and scales.dtype is torch.float16 and
-              (out_dtype is torch.float32 or out_dtype is torch.float16) and device.type == "cuda" and
-              q.device == device and scales.device == device and len(qs) == 2 + lead and ss[:-1] == qs[:-1] and
-              k == 2 * qs[-1] and groups > 0 and k > 0 and k % (32 * groups) == 0 and
-              qt[-1] == 1 and (qs[-2] <= 1 or (qt[-2] >= qs[-1] and qt[-2] % 16 == 0)) and
-              (lead == 0 or qs[0] <= 1 or qt[0] % 16 == 0) and q.data_ptr() % 16 == 0 and
-              (groups == 1 or st[-1] == 1) and (qs[-2] <= 1 or st[-2] >= groups) and
-              (x.is_contiguous() or (x.stride(1) == 1 and (rows <= 1 or x.stride(0) >= k))))
-        if ok and zeros is not None:
-            zt = zeros.stride()
-            ok = (zeros.dtype is torch.uint8 and zeros.shape == ss and zeros.device == device and
-                  (groups == 1 or zt[-1] == 1) and (qs[-2] <= 1 or zt[-2] >= groups))
-        return ok and not (torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or (
-            row_weights is not None and row_weights.requires_grad)))
-    except (AttributeError, TypeError, ValueError, IndexError):
-        return False
-
-
-def _check_w4(x, q, scales, zeros, row_weights, lead, out_dtype):
-    """Checks shared by the two products: lead is the number of dimensions ahead of a matrix's two."""
+def _check_w4(x, q, scales, zeros, counts, order, row_weights, out_dtype, lead=0) -> None:
+    """Says what is wrong with the arguments of the products (the binding has the same checks); lead: dimensions ahead of
+    a matrix's two."""
     if row_weights is not None and not isinstance(row_weights, torch.Tensor):
         raise TypeError("row_weights must be a torch.Tensor")
     if not isinstance(x, torch.Tensor) or not isinstance(q, torch.Tensor) or not isinstance(scales, torch.Tensor):
@@ -573,26 +500,6 @@ def _check_w4(x, q, scales, zeros, row_weights, lead, out_dtype):
         raise RuntimeError("the products with 4-bit weights have no gradient: detach x, scales and row_weights")
 
 
-def _w4(x, q, scales, zeros, rows, experts, counts, order, row_weights, out_dtype):
-    n, half = q.shape[-2:]
-    groups = scales.shape[-1]
-    device = x.device
-    y = torch.empty((rows, n), dtype=out_dtype, device=device)
-    if rows == 0 or n == 0:
-        return y
-    qt, st = q.stride(), scales.stride()
-    zt = zeros.stride() if zeros is not None else st
-    several = experts > 1
-    _launch("ggk_w4_multiply", _lib.GGKW4Args(
-        rows, x.shape[0], n, 2 * half, 2 * half // groups, experts, x.data_ptr(), _row_stride(x),
-        q.data_ptr(), qt[-2] if n > 1 else half, qt[0] if several else 0,
-        scales.data_ptr(), st[-2] if n > 1 else groups, st[0] if several else 0,
-        None if zeros is None else zeros.data_ptr(), zt[-2] if n > 1 else groups, zt[0] if several else 0,
-        None if counts is None else counts.data_ptr(), None if order is None else order.data_ptr(),
-        None if row_weights is None else row_weights.data_ptr(), y.data_ptr(), n, _TYPES[out_dtype]), device)
-    return y
-
-
 def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
               out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """y = x @ w.T for a few rows x (float16 [M, K]) and a matrix w [N, K] of 4-bit weights:
@@ -606,9 +513,7 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
 
     Runs on the current stream of x's device, without waiting; no gradient (inputs that require one are
     refused).  Any number of rows is right; it is made for up to 64 or so."""
-    if not _w4_in_order(x, q, scales, zeros, None, 0, out_dtype):
-        _check_w4(x, q, scales, zeros, None, 0, out_dtype)
-    return _w4(x, q, scales, zeros, x.shape[0], 0, None, None, None, out_dtype)
+    return _w4(_check_w4, x, q, scales, zeros, None, None, None, out_dtype)
 
 
 def moe_w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, counts: torch.Tensor, order: torch.Tensor,
@@ -625,10 +530,29 @@ def moe_w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, counts
     entries (e.g. the routing's weights), 1 if not given.  Counts and order stay on the GPU and
     are not trusted: a negative count is taken as 0, counts past R and entries outside [0, R) are dropped;
     rows that order does not name are left unwritten."""
+    if counts is None or order is None:
+        raise TypeError("counts and order must be torch.Tensors")
+    return _w4(_check_moe_w4, x, q, scales, zeros, counts, order, row_weights, out_dtype)
+
+
+def _w4(check, x, q, scales, zeros, counts, order, row_weights, out_dtype):
+    try:
+        out = _binding().w4(x, q, scales, zeros, counts, order, row_weights, out_dtype)
+    except TypeError:  # an argument of another kind
+        check(x, q, scales, zeros, counts, order, row_weights, out_dtype)
+        raise
+    if isinstance(out, torch.Tensor):
+        return out
+    if out is None:
+        check(x, q, scales, zeros, counts, order, row_weights, out_dtype)
+        raise ValueError("products with 4-bit weights: arguments not in order")
+    raise _lib.HipError(out, "ggk_w4_multiply")
+
+
+def _check_moe_w4(x, q, scales, zeros, counts, order, row_weights, out_dtype) -> None:
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise ValueError("q must be [experts, N, K / 2]")
-    if not _w4_in_order(x, q, scales, zeros, row_weights, 1, out_dtype):
-        _check_w4(x, q, scales, zeros, row_weights, 1, out_dtype)
+    _check_w4(x, q, scales, zeros, counts, order, row_weights, out_dtype, lead=1)
     experts = q.shape[0]
     if not 1 <= experts <= _lib.GGK_MOE_MAX_EXPERTS:
         raise ValueError(f"q has {experts} experts, expected 1 to {_lib.GGK_MOE_MAX_EXPERTS}")
@@ -643,7 +567,6 @@ def moe_w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, counts
         raise ValueError(f"order has {rows} entries, not a multiple of x's {x.shape[0]} rows")
     if row_weights is not None:
         _check_vector(row_weights, "row_weights", torch.float32, rows, x.device)
-    return _w4(x, q, scales, zeros, rows, experts, counts, order, row_weights, out_dtype)
 
 
 # ---------------------------------------------------------------- custom op

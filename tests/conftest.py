@@ -22,6 +22,10 @@ def _ensure_built():
         from grouped_gemm_gpu_kernel_amd import build
 
         build.build_library()
+    if not _lib.TORCH_PATH.exists():
+        from grouped_gemm_gpu_kernel_amd import build
+
+        build.build_torch_binding()
     if not (ROOT / "oracle" / "liboracle.so").exists():
         from oracle import oracle
 
