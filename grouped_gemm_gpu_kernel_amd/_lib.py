@@ -155,7 +155,7 @@ class GGKRouteGradientArgs(ctypes.Structure):
     _fields_ = [
         ("tokens", ctypes.c_int), ("experts", ctypes.c_int), ("slots", ctypes.c_int), ("type", ctypes.c_int),
         ("logits", ctypes.c_void_p), ("ld", ctypes.c_longlong), ("ids", ctypes.c_void_p),
-        ("slope", ctypes.c_void_p), ("normalize", ctypes.c_int), ("scale", ctypes.c_float),
+        ("distinct", ctypes.c_int), ("slope", ctypes.c_void_p), ("normalize", ctypes.c_int), ("scale", ctypes.c_float),
         ("d_weights", ctypes.c_void_p), ("d_loss", ctypes.c_void_p), ("d_logits", ctypes.c_void_p),
     ]
 

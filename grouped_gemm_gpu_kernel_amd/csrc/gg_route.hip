@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kWave = 64;
 constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / kWave;
+constexpr int kSmallThreads = 1024;  // of the workgroup that routes a few tokens by itself
 constexpr int kMaxExperts = GGK_MOE_MAX_EXPERTS;
 
 typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
@@ -101,7 +101,7 @@ __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f
 // lane adds the same pairs and ends with the same bits -- and across rows by the lane swaps of gfx950.
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true);  // every lane reads a lane of its row
 }
 
 template <int L, class Op>
@@ -206,17 +206,24 @@ struct Workspace {
   int* routed;  // [blocks]
 };
 
-// At most this many entries of `count` are summed by every block of the order kernel itself.
+// At most this many entries of `count` are summed by every block of the order kernel itself: with 64 experts and
+// 16384 tokens, two launches of 256 blocks instead of three of 512.
 constexpr int kMaxOwnSums = 20 * 1024;
 constexpr int kMaxBlocks = 512;
 
 Plan plan_blocks(int tokens, int experts) {
   const int least = kThreads / 16;  // one token a group
-  int rows = (tokens + kMaxBlocks - 1) / kMaxBlocks;
+  const int own = kMaxOwnSums / experts;
+  const int most = own >= kMaxBlocks / 2 && own < kMaxBlocks ? own : kMaxBlocks;
+  int rows = (tokens + most - 1) / most;
   rows = rows < least ? least : (rows + least - 1) / least * least;
   const int blocks = tokens > 0 ? (tokens + rows - 1) / rows : 1;
   return {blocks, rows, (long long)blocks * experts > kMaxOwnSums, false};
 }
+
+// So many tokens are routed by one workgroup, 64 at a time: 4.5 us for the first, 2.4 for each further 64, where two
+// launches take 10.  Its counts per wave have to fit 64 KB of LDS.
+bool is_small(int tokens, int experts) { return tokens <= 128 && experts <= 768; }
 
 size_t workspace_ints(int experts, int blocks) {
   return (size_t)experts * blocks + (size_t)(experts + 1) * blocks + (size_t)blocks;
@@ -230,26 +237,47 @@ Workspace carve(void* base, int experts, int blocks) {
   return w;
 }
 
+// What a group holds of a token before it is routed.
+template <class T, int V>
+struct Token {
+  T z[V];
+  bool live;
+};
+
+// Does routing need every logit of a token?
+__device__ __forceinline__ bool needs_all(const ggk_route_args& a) {
+  return a.given_ids == nullptr || !a.normalize || a.loss != nullptr;
+}
+
+template <class T, int L, int V>
+__device__ __forceinline__ void load_token(const ggk_route_args& a, bool vectors, int t, int last, Token<T, V>& token) {
+  const bool in = t < last;
+  token.live = in && (a.token_mask == nullptr || a.token_mask[t] != 0);
+  if (needs_all(a)) {
+    // Of a padding token too: waiting for the mask first would put one load behind the other.
+    load_row<T, L, V>(static_cast<const T*>(a.logits) + (long long)(in ? t : 0) * a.ld, threadIdx.x % L,
+                      in ? a.experts : 0, vectors, Logit<T>::store(-__builtin_inff()), token.z);
+  }
+}
+
 // One token by its group: ids and weights to memory, slots counted in s_count, p added to sums.  Every lane
 // of the wave calls it; `t` at or past `last` does nothing.  Returns whether the token was routed.
 template <class T, int L, int V>
-__device__ __forceinline__ bool route_token(const ggk_route_args& a, bool vectors, int t, int last, int* s_count,
-                                            float (&sums)[V]) {
+__device__ __forceinline__ bool route_token(const ggk_route_args& a, const Token<T, V>& token, int t, int last,
+                                            int* s_count, float (&sums)[V]) {
   using Z = Logit<T>;
   using C = Columns<L, V>;
   const int lane = threadIdx.x % L;
-  const bool in = t < last;
-  const bool live = in && (a.token_mask == nullptr || a.token_mask[t] != 0);
+  const bool in = t < last, live = token.live;
   const T* row = static_cast<const T*>(a.logits) + (long long)(in ? t : 0) * a.ld;
   const long long slot0 = (long long)t * a.slots;
-  const T closed = Z::store(-__builtin_inff());
-  const bool all = a.given_ids == nullptr || !a.normalize || a.loss != nullptr;  // every logit is needed
   uint32_t key[V], best = 0;
   T z[V];
-  if (all) {
-    load_row<T, L, V>(row, lane, live ? a.experts : 0, vectors, closed, z);
+  if (needs_all(a)) {
+    const T closed = Z::store(-__builtin_inff());
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      z[j] = live ? token.z[j] : closed;
       key[j] = Z::key(z[j], C::expert(lane, j));
       best = key[j] > best ? key[j] : best;
     }
@@ -273,14 +301,19 @@ __device__ __forceinline__ bool route_token(const ggk_route_args& a, bool vector
     }
     routed = group_any<L>(my_id >= 0);
   }
-  // The softmax over all experts, before the choice takes its keys away.
+  // The softmax over all experts, before the choice takes its keys away.  A token that is not routed has every expert
+  // closed, or none of its own: zeros.
   if (!a.normalize || a.loss != nullptr) {
+    const float shift = routed ? top : 0.0f;
     float p[V], total = 0.0f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      p[j] = routed ? exp_of(Z::value(z[j]) - top) : 0.0f;
-      total += p[j];
+    for (int j = 0; j < V; ++j) p[j] = exp_of(Z::value(z[j]) - shift);
+    if (a.given_ids != nullptr) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[j] = routed ? p[j] : 0.0f;
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) total += p[j];
     total = group_sum<L>(total);
     inv = routed ? 1.0f / total : 0.0f;
     if (a.loss != nullptr) {
@@ -289,40 +322,33 @@ __device__ __forceinline__ bool route_token(const ggk_route_args& a, bool vector
     }
   }
   if (a.given_ids == nullptr) {
+    const int base = C::expert(lane, 0);
     for (int s = 0;; ++s) {
       const bool open = best > Z::kClosed;
       uint32_t at;
-      bool first[V];
       if constexpr (Z::kDistinct) {
         at = 0xffffu - (best & 0xffffu);
       } else {
         // The lowest expert among those with the best key: a lane's first, then the least over lanes.
         at = 0xffffffffu;
-        bool none = true;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          first[j] = none && key[j] == best;
-          none = none && key[j] != best;
-          at = first[j] ? (uint32_t)C::expert(lane, j) : at;
-        }
-        const uint32_t mine = at;
+        for (int j = V - 1; j >= 0; --j) at = key[j] == best ? (uint32_t)C::expert(0, j) : at;
+        at = at == 0xffffffffu ? at : at + base;
         at = group_min<L>(at);
-        const bool owner = mine == at;
-#pragma unroll
-        for (int j = 0; j < V; ++j) first[j] = first[j] && owner;
       }
       if (lane == s && open) {
         my_id = (int)at;
         my_z = Z::of_key(best);
       }
       if (s + 1 == a.slots || __ballot(open) == 0) break;
+      const int here = (int)at - base;  // the value's place, if it is one of the lane's
       uint32_t next = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if constexpr (Z::kDistinct) {
           key[j] = key[j] == best ? 0u : key[j];
         } else {
-          key[j] = first[j] ? 0u : key[j];
+          key[j] = here == C::expert(0, j) ? 0u : key[j];
         }
         next = key[j] > next ? key[j] : next;
       }
@@ -346,8 +372,26 @@ __device__ __forceinline__ bool route_token(const ggk_route_args& a, bool vector
   return routed;
 }
 
-// The block's sums of p (balance) over its groups, to out[e].  s_part: kWaves * experts floats.
-template <int L, int V>
+// Tokens [first, last) by the groups of the workgroup, each group's next logits loaded while it routes a token.
+// Returns the number of tokens that this lane's group has routed.
+template <class T, int L, int V, int THREADS>
+__device__ __forceinline__ int route_tokens(const ggk_route_args& a, bool vectors, int first, int last, int* s_count,
+                                            float (&sums)[V]) {
+  constexpr int kGroups = THREADS / L;
+  const int group = threadIdx.x / L;
+  int routed = 0;
+  Token<T, V> next;
+  load_token<T, L, V>(a, vectors, first + group, last, next);
+  for (int t0 = first; t0 < last; t0 += kGroups) {
+    const Token<T, V> token = next;
+    if (t0 + kGroups < last) load_token<T, L, V>(a, vectors, t0 + kGroups + group, last, next);
+    routed += route_token<T, L, V>(a, token, t0 + group, last, s_count, sums) ? 1 : 0;
+  }
+  return routed;
+}
+
+// The block's sums of p (balance) over its groups, to out[e].  s_part: a row of `experts` floats a wave.
+template <int L, int V, int THREADS>
 __device__ __forceinline__ void block_sums(float (&sums)[V], int experts, float* s_part, float* out) {
   using C = Columns<L, V>;
   const int tid = threadIdx.x, lane = tid % L, wave = tid / kWave;
@@ -363,16 +407,16 @@ __device__ __forceinline__ void block_sums(float (&sums)[V], int experts, float*
     if (tid % kWave < L && e < experts) s_part[wave * experts + e] = sums[j];
   }
   __syncthreads();
-  for (int e = tid; e < experts; e += kThreads) {
+  for (int e = tid; e < experts; e += THREADS) {
     float x = 0.0f;
-    for (int w = 0; w < kWaves; ++w) x += s_part[w * experts + e];
+    for (int w = 0; w < THREADS / kWave; ++w) x += s_part[w * experts + e];
     out[e] = x;
   }
 }
 
 template <class T, int L, int V>
-__global__ __launch_bounds__(kThreads) void route_rows_kernel(ggk_route_args a, Workspace ws, Plan plan) {
-  extern __shared__ int shared[];  // counts [experts + 1], routed, then (balance) kWaves * experts floats
+__global__ __launch_bounds__(kThreads, 4) void route_rows_kernel(ggk_route_args a, Workspace ws, Plan plan) {
+  extern __shared__ int shared[];  // counts [experts + 1], routed, then (balance) `experts` floats a wave
   int* s_count = shared;
   int* s_routed = shared + a.experts + 1;
   const int tid = threadIdx.x;
@@ -383,13 +427,10 @@ __global__ __launch_bounds__(kThreads) void route_rows_kernel(ggk_route_args a, 
   for (int j = 0; j < V; ++j) sums[j] = 0.0f;
   const int first = blockIdx.x * plan.rows;
   const int last = min(a.tokens, first + plan.rows);
-  int routed = 0;
-  for (int t0 = first; t0 < last; t0 += kThreads / L) {
-    routed += route_token<T, L, V>(a, plan.vectors, t0 + tid / L, last, s_count, sums) ? 1 : 0;
-  }
+  const int routed = route_tokens<T, L, V, kThreads>(a, plan.vectors, first, last, s_count, sums);
   if (tid % L == 0 && routed > 0) atomicAdd(s_routed, routed);
   if (a.loss != nullptr) {
-    block_sums<L, V>(sums, a.experts, reinterpret_cast<float*>(shared + a.experts + 2),
+    block_sums<L, V, kThreads>(sums, a.experts, reinterpret_cast<float*>(shared + a.experts + 2),
                      ws.p + (size_t)blockIdx.x * a.experts);
   }
   __syncthreads();
@@ -444,6 +485,7 @@ __global__ __launch_bounds__(kThreads) void route_columns_kernel(ggk_route_args 
 }
 
 // Exclusive prefix sum of one value per thread in thread order; ends with a barrier.
+template <int THREADS>
 __device__ __forceinline__ int block_before(int v, int* s_waves) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int x = v;
@@ -456,16 +498,17 @@ __device__ __forceinline__ int block_before(int v, int* s_waves) {
   __syncthreads();
   int before = x - v;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) before += w < wave ? s_waves[w] : 0;
+  for (int w = 0; w < THREADS / kWave; ++w) before += w < wave ? s_waves[w] : 0;
   __syncthreads();
   return before;
 }
 
 // Turns s_at[e], the places taken before this block's slots of each expert, into places in the order, adding the
 // experts before (total[e]: all slots of e; the slots without an expert come last).
+template <int THREADS>
 __device__ __forceinline__ void add_experts_before(int* s_at, const int* total, int experts, int* s_waves) {
   const int tid = threadIdx.x;
-  constexpr int kPer = (kMaxExperts + 1 + kThreads - 1) / kThreads;
+  constexpr int kPer = (kMaxExperts + 1 + THREADS - 1) / THREADS;
   int mine[kPer], sum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -473,7 +516,7 @@ __device__ __forceinline__ void add_experts_before(int* s_at, const int* total, 
     mine[i] = e < experts ? total[e] : 0;
     sum += mine[i];
   }
-  int before = block_before(sum, s_waves);
+  int before = block_before<THREADS>(sum, s_waves);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = tid * kPer + i;
@@ -484,24 +527,37 @@ __device__ __forceinline__ void add_experts_before(int* s_at, const int* total, 
 }
 
 // Places slots [first, last) by expert, in their own order within one.  s_at: the next place of each expert;
-// s_wave: kWaves * (experts + 1) ints.  Every wave takes a run of slots, 64 at a time: it counts its slots of
+// s_wave: experts + 1 ints a wave; id0: this lane's first id, loaded before the counts were known.  Every wave takes a run of slots, 64 at a time: it counts its slots of
 // each expert, the waves' counts become their first places, and a slot goes to its wave's next place plus the number of
 // lanes below with the same expert.  Waves write only their own row of s_wave.
-__device__ __forceinline__ void place_slots(const ggk_route_args& a, long long first, long long last, const int* s_at,
-                                            int* s_wave) {
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, width = a.experts + 1;
-  for (int i = tid; i < kWaves * width; i += kThreads) s_wave[i] = 0;
-  __syncthreads();
+// Waves write only their own row of s_wave.
+struct Run {
+  long long begin, end;  // of the wave's slots
+};
+
+template <int THREADS>
+__device__ __forceinline__ Run run_of_wave(long long first, long long last) {
+  constexpr int kWaves = THREADS / kWave;
   const long long each = ((last - first + kWaves - 1) / kWaves + kWave - 1) / kWave * kWave;
-  const long long mine = first + wave * each, end = min(last, mine + each);
+  const long long begin = first + (threadIdx.x / kWave) * each;
+  return {begin, min(last, begin + each)};
+}
+
+template <int THREADS>
+__device__ __forceinline__ void place_slots(const ggk_route_args& a, const Run& run, int id0, const int* s_at,
+                                            int* s_wave) {
+  constexpr int kWaves = THREADS / kWave;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, width = a.experts + 1;
+  for (int i = tid; i < kWaves * width; i += THREADS) s_wave[i] = 0;
+  __syncthreads();
   int* my = s_wave + wave * width;
   const int bits = 32 - __builtin_clz(a.experts);
-  for (long long i = mine + lane; i < end; i += kWave) {
-    const int id = a.ids[i];
+  for (long long i = run.begin + lane; i < run.end; i += kWave) {
+    const int id = i == run.begin + lane ? id0 : a.ids[i];
     atomicAdd(&my[id < 0 ? a.experts : id], 1);
   }
   __syncthreads();
-  for (int e = tid; e < width; e += kThreads) {
+  for (int e = tid; e < width; e += THREADS) {
     int at = s_at[e];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
@@ -511,9 +567,9 @@ __device__ __forceinline__ void place_slots(const ggk_route_args& a, long long f
     }
   }
   __syncthreads();
-  for (long long i0 = mine; i0 < end; i0 += kWave) {
-    const bool in = i0 + lane < end;
-    int id = in ? a.ids[i0 + lane] : -1;
+  for (long long i0 = run.begin; i0 < run.end; i0 += kWave) {
+    const bool in = i0 + lane < run.end;
+    int id = i0 == run.begin ? id0 : (in ? a.ids[i0 + lane] : -1);
     id = id < 0 ? a.experts : id;
     unsigned long long same = __ballot(in);
     for (int bit = 0; bit < bits; ++bit) {
@@ -559,20 +615,28 @@ __device__ __forceinline__ int all_routed(const Workspace& ws, int blocks) {
   return routed;
 }
 
-// The order of one block's slots; the last block also computes the loss.  Without the columns kernel every block
-// adds up the counts of all blocks itself, and the last one the sums of p.
+// The order of one block's slots; one more block computes the loss.  Without the columns kernel every block adds up
+// the counts of all blocks itself, and the last one the sums of p.
 __global__ __launch_bounds__(kThreads) void route_order_kernel(ggk_route_args a, Workspace ws, Plan plan) {
   extern __shared__ int shared[];  // s_at, s_total [experts + 1] each, then s_wave
-  __shared__ int s_waves[kWaves];
+  __shared__ int s_waves[kThreads / kWave];
   const int tid = threadIdx.x, width = a.experts + 1, block = blockIdx.x;
   int* s_at = shared;
   int* s_total = shared + width;
   int* s_wave = shared + 2 * width;
-  const bool last_block = block == (int)gridDim.x - 1;
+  const bool loss_block = block == plan.blocks;
+  if (loss_block && plan.columns) {
+    if (tid < kWave) balance_loss(a, ws.p, a.counts, all_routed(ws, plan.blocks));
+    return;
+  }
+  const long long first = (long long)block * plan.rows * a.slots;
+  const Run run = run_of_wave<kThreads>(
+      first, min((long long)a.tokens * a.slots, first + (long long)plan.rows * a.slots));
+  const int id0 = !loss_block && run.begin + tid % kWave < run.end ? a.ids[run.begin + tid % kWave] : -1;
   if (plan.columns) {
     for (int e = tid; e < width; e += kThreads) s_at[e] = ws.count[(size_t)block * width + e];
     __syncthreads();
-    add_experts_before(s_at, a.counts, a.experts, s_waves);
+    add_experts_before<kThreads>(s_at, a.counts, a.experts, s_waves);
   } else {
     // Threads take (slice of blocks, expert): slices of the columns are added up in LDS.
     for (int e = tid; e < 2 * width; e += kThreads) shared[e] = 0;
@@ -581,7 +645,7 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(ggk_route_args a,
     for (int i = tid; i < slices * width; i += kThreads) {
       const int e = i % width, b0 = i / width * each, b1 = min(plan.blocks, b0 + each);
       int before = 0, total = 0;
-#pragma unroll 8
+#pragma unroll 16
       for (int b = b0; b < b1; ++b) {
         const int n = ws.count[(size_t)b * width + e];
         before += b < block ? n : 0;
@@ -591,75 +655,73 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(ggk_route_args a,
       atomicAdd(&s_total[e], total);
     }
     __syncthreads();
-    add_experts_before(s_at, s_total, a.experts, s_waves);
-    if (last_block) {
+    if (loss_block) {
+      // Sums of p: slices of the blocks per expert, then the slices in their order.
+      float* s_p = reinterpret_cast<float*>(s_wave);
+      const int parts = min(kThreads / kWave, max(1, kThreads / a.experts)), rows = (plan.blocks + parts - 1) / parts;
+      for (int i = tid; i < parts * a.experts; i += kThreads) {
+        const int e = i % a.experts, b0 = i / a.experts * rows, b1 = min(plan.blocks, b0 + rows);
+        float p = 0.0f;
+#pragma unroll 16
+        for (int b = b0; b < b1; ++b) p += ws.p[(size_t)b * a.experts + e];
+        s_p[i] = p;
+      }
+      __syncthreads();
+      for (int e = tid; e < a.experts; e += kThreads) {
+        float p = s_p[e];
+        for (int i = 1; i < parts; ++i) p += s_p[i * a.experts + e];
+        s_p[e] = p;
+      }
+      __syncthreads();
+      if (tid < kWave) balance_loss(a, s_p, s_total, all_routed(ws, plan.blocks));
+      return;
+    }
+    add_experts_before<kThreads>(s_at, s_total, a.experts, s_waves);
+    if (block == 0) {
       for (int e = tid; e < a.experts; e += kThreads) a.counts[e] = s_total[e];
     }
   }
-  const long long all = (long long)a.tokens * a.slots;
-  const long long first = (long long)block * plan.rows * a.slots;
-  place_slots(a, first, min(all, first + (long long)plan.rows * a.slots), s_at, s_wave);
-  if (last_block && a.loss != nullptr) {
-    __syncthreads();
-    if (plan.columns) {
-      if (tid < kWave) balance_loss(a, ws.p, a.counts, all_routed(ws, plan.blocks));
-      return;
-    }
-    // Sums of p: slices of the blocks per expert, then the slices in their order.
-    float* s_p = reinterpret_cast<float*>(s_wave);
-    const int slices = min(kWaves, max(1, kThreads / a.experts)), each = (plan.blocks + slices - 1) / slices;
-    for (int i = tid; i < slices * a.experts; i += kThreads) {
-      const int e = i % a.experts, b0 = i / a.experts * each, b1 = min(plan.blocks, b0 + each);
-      float p = 0.0f;
-#pragma unroll 8
-      for (int b = b0; b < b1; ++b) p += ws.p[(size_t)b * a.experts + e];
-      s_p[i] = p;
-    }
-    __syncthreads();
-    for (int e = tid; e < a.experts; e += kThreads) {
-      float p = s_p[e];
-      for (int s = 1; s < slices; ++s) p += s_p[s * a.experts + e];
-      s_p[e] = p;
-    }
-    __syncthreads();
-    if (tid < kWave) balance_loss(a, s_p, s_total, all_routed(ws, plan.blocks));
-  }
+  place_slots<kThreads>(a, run, id0, s_at, s_wave);
 }
 
 // All of it for a few tokens, in one workgroup.
 template <class T, int L, int V>
-__global__ __launch_bounds__(kThreads) void route_small_kernel(ggk_route_args a, bool vectors) {
+__global__ __launch_bounds__(kSmallThreads) void route_small_kernel(ggk_route_args a, bool vectors) {
   extern __shared__ int shared[];  // counts [experts + 1], routed, s_at [experts + 1], then s_part / s_wave
-  __shared__ int s_waves[kWaves];
+  __shared__ int s_waves[kSmallThreads / kWave];
   const int tid = threadIdx.x, width = a.experts + 1;
   int* s_count = shared;
   int* s_routed = shared + width;
   int* s_at = shared + width + 1;
   int* s_rest = shared + 2 * width + 1;
-  for (int e = tid; e < 2 * width + 1; e += kThreads) shared[e] = 0;
+  for (int e = tid; e < 2 * width + 1; e += kSmallThreads) shared[e] = 0;
   __syncthreads();
   float sums[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) sums[j] = 0.0f;
-  int routed = 0;
-  for (int t0 = 0; t0 < a.tokens; t0 += kThreads / L) {
-    routed += route_token<T, L, V>(a, vectors, t0 + tid / L, a.tokens, s_count, sums) ? 1 : 0;
-  }
+  const int routed = route_tokens<T, L, V, kSmallThreads>(a, vectors, 0, a.tokens, s_count, sums);
   if (tid % L == 0 && routed > 0) atomicAdd(s_routed, routed);
   __syncthreads();  // ids are read back below by other threads of this workgroup
+  const Run run = run_of_wave<kSmallThreads>(0, (long long)a.tokens * a.slots);
+  const int id0 = run.begin + tid % kWave < run.end ? a.ids[run.begin + tid % kWave] : -1;
   if (a.loss != nullptr) {
     float* s_part = reinterpret_cast<float*>(s_rest);
-    block_sums<L, V>(sums, a.experts, s_part, s_part);
+    block_sums<L, V, kSmallThreads>(sums, a.experts, s_part, s_part);
     __syncthreads();
     if (tid < kWave) balance_loss(a, s_part, s_count, *s_routed);
     __syncthreads();
   }
-  for (int e = tid; e < a.experts; e += kThreads) a.counts[e] = s_count[e];
-  add_experts_before(s_at, s_count, a.experts, s_waves);
-  place_slots(a, 0, (long long)a.tokens * a.slots, s_at, s_rest);
+  for (int e = tid; e < a.experts; e += kSmallThreads) a.counts[e] = s_count[e];
+  add_experts_before<kSmallThreads>(s_at, s_count, a.experts, s_waves);
+  place_slots<kSmallThreads>(a, run, id0, s_at, s_rest);
 }
 
 // ---------------------------------------------------------------- backward
+
+// A group's row of the gradient in LDS, where the chosen experts' parts are added to it: comparing every slot's
+// expert with each of a lane's takes 3 instructions for each pair, 384 a wave with 8 slots and 16 values.
+template <int L, int V>
+constexpr bool kRowInLds = V >= 8;
 
 template <class T, int L, int V>
 __global__ __launch_bounds__(kThreads) void route_gradient_kernel(ggk_route_gradient_args a, bool vectors) {
@@ -667,7 +729,8 @@ __global__ __launch_bounds__(kThreads) void route_gradient_kernel(ggk_route_grad
   using C = Columns<L, V>;
   constexpr int W = C::W;
   constexpr int kGroups = kThreads / L;
-  const int lane = threadIdx.x % L;
+  __shared__ alignas(16) float s_rows[kRowInLds<L, V> ? kGroups : 1][kRowInLds<L, V> ? L * V : 1];
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
   const float d_loss = a.d_loss != nullptr ? *a.d_loss : 0.0f;
   // Without a loss, normalized weights depend on the chosen logits alone.
   const bool softmax = a.d_loss != nullptr || !a.normalize;
@@ -677,30 +740,48 @@ __global__ __launch_bounds__(kThreads) void route_gradient_kernel(ggk_route_grad
     const int e = C::expert(lane, j);
     c[j] = a.d_loss != nullptr && e < a.experts ? d_loss * a.slope[e] : 0.0f;
   }
-  for (long long t0 = (long long)blockIdx.x * kGroups; t0 < a.tokens; t0 += (long long)gridDim.x * kGroups) {
-    const int t = (int)t0 + threadIdx.x / L;
+  struct Loaded {
+    T z[V];
+    int id;
+    float g;
+  };
+  auto load = [&](long long t0, Loaded& x) {
+    const long long t = t0 + group;
     const bool in = t < a.tokens;
-    const T* row = static_cast<const T*>(a.logits) + (long long)(in ? t : 0) * a.ld;
-    const long long slot0 = (long long)t * a.slots;
-    const int my_id = in && lane < a.slots ? a.ids[slot0 + lane] : -1;
-    const bool has = my_id >= 0 && my_id < a.experts;
+    const long long slot = t * a.slots + lane;
+    x.id = in && lane < a.slots ? a.ids[slot] : -1;
+    x.g = in && lane < a.slots && a.d_weights != nullptr ? a.scale * a.d_weights[slot] : 0.0f;
+    if (softmax) {
+      load_row<T, L, V>(static_cast<const T*>(a.logits) + (in ? t : 0) * a.ld, lane, in ? a.experts : 0, vectors,
+                        Z::store(-__builtin_inff()), x.z);
+    }
+  };
+  Loaded next;
+  long long t0 = (long long)blockIdx.x * kGroups;
+  const long long stride = (long long)gridDim.x * kGroups;
+  load(t0, next);
+  for (; t0 < a.tokens; t0 += stride) {
+    const Loaded now = next;
+    if (t0 + stride < a.tokens) load(t0 + stride, next);
+    const long long t = t0 + group;
+    const bool in = t < a.tokens;
+    const bool has = now.id >= 0 && now.id < a.experts;
     const bool routed = group_any<L>(has);
-    const float g = has && a.d_weights != nullptr ? a.scale * a.d_weights[slot0 + lane] : 0.0f;
-    const float my_z = has ? Z::value(row[my_id]) : -__builtin_inff();
+    const float g = has ? now.g : 0.0f;
+    // The chosen logits: again from memory (the cache has them), by the lanes of the slots.
+    const float my_z = has ? Z::value((static_cast<const T*>(a.logits) + t * a.ld)[now.id]) : -__builtin_inff();
     float d[V], top = 0.0f, inv = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = 0.0f;
     if (softmax) {
-      T z[V];
-      load_row<T, L, V>(row, lane, in ? a.experts : 0, vectors, Z::store(-__builtin_inff()), z);
       top = -__builtin_inff();
       float total = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) top = fmaxf(top, Z::value(z[j]));
+      for (int j = 0; j < V; ++j) top = fmaxf(top, Z::value(now.z[j]));
       top = group_max<L>(top);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        d[j] = routed ? exp_of(Z::value(z[j]) - top) : 0.0f;
+        d[j] = routed ? exp_of(Z::value(now.z[j]) - top) : 0.0f;
         total += d[j];
       }
       total = group_sum<L>(total);
@@ -728,15 +809,39 @@ __global__ __launch_bounds__(kThreads) void route_gradient_kernel(ggk_route_grad
       for (int j = 0; j < V; ++j) d[j] = routed ? d[j] * (c[j] - dot) : 0.0f;
     }
     if (a.d_weights != nullptr) {
-      // Slot by slot, so that an expert named twice is added in the slots' order.
-      for (int s = 0; s < a.slots; ++s) {
-        const int id = __shfl(has ? my_id : -1, s, L);
-        const float part = __shfl(my_d, s, L);
+      if constexpr (kRowInLds<L, V>) {
+        float* row = s_rows[group];
+        typedef struct alignas(16) {
+          float v[4];
+        } Four;
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] += id == C::expert(lane, j) ? part : 0.0f;
+        for (int j = 0; j < V; j += 4) *reinterpret_cast<Four*>(row + C::expert(lane, j)) = {d[j], d[j + 1], d[j + 2], d[j + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (a.distinct) {
+          if (has) row[now.id] += my_d;
+        } else {  // one slot after the other, so that an expert named twice is added in the slots' order
+          for (int s = 0; s < a.slots; ++s) {
+            if (lane == s && has) row[now.id] += my_d;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const Four x = *reinterpret_cast<const Four*>(row + C::expert(lane, j));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[j + i] = x.v[i];
+        }
+      } else {
+        for (int s = 0; s < a.slots; ++s) {
+          const int id = __shfl(has ? now.id : -1, s, L);
+          const float part = __shfl(my_d, s, L);
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[j] += id == C::expert(lane, j) ? part : 0.0f;
+        }
       }
     }
-    T* out = static_cast<T*>(a.d_logits) + (long long)t * a.experts;
+    T* out = static_cast<T*>(a.d_logits) + t * a.experts;
     typedef struct alignas(sizeof(T) * W) {
       T v[W];
     } Vector;
@@ -762,22 +867,19 @@ __global__ __launch_bounds__(kThreads) void route_gradient_kernel(ggk_route_grad
 
 // ---------------------------------------------------------------- launches
 
-// At most this many tokens are routed by one workgroup.
-constexpr int kSmallTokens = 128;
-
 template <class T, int L, int V>
 hipError_t launch_route(const ggk_route_args& a, Plan plan, hipStream_t stream) {
   const size_t width = a.experts + 1;
-  const size_t waves = sizeof(int) * kWaves * width;
+  const size_t wave_row = sizeof(int) * width;  // of every wave, beside what the workgroup shares
   plan.vectors = whole_vectors<T, V>(a.logits, a.tokens > 1 ? a.ld : 0, a.experts);
-  if (a.tokens <= kSmallTokens) {
-    hipLaunchKernelGGL((route_small_kernel<T, L, V>), dim3(1), dim3(kThreads), sizeof(int) * (2 * width + 1) + waves,
-                       stream, a, plan.vectors);
+  if (is_small(a.tokens, a.experts)) {
+    hipLaunchKernelGGL((route_small_kernel<T, L, V>), dim3(1), dim3(kSmallThreads),
+                       sizeof(int) * (2 * width + 1) + kSmallThreads / kWave * wave_row, stream, a, plan.vectors);
     return hipGetLastError();
   }
   const Workspace ws = carve(a.workspace, a.experts, plan.blocks);
   hipLaunchKernelGGL((route_rows_kernel<T, L, V>), dim3(plan.blocks), dim3(kThreads),
-                     sizeof(int) * (width + 1) + (a.loss != nullptr ? waves : 0), stream, a, ws, plan);
+                     sizeof(int) * (width + 1) + (a.loss != nullptr ? kThreads / kWave * wave_row : 0), stream, a, ws, plan);
   hipError_t st = hipGetLastError();
   if (st != hipSuccess) return st;
   if (plan.columns) {
@@ -786,8 +888,8 @@ hipError_t launch_route(const ggk_route_args& a, Plan plan, hipStream_t stream) 
     st = hipGetLastError();
     if (st != hipSuccess) return st;
   }
-  hipLaunchKernelGGL(route_order_kernel, dim3(plan.blocks), dim3(kThreads), sizeof(int) * 2 * width + waves, stream, a,
-                     ws, plan);
+  hipLaunchKernelGGL(route_order_kernel, dim3(plan.blocks + (a.loss != nullptr ? 1 : 0)), dim3(kThreads),
+                     sizeof(int) * 2 * width + kThreads / kWave * wave_row, stream, a, ws, plan);
   return hipGetLastError();
 }
 
@@ -834,7 +936,7 @@ bool bad_sizes(int tokens, int experts, int slots, int type, long long ld) {
 }  // namespace
 
 extern "C" size_t ggk_route_workspace(int tokens, int experts) {
-  if (tokens <= kSmallTokens || experts < 1 || experts > kMaxExperts) return 0;
+  if (tokens < 0 || experts < 1 || experts > kMaxExperts || is_small(tokens, experts)) return 0;
   return sizeof(int) * workspace_ints(experts, plan_blocks(tokens, experts).blocks);
 }
 
@@ -844,7 +946,7 @@ extern "C" hipError_t ggk_route_check(const ggk_route_args* args) {
   if (bad_sizes(a.tokens, a.experts, a.slots, a.type, a.ld)) return hipErrorInvalidValue;
   if (a.given_ids == nullptr && a.slots > a.experts) return hipErrorInvalidValue;
   if (a.workspace_bytes < ggk_route_workspace(a.tokens, a.experts)) return hipErrorInvalidValue;
-  if (a.counts == nullptr || (a.workspace == nullptr && a.tokens > kSmallTokens) || (a.loss == nullptr) != (a.slope == nullptr) ||
+  if (a.counts == nullptr || (a.workspace == nullptr && !is_small(a.tokens, a.experts)) || (a.loss == nullptr) != (a.slope == nullptr) ||
       (a.tokens > 0 && (a.logits == nullptr || a.weights == nullptr || a.ids == nullptr || a.order == nullptr))) {
     return hipErrorInvalidDevicePointer;
   }

@@ -144,6 +144,7 @@ struct Route : torch::autograd::Function<Route> {
     RouteOutputs o = route(c);
     TORCH_CHECK(o.status == 0, "ggk_route failed with hipError_t ", o.status);
     ctx->save_for_backward({logits, o.ids, o.slope});
+    ctx->saved_data["distinct"] = !c.ids.has_value();
     ctx->saved_data["normalize"] = c.normalize;
     ctx->saved_data["scale"] = c.scale;
     ctx->mark_non_differentiable({o.ids, o.counts, o.order});
@@ -170,6 +171,7 @@ struct Route : torch::autograd::Function<Route> {
       a.logits = z.const_data_ptr();
       a.ld = row_stride(z);
       a.ids = ids.const_data_ptr<int>();
+      a.distinct = ctx->saved_data["distinct"].toBool();
       a.slope = slope.defined() ? slope.const_data_ptr<float>() : nullptr;
       a.normalize = ctx->saved_data["normalize"].toBool();
       a.scale = static_cast<float>(ctx->saved_data["scale"].toDouble());

@@ -421,6 +421,7 @@ typedef struct ggk_route_gradient_args {
   const void* logits;
   long long ld;
   const int* ids;
+  int distinct; /* no token names an expert twice, as where the largest logits were taken */
   const float* slope;
   int normalize;
   float scale;
