@@ -17,6 +17,8 @@
 #include <hip/hip_bf16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "grouped_gemm_amd_kernels.h"
 
 namespace {
@@ -260,6 +262,107 @@ __device__ __forceinline__ void load_token(const ggk_route_args& a, bool vectors
   }
 }
 
+// The choice: slot s of a group's token to its lane s, as the s-th best key's expert and logit.  best: the best of all.
+// With few values a lane, each round looks all of them over and takes the chosen one out.
+template <class T, int L, int V>
+__device__ __forceinline__ void choose(int slots, uint32_t (&key)[V], uint32_t best, int& my_id, float& my_z) {
+  using Z = Logit<T>;
+  using C = Columns<L, V>;
+  const int lane = threadIdx.x % L, base = C::expert(lane, 0);
+  for (int s = 0;; ++s) {
+    const bool open = best > Z::kClosed;
+    uint32_t at;
+    if constexpr (Z::kDistinct) {
+      at = 0xffffu - (best & 0xffffu);
+    } else {
+      // The lowest expert among those with the best key: a lane's first, then the least over lanes.
+      at = 0xffffffffu;
+#pragma unroll
+      for (int j = V - 1; j >= 0; --j) at = key[j] == best ? (uint32_t)C::expert(lane, j) : at;
+      at = group_min<L>(at);
+    }
+    if (lane == s && open) {
+      my_id = (int)at;
+      my_z = Z::of_key(best);
+    }
+    if (s + 1 == slots || __ballot(open) == 0) break;
+    const int here = (int)at - base;  // the value's place, if it is one of the lane's
+    uint32_t next = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if constexpr (Z::kDistinct) {
+        key[j] = key[j] == best ? 0u : key[j];
+      } else {
+        key[j] = here == C::expert(0, j) ? 0u : key[j];
+      }
+      next = key[j] > next ? key[j] : next;
+    }
+    best = group_max<L>(next);
+  }
+}
+
+// With many, a lane keeps its three best in order and a round looks at the first alone.  A lane that has given all
+// three makes them anew, from what comes after the last choice; with 8 slots of 256 experts one token in 50 has
+// such a lane.  A round of 16 values costs 30 instructions instead of 105: 65521
+// tokens of 256 float logits with their softmax 36 instead of 39 us, of which 26 are vector instructions issued.
+template <class T, int L, int V>
+__device__ __forceinline__ void choose_queued(int slots, const uint32_t (&key)[V], uint32_t best, int& my_id, float& my_z) {
+  using Z = Logit<T>;
+  using C = Columns<L, V>;
+  const int lane = threadIdx.x % L;
+  uint32_t q0, q1, q2;
+  int e0, e1, e2;
+  // The best three of all keys, or of those after (key `below`, expert `after`) in the order of the choice.
+  auto fill = [&](auto all, uint32_t below, int after) {
+    q0 = q1 = q2 = 0;
+    e0 = e1 = e2 = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int e = C::expert(lane, j);
+      const bool in = decltype(all)::value || key[j] < below || (!Z::kDistinct && key[j] == below && e > after);
+      const uint32_t k = in ? key[j] : 0u;
+      if constexpr (!Z::kDistinct) {  // equal keys keep the lower expert, which comes first, ahead
+        const bool b0 = k > q0, b1 = k > q1, b2 = k > q2;
+        e2 = b1 ? e1 : (b2 ? e : e2);
+        e1 = b0 ? e0 : (b1 ? e : e1);
+        e0 = b0 ? e : e0;
+      }
+      const uint32_t r = min(q0, k), r1 = min(q1, r);
+      q0 = max(q0, k);
+      q1 = max(q1, r);
+      q2 = max(q2, r1);
+    }
+  };
+  fill(std::true_type{}, 0, 0);
+  int given = 0;
+  for (int s = 0;; ++s) {
+    const bool open = best > Z::kClosed;
+    uint32_t at;
+    if constexpr (Z::kDistinct) {
+      at = 0xffffu - (best & 0xffffu);
+    } else {
+      at = group_min<L>(q0 == best ? (uint32_t)e0 : 0xffffffffu);
+    }
+    if (lane == s && open) {
+      my_id = (int)at;
+      my_z = Z::of_key(best);
+    }
+    if (s + 1 == slots || __ballot(open) == 0) break;
+    const bool mine = q0 == best && (Z::kDistinct || e0 == (int)at);
+    q0 = mine ? q1 : q0;
+    q1 = mine ? q2 : q1;
+    q2 = mine ? 0u : q2;
+    e0 = mine ? e1 : e0;
+    e1 = mine ? e2 : e1;
+    given += mine ? 1 : 0;
+    if (__ballot(given == 3) != 0) {
+      fill(std::false_type{}, best, (int)at);
+      given = 0;
+    }
+    best = group_max<L>(q0);
+  }
+}
+
 // One token by its group: ids and weights to memory, slots counted in s_count, p added to sums.  Every lane
 // of the wave calls it; `t` at or past `last` does nothing.  Returns whether the token was routed.
 template <class T, int L, int V>
@@ -322,37 +425,10 @@ __device__ __forceinline__ bool route_token(const ggk_route_args& a, const Token
     }
   }
   if (a.given_ids == nullptr) {
-    const int base = C::expert(lane, 0);
-    for (int s = 0;; ++s) {
-      const bool open = best > Z::kClosed;
-      uint32_t at;
-      if constexpr (Z::kDistinct) {
-        at = 0xffffu - (best & 0xffffu);
-      } else {
-        // The lowest expert among those with the best key: a lane's first, then the least over lanes.
-        at = 0xffffffffu;
-#pragma unroll
-        for (int j = V - 1; j >= 0; --j) at = key[j] == best ? (uint32_t)C::expert(0, j) : at;
-        at = at == 0xffffffffu ? at : at + base;
-        at = group_min<L>(at);
-      }
-      if (lane == s && open) {
-        my_id = (int)at;
-        my_z = Z::of_key(best);
-      }
-      if (s + 1 == a.slots || __ballot(open) == 0) break;
-      const int here = (int)at - base;  // the value's place, if it is one of the lane's
-      uint32_t next = 0;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if constexpr (Z::kDistinct) {
-          key[j] = key[j] == best ? 0u : key[j];
-        } else {
-          key[j] = here == C::expert(0, j) ? 0u : key[j];
-        }
-        next = key[j] > next ? key[j] : next;
-      }
-      best = group_max<L>(next);
+    if constexpr (V >= 8) {
+      choose_queued<T, L, V>(a.slots, key, best, my_id, my_z);
+    } else {
+      choose<T, L, V>(a.slots, key, best, my_id, my_z);
     }
   }
   const bool has = my_id >= 0;

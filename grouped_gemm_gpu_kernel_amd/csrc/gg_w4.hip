@@ -33,7 +33,6 @@ typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 constexpr int kWave = 64;
 constexpr int kCus = 256;
 constexpr int kStep = 128;  // values of k a wave takes at once: 16 bytes of each of 16 rows of q in 4 lanes
-constexpr int kMaxExperts = GGK_MOE_MAX_EXPERTS;
 
 // The 8 weights of a dword (nibble i: k + i) less a zero point, times 2^-9; minus_zero: the zero point times -2^-9.  An
 // integer up to 15 as the bits of a binary16 is a subnormal, that many times 2^-24: the nibbles become halves by two
@@ -71,9 +70,10 @@ struct RowTile {
 // Places and row tiles of every expert, made once a workgroup: expert e has places [first[e], first[e + 1]) and tiles
 // [tile[e], tile[e + 1]); "expert" a.experts has the places that the counts leave.  Counts are clamped to >= 0 and
 // their sums to the rows there are.
+template <int MOST>
 struct Experts {
-  int first[kMaxExperts + 2];
-  int tile[kMaxExperts + 2];
+  int first[MOST + 2];
+  int tile[MOST + 2];
   int waves[32];
 };
 
@@ -106,8 +106,8 @@ __device__ int block_before(int v, int limit, int* s_waves, int* total) {
   return add_up_to(before, ahead, limit);
 }
 
-template <int THREADS, int ROWS>
-__device__ void list_experts(const ggk_w4_args& a, Experts& s) {
+template <int THREADS, int ROWS, class Table>
+__device__ void list_experts(const ggk_w4_args& a, Table& s) {
   int placed = 0, tiles = 0;
   for (int e0 = 0; e0 < a.experts; e0 += THREADS) {
     const int e = e0 + threadIdx.x;
@@ -133,8 +133,8 @@ __device__ void list_experts(const ggk_w4_args& a, Experts& s) {
   __syncthreads();
 }
 
-template <int ROWS>
-__device__ RowTile expert_tile(const ggk_w4_args& a, const Experts& s, int tile) {
+template <int ROWS, class Table>
+__device__ RowTile expert_tile(const ggk_w4_args& a, const Table& s, int tile) {
   const int lane = threadIdx.x % kWave;
   int before = 0;  // entries of s.tile at or below `tile`: the last of them is the one that holds it
   for (int e0 = 0; e0 <= a.experts; e0 += kWave) {
@@ -152,9 +152,13 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kDepth = 4;  // steps of weights a wave has in flight
 
 // Steps of every wave that a chunk of x holds: four, less where two chunks of R rows would not fit 64 KB (32 KB beside
-// the experts' table), so that a CU holds two workgroups.  A load instruction takes 512 values of one row.
+// the full table of experts), so that a CU holds two workgroups.  A load instruction takes 512 values of one row.
 template <int R, int WK, bool EXPERTS>
-constexpr int kChunk = R * WK <= (EXPERTS ? 16 : 32) ? 4 : (EXPERTS ? 64 : 128) / (R * WK);
+constexpr int kChunk = R * WK <= (EXPERTS && R < 32 ? 16 : 32) ? 4 : (EXPERTS ? 64 : 128) / (R * WK);
+
+// Experts that the table of a kernel with R-row tiles holds: all, or as many as leave room for two workgroups.
+template <int R>
+constexpr int kTable = R < 32 ? GGK_MOE_MAX_EXPERTS : 256;
 
 // Length in values of a row of x in LDS: 16 bytes more than its chunk, so that the 16 rows of an instruction's
 // operand lie in distinct banks.
@@ -393,7 +397,7 @@ __global__ __launch_bounds__(kThreads, 4) void w4_kernel(Launch l) {
     }
   } else {
     __shared__ int s_slot[R], s_x_row[R];
-    __shared__ Experts s_experts;
+    __shared__ Experts<kTable<R>> s_experts;
     const Shared s{s_x, s_w, s_sz, s_slot, s_x_row};
     const int fan = a.rows / a.x_rows;
     list_experts<kThreads, R>(a, s_experts);
@@ -417,6 +421,8 @@ __global__ __launch_bounds__(kThreads, 4) void w4_kernel(Launch l) {
         // The rows are a constant of the whole loop over K: the compiler leaves out the wait between a matrix
         // instruction and the use of its result when a branch on them lies between.
         run_item<4, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
+      } else if (R > 16 && t.rows <= 16) {
+        run_item<16, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
       } else {
         run_item<R, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
       }
@@ -433,6 +439,7 @@ __global__ __launch_bounds__(kThreads, 4) void w4_kernel(Launch l) {
 
 template <int R, int WK, bool EXPERTS>
 hipError_t launch(const ggk_w4_args& a, hipStream_t stream) {
+  if (EXPERTS && a.experts > kTable<R>) return hipErrorInvalidValue;
   const bool fine = a.group % kStep != 0;
   auto kernel = fine ? (a.zeros != nullptr ? w4_kernel<R, WK, EXPERTS, true, true> : w4_kernel<R, WK, EXPERTS, true, false>)
                      : (a.zeros != nullptr ? w4_kernel<R, WK, EXPERTS, false, true> : w4_kernel<R, WK, EXPERTS, false, false>);
@@ -495,6 +502,7 @@ extern "C" hipError_t ggk_w4_multiply(const ggk_w4_args* args, hipStream_t strea
   const long long columns = (a.n + 15) / 16;
   if (a.experts > 0) {
     const long long waves = columns * min(a.rows, a.experts);
+    if (waves >= 1024 && a.experts <= kTable<32>) return launch<32, 1, true>(a, stream);
     return waves >= 1024 ? launch<16, 1, true>(a, stream) : waves >= 512 ? launch<16, 2, true>(a, stream) : launch<16, 4, true>(a, stream);
   }
   if (a.rows > 16) {

@@ -330,6 +330,30 @@ def test_nan_and_infinity_show(torch_cuda, experts, normalize):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("experts", [100, 128, 255, 256, 300, 512, 1000, 1024])
+def test_choices_held_by_few_lanes(torch_cuda, experts, dtype):
+    """The best logits next to each other or in steps that put them all in one lane, sorted both ways, equal in runs,
+    and with NaN at the first and last expert."""
+    z = torch.zeros(12, experts)
+    step = torch.arange(experts, dtype=torch.float32)
+    z[0], z[1] = step / 64, -step / 64
+    z[2, :20] = 4 + torch.arange(20) / 16
+    z[3, -20:] = 4 - torch.arange(20) / 16
+    for row, stride in ((4, 4), (5, 16), (6, 64)):
+        z[row, ::stride] = 3 + torch.arange(len(z[row, ::stride])) / 64
+    z[7] = (step / 7).floor()
+    z[8] = -(step / 50).floor()
+    z[9, 0] = z[9, -1] = math.nan
+    z[10, 1::64] = 5
+    z[11, 4:8] = torch.tensor([7.0, 6, 7, 6])
+    z = z.repeat(13, 1).to(TYPES[dtype]).cuda()
+    for top_k in (1, 3, 4, 9, 16, 17, 40):
+        dw = torch.randn(len(z), top_k, generator=torch.Generator().manual_seed(1)).cuda()
+        _check(z, top_k, d_weights=dw, d_loss=0.5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("experts,slots", [(5, 3), (64, 4), (70, 64), (500, 6)])
 @pytest.mark.parametrize("normalize", [True, False])
 def test_given_experts(torch_cuda, experts, slots, normalize):
