@@ -199,14 +199,16 @@ struct Plan {
   bool vectors;
 };
 
-// Workspace, written by the rows kernel: per block and expert the sum of p and the slots taken (one more
-// column: slots without an expert), then per block the routed tokens.  The columns kernel turns the
-// counts into sums over the blocks before, and the first block's sums of p into those over all.
+// Workspace, written by the rows kernel: per block and expert the slots taken (one more column: slots without an
+// expert; rows padded to whole vectors of four) and the sum of p, then per block the routed tokens.  The columns
+// kernel turns the counts into sums over the blocks before, and the first block's sums of p into those over all.
 struct Workspace {
+  int* count;   // [blocks][pitch]
   float* p;     // [blocks][experts]
-  int* count;   // [blocks][experts + 1]
   int* routed;  // [blocks]
 };
+
+__host__ __device__ inline int count_pitch(int experts) { return (experts + 4) / 4 * 4; }
 
 // At most this many entries of `count` are summed by every block of the order kernel itself: with 64 experts and
 // 16384 tokens, two launches of 256 blocks instead of three of 512.
@@ -228,14 +230,14 @@ Plan plan_blocks(int tokens, int experts) {
 bool is_small(int tokens, int experts) { return tokens <= 128 && experts <= 768; }
 
 size_t workspace_ints(int experts, int blocks) {
-  return (size_t)experts * blocks + (size_t)(experts + 1) * blocks + (size_t)blocks;
+  return (size_t)count_pitch(experts) * blocks + (size_t)experts * blocks + (size_t)blocks;
 }
 
 Workspace carve(void* base, int experts, int blocks) {
   Workspace w;
-  w.p = static_cast<float*>(base);
-  w.count = reinterpret_cast<int*>(w.p + (size_t)experts * blocks);
-  w.routed = w.count + (size_t)(experts + 1) * blocks;
+  w.count = static_cast<int*>(base);
+  w.p = reinterpret_cast<float*>(w.count + (size_t)count_pitch(experts) * blocks);
+  w.routed = reinterpret_cast<int*>(w.p + (size_t)experts * blocks);
   return w;
 }
 
@@ -510,7 +512,8 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows_kernel(ggk_route_args 
                      ws.p + (size_t)blockIdx.x * a.experts);
   }
   __syncthreads();
-  for (int e = tid; e <= a.experts; e += kThreads) ws.count[(size_t)blockIdx.x * (a.experts + 1) + e] = s_count[e];
+  const int pitch = count_pitch(a.experts);
+  for (int e = tid; e < pitch; e += kThreads) ws.count[(size_t)blockIdx.x * pitch + e] = e <= a.experts ? s_count[e] : 0;
   if (tid == 0) ws.routed[blockIdx.x] = *s_routed;
 }
 
@@ -523,7 +526,7 @@ __global__ __launch_bounds__(kThreads) void route_columns_kernel(ggk_route_args 
   __shared__ int s_count[kSlices][kColumns];
   __shared__ float s_p[kSlices][kColumns];
   const int tid = threadIdx.x, c = tid % kColumns, slice = tid / kColumns;
-  const int e = blockIdx.x * kColumns + c, width = a.experts + 1;
+  const int e = blockIdx.x * kColumns + c, width = a.experts + 1, pitch = count_pitch(a.experts);
   constexpr int kPer = kMaxBlocks / kSlices;
   const int each = (blocks + kSlices - 1) / kSlices;
   const int b0 = slice * each, rows = max(0, min(each, blocks - b0));
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(kThreads) void route_columns_kernel(ggk_route_args 
   float p = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    count[i] = i < rows && e < width ? ws.count[(size_t)(b0 + i) * width + e] : 0;
+    count[i] = i < rows && e < width ? ws.count[(size_t)(b0 + i) * pitch + e] : 0;
     sum += count[i];
   }
   if (a.loss != nullptr) {
@@ -551,7 +554,7 @@ __global__ __launch_bounds__(kThreads) void route_columns_kernel(ggk_route_args 
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    if (i < rows && e < width) ws.count[(size_t)(b0 + i) * width + e] = before;
+    if (i < rows && e < width) ws.count[(size_t)(b0 + i) * pitch + e] = before;
     before += count[i];
   }
   if (slice == 0 && e < a.experts) {
@@ -710,25 +713,37 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(ggk_route_args a,
       first, min((long long)a.tokens * a.slots, first + (long long)plan.rows * a.slots));
   const int id0 = !loss_block && run.begin + tid % kWave < run.end ? a.ids[run.begin + tid % kWave] : -1;
   if (plan.columns) {
-    for (int e = tid; e < width; e += kThreads) s_at[e] = ws.count[(size_t)block * width + e];
+    for (int e = tid; e < width; e += kThreads) s_at[e] = ws.count[(size_t)block * count_pitch(a.experts) + e];
     __syncthreads();
     add_experts_before<kThreads>(s_at, a.counts, a.experts, s_waves);
   } else {
-    // Threads take (slice of blocks, expert): slices of the columns are added up in LDS.
+    // Threads take four columns of a slice of the blocks; the slices are added up in LDS.
     for (int e = tid; e < 2 * width; e += kThreads) shared[e] = 0;
     __syncthreads();
-    const int slices = max(1, kThreads / width), each = (plan.blocks + slices - 1) / slices;
-    for (int i = tid; i < slices * width; i += kThreads) {
-      const int e = i % width, b0 = i / width * each, b1 = min(plan.blocks, b0 + each);
-      int before = 0, total = 0;
-#pragma unroll 16
+    typedef struct alignas(16) {
+      int v[4];
+    } Four;
+    const int quads = count_pitch(a.experts) / 4, slices = max(1, kThreads / quads);
+    const int each = (plan.blocks + slices - 1) / slices;
+    for (int i = tid; i < slices * quads; i += kThreads) {
+      const int quad = i % quads, b0 = i / quads * each, b1 = min(plan.blocks, b0 + each);
+      int before[4] = {0, 0, 0, 0}, total[4] = {0, 0, 0, 0};
+#pragma unroll 8
       for (int b = b0; b < b1; ++b) {
-        const int n = ws.count[(size_t)b * width + e];
-        before += b < block ? n : 0;
-        total += n;
+        const Four n = reinterpret_cast<const Four*>(ws.count)[(size_t)b * quads + quad];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          before[c] += b < block ? n.v[c] : 0;
+          total[c] += n.v[c];
+        }
       }
-      atomicAdd(&s_at[e], before);
-      atomicAdd(&s_total[e], total);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (4 * quad + c < width) {
+          atomicAdd(&s_at[4 * quad + c], before[c]);
+          atomicAdd(&s_total[4 * quad + c], total[c]);
+        }
+      }
     }
     __syncthreads();
     if (loss_block) {
@@ -1021,7 +1036,9 @@ extern "C" hipError_t ggk_route_check(const ggk_route_args* args) {
   const ggk_route_args& a = *args;
   if (bad_sizes(a.tokens, a.experts, a.slots, a.type, a.ld)) return hipErrorInvalidValue;
   if (a.given_ids == nullptr && a.slots > a.experts) return hipErrorInvalidValue;
-  if (a.workspace_bytes < ggk_route_workspace(a.tokens, a.experts)) return hipErrorInvalidValue;
+  if (a.workspace_bytes < ggk_route_workspace(a.tokens, a.experts) || reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) {
+    return hipErrorInvalidValue;
+  }
   if (a.counts == nullptr || (a.workspace == nullptr && !is_small(a.tokens, a.experts)) || (a.loss == nullptr) != (a.slope == nullptr) ||
       (a.tokens > 0 && (a.logits == nullptr || a.weights == nullptr || a.ids == nullptr || a.order == nullptr))) {
     return hipErrorInvalidDevicePointer;

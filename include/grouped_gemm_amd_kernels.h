@@ -375,8 +375,8 @@ hipError_t ggk_launch_grouped_device_done(int variant, int path, int addressing,
  *                   such token; slope[e] = d loss / d (sum of softmax(z_t)[e]).
  * loss and slope may be NULL, both or neither.  Sums are made in a fixed
  * order: the same call gives the same bits.  workspace holds
- * ggk_route_workspace(tokens, experts) bytes (0 for a few tokens), written
- * before they are read; calls that may overlap need one each.  1 <= experts <=
+ * ggk_route_workspace(tokens, experts) bytes (0 for a few tokens) from a
+ * multiple of 16 on, written before they are read; calls that may overlap need one each.  1 <= experts <=
  * GGK_MOE_MAX_EXPERTS, 1 <= slots <= GGK_ROUTE_MAX_SLOTS and, without
  * given_ids, slots <= experts; tokens * slots <= GGK_ROUTE_MAX_TOTAL_SLOTS. */
 enum { GGK_TYPE_F32 = 0, GGK_TYPE_F16 = 1, GGK_TYPE_BF16 = 2 };

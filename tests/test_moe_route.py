@@ -136,6 +136,7 @@ def _route_args(**over):
     ({"counts": None}, 17), ({"order": None}, 17), ({"loss": 0x1000}, 17), ({"slope": 0x1000}, 17),
     ({"loss": 0x1000, "slope": 0x1000}, 0), ({"tokens": (1 << 29) + 1}, 1), ({"tokens": 1 << 29}, 0),
     ({"tokens": 1000, "workspace_bytes": 0}, 1), ({"tokens": 1000, "workspace": None}, 17),
+    ({"tokens": 1000, "workspace": 0x1008}, 1),
     ({"tokens": 0, "logits": None, "weights": None, "ids": None, "order": None}, 0)])
 def test_route_arguments_are_checked_on_the_host(over, status):
     assert _lib.lib().ggk_route_check(ctypes.byref(_route_args(**over))) == status

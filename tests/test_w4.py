@@ -8,6 +8,9 @@ no larger than S: at most n u S for a chain of n additions.  Sums here are made 
 terms by a few u: (K / 32 + 128) u S in all, and half a step of the output's type."""
 import ctypes
 import math
+import re
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -112,6 +115,54 @@ def test_refusals_of_the_torch_calls():
                                (t(6, dtype=torch.float32).requires_grad_(True), RuntimeError, "no gradient")]:
             with pytest.raises(error, match=text):
                 torch_ops.moe_w4_matmul(x, q3, s3, counts, order, row_weights=w)
+
+
+def test_matrix_results_are_read_behind_their_wait_states(tmp_path):
+    """A matrix instruction's result may be read by another kind of instruction 8 wait states later at the earliest.  The
+    compiler sees to it inside a basic block, but was seen to leave it out where a branch lies between (row tiles skipped
+    inside the loop over K gave wrong sums): in the built kernels no result is read, and no branch taken, before
+    that."""
+    root = Path(__file__).resolve().parents[1]
+    built = root / "grouped_gemm_gpu_kernel_amd" / "_build" / "gg_w4.o"
+    if not built.exists():
+        pytest.skip("no regular build in the tree (build first)")
+    llvm = Path("/opt/rocm/llvm/bin")
+    subprocess.run([str(llvm / "llvm-objcopy"), f"--dump-section=.hip_fatbin={tmp_path / 'fat'}", str(built),
+                    str(tmp_path / "copy.o")], check=True)
+    subprocess.run([str(llvm / "clang-offload-bundler"), "--unbundle", "--type=o",
+                    "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", f"--input={tmp_path / 'fat'}",
+                    f"--output={tmp_path / 'gfx950.o'}"], check=True)
+    text = subprocess.run([str(llvm / "llvm-objdump"), "-d", "--mcpu=gfx950", str(tmp_path / "gfx950.o")], check=True,
+                          capture_output=True, text=True).stdout
+    code = [line.split("//")[0].strip() for line in text.splitlines() if line.startswith("\t")]
+
+    def registers(operands):
+        found = set()
+        for first, last, one in re.findall(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b", operands):
+            found |= {int(one)} if one else set(range(int(first), int(last) + 1))
+        return found
+
+    bad, seen = [], 0
+    for i, line in enumerate(code):
+        if not line.startswith("v_mfma"):
+            continue
+        seen += 1
+        result, states = registers(line.split(",")[0]), 0
+        for after in code[i + 1:]:
+            if states >= 8:
+                break
+            kind = after.split()[0]
+            operands = after.split(",")
+            if kind.startswith("v_mfma"):
+                if result & registers(",".join(operands[1:3])):
+                    bad.append((line, after, states))
+                if result & registers(after):  # the next of a chain: checked as the one before
+                    break
+            elif result & registers(after) or kind.startswith(("s_cbranch", "s_branch", "s_setpc")):
+                bad.append((line, after, states))
+                break
+            states += int(after.split()[1], 0) + 1 if kind == "s_nop" else 1
+    assert seen > 100 and not bad, bad[:3]
 
 
 # ---------------------------------------------------------------- GPU
