@@ -32,6 +32,7 @@ typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 
 constexpr int kWave = 64;
 constexpr int kCus = 256;
+constexpr int kXcds = 8;  // neighbouring workgroups go to different ones, each with an L2 of its own
 constexpr int kStep = 128;  // values of k a wave takes at once: 16 bytes of each of 16 rows of q in 4 lanes
 
 // The 8 weights of a dword (nibble i: k + i) less a zero point, times 2^-9; minus_zero: the zero point times -2^-9.  An
@@ -200,25 +201,36 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
   const int my_column = lane / 4, my_piece = lane % 4;  // of the lane in a load
   const int steps = (a.k + kStep - 1) / kStep;
   const int turns = (steps + WK - 1) / WK;  // steps of a wave, at most
+  const int units = (turns + kDepth - 1) / kDepth;
+  // The turns are made in units of kDepth.  In step, the workgroups would all read the same lines of x at the same time,
+  // and rows a power of two apart lie in a few channels of the L2: where it costs nothing else, each begins with
+  // another unit and goes on around the end (64 rows of 8192 values, groups of 128: 25.2 us in step, 22.9 us so;
+  // groups of 64: 26.6 and 27.2, and experts' items begin at their own times as it is).
+  constexpr bool kTurned = !EXPERTS && !FINE;
+  int unit = kTurned ? (int)((blockIdx.x / kXcds % (kCus / kXcds)) * units / (kCus / kXcds)) : 0;
+  auto after = [&](int u) { return kTurned && u + 1 == units ? 0 : u + 1; };
 
-  // A chunk of x into its half of s.x, 512 values of a row an instruction; zeros past K by the resource's range check.
-  auto stage = [&](int chunk) {
+  // A chunk of x into half `half` of s.x, 512 values of a row an instruction; zeros past K by the resource's range
+  // check.  chunk: from the first turn on.
+  auto stage = [&](int chunk, int half) {
     constexpr int kLoads = kTurns * WK / 4;  // of a row
     static_assert(kTurns * WK % 4 == 0, "whole instructions a row");
     const int k0 = chunk * kTurns * WK * kStep;
 #pragma unroll
     for (int i = 0; i < (R * kLoads + kWaves - 1) / kWaves; ++i) {
       const int at = wave + i * kWaves, r = at / kLoads, k = k0 + at % kLoads * 512;
+      const int place = 2 * ((half * R + r) * kLength + at % kLoads * 512);  // in bytes
       if (r < t.rows && k < a.k) {
-        const _Float16* x = static_cast<const _Float16*>(a.x) + (EXPERTS ? __builtin_amdgcn_readfirstlane(s.x_row[r]) : t.first + r) * a.ldx + k;
-        gg::load_to_lds16(x, 2 * (a.k - k < 512 ? a.k - k : 512),
-                          gg::lds_address(s.x) + 2 * ((chunk % 2 * R + r) * kLength + at % kLoads * 512), 16 * lane, 0);
+        const _Float16* x = static_cast<const _Float16*>(a.x) +
+                            (EXPERTS ? __builtin_amdgcn_readfirstlane(s.x_row[r]) : t.first + r) * a.ldx + k;
+        gg::load_to_lds16(x, 2 * (a.k - k < 512 ? a.k - k : 512), gg::lds_address(s.x) + place, 16 * lane, 0);
       } else if (r < t.rows) {  // a chunk that K does not reach the end of
-        *reinterpret_cast<uint4v*>(s.x + 2 * ((chunk % 2 * R + r) * kLength + at % kLoads * 512) + 16 * lane) = uint4v{0, 0, 0, 0};
+        *reinterpret_cast<uint4v*>(s.x + place + 16 * lane) = uint4v{0, 0, 0, 0};
       }
     }
   };
-  stage(0);
+  constexpr int kChunks = kDepth / kTurns;  // of a unit
+  stage(unit * kChunks, 0);
 
   const long long j = min(column0 + my_column, a.n - 1);
   const unsigned char* q = a.q + t.expert * a.stride_q + j * a.ldq;
@@ -227,9 +239,20 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
   // Scale (low half) and zero point of the group that holds the lane's k, which goes from load to load in equal
   // strides: the group goes on by the whole groups of a stride, and one more where the rest has come to one.
   constexpr int kStride = (FINE ? 1 : kDepth) * WK * kStep;
-  int scale_k = FINE ? wk * kStep + 32 * my_piece : (my_piece * WK + wk) * kStep;  // below 2^12: the product below is exact
-  int group = (int)__umulhi((uint32_t)scale_k, l.group_inverse), rest = scale_k - group * a.group;
+  const int first_k = FINE ? wk * kStep + 32 * my_piece : (my_piece * WK + wk) * kStep;  // below 2^12: the product is exact
+  const int first_group = (int)__umulhi((uint32_t)first_k, l.group_inverse);
+  int scale_k = first_k, group = first_group, rest = first_k - first_group * a.group;
+  if (kTurned && unit > 0) {
+    scale_k += unit * kStride;
+    group = scale_k / a.group;
+    rest = scale_k - group * a.group;
+  }
   const int last_group = a.k / a.group - 1;
+  auto from_start = [&]() {
+    scale_k = first_k;
+    group = first_group;
+    rest = first_k - first_group * a.group;
+  };
   auto next_scale = [&]() {
     const int g = min(group, last_group);
     uint32_t v = *reinterpret_cast<const uint16_t*>(scales + g);
@@ -268,7 +291,7 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
   };
   if constexpr (!FINE) sz[0] = next_scale();
 #pragma unroll
-  for (int d = 0; d < kDepth; ++d) load(d, d);
+  for (int d = 0; d < kDepth; ++d) load(unit * kDepth + d, d);
 #pragma unroll
   for (int m = 0; m < M; ++m) sum[m] = float4v{};
   const unsigned char* x[M];  // the lane's rows in LDS
@@ -277,22 +300,28 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
     x[m] = s.x + 2 * (min(16 * m + column, R - 1) * kLength + wk * kStep + (FINE ? 8 : 32) * row);
   }
   uint4v v, g, four;
+  int next = units > 1 ? after(unit) : units;  // units: past the end, where loads repeat the last values
+  if (kTurned && next == 0) from_start();
   write(0);
-  load(kDepth, 0);
+  load(next * kDepth, 0);
   read(v, g);
-  for (int turn0 = 0; turn0 < turns; turn0 += kDepth) {
+  for (int done = 0; done < units; ++done) {
+    const int second = done + 2 < units ? after(next) : units;
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
-      const int turn = turn0 + d;
-      if (turn >= turns) break;
+      if (units == 1 && d >= turns) break;
+      const int half = kTurns == kDepth ? done % 2 : d / kTurns % 2;
       if (d % kTurns == 0) {
         // This chunk's loads are older than the weights' of the last kTurns steps; behind the barrier every wave's have
         // landed, and every wave is done with the chunk before, whose place the next one takes.
-        const int chunk = turn / kTurns;
         asm volatile("" ::: "memory");
         gg::wait_vmcnt<kTurns>();
         gg::stage_barrier();
-        if (turn + kTurns < turns) stage(chunk + 1);
+        if (d / kTurns + 1 < kChunks) {
+          stage(unit * kChunks + d / kTurns + 1, 1 - half);
+        } else if (done + 1 < units) {
+          stage(next * kChunks, 1 - half);
+        }
         if constexpr (FINE) asm volatile("" ::: "memory");
       }
       if constexpr (!FINE) {
@@ -300,11 +329,12 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
           s.sz[wave][my_column][my_piece] = sz[0];
           four = *reinterpret_cast<const uint4v*>(s.sz[wave][column]);
           sz[0] = next_scale();
+          if (kTurned && second == 0) from_start();
         }
       }
       uint4v next_v, next_g;
       write((d + 1) % kDepth);
-      load(turn + 1 + kDepth, (d + 1) % kDepth);
+      load(d + 1 < kDepth ? next * kDepth + d + 1 : second * kDepth, (d + 1) % kDepth);
       read(next_v, next_g);
       if constexpr (!FINE) g = uint4v{four[d], four[d], four[d], four[d]};
       half8v b[4];
@@ -317,7 +347,7 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
         }
         b[i] = unpack(v[i], minus_zero);
       }
-      const int at = 2 * ((turn / kTurns % 2) * R * kLength + turn % kTurns * WK * kStep);
+      const int at = 2 * (half * R * kLength + d % kTurns * WK * kStep);
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         float4v part = float4v{};
@@ -336,6 +366,8 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
       v = next_v;
       g = next_g;
     }
+    unit = next;
+    next = second;
   }
 }
 

@@ -207,6 +207,17 @@ def test_larger(torch_cuda, rows, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group", [128, 640, 64])
+@pytest.mark.parametrize("rows,n", [(3, 4200), (12, 2064), (9, 8500), (4, 24000), (40, 4100), (35, 24000)])
+def test_each_start_along_k(torch_cuda, rows, n, group):
+    """Columns enough that workgroups begin with every part of K, the last part not a whole one."""
+    k = 128 * 85
+    q, s, z = _weights((), n, k, group, rows % 2 == 0, n + group)
+    x = _x(rows, k, n)
+    check(torch_ops.w4_matmul(x, q, s, z), x.double(), values(q, s, z))
+
+
+@pytest.mark.gpu
 def test_strides_and_alignment(torch_cuda):
     """Column slices of wider x, scales and zeros at any offset, q by 16 bytes."""
     q, s, z = _weights((), 50, 512, 64, True, 4)
