@@ -50,6 +50,7 @@ GG_MOE_NOALLOC_SCRATCH_BYTES = 99840
 GGK_TYPE_F32, GGK_TYPE_F16, GGK_TYPE_BF16 = 0, 1, 2
 GGK_ROUTE_MAX_SLOTS = 64
 GGK_ROUTE_MAX_TOTAL_SLOTS = 1 << 30
+GGK_W4_MAX_EXTENT = 1 << 28
 
 c_int_p = ctypes.POINTER(ctypes.c_int)
 c_ll_p = ctypes.POINTER(ctypes.c_longlong)

@@ -28,7 +28,6 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
-typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 
 constexpr int kWave = 64;
 constexpr int kCus = 256;
@@ -500,7 +499,8 @@ hipError_t launch(const ggk_w4_args& a, hipStream_t stream) {
 extern "C" hipError_t ggk_w4_check(const ggk_w4_args* args) {
   if (args == nullptr) return hipErrorInvalidValue;
   const ggk_w4_args& a = *args;
-  if (a.rows < 0 || a.rows > GGK_ROUTE_MAX_TOTAL_SLOTS || a.x_rows < 0 || a.n < 0 || a.k < 1 || a.experts < 0 || a.experts > GGK_MOE_MAX_EXPERTS ||
+  if (a.rows < 0 || a.rows > GGK_ROUTE_MAX_TOTAL_SLOTS || a.x_rows < 0 || a.n < 0 || a.n > GGK_W4_MAX_EXTENT ||
+      a.k < 1 || a.k > GGK_W4_MAX_EXTENT || a.experts < 0 || a.experts > GGK_MOE_MAX_EXPERTS ||
       a.group < 32 || a.group % 32 != 0 || a.k % a.group != 0 || (a.y_type != GGK_TYPE_F32 && a.y_type != GGK_TYPE_F16)) {
     return hipErrorInvalidValue;
   }

@@ -253,7 +253,7 @@ py::object w4_call(const Tensor& x, const Tensor& q, const Tensor& scales, const
       return py::none();
     }
   }
-  if (rows > GGK_ROUTE_MAX_TOTAL_SLOTS || n > INT32_MAX || k > INT32_MAX) return py::none();
+  if (rows > GGK_ROUTE_MAX_TOTAL_SLOTS || n > GGK_W4_MAX_EXTENT || k > GGK_W4_MAX_EXTENT) return py::none();
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || scales.requires_grad() || (row_weights && row_weights->requires_grad()))) {
     return py::none();

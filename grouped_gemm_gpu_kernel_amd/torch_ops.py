@@ -404,8 +404,9 @@ def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optiona
     is none.
 
     weights and balance_loss carry gradients to logits (f_e counts as a constant).  Everything runs on the
-    current stream of the logits' device without waiting for it, and can be captured in a graph; the
-    same call gives the same bits.  E at most 1024, k at most 64."""
+    current stream of the logits' device without waiting for it, and can be captured in a graph (with its
+    backward pass, where no eager graph of the same leaves is alive, as for any backward pass); the same
+    call gives the same bits.  E at most 1024, k at most 64."""
     try:
         out = _binding().route(logits, top_k, ids, token_mask, normalize, scale, balance)
     except TypeError:  # an argument of another kind
@@ -493,6 +494,8 @@ def _check_w4(x, q, scales, zeros, counts, order, row_weights, out_dtype, lead=0
     groups = scales.shape[-1]
     if groups < 1 or k % groups != 0 or (k // groups) % 32 != 0 or k == 0:
         raise ValueError(f"scales has {groups} groups for K = {k}: a group is a multiple of 32 values that divides K")
+    if max(k, q.shape[-2]) > _lib.GGK_W4_MAX_EXTENT:
+        raise ValueError(f"q stands for [{q.shape[-2]}, {k}] weights: N and K are at most 2^28")
     if q.data_ptr() % 16 != 0 or any(n > 1 and s % 16 != 0 for n, s in zip(q.shape[:-1], q.stride()[:-1])):
         raise ValueError("q must start on a multiple of 16 bytes, and so must its rows and matrices")
     if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or
@@ -529,7 +532,7 @@ def moe_w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, counts
     Slots without an expert (the end of order, past the counts' sum) get zeros.  row_weights: float32, R
     entries (e.g. the routing's weights), 1 if not given.  Counts and order stay on the GPU and
     are not trusted: a negative count is taken as 0, counts past R and entries outside [0, R) are dropped;
-    rows that order does not name are left unwritten."""
+    rows that order does not name are left unwritten, and one that it names twice gets one of its products."""
     if counts is None or order is None:
         raise TypeError("counts and order must be torch.Tensors")
     return _w4(_check_moe_w4, x, q, scales, zeros, counts, order, row_weights, out_dtype)

@@ -450,8 +450,11 @@ hipError_t ggk_route_gradient(const ggk_route_gradient_args* args, hipStream_t s
  * o = order[r] reads x row o / (rows / x_rows) and writes y row o, times
  * row_weights[o] if given; slots past the counts' sum are set to 0.  Counts
  * are not trusted: a negative one is taken as 0, what goes past `rows` is
- * dropped, and an order entry outside [0, rows) is passed over.  rows <=
- * GGK_ROUTE_MAX_TOTAL_SLOTS. */
+ * dropped, and an order entry outside [0, rows) is passed over; what a
+ * slot named twice gets is one of its products.  rows <= GGK_ROUTE_MAX_TOTAL_SLOTS, n and k <=
+ * GGK_W4_MAX_EXTENT. */
+#define GGK_W4_MAX_EXTENT (1 << 28)
+
 typedef struct ggk_w4_args {
   int rows; /* of y */
   int x_rows;

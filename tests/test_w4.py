@@ -62,7 +62,9 @@ MOE = dict(experts=3, counts=0x1000, order=0x1000, stride_q=512, stride_s=16)
     ({"y": None}, 17), ({"rows": 0, "x_rows": 0, "x": None, "y": None}, 0), ({"n": 0, "q": None}, 0), (MOE, 0),
     ({**MOE, "rows": 8}, 0), ({**MOE, "rows": 7}, 1), ({**MOE, "x_rows": 0}, 1), ({**MOE, "counts": None}, 17),
     ({**MOE, "order": None}, 17), ({**MOE, "stride_q": 520}, 1), ({**MOE, "stride_q": -512}, 1),
-    ({**MOE, "experts": 1025}, 1), ({**MOE, "experts": -1}, 1)])
+    ({**MOE, "experts": 1025}, 1), ({**MOE, "experts": -1}, 1),
+    ({"n": (1 << 28) + 1}, 1), ({"k": (1 << 28) + 64, "ldx": 1 << 29, "ldq": 1 << 28, "lds": 1 << 23}, 1),
+    ({"n": 1 << 28, "k": 1 << 28, "ldx": 1 << 28, "ldq": 1 << 27, "lds": 1 << 22, "ldy": 1 << 28}, 0)])
 def test_arguments_are_checked_on_the_host(over, status):
     args = _lib.GGKW4Args(**{**BASE, **over})
     assert _lib.lib().ggk_w4_check(ctypes.byref(args)) == status
@@ -92,7 +94,9 @@ def test_refusals_of_the_torch_calls():
                 ((x, q.cpu(), s), ValueError, "q is on"), ((x, t(64, 6, dtype=torch.uint8).t(), s), ValueError, "contiguous"),
                 ((x, t(6, 72, dtype=torch.uint8)[:, :64], s), ValueError, "16 bytes"),
                 ((x, t(1, 64, dtype=torch.uint8).expand(6, 64), s), ValueError, "overlap"),
-                ((x, t(2, 6, 64, dtype=torch.uint8), s), ValueError, "dimensions")]:
+                ((x, t(2, 6, 64, dtype=torch.uint8), s), ValueError, "dimensions"),
+                ((x, t((1 << 28) + 1, 64, dtype=torch.uint8), t((1 << 28) + 1, 2)), ValueError, "at most"),
+                ((t(1, (1 << 28) + 64), t(1, (1 << 27) + 32, dtype=torch.uint8), t(1, 1)), ValueError, "at most")]:
             with pytest.raises(error, match=text):
                 torch_ops.w4_matmul(*bad)
         with pytest.raises(TypeError, match="out_dtype"):
