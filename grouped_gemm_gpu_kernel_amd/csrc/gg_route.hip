@@ -211,7 +211,8 @@ struct Workspace {
 __host__ __device__ inline int count_pitch(int experts) { return (experts + 4) / 4 * 4; }
 
 // At most this many entries of `count` are summed by every block of the order kernel itself: with 64 experts and
-// 16384 tokens, two launches of 256 blocks instead of three of 512.
+// 16384 tokens, two launches of 256 blocks, 10.2 us, instead of three of 512, 11.6.  With 128 experts and 8192 tokens
+// (32 K entries) it took 15.0 us, against 12.9 with the columns kernel.
 constexpr int kMaxOwnSums = 20 * 1024;
 constexpr int kMaxBlocks = 512;
 
@@ -492,6 +493,8 @@ __device__ __forceinline__ void block_sums(float (&sums)[V], int experts, float*
   }
 }
 
+// The tokens of one block: choice, weights, counts and sums of p.  65521 tokens of 256 float logits, 8 slots, loss: 37 us
+// for 67 MB, bound by vector instructions (985 a wave for its 4 tokens, 26 us); 16384 of 64: 4.7 us, start and latency.
 template <class T, int L, int V>
 __global__ __launch_bounds__(kThreads, 4) void route_rows_kernel(ggk_route_args a, Workspace ws, Plan plan) {
   extern __shared__ int shared[];  // counts [experts + 1], routed, then (balance) `experts` floats a wave
@@ -518,7 +521,8 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows_kernel(ggk_route_args 
 }
 
 // Sums over the blocks, kColumns columns a workgroup: each column's slices of blocks are added up, then the
-// counts become the sums over the blocks before, the totals go to a.counts, and the sums of p to block 0's.
+// counts become the sums over the blocks before, the totals go to a.counts, and the sums of p to block 0's.  5 us for
+// 512 blocks of 256 experts.
 constexpr int kColumns = 16;
 constexpr int kSlices = kThreads / kColumns;
 
@@ -605,13 +609,8 @@ __device__ __forceinline__ void add_experts_before(int* s_at, const int* total, 
   __syncthreads();
 }
 
-// Places slots [first, last) by expert, in their own order within one.  s_at: the next place of each expert;
-// s_wave: experts + 1 ints a wave; id0: this lane's first id, loaded before the counts were known.  Every wave takes a run of slots, 64 at a time: it counts its slots of
-// each expert, the waves' counts become their first places, and a slot goes to its wave's next place plus the number of
-// lanes below with the same expert.  Waves write only their own row of s_wave.
-// Waves write only their own row of s_wave.
 struct Run {
-  long long begin, end;  // of the wave's slots
+  long long begin, end;  // a wave's slots
 };
 
 template <int THREADS>
@@ -622,6 +621,11 @@ __device__ __forceinline__ Run run_of_wave(long long first, long long last) {
   return {begin, min(last, begin + each)};
 }
 
+// Places the workgroup's slots by expert, in their own order within one.  s_at: the next place of each expert; s_wave:
+// experts + 1 ints a wave; id0: this lane's first id, loaded before the counts were known.  Every wave takes its run
+// of slots, 64 at a time: it counts its slots of each expert, the waves' counts become their first places, and a slot
+// goes to its wave's next place plus the number of lanes below with the same expert.  Waves write only their own row
+// of s_wave.
 template <int THREADS>
 __device__ __forceinline__ void place_slots(const ggk_route_args& a, const Run& run, int id0, const int* s_at,
                                             int* s_wave) {
@@ -695,7 +699,8 @@ __device__ __forceinline__ int all_routed(const Workspace& ws, int blocks) {
 }
 
 // The order of one block's slots; one more block computes the loss.  Without the columns kernel every block adds up
-// the counts of all blocks itself, and the last one the sums of p.
+// the counts of all blocks itself, and the last one the sums of p.  6.2 us for 16384 tokens of 2 slots on 64 experts, 9.8
+// for 65521 of 8 on 256: latency of a few dependent passes, not bytes.
 __global__ __launch_bounds__(kThreads) void route_order_kernel(ggk_route_args a, Workspace ws, Plan plan) {
   extern __shared__ int shared[];  // s_at, s_total [experts + 1] each, then s_wave
   __shared__ int s_waves[kThreads / kWave];
@@ -814,6 +819,10 @@ __global__ __launch_bounds__(kSmallThreads) void route_small_kernel(ggk_route_ar
 template <int L, int V>
 constexpr bool kRowInLds = V >= 8;
 
+// The formulas: with a the chosen weights over scale, g = scale * dw, c_e = d_loss * slope_e and p the softmax,
+//   dz_e = p_e (c_e - sum_j p_j c_j)   and   normalize: + a_s (g_s - sum_j a_j g_j) at the chosen
+//                                            else:      + p_e (g_e - sum_j p_j g_j), g 0 where not chosen.
+// 65521 tokens of 256 float logits: 32 us for 138 MB, near the rate of a copy.
 template <class T, int L, int V>
 __global__ __launch_bounds__(kThreads) void route_gradient_kernel(ggk_route_gradient_args a, bool vectors) {
   using Z = Logit<T>;
@@ -1039,7 +1048,8 @@ extern "C" hipError_t ggk_route_check(const ggk_route_args* args) {
   if (a.workspace_bytes < ggk_route_workspace(a.tokens, a.experts) || reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) {
     return hipErrorInvalidValue;
   }
-  if (a.counts == nullptr || (a.workspace == nullptr && !is_small(a.tokens, a.experts)) || (a.loss == nullptr) != (a.slope == nullptr) ||
+  if (a.counts == nullptr || (a.workspace == nullptr && !is_small(a.tokens, a.experts)) ||
+      (a.loss == nullptr) != (a.slope == nullptr) ||
       (a.tokens > 0 && (a.logits == nullptr || a.weights == nullptr || a.ids == nullptr || a.order == nullptr))) {
     return hipErrorInvalidDevicePointer;
   }
