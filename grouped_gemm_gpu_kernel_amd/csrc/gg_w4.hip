@@ -14,8 +14,9 @@
 // registers, four steps ahead, then written to the wave's own LDS and read back in the instruction's order.  x is
 // loaded by the workgroup straight into LDS, a chunk of K ahead.
 //
-// A workgroup of 8 waves computes 16 (8 / WK) columns of up to R rows: WK waves split K among them, step by step, so
-// that a narrow matrix still gives every CU loads to wait for, and their sums are joined in LDS in the waves' order.
+// A workgroup of 8 or 16 waves computes 16 columns for each WK of them, of up to R rows: WK waves split K among them, step
+// by step, so that a narrow matrix still gives every CU loads to wait for, and their sums are joined in LDS in the
+// waves' order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -147,8 +148,8 @@ __device__ RowTile expert_tile(const ggk_w4_args& a, const Table& s, int tile) {
   return t;
 }
 
-constexpr int kWaves = 8;
-constexpr int kThreads = kWaves * kWave;
+constexpr int kWaves = 8;       // of a workgroup, two on a CU,
+constexpr int kManyWaves = 16;  // or of one on a CU
 constexpr int kDepth = 4;  // steps of weights a wave has in flight
 
 // Steps of every wave that a chunk of x holds: four, less where two chunks of R rows would not fit 64 KB (32 KB beside
@@ -166,10 +167,10 @@ template <int R, int WK, bool EXPERTS>
 constexpr int kRowLength = kChunk<R, WK, EXPERTS> * WK * kStep + 8;
 
 // Bytes of two chunks of x, or of the waves' sums at the end.
-template <int R, int WK, bool EXPERTS>
-constexpr int kXBytes = 4 * R * kRowLength<R, WK, EXPERTS> > kWaves * (R < 16 ? 16 : R) * 64
+template <int WAVES, int R, int WK, bool EXPERTS>
+constexpr int kXBytes = 4 * R * kRowLength<R, WK, EXPERTS> > WAVES * (R < 16 ? 16 : R) * 64
                             ? 4 * R * kRowLength<R, WK, EXPERTS>
-                            : kWaves * (R < 16 ? 16 : R) * 64;
+                            : WAVES * (R < 16 ? 16 : R) * 64;
 
 // What a workgroup keeps in LDS: pointers to arrays of their own, so that accesses to one may pass those to another.
 struct Shared {
@@ -189,7 +190,7 @@ __device__ __forceinline__ int piece(int column, int p) { return column * 64 + (
 // each instruction's 32 values lie in one; else a step lies in one group.  Every load of weights is made without a
 // condition, past K too (there it reads the row's last values, with a scale of 0): the waits before a load's use
 // are counted in the loads made since, and a load that may not have been made does not count.
-template <int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
+template <int WAVES, int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
 __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t, int column0, const Shared& s,
                                               float4v (&sum)[(R + 15) / 16]) {
   const ggk_w4_args& a = l.a;
@@ -206,6 +207,10 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
   // another unit and goes on around the end (64 rows of 8192 values, groups of 128: 25.2 us in step, 22.9 us so;
   // groups of 64: 26.6 and 27.2, and experts' items begin at their own times as it is).
   constexpr bool kTurned = !EXPERTS && !FINE;
+  // The wait for the next step's weights also waits for what was loaded before their last kDepth - 1 loads; ahead of the
+  // chunk's loads it waits for fewer of those (64 rows of 8192, groups of 64: 24.1 instead of 25.1 us).  With fewer rows
+  // it gains nothing, and experts lose 1%.
+  constexpr bool kWriteFirst = WAVES > kWaves;
   int unit = kTurned ? (int)((blockIdx.x / kXcds % (kCus / kXcds)) * units / (kCus / kXcds)) : 0;
   auto after = [&](int u) { return kTurned && u + 1 == units ? 0 : u + 1; };
 
@@ -216,8 +221,8 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
     static_assert(kTurns * WK % 4 == 0, "whole instructions a row");
     const int k0 = chunk * kTurns * WK * kStep;
 #pragma unroll
-    for (int i = 0; i < (R * kLoads + kWaves - 1) / kWaves; ++i) {
-      const int at = wave + i * kWaves, r = at / kLoads, k = k0 + at % kLoads * 512;
+    for (int i = 0; i < (R * kLoads + WAVES - 1) / WAVES; ++i) {
+      const int at = wave + i * WAVES, r = at / kLoads, k = k0 + at % kLoads * 512;
       const int place = 2 * ((half * R + r) * kLength + at % kLoads * 512);  // in bytes
       if (r < t.rows && k < a.k) {
         const _Float16* x = static_cast<const _Float16*>(a.x) +
@@ -309,6 +314,7 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       if (units == 1 && d >= turns) break;
+      if constexpr (kWriteFirst) write((d + 1) % kDepth);
       const int half = kTurns == kDepth ? done % 2 : d / kTurns % 2;
       if (d % kTurns == 0) {
         // This chunk's loads are older than the weights' of the last kTurns steps; behind the barrier every wave's have
@@ -332,7 +338,7 @@ __device__ __forceinline__ void multiply_item(const Launch& l, const RowTile& t,
         }
       }
       uint4v next_v, next_g;
-      write((d + 1) % kDepth);
+      if constexpr (!kWriteFirst) write((d + 1) % kDepth);
       load(d + 1 < kDepth ? next * kDepth + d + 1 : second * kDepth, (d + 1) % kDepth);
       read(next_v, next_g);
       if constexpr (!FINE) g = uint4v{four[d], four[d], four[d], four[d]};
@@ -380,14 +386,14 @@ __device__ __forceinline__ void store_y(const ggk_w4_args& a, int slot, int j, f
 }
 
 // One tile of rows by the workgroup's columns from block0 on: sums, their join over the waves that split K, y.
-template <int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
+template <int WAVES, int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
 __device__ __forceinline__ void run_item(const Launch& l, const RowTile& t, int block0, const Shared& s) {
   const ggk_w4_args& a = l.a;
-  constexpr int M = (R + 15) / 16, kColumns = 16 * (kWaves / WK);
+  constexpr int M = (R + 15) / 16, kColumns = 16 * (WAVES / WK);
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int column = lane % 16, row = lane / 16, wn = wave / WK, wk = wave % WK;
   float4v sum[M];
-  multiply_item<R, WK, EXPERTS, FINE, ZEROS>(l, t, block0 + wn * 16, s, sum);
+  multiply_item<WAVES, R, WK, EXPERTS, FINE, ZEROS>(l, t, block0 + wn * 16, s, sum);
   float* s_sum = reinterpret_cast<float*>(s.x);  // [WK][16 M][kColumns]
   gg::stage_barrier();
 #pragma unroll
@@ -396,7 +402,7 @@ __device__ __forceinline__ void run_item(const Launch& l, const RowTile& t, int 
     for (int i = 0; i < 4; ++i) s_sum[(wk * 16 * M + 16 * m + 4 * row + i) * kColumns + 16 * wn + column] = sum[m][i];
   }
   gg::stage_barrier();
-  for (int i = tid; i < t.rows * kColumns; i += kThreads) {
+  for (int i = tid; i < t.rows * kColumns; i += WAVES * kWave) {
     const int r = i / kColumns, c = i % kColumns, j = block0 + c, slot = EXPERTS ? s.slot[r] : t.first + r;
     if (j < a.n && slot >= 0) {
       float y = 0.0f;
@@ -409,25 +415,26 @@ __device__ __forceinline__ void run_item(const Launch& l, const RowTile& t, int 
   }
 }
 
-// R: rows of an item, at most.  Measured, among others: one row of 4096 by 14336 columns, 30 MB, 10 us, of which the
-// workgroups' start is 3.2 and the rest runs at 4.4 TB/s, from the cache at 5.7; 64 experts' matrices of that size,
+// R: rows of an item, at most.  Measured, among others: one row of 4096 by 14336 columns, 30 MB, 9.4 us, of which the
+// workgroups' start is 3.2 and the rest runs at 4.9 TB/s, from the cache at 5.7; 64 experts' matrices of that size,
 // 256 slots on 46 of them, 1.4 GB, 312 us (4.5 TB/s, where a sum over 4 GB reads 4.0); 64 rows of 8192 by 8192 with
-// groups of 64, 27 us: 22 without the loads of x, 25 without unpacking, 26 without reading x from LDS, 3.6 in the
-// matrix instructions alone: the parts overlap badly with a barrier every 512 values of K, none bounds it by itself.
-template <int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
-__global__ __launch_bounds__(kThreads, 4) void w4_kernel(Launch l) {
+// groups of 64, 24 us; by 8 waves it took 27, and 22 without the loads of x, 25 without unpacking, 26 without reading x
+// from LDS, 3.6 in the matrix instructions alone: the parts overlap badly with a barrier every 512 values of K, and
+// sharing x among more columns took off most.
+template <int WAVES, int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
+__global__ __launch_bounds__(WAVES * kWave, 4) void w4_kernel(Launch l) {
   const ggk_w4_args& a = l.a;
-  constexpr int kColumns = 16 * (kWaves / WK);
-  __shared__ alignas(16) unsigned char s_x[kXBytes<R, WK, EXPERTS>];
-  __shared__ alignas(16) unsigned char s_w[kWaves][16 * 64];
-  __shared__ alignas(16) uint32_t s_sz[kWaves][16][4];
+  constexpr int kColumns = 16 * (WAVES / WK);
+  __shared__ alignas(16) unsigned char s_x[kXBytes<WAVES, R, WK, EXPERTS>];
+  __shared__ alignas(16) unsigned char s_w[WAVES][16 * 64];
+  __shared__ alignas(16) uint32_t s_sz[WAVES][16][4];
   const int tid = threadIdx.x;
   if constexpr (!EXPERTS) {
     const Shared s{s_x, s_w, s_sz, nullptr, nullptr};
     const int tiles = (a.rows + R - 1) / R;
     for (int tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
       const RowTile t{0, tile * R, min(R, a.rows - tile * R)};
-      run_item<R, WK, false, FINE, ZEROS>(l, t, blockIdx.x * kColumns, s);
+      run_item<WAVES, R, WK, false, FINE, ZEROS>(l, t, blockIdx.x * kColumns, s);
       gg::stage_barrier();
     }
   } else {
@@ -435,12 +442,12 @@ __global__ __launch_bounds__(kThreads, 4) void w4_kernel(Launch l) {
     __shared__ Experts<kTable<R>> s_experts;
     const Shared s{s_x, s_w, s_sz, s_slot, s_x_row};
     const int fan = a.rows / a.x_rows;
-    list_experts<kThreads, R>(a, s_experts);
+    list_experts<WAVES * kWave, R>(a, s_experts);
     const int tiles = s_experts.tile[a.experts + 1];
     int tile = blockIdx.x / l.blocks, block = blockIdx.x % l.blocks;
     while (tile < tiles) {
       const RowTile t = expert_tile<R>(a, s_experts, tile);
-      for (int i = tid; i < t.rows; i += kThreads) {
+      for (int i = tid; i < t.rows; i += WAVES * kWave) {
         int slot = a.order[t.first + i];
         if (slot >= a.rows) slot = -1;
         s.slot[i] = slot;
@@ -448,18 +455,18 @@ __global__ __launch_bounds__(kThreads, 4) void w4_kernel(Launch l) {
       }
       gg::stage_barrier();
       if (t.expert == a.experts) {
-        for (int i = tid; i < t.rows * kColumns; i += kThreads) {
+        for (int i = tid; i < t.rows * kColumns; i += WAVES * kWave) {
           const int slot = s.slot[i / kColumns], j = block * kColumns + i % kColumns;
           if (j < a.n && slot >= 0) store_y(a, slot, j, 0.0f);
         }
       } else if (R > 4 && t.rows <= 4) {
         // The rows are a constant of the whole loop over K: the compiler leaves out the wait between a matrix
         // instruction and the use of its result when a branch on them lies between.
-        run_item<4, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
+        run_item<WAVES, 4, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
       } else if (R > 16 && t.rows <= 16) {
-        run_item<16, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
+        run_item<WAVES, 16, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
       } else {
-        run_item<R, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
+        run_item<WAVES, R, WK, true, FINE, ZEROS>(l, t, block * kColumns, s);
       }
       gg::stage_barrier();
       tile += l.stride_tiles;
@@ -472,13 +479,14 @@ __global__ __launch_bounds__(kThreads, 4) void w4_kernel(Launch l) {
   }
 }
 
-template <int R, int WK, bool EXPERTS>
+template <int R, int WK, bool EXPERTS, int WAVES = kWaves>
 hipError_t launch(const ggk_w4_args& a, hipStream_t stream) {
   if (EXPERTS && a.experts > kTable<R>) return hipErrorInvalidValue;
   const bool fine = a.group % kStep != 0;
-  auto kernel = fine ? (a.zeros != nullptr ? w4_kernel<R, WK, EXPERTS, true, true> : w4_kernel<R, WK, EXPERTS, true, false>)
-                     : (a.zeros != nullptr ? w4_kernel<R, WK, EXPERTS, false, true> : w4_kernel<R, WK, EXPERTS, false, false>);
-  constexpr int kColumns = 16 * (kWaves / WK);
+  auto with_zeros = fine ? w4_kernel<WAVES, R, WK, EXPERTS, true, true> : w4_kernel<WAVES, R, WK, EXPERTS, false, true>;
+  auto without = fine ? w4_kernel<WAVES, R, WK, EXPERTS, true, false> : w4_kernel<WAVES, R, WK, EXPERTS, false, false>;
+  auto kernel = a.zeros != nullptr ? with_zeros : without;
+  constexpr int kColumns = 16 * (WAVES / WK);
   const int stride = (fine ? 1 : kDepth) * WK * kStep;
   Launch l{};
   l.a = a;
@@ -494,7 +502,7 @@ hipError_t launch(const ggk_w4_args& a, hipStream_t stream) {
     l.stride_tiles = (int)grid.x / l.blocks;
     l.stride_blocks = (int)grid.x % l.blocks;
   }
-  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, l);
+  hipLaunchKernelGGL(kernel, grid, dim3(WAVES * kWave), 0, stream, l);
   return hipGetLastError();
 }
 
@@ -533,21 +541,33 @@ extern "C" hipError_t ggk_w4_multiply(const ggk_w4_args* args, hipStream_t strea
   const hipError_t st = ggk_w4_check(args);
   if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
   const ggk_w4_args& a = *args;
-  // Waves that split K, by the waves there would be without: 8192 fill the GPU, and more than about 3000 only add the
-  // fixed cost of a workgroup (3.2 us for 224 of them, 6.5 for 896) to a launch of a few microseconds.
   const long long columns = (a.n + 15) / 16;
   if (a.experts > 0) {
+    // Waves that split K, where there are few without.
     const long long waves = columns * min(a.rows, a.experts);
     if (waves >= 1024 && a.experts <= kTable<32>) return launch<32, 1, true>(a, stream);
     if (waves >= 512) return waves >= 1024 ? launch<16, 1, true>(a, stream) : launch<16, 2, true>(a, stream);
     return launch<16, 4, true>(a, stream);
   }
+  // The form by what the busiest CU gets: its workgroups, each with its columns and a fixed cost as of `fixed` columns.
+  const long long tiles = a.rows > 16 ? (a.rows + 31) / 32 : 1;
+  const int fixed = a.rows > 16 ? 32 : 8;
+  auto cost = [&](int width) {
+    const long long workgroups = (a.n + width - 1) / width * tiles;
+    return (workgroups + kCus - 1) / kCus * (width + fixed);
+  };
   if (a.rows > 16) {
-    const long long waves = columns * ((a.rows + 31) / 32);
-    return waves > 1344 ? launch<32, 2, false>(a, stream) : launch<32, 4, false>(a, stream);
+    // us of the three, narrow to wide: 40 rows of 2048 by 2048 6.2, 7.4, 10.2; 64 of 8192 by 8192 28, 24, 38; 64 of 4096
+    // by 14336 26, 24, 18; 90 of 4096 by 8192 21, 23, 18.
+    const long long narrow = cost(32), wide = cost(64), widest = cost(128);
+    if (widest <= wide && widest <= narrow) return launch<32, 2, false, kManyWaves>(a, stream);
+    return wide <= narrow ? launch<32, 4, false, kManyWaves>(a, stream) : launch<32, 4, false>(a, stream);
   }
+  // us: one row of 4096 by 8192 in workgroups of 32 and 64 columns 6.8, 8.8, by 14336 10.0, 9.4, by 20480 13.1, 13.4;
+  // 13 rows of 4096 by 6400 in 16, 32 and 64 8.7, 7.7, 9.9, by 10240 12.3, 10.6, 10.0, by 28672 23.7, 19.4, 15.9.
   const bool few = a.rows <= 4;
-  if (columns <= 384) return few ? launch<4, 8, false>(a, stream) : launch<16, 8, false>(a, stream);
-  if (columns <= 1344) return few ? launch<4, 4, false>(a, stream) : launch<16, 4, false>(a, stream);
-  return few ? launch<4, 2, false>(a, stream) : launch<16, 2, false>(a, stream);
+  const long long narrow = cost(16), wide = cost(32), widest = cost(64);
+  if (widest <= wide && widest <= narrow) return few ? launch<4, 2, false>(a, stream) : launch<16, 2, false>(a, stream);
+  if (wide <= narrow) return few ? launch<4, 4, false>(a, stream) : launch<16, 4, false>(a, stream);
+  return few ? launch<4, 8, false>(a, stream) : launch<16, 8, false>(a, stream);
 }

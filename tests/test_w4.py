@@ -212,7 +212,7 @@ def test_larger(torch_cuda, rows, n, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("group", [128, 640, 64])
-@pytest.mark.parametrize("rows,n", [(3, 4200), (12, 2064), (9, 8500), (4, 24000), (40, 4100), (35, 24000)])
+@pytest.mark.parametrize("rows,n", [(3, 4200), (12, 2064), (9, 8500), (4, 24000), (40, 4100), (35, 24000), (50, 14300)])
 def test_each_start_along_k(torch_cuda, rows, n, group):
     """Columns enough that workgroups begin with every part of K, the last part not a whole one."""
     k = 128 * 85
@@ -285,6 +285,19 @@ def test_sums_of_integers_are_exact(torch_cuda, rows, group):
     assert torch.equal(torch_ops.w4_matmul(x, q, s, z).double(), want)
     want = x.double() @ values(q, s).t()
     assert torch.equal(torch_ops.w4_matmul(x, q, s).double(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(2, 2000), (2, 8000), (2, 14300), (9, 2000), (9, 6400), (9, 14300), (33, 2000),
+                                    (40, 4100), (50, 14300)])
+@pytest.mark.parametrize("group", [64, 128])
+def test_each_width_is_exact(torch_cuda, rows, n, group):
+    """The same for narrow and wide matrices, whose workgroups take other numbers of columns."""
+    q, s, _ = _weights((), n, 1408, group, False, 19)
+    s.fill_(1.0)
+    x = torch.randint(-1, 2, (rows, 1408), generator=torch.Generator().manual_seed(20)).half().cuda()
+    x[:, 7::512] = 2048.0
+    assert torch.equal(torch_ops.w4_matmul(x, q, s).double(), x.double() @ values(q, s).t())
 
 
 @pytest.mark.gpu
