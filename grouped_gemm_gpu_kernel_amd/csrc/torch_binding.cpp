@@ -13,10 +13,14 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
+#include <unordered_set>
+#include <vector>
 
 #include "grouped_gemm_amd_kernels.h"
 
@@ -139,6 +143,30 @@ RouteOutputs route(const RouteCall& c) {
   return o;
 }
 
+bool is_capturing(c10::Device device) {
+  const c10::OptionalDeviceGuard guard(device);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device.index()).stream(), &status) == hipSuccess &&
+         status != hipStreamCaptureStatusNone;
+}
+
+// Does the backward pass go on from `node` to a leaf whose gradient belongs to the default stream?
+bool reaches_default_stream(const torch::autograd::Node* node) {
+  std::vector<const torch::autograd::Node*> left{node};
+  std::unordered_set<const torch::autograd::Node*> seen;
+  while (!left.empty()) {
+    const torch::autograd::Node* at = left.back();
+    left.pop_back();
+    if (at == nullptr || !seen.insert(at).second) continue;
+    if (auto* leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(at)) {
+      const auto stream = const_cast<torch::autograd::AccumulateGrad*>(leaf)->stream();
+      if (stream && stream->id() == 0) return true;
+    }
+    for (const auto& edge : at->next_edges()) left.push_back(edge.function.get());
+  }
+  return false;
+}
+
 struct Route : torch::autograd::Function<Route> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const RouteCall& c) {
     RouteOutputs o = route(c);
@@ -159,6 +187,10 @@ struct Route : torch::autograd::Function<Route> {
     const Tensor &z = saved[0], &ids = saved[1], &slope = saved[2];
     const Tensor d_loss = grads.size() > 4 ? grads[4] : Tensor();
     if (!grads[0].defined() && !d_loss.defined()) return {Tensor(), Tensor()};
+    // The engine would join the leaf's stream to the capture, which for the default stream ends the process.
+    TORCH_CHECK(!is_capturing(z.device()) || !reaches_default_stream(torch::autograd::get_current_node().get()),
+                "moe_route: a backward pass is being captured while an eager graph of the same leaves, made on the default "
+                "stream, is alive: free it first, or make it on a side stream");
     // The weights' gradient may come expanded (a sum's) or in any strides.
     const Tensor d_weights = grads[0].defined() ? grads[0].contiguous() : Tensor();
     Tensor d = at::empty({z.size(0), z.size(1)}, z.options().requires_grad(false));

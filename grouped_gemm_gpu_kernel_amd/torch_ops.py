@@ -404,9 +404,9 @@ def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optiona
     is none.
 
     weights and balance_loss carry gradients to logits (f_e counts as a constant).  Everything runs on the
-    current stream of the logits' device without waiting for it, and can be captured in a graph (with its
-    backward pass, where no eager graph of the same leaves is alive, as for any backward pass); the same
-    call gives the same bits.  E at most 1024, k at most 64."""
+    current stream of the logits' device without waiting for it, and can be captured in a graph (its
+    backward pass too, unless an eager graph of the same leaves made on the default stream is alive, which is
+    refused); the same call gives the same bits.  E at most 1024, k at most 64."""
     try:
         out = _binding().route(logits, top_k, ids, token_mask, normalize, scale, balance)
     except TypeError:  # an argument of another kind

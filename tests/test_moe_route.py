@@ -502,6 +502,32 @@ def test_streams_and_two_calls_at_once(torch_cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("leaf", [True, False])
+def test_capture_with_an_eager_graph_alive_is_refused(torch_cuda, leaf):
+    """The leaf's gradient belongs to the default stream while an eager graph made there lives."""
+    z = _logits(300, 16, "f32", 0).requires_grad_(True)
+
+    def forward():
+        return torch_ops.moe_route(z if leaf else z * 2.0, 2, balance=True)
+
+    alive = forward()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(forward().balance_loss, z)
+    torch.cuda.synchronize()
+    del graph
+    want, = torch.autograd.grad(alive.balance_loss, z)  # eager calls go on as before
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(forward().balance_loss, z)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_captured_and_replayed(torch_cuda):
     """Forward and backward in a graph, replayed with new logits between the program's own calls."""
     static = _logits(700, 48, "f32", 0).requires_grad_(True)
