@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -58,6 +59,9 @@ bool vector_in_order(const Tensor& t, at::ScalarType type, int64_t count, c10::D
   return t.scalar_type() == type && t.device() == device && t.numel() == count && t.is_contiguous();
 }
 
+// A tangent of forward-mode differentiation: a dual tensor does not have to require a gradient.
+bool has_tangent(const Tensor& t) { return torch::autograd::isFwGradDefined(t); }
+
 template <class Args>
 int launch(hipError_t (*entry)(const Args*, hipStream_t), const Args& args, c10::Device device) {
   const c10::OptionalDeviceGuard guard(device);
@@ -82,7 +86,7 @@ struct RouteOutputs {
 
 bool route_in_order(const RouteCall& c) {
   const Tensor& z = c.logits;
-  if (!z.is_cuda() || type_of(z.scalar_type()) < 0 || !matrix_in_order(z)) return false;
+  if (!z.is_cuda() || type_of(z.scalar_type()) < 0 || !matrix_in_order(z) || has_tangent(z)) return false;
   const int64_t tokens = z.size(0), experts = z.size(1);
   if (experts < 1 || experts > GGK_MOE_MAX_EXPERTS || c.slots < 1 || c.slots > GGK_ROUTE_MAX_SLOTS ||
       (!c.ids && c.slots > experts) || tokens > GGK_ROUTE_MAX_TOTAL_SLOTS / c.slots) {
@@ -187,6 +191,8 @@ struct Route : torch::autograd::Function<Route> {
     const Tensor &z = saved[0], &ids = saved[1], &slope = saved[2];
     const Tensor d_loss = grads.size() > 4 ? grads[4] : Tensor();
     if (!grads[0].defined() && !d_loss.defined()) return {Tensor(), Tensor()};
+    TORCH_CHECK(!has_tangent(grads[0]) && !has_tangent(d_loss),
+                "moe_route's gradient has no forward-mode derivative: it was given a dual tensor");
     // The engine would join the leaf's stream to the capture, which for the default stream ends the process.
     TORCH_CHECK(!is_capturing(z.device()) || !reaches_default_stream(torch::autograd::get_current_node().get()),
                 "moe_route: a backward pass is being captured while an eager graph of the same leaves, made on the default "

@@ -382,6 +382,12 @@ def _check_vector(t: torch.Tensor, name: str, dtype: torch.dtype, count: int, de
         raise ValueError(f"{name} must be contiguous")
 
 
+def _check_no_tangent(what: str, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} no forward-mode derivative: {name} is a dual tensor (take its primal)")
+
+
 def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optional[torch.Tensor] = None,
               token_mask: Optional[torch.Tensor] = None, normalize: bool = True, scale: float = 1.0,
               balance: bool = False) -> Routing:
@@ -403,7 +409,8 @@ def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optiona
     counted slots and P_e the mean of softmax(logits)[:, e] over the tokens with an expert; 0 if there
     is none.
 
-    weights and balance_loss carry gradients to logits (f_e counts as a constant).  Everything runs on the
+    weights and balance_loss carry gradients to logits (f_e counts as a constant; no second derivative, and no
+    forward-mode one: dual tensors are refused).  Everything runs on the
     current stream of the logits' device without waiting for it, and can be captured in a graph (its
     backward pass too, unless an eager graph of the same leaves made on the default stream is alive, which is
     refused); the same call gives the same bits.  E at most 1024, k at most 64."""
@@ -451,6 +458,7 @@ def _check_route(logits, top_k, ids, token_mask) -> None:
         raise ValueError(f"{tokens} tokens with {slots} slots each: more than 2^30 slots")
     if token_mask is not None:
         _check_vector(token_mask, "token_mask", torch.bool, tokens, logits.device)
+    _check_no_tangent("moe_route has", logits=logits)
 
 
 # ---------------------------------------------------------------- 4-bit weights

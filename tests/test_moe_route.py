@@ -195,6 +195,23 @@ def test_refusals_of_the_torch_call():
             torch_ops.moe_route(logits((1 << 27) + 1, 8), 8)
 
 
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_derivatives_are_refused(requires_grad):
+    """A dual tensor does not require a gradient by itself; its tangent would be lost without a word."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+
+    with FakeTensorMode(), forward_ad.dual_level():
+        z = torch.empty(6, 8, device="cuda:0")
+        dual = forward_ad.make_dual(z.requires_grad_(requires_grad), torch.empty(6, 8, device="cuda:0"))
+        ids = torch.empty(6, 2, dtype=torch.int32, device="cuda:0")
+        for arguments in ({"top_k": 2}, {"top_k": 2, "balance": True}, {"ids": ids}):
+            with pytest.raises(RuntimeError, match="forward-mode derivative: logits"):
+                torch_ops.moe_route(dual, **arguments)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode derivative: logits"):
+                torch_ops.moe_route(dual, **arguments)
+
+
 # ---------------------------------------------------------------- GPU
 
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
@@ -434,6 +451,21 @@ def test_a_second_derivative_is_refused(torch_cuda):
     d, = torch.autograd.grad((r.weights.square().sum() + r.balance_loss,), z, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         d.sum().backward()
+
+
+@pytest.mark.gpu
+def test_a_gradient_of_dual_tensors_is_refused(torch_cuda):
+    """Forward mode over the backward pass: the tangents of the incoming gradients would be lost."""
+    from torch.autograd import forward_ad
+
+    z = _logits(20, 8, "f32", 2).requires_grad_(True)
+    r = torch_ops.moe_route(z, 2, balance=True)
+    dw, dl = torch.ones(20, 2, device="cuda"), torch.ones((), device="cuda")
+    with forward_ad.dual_level():
+        for grads in ((forward_ad.make_dual(dw, dw), dl), (dw, forward_ad.make_dual(dl, dl))):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                torch.autograd.grad((r.weights, r.balance_loss), z, grads, retain_graph=True)
+        torch.autograd.grad((r.weights, r.balance_loss), z, (dw, dl))
 
 
 @pytest.mark.gpu
