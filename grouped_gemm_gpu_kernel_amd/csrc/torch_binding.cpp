@@ -292,6 +292,7 @@ py::object w4_call(const Tensor& x, const Tensor& q, const Tensor& scales, const
     }
   }
   if (rows > GGK_ROUTE_MAX_TOTAL_SLOTS || n > GGK_W4_MAX_EXTENT || k > GGK_W4_MAX_EXTENT) return py::none();
+  if (has_tangent(x) || has_tangent(scales) || (row_weights && has_tangent(*row_weights))) return py::none();
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || scales.requires_grad() || (row_weights && row_weights->requires_grad()))) {
     return py::none();

@@ -509,6 +509,7 @@ def _check_w4(x, q, scales, zeros, counts, order, row_weights, out_dtype, lead=0
     if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or
                                     (row_weights is not None and row_weights.requires_grad)):
         raise RuntimeError("the products with 4-bit weights have no gradient: detach x, scales and row_weights")
+    _check_no_tangent("the products with 4-bit weights have", x=x, scales=scales, row_weights=row_weights)
 
 
 def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
@@ -523,7 +524,7 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
     never rounded: products and sums are float32, y is float32 or float16, rounded once.
 
     Runs on the current stream of x's device, without waiting; no gradient (inputs that require one are
-    refused).  Any number of rows is right; it is made for up to 64 or so."""
+    refused, and dual tensors of forward mode).  Any number of rows is right; it is made for up to 64 or so."""
     return _w4(_check_w4, x, q, scales, zeros, None, None, None, out_dtype)
 
 

@@ -121,6 +121,32 @@ def test_refusals_of_the_torch_calls():
                 torch_ops.moe_w4_matmul(x, q3, s3, counts, order, row_weights=w)
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor does not require a gradient by itself; its tangent would be lost without a word."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+
+    with FakeTensorMode(), forward_ad.dual_level():
+        def t(*shape, dtype=torch.float16):
+            return torch.empty(*shape, dtype=dtype, device="cuda:0")
+
+        def dual(a):
+            return forward_ad.make_dual(a, torch.empty_like(a))
+
+        x, q, s = t(3, 128), t(6, 64, dtype=torch.uint8), t(6, 2)
+        q3, s3, w = t(2, 6, 64, dtype=torch.uint8), t(2, 6, 2), t(6, dtype=torch.float32)
+        counts, order = t(2, dtype=torch.int32), t(6, dtype=torch.int32)
+        for name, call in [
+                ("x", lambda: torch_ops.w4_matmul(dual(x), q, s)), ("scales", lambda: torch_ops.w4_matmul(x, q, dual(s))),
+                ("x", lambda: torch_ops.moe_w4_matmul(dual(x), q3, s3, counts, order)),
+                ("scales", lambda: torch_ops.moe_w4_matmul(x, q3, dual(s3), counts, order)),
+                ("row_weights", lambda: torch_ops.moe_w4_matmul(x, q3, s3, counts, order, row_weights=dual(w)))]:
+            with pytest.raises(RuntimeError, match=f"forward-mode derivative: {name}"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match=f"forward-mode derivative: {name}"):
+                call()
+
+
 def test_matrix_results_are_read_behind_their_wait_states(tmp_path):
     """A matrix instruction's result may be read by another kind of instruction 8 wait states later at the earliest.  The
     compiler sees to it inside a basic block, but was seen to leave it out where a branch lies between (row tiles skipped
