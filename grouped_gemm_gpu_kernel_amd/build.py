@@ -11,7 +11,8 @@ Produces, in-tree:
 Steps: hipcc compiles the kernels for gfx950 with the compiler's resource
 report, which is parsed into a table the library links in; g++ compiles the
 plain C++ host runtime; hipcc links everything into one shared library.
-Usage: python -m grouped_gemm_gpu_kernel_amd.build [--no-tests] [--no-oracle]
+Usage: python -m grouped_gemm_gpu_kernel_amd.build [--no-tests] [--no-oracle] [--no-torch]
+Only gg_torch.so needs torch and the Python headers; without them it is left out, with a note.
 """
 from __future__ import annotations
 
@@ -170,9 +171,22 @@ def build_host_sanitized(out_path: Path) -> Path:
     return out
 
 
-def build_torch_binding() -> Path:
+def torch_binding_lacks() -> str | None:
+    """What the C++ part of torch_ops cannot be built without and is not there; None if all of it is."""
+    if importlib.util.find_spec("torch") is None:
+        return "torch is not installed"
+    headers = Path(sysconfig.get_paths()["include"])
+    return None if (headers / "Python.h").exists() else f"{headers} has no Python.h"
+
+
+def build_torch_binding() -> Path | None:
     """The C++ part of torch_ops (csrc/torch_binding.cpp), a Python module linked against the library beside it; torch's
-    own libraries are those that `import torch` has loaded."""
+    own libraries are those that `import torch` has loaded.  Returns None, with a note, where torch or the Python headers
+    are missing: the C, C++ and ctypes sides do without."""
+    lacks = torch_binding_lacks()
+    if lacks is not None:
+        print(f"gg_torch.so is not built: {lacks} (the PyTorch routing and 4-bit products need it)")
+        return None
     torch = Path(importlib.util.find_spec("torch").origin).parent
     out = LIB_DIR / "gg_torch.so"
     tmp = out.parent / (out.name + ".tmp")
@@ -232,7 +246,8 @@ def build_oracle() -> Path:
 
 def main(argv: list[str]) -> int:
     build_library()
-    build_torch_binding()
+    if "--no-torch" not in argv:
+        build_torch_binding()
     if "--no-oracle" not in argv:
         build_oracle()
     if "--no-tests" not in argv:
