@@ -190,7 +190,9 @@ def build_torch_binding() -> Path | None:
     torch = Path(importlib.util.find_spec("torch").origin).parent
     out = LIB_DIR / "gg_torch.so"
     tmp = out.parent / (out.name + ".tmp")
+    version = re.search(r"^__version__ = '(.+)'$", (torch / "version.py").read_text(), re.M).group(1)
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+          f'-DGG_TORCH_VERSION="{version}"',
           f"-I{ROOT / 'include'}", "-isystem", str(torch / "include"),
           "-isystem", str(torch / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(ROCM / "include"),
           "-isystem", sysconfig.get_paths()["include"], str(CSRC_DIR / "torch_binding.cpp"), "-o", str(tmp),

@@ -336,6 +336,7 @@ py::object w4_call(const Tensor& x, const Tensor& q, const Tensor& scales, const
 }  // namespace
 
 PYBIND11_MODULE(gg_torch, m) {
+  m.attr("torch_version") = GG_TORCH_VERSION;  // whose classes this was compiled with; the loader compares
   m.def("route", &route_call);
   m.def("w4", &w4_call);
 }

@@ -355,7 +355,8 @@ class Routing(NamedTuple):
 
 
 def _binding():
-    """The C++ binding of the calls below (csrc/torch_binding.cpp); raises if it has not been built."""
+    """The C++ binding of the calls below (csrc/torch_binding.cpp); raises if it has not been built, or with another torch:
+    tensors and autograd nodes are C++ classes whose layout may differ from version to version."""
     global _gg_torch
     if _gg_torch is None:
         if not _lib.TORCH_PATH.exists():
@@ -363,8 +364,15 @@ def _binding():
                                "(or __graft_entry__.build()); there is no fallback implementation")
         _lib.lib()
         spec = importlib.util.spec_from_file_location("gg_torch", _lib.TORCH_PATH)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        again = "build it again with `python -m grouped_gemm_gpu_kernel_amd.build`"
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as error:  # symbols that this torch does not have, or another Python
+            raise RuntimeError(f"{_lib.TORCH_PATH} does not fit this torch ({torch.__version__}): {again}") from error
+        built_for = getattr(module, "torch_version", "another version")
+        if built_for != str(torch.__version__):
+            raise RuntimeError(f"{_lib.TORCH_PATH} was built for torch {built_for}, this is {torch.__version__}: {again}")
         _gg_torch = module
     return _gg_torch
 

@@ -1,5 +1,5 @@
 """The build recipe where torch, or the Python headers, are missing: everything but the PyTorch binding is
-built, as C, C++ and ctypes users need it."""
+built, as C, C++ and ctypes users need it.  A binding that was built for another torch is refused."""
 import importlib.util
 import sysconfig
 
@@ -53,3 +53,28 @@ def test_no_torch_asks_for_nothing(made, missing, capsys):
 
 def test_here_both_are_there():
     assert build.torch_binding_lacks() is None
+
+
+def test_a_binding_of_another_torch_is_refused(monkeypatch):
+    """Built, then torch was exchanged: nothing in the old binary is called."""
+    import torch
+
+    from grouped_gemm_gpu_kernel_amd import torch_ops
+
+    assert torch_ops._binding().torch_version == torch.__version__
+    monkeypatch.setattr(torch_ops, "_gg_torch", None)
+    with monkeypatch.context() as other:
+        other.setattr(torch, "__version__", "2.9.1+rocm6.4")
+        with pytest.raises(RuntimeError, match="was built for torch .* this is 2.9.1.*build it again"):
+            torch_ops.moe_route(torch.zeros(3, 4), 2)
+    assert torch_ops._binding() is not None
+
+
+def test_a_binding_that_does_not_load_says_so(monkeypatch, tmp_path):
+    from grouped_gemm_gpu_kernel_amd import _lib, torch_ops
+
+    (tmp_path / "gg_torch.so").write_bytes(b"no library")
+    monkeypatch.setattr(torch_ops, "_gg_torch", None)
+    monkeypatch.setattr(_lib, "TORCH_PATH", tmp_path / "gg_torch.so")
+    with pytest.raises(RuntimeError, match="does not fit this torch.*build it again"):
+        torch_ops._binding()
