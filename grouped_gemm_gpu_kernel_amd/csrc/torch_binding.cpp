@@ -62,6 +62,19 @@ bool vector_in_order(const Tensor& t, at::ScalarType type, int64_t count, c10::D
 // A tangent of forward-mode differentiation: a dual tensor does not have to require a gradient.
 bool has_tangent(const Tensor& t) { return torch::autograd::isFwGradDefined(t); }
 
+// The address of a tensor's data, by its type: this form of the accessor throws where a tensor has elements but no data
+// (a fake one), for which the one without a type gives the null pointer that stands for an argument left out.
+const void* data(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return t.const_data_ptr<float>();
+    case at::kHalf: return t.const_data_ptr<at::Half>();
+    case at::kBFloat16: return t.const_data_ptr<at::BFloat16>();
+    case at::kInt: return t.const_data_ptr<int>();
+    case at::kBool: return t.const_data_ptr<bool>();
+    default: return t.const_data_ptr<uint8_t>();
+  }
+}
+
 template <class Args>
 int launch(hipError_t (*entry)(const Args*, hipStream_t), const Args& args, c10::Device device) {
   const c10::OptionalDeviceGuard guard(device);
@@ -125,9 +138,9 @@ RouteOutputs route(const RouteCall& c) {
   a.experts = static_cast<int>(experts);
   a.slots = static_cast<int>(c.slots);
   a.type = type_of(z.scalar_type());
-  a.logits = z.const_data_ptr();
+  a.logits = data(z);
   a.ld = row_stride(z);
-  a.token_mask = c.mask ? static_cast<const unsigned char*>(c.mask->const_data_ptr()) : nullptr;
+  a.token_mask = c.mask ? static_cast<const unsigned char*>(data(*c.mask)) : nullptr;
   a.given_ids = c.ids ? c.ids->const_data_ptr<int>() : nullptr;
   a.normalize = c.normalize;
   a.scale = static_cast<float>(c.scale);
@@ -206,7 +219,7 @@ struct Route : torch::autograd::Function<Route> {
       a.experts = static_cast<int>(z.size(1));
       a.slots = static_cast<int>(ids.size(1));
       a.type = type_of(z.scalar_type());
-      a.logits = z.const_data_ptr();
+      a.logits = data(z);
       a.ld = row_stride(z);
       a.ids = ids.const_data_ptr<int>();
       a.distinct = ctx->saved_data["distinct"].toBool();
@@ -308,16 +321,16 @@ py::object w4_call(const Tensor& x, const Tensor& q, const Tensor& scales, const
   a.k = static_cast<int>(k);
   a.group = static_cast<int>(k / groups);
   a.experts = static_cast<int>(experts);
-  a.x = x.const_data_ptr();
+  a.x = data(x);
   a.ldx = row_stride(x);
-  a.q = static_cast<const unsigned char*>(q.const_data_ptr());
+  a.q = static_cast<const unsigned char*>(data(q));
   a.ldq = ld(q);
   a.stride_q = matrix(q);
-  a.scales = scales.const_data_ptr();
+  a.scales = data(scales);
   a.lds = ld(scales);
   a.stride_s = matrix(scales);
   if (zeros) {
-    a.zeros = static_cast<const unsigned char*>(zeros->const_data_ptr());
+    a.zeros = static_cast<const unsigned char*>(data(*zeros));
     a.ldz = ld(*zeros);
     a.stride_z = matrix(*zeros);
   }

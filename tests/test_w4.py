@@ -147,6 +147,24 @@ def test_forward_mode_derivatives_are_refused():
                 call()
 
 
+def test_tensors_without_data_are_refused():
+    """Fake tensors never come to a launch, where their null addresses would stand for zero points and masks left out."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        def t(*shape, dtype=torch.float16):
+            return torch.empty(*shape, dtype=dtype, device="cuda:0")
+
+        x, q, s, z = t(3, 128), t(6, 64, dtype=torch.uint8), t(6, 2), t(6, 2, dtype=torch.uint8)
+        q3, s3, counts, order = t(2, 6, 64, dtype=torch.uint8), t(2, 6, 2), t(2, dtype=torch.int32), t(6, dtype=torch.int32)
+        for call in (lambda: torch_ops.w4_matmul(x, q, s), lambda: torch_ops.w4_matmul(x, q, s, z),
+                     lambda: torch_ops.moe_w4_matmul(x, q3, s3, counts, order),
+                     lambda: torch_ops.moe_route(t(600, 8), 2),
+                     lambda: torch_ops.moe_route(t(600, 8), 2, token_mask=t(600, dtype=torch.bool))):
+            with pytest.raises(RuntimeError, match="data is not allocated"):
+                call()
+
+
 def test_matrix_results_are_read_behind_their_wait_states(tmp_path):
     """A matrix instruction's result may be read by another kind of instruction 8 wait states later at the earliest.  The
     compiler sees to it inside a basic block, but was seen to leave it out where a branch lies between (row tiles skipped
