@@ -47,8 +47,12 @@ bool rows_in_order(const Tensor& t, int64_t rows, int64_t columns, int64_t row_s
   return (columns <= 1 || column_stride == 1) && (rows <= 1 || row_stride >= std::max<int64_t>(1, columns));
 }
 
+// Does the memory hold the values?  Not where they are its negatives (the negative bit, as of the imaginary part of a
+// conjugate) or it is not there (a zero tensor).
+bool is_stored(const Tensor& t) { return !t.is_neg() && !t._is_zerotensor(); }
+
 bool matrix_in_order(const Tensor& t) {
-  return t.dim() == 2 && rows_in_order(t, t.size(0), t.size(1), t.stride(0), t.stride(1));
+  return t.dim() == 2 && is_stored(t) && rows_in_order(t, t.size(0), t.size(1), t.stride(0), t.stride(1));
 }
 
 int64_t row_stride(const Tensor& t) {
@@ -56,7 +60,8 @@ int64_t row_stride(const Tensor& t) {
 }
 
 bool vector_in_order(const Tensor& t, at::ScalarType type, int64_t count, c10::Device device) {
-  return t.scalar_type() == type && t.device() == device && t.numel() == count && t.is_contiguous();
+  return t.scalar_type() == type && t.device() == device && t.numel() == count && t.is_contiguous() &&
+         is_stored(t);
 }
 
 // A tangent of forward-mode differentiation: a dual tensor does not have to require a gradient.
@@ -202,16 +207,20 @@ struct Route : torch::autograd::Function<Route> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &z = saved[0], &ids = saved[1], &slope = saved[2];
-    const Tensor d_loss = grads.size() > 4 ? grads[4] : Tensor();
-    if (!grads[0].defined() && !d_loss.defined()) return {Tensor(), Tensor()};
-    TORCH_CHECK(!has_tangent(grads[0]) && !has_tangent(d_loss),
+    // Incoming gradients may be expanded (a sum's) or in any strides, and hold their values' negatives, or none where all
+    // are zero.
+    const auto incoming = [&](size_t i) {
+      return i >= grads.size() || !grads[i].defined() || grads[i]._is_zerotensor() ? Tensor()
+                                                                                   : grads[i].resolve_neg().contiguous();
+    };
+    if (!grads[0].defined() && (grads.size() < 5 || !grads[4].defined())) return {Tensor(), Tensor()};
+    const Tensor d_weights = incoming(0), d_loss = incoming(4);
+    TORCH_CHECK(!has_tangent(d_weights) && !has_tangent(d_loss),
                 "moe_route's gradient has no forward-mode derivative: it was given a dual tensor");
     // The engine would join the leaf's stream to the capture, which for the default stream ends the process.
     TORCH_CHECK(!is_capturing(z.device()) || !reaches_default_stream(torch::autograd::get_current_node().get()),
                 "moe_route: a backward pass is being captured while an eager graph of the same leaves, made on the default "
                 "stream, is alive: free it first, or make it on a side stream");
-    // The weights' gradient may come expanded (a sum's) or in any strides.
-    const Tensor d_weights = grads[0].defined() ? grads[0].contiguous() : Tensor();
     Tensor d = at::empty({z.size(0), z.size(1)}, z.options().requires_grad(false));
     if (z.size(0) > 0) {
       ggk_route_gradient_args a{};
@@ -263,7 +272,7 @@ py::object route_call(const Tensor& logits, std::optional<int64_t> top_k, const 
 // `align` elements.
 bool weights_in_order(const Tensor& t, const Tensor& q, at::ScalarType type, c10::Device device, int64_t align) {
   const int64_t dim = q.dim(), n = q.size(dim - 2);
-  if (t.scalar_type() != type || t.device() != device || t.dim() != dim) return false;
+  if (t.scalar_type() != type || t.device() != device || t.dim() != dim || !is_stored(t)) return false;
   for (int64_t i = 0; i + 1 < dim; ++i) {
     if (t.size(i) != q.size(i)) return false;
   }

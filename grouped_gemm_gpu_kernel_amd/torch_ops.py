@@ -390,6 +390,12 @@ def _check_vector(t: torch.Tensor, name: str, dtype: torch.dtype, count: int, de
         raise ValueError(f"{name} must be contiguous")
 
 
+def _check_stored(**tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and (t.is_neg() or t._is_zerotensor()):
+            raise ValueError(f"{name} is a view whose memory does not hold its values: call resolve_neg() (or add 0)")
+
+
 def _check_no_tangent(what: str, **tensors) -> None:
     for name, t in tensors.items():
         if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
@@ -466,6 +472,7 @@ def _check_route(logits, top_k, ids, token_mask) -> None:
         raise ValueError(f"{tokens} tokens with {slots} slots each: more than 2^30 slots")
     if token_mask is not None:
         _check_vector(token_mask, "token_mask", torch.bool, tokens, logits.device)
+    _check_stored(logits=logits, ids=ids, token_mask=token_mask)
     _check_no_tangent("moe_route has", logits=logits)
 
 
@@ -514,6 +521,7 @@ def _check_w4(x, q, scales, zeros, counts, order, row_weights, out_dtype, lead=0
         raise ValueError(f"q stands for [{q.shape[-2]}, {k}] weights: N and K are at most 2^28")
     if q.data_ptr() % 16 != 0 or any(n > 1 and s % 16 != 0 for n, s in zip(q.shape[:-1], q.stride()[:-1])):
         raise ValueError("q must start on a multiple of 16 bytes, and so must its rows and matrices")
+    _check_stored(x=x, q=q, scales=scales, zeros=zeros, row_weights=row_weights)
     if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad or
                                     (row_weights is not None and row_weights.requires_grad)):
         raise RuntimeError("the products with 4-bit weights have no gradient: detach x, scales and row_weights")
@@ -587,6 +595,7 @@ def _check_moe_w4(x, q, scales, zeros, counts, order, row_weights, out_dtype) ->
         raise ValueError(f"order has {rows} entries, not a multiple of x's {x.shape[0]} rows")
     if row_weights is not None:
         _check_vector(row_weights, "row_weights", torch.float32, rows, x.device)
+    _check_stored(counts=counts, order=order)
 
 
 # ---------------------------------------------------------------- custom op

@@ -469,6 +469,37 @@ def test_a_gradient_of_dual_tensors_is_refused(torch_cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("normalize", [True, False])
+def test_incoming_gradients_held_as_negatives_or_not_at_all(torch_cuda, normalize):
+    """A lazily conjugated complex value's imaginary part holds its values' negatives, and a zero tensor nothing: the
+    gradient of what they stand for."""
+    z = _logits(40, 8, "f32", 2).requires_grad_(True)
+    dw = torch.randn(40, 2, generator=torch.Generator().manual_seed(1)).cuda()
+    dl = torch.full((), 0.3, device="cuda")
+
+    def gradient(d_weights, d_loss):
+        r = torch_ops.moe_route(z, 2, normalize=normalize, balance=True)
+        return torch.autograd.grad((r.weights, r.balance_loss), z, (d_weights, d_loss))[0]
+
+    def negative(t):
+        t = torch.imag(torch.complex(t, -t).conj())
+        assert t.is_neg()
+        return t
+
+    want = gradient(dw, dl)
+    assert torch.equal(gradient(negative(dw), dl), want)
+    assert torch.equal(gradient(dw, negative(dl)), want)
+    none = torch._efficientzerotensor((40, 2), device="cuda")
+    assert torch.equal(gradient(none, dl), gradient(torch.zeros_like(dw), dl))
+    assert torch.equal(gradient(none, torch._efficientzerotensor((), device="cuda")), torch.zeros_like(z))
+    # through torch's own operators
+    r = torch_ops.moe_route(z, 2, normalize=normalize, balance=True)
+    back, = torch.autograd.grad(torch.imag(torch.complex(dl, r.balance_loss).conj()), z)
+    r = torch_ops.moe_route(z, 2, normalize=normalize, balance=True)
+    assert torch.equal(back, torch.autograd.grad(-r.balance_loss, z)[0])
+
+
+@pytest.mark.gpu
 def test_saved_tensors_changed_in_place_are_noticed(torch_cuda):
     """ids changed before the backward pass raise; counts and order, which it does not read, may be."""
     z = _logits(200, 8, "f32", 2).requires_grad_(True)

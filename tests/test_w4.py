@@ -165,6 +165,30 @@ def test_tensors_without_data_are_refused():
                 call()
 
 
+def test_views_whose_memory_holds_other_values_are_refused():
+    """Views with the negative bit (the imaginary part of a conjugate): memory holds the values' negatives."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        def t(*shape, dtype=torch.float16):
+            return torch.empty(*shape, dtype=dtype, device="cuda:0")
+
+        x, q, s = t(1, 128), t(6, 64, dtype=torch.uint8), t(6, 2)
+        q3, s3, counts, order = t(2, 6, 64, dtype=torch.uint8), t(2, 6, 2), t(2, dtype=torch.int32), t(1, dtype=torch.int32)
+        w = torch.imag(t(1, dtype=torch.complex64).conj())
+        assert w.is_neg() and w.is_contiguous()
+        with pytest.raises(ValueError, match="row_weights is a view"):
+            torch_ops.moe_w4_matmul(x, q3, s3, counts, order, row_weights=w)
+        with pytest.raises(ValueError, match="x is a view"):
+            torch_ops.w4_matmul(torch._neg_view(x), q, s)
+        with pytest.raises(ValueError, match="scales is a view"):
+            torch_ops.w4_matmul(x, q, torch._neg_view(s))
+        with pytest.raises(ValueError, match="logits is a view"):
+            torch_ops.moe_route(torch._neg_view(t(600, 8)), 2)
+        with pytest.raises(ValueError, match="logits is a view"):
+            torch_ops.moe_route(torch._efficientzerotensor((600, 8), device="cuda:0"), 2)
+
+
 def test_matrix_results_are_read_behind_their_wait_states(tmp_path):
     """A matrix instruction's result may be read by another kind of instruction 8 wait states later at the earliest.  The
     compiler sees to it inside a basic block, but was seen to leave it out where a branch lies between (row tiles skipped
