@@ -197,7 +197,18 @@ struct Plan {
   int blocks, rows;
   bool columns;  // the columns kernel runs between the rows and the order
   bool vectors;
+  int run;  // tokens of a group whose p are added up in its registers before they go to LDS; 0: all of them
 };
+
+// A float sum of n terms is off by up to n half steps, and terms that are alike make that much of it.  Sums of p over a
+// group's tokens are made in runs of about the root of their number, but of 64 at least, and the runs added up in LDS:
+// 2^25 tokens of two experts, 2048 a group, were off by 253 half steps in one sum.
+int tokens_a_run(int tokens) {
+  if (tokens <= 64) return 0;
+  int run = 64;
+  while ((long long)run * run < tokens) ++run;
+  return run;
+}
 
 // Workspace, written by the rows kernel: per block and expert the slots taken (one more column: slots without an
 // expert; rows padded to whole vectors of four) and the sum of p, then per block the routed tokens.  The columns
@@ -223,7 +234,7 @@ Plan plan_blocks(int tokens, int experts) {
   int rows = (tokens + most - 1) / most;
   rows = rows < least ? least : (rows + least - 1) / least * least;
   const int blocks = tokens > 0 ? (tokens + rows - 1) / rows : 1;
-  return {blocks, rows, (long long)blocks * experts > kMaxOwnSums, false};
+  return {blocks, rows, (long long)blocks * experts > kMaxOwnSums, false, 0};
 }
 
 // So many tokens are routed by one workgroup, 64 at a time: 4.5 us for the first, 2.4 for each further 64, where two
@@ -451,40 +462,59 @@ __device__ __forceinline__ bool route_token(const ggk_route_args& a, const Token
   return routed;
 }
 
+// The wave's sums of p over its groups go to its row of s_part, a row of `experts` floats a wave: stored, or added to
+// what is there.
+template <int L, int V>
+__device__ __forceinline__ void wave_sums(const float (&sums)[V], int experts, float* s_part, bool add) {
+  using C = Columns<L, V>;
+  const int tid = threadIdx.x, lane = tid % L, wave = tid / kWave;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    float x = sums[j];
+    if constexpr (L < kWave) {
+      uint2v r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+      r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    const int e = C::expert(lane, j);
+    if (tid % kWave < L && e < experts) s_part[wave * experts + e] = add ? s_part[wave * experts + e] + x : x;
+  }
+}
+
 // Tokens [first, last) by the groups of the workgroup, each group's next logits loaded while it routes a token.
-// Returns the number of tokens that this lane's group has routed.
-template <class T, int L, int V, int THREADS>
+// Returns the number of tokens that this lane's group has routed.  RUNS: after every `run` tokens of a group its sums of p
+// are added to s_part, which has been cleared.
+template <class T, int L, int V, int THREADS, bool RUNS>
 __device__ __forceinline__ int route_tokens(const ggk_route_args& a, bool vectors, int first, int last, int* s_count,
-                                            float (&sums)[V]) {
+                                            float (&sums)[V], int run, float* s_part) {
   constexpr int kGroups = THREADS / L;
   const int group = threadIdx.x / L;
-  int routed = 0;
+  int routed = 0, in_run = 0;
   Token<T, V> next;
   load_token<T, L, V>(a, vectors, first + group, last, next);
   for (int t0 = first; t0 < last; t0 += kGroups) {
     const Token<T, V> token = next;
     if (t0 + kGroups < last) load_token<T, L, V>(a, vectors, t0 + kGroups + group, last, next);
     routed += route_token<T, L, V>(a, token, t0 + group, last, s_count, sums) ? 1 : 0;
+    if constexpr (RUNS) {
+      if (++in_run == run) {
+        wave_sums<L, V>(sums, a.experts, s_part, true);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sums[j] = 0.0f;
+        in_run = 0;
+      }
+    }
   }
   return routed;
 }
 
-// The block's sums of p (balance) over its groups, to out[e].  s_part: a row of `experts` floats a wave.
+// The block's sums of p (balance) over its groups, to out[e].  s_part: a row of `experts` floats a wave; add: with runs'
+// sums in it.
 template <int L, int V, int THREADS>
-__device__ __forceinline__ void block_sums(float (&sums)[V], int experts, float* s_part, float* out) {
-  using C = Columns<L, V>;
-  const int tid = threadIdx.x, lane = tid % L, wave = tid / kWave;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if constexpr (L < kWave) {
-      uint2v r = __builtin_amdgcn_permlane16_swap(__float_as_uint(sums[j]), __float_as_uint(sums[j]), false, false);
-      float x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-      r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-      sums[j] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    const int e = C::expert(lane, j);
-    if (tid % kWave < L && e < experts) s_part[wave * experts + e] = sums[j];
-  }
+__device__ __forceinline__ void block_sums(const float (&sums)[V], int experts, float* s_part, float* out, bool add) {
+  const int tid = threadIdx.x;
+  wave_sums<L, V>(sums, experts, s_part, add);
   __syncthreads();
   for (int e = tid; e < experts; e += THREADS) {
     float x = 0.0f;
@@ -495,24 +525,25 @@ __device__ __forceinline__ void block_sums(float (&sums)[V], int experts, float*
 
 // The tokens of one block: choice, weights, counts and sums of p.  65521 tokens of 256 float logits, 8 slots, loss: 37 us
 // for 67 MB, bound by vector instructions (985 a wave for its 4 tokens, 26 us); 16384 of 64: 4.7 us, start and latency.
-template <class T, int L, int V>
+template <class T, int L, int V, bool RUNS>
 __global__ __launch_bounds__(kThreads, 4) void route_rows_kernel(ggk_route_args a, Workspace ws, Plan plan) {
   extern __shared__ int shared[];  // counts [experts + 1], routed, then (balance) `experts` floats a wave
   int* s_count = shared;
   int* s_routed = shared + a.experts + 1;
   const int tid = threadIdx.x;
-  for (int e = tid; e < a.experts + 2; e += kThreads) shared[e] = 0;
+  float* s_part = reinterpret_cast<float*>(shared + a.experts + 2);
+  const int clear = a.experts + 2 + (RUNS ? kThreads / kWave * a.experts : 0);
+  for (int e = tid; e < clear; e += kThreads) shared[e] = 0;
   __syncthreads();
   float sums[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) sums[j] = 0.0f;
   const int first = blockIdx.x * plan.rows;
   const int last = min(a.tokens, first + plan.rows);
-  const int routed = route_tokens<T, L, V, kThreads>(a, plan.vectors, first, last, s_count, sums);
+  const int routed = route_tokens<T, L, V, kThreads, RUNS>(a, plan.vectors, first, last, s_count, sums, plan.run, s_part);
   if (tid % L == 0 && routed > 0) atomicAdd(s_routed, routed);
   if (a.loss != nullptr) {
-    block_sums<L, V, kThreads>(sums, a.experts, reinterpret_cast<float*>(shared + a.experts + 2),
-                     ws.p + (size_t)blockIdx.x * a.experts);
+    block_sums<L, V, kThreads>(sums, a.experts, s_part, ws.p + (size_t)blockIdx.x * a.experts, RUNS);
   }
   __syncthreads();
   const int pitch = count_pitch(a.experts);
@@ -795,14 +826,14 @@ __global__ __launch_bounds__(kSmallThreads) void route_small_kernel(ggk_route_ar
   float sums[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) sums[j] = 0.0f;
-  const int routed = route_tokens<T, L, V, kSmallThreads>(a, vectors, 0, a.tokens, s_count, sums);
+  const int routed = route_tokens<T, L, V, kSmallThreads, false>(a, vectors, 0, a.tokens, s_count, sums, 0, nullptr);
   if (tid % L == 0 && routed > 0) atomicAdd(s_routed, routed);
   __syncthreads();  // ids are read back below by other threads of this workgroup
   const Run run = run_of_wave<kSmallThreads>(0, (long long)a.tokens * a.slots);
   const int id0 = run.begin + tid % kWave < run.end ? a.ids[run.begin + tid % kWave] : -1;
   if (a.loss != nullptr) {
     float* s_part = reinterpret_cast<float*>(s_rest);
-    block_sums<L, V, kSmallThreads>(sums, a.experts, s_part, s_part);
+    block_sums<L, V, kSmallThreads>(sums, a.experts, s_part, s_part, false);
     __syncthreads();
     if (tid < kWave) balance_loss(a, s_part, s_count, *s_routed);
     __syncthreads();
@@ -977,8 +1008,11 @@ hipError_t launch_route(const ggk_route_args& a, Plan plan, hipStream_t stream) 
                        sizeof(int) * (2 * width + 1) + kSmallThreads / kWave * wave_row, stream, a, plan.vectors);
     return hipGetLastError();
   }
+  plan.run = a.loss != nullptr ? tokens_a_run(plan.rows / (kThreads / L)) : 0;
   const Workspace ws = carve(a.workspace, a.experts, plan.blocks);
-  hipLaunchKernelGGL((route_rows_kernel<T, L, V>), dim3(plan.blocks), dim3(kThreads),
+  // A kernel of its own for runs: with them the one for fewer tokens spilled or lost 1%.
+  auto rows_kernel = plan.run > 0 ? route_rows_kernel<T, L, V, true> : route_rows_kernel<T, L, V, false>;
+  hipLaunchKernelGGL(rows_kernel, dim3(plan.blocks), dim3(kThreads),
                      sizeof(int) * (width + 1) + (a.loss != nullptr ? kThreads / kWave * wave_row : 0), stream, a, ws, plan);
   hipError_t st = hipGetLastError();
   if (st != hipSuccess) return st;

@@ -374,7 +374,9 @@ hipError_t ggk_launch_grouped_device_done(int variant, int path, int addressing,
  *                   softmax(z_t)[e] over the tokens with an expert), 0 with no
  *                   such token; slope[e] = d loss / d (sum of softmax(z_t)[e]).
  * loss and slope may be NULL, both or neither.  Sums are made in a fixed
- * order: the same call gives the same bits.  workspace holds
+ * order: the same call gives the same bits; sums over the tokens are float32
+ * in runs of about the root of their number, off by some 200 half steps at most
+ * for 2^25 tokens.  workspace holds
  * ggk_route_workspace(tokens, experts) bytes (0 for a few tokens) from a
  * multiple of 16 on, written before they are read; calls that may overlap need one each.  1 <= experts <=
  * GGK_MOE_MAX_EXPERTS, 1 <= slots <= GGK_ROUTE_MAX_SLOTS and, without

@@ -524,6 +524,35 @@ def test_no_tokens(torch_cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,top_k", [(2 ** 25 + 7, 2, 1), (2 ** 21 + 3, 32, 17), (2 ** 20 + 5, 300, 4)])
+@pytest.mark.parametrize("step", [0.25, 0.6, 0.9])
+def test_loss_over_many_tokens(torch_cuda, tokens, experts, top_k, step):
+    """The same logits for every token, so that the roundings of a running sum of p all go the same way.
+
+    Sums of p make chains of at most 64 additions in a lane and 64 of such runs (2^25 tokens by 512 blocks of 32 groups
+    are 2048 a lane), 10 over a block's groups and waves, 512 / 8 + 8 over the blocks: 210 u, and 16 u for p and what
+    follows the sums."""
+    row = (-torch.arange(experts) * step).bfloat16()
+    row[experts // 2:] -= 1
+    z = row.cuda().repeat(tokens, 1)
+    r = torch_ops.moe_route(z, top_k, balance=True)
+    p = np.exp(row.double().numpy())
+    p /= p.sum()
+    want = experts / top_k * p[:top_k].sum()
+    assert r.counts.tolist() == [tokens] * top_k + [0] * (experts - top_k)
+    assert abs(float(r.balance_loss) - want) <= 226 * U * want, (float(r.balance_loss) / want - 1) / U
+    z.requires_grad_(True)
+    r = torch_ops.moe_route(z, top_k, balance=True)
+    got, = torch.autograd.grad(r.balance_loss, z, torch.full((), float(tokens), device="cuda"))
+    c = np.where(np.arange(experts) < top_k, experts / top_k, 0.0)
+    grad = p * (c - (p * c).sum())
+    size = p * (c + (p * c).sum())
+    bound = size * 4 * (20 + 32) * U + np.abs(grad) * 2.0 ** -8 * 1.01 + TINY
+    assert (got == got[0]).all()  # equal rows, wherever they stand
+    assert (np.abs(got[-1].double().cpu().numpy() - grad) <= bound).all()
+
+
+@pytest.mark.gpu
 def test_rows_past_32_bits(torch_cuda):
     """Logits whose last rows lie past 2^31 elements: 9 GB of bfloat16, of which a few rows are looked at."""
     experts, tokens = 1024, 2 ** 31 // 1024 + 1000
@@ -546,6 +575,40 @@ def test_rows_past_32_bits(torch_cuda):
     e = (tokens - 1) % experts
     assert abs(float(last[e]) - want * (1 - want)) <= want * 2.0 ** -8
     assert not got[:-1].any()
+
+
+@pytest.mark.gpu
+def test_loss_and_its_gradient_past_32_bits(torch_cuda):
+    """The loss over rows that end past 2^31 elements, and its gradient there.  Chains of additions as in
+    test_loss_over_many_tokens, shorter ones (514 tokens a lane)."""
+    experts, tokens = 1024, 2 ** 31 // 1024 + 1000
+    z = torch.zeros(tokens, experts, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([5, tokens - 900, tokens - 1], device="cuda")
+    z[at, at % experts] = 3.0
+    z.requires_grad_(True)
+    r = torch_ops.moe_route(z, 1, balance=True)
+    chosen = (at % experts).tolist()
+    counts = np.zeros(experts)
+    counts[0] = tokens - len(chosen)
+    p_sum = np.full(experts, (tokens - len(chosen)) / experts)
+    total = math.exp(3.0) + experts - 1
+    for e in chosen:
+        counts[e] += 1
+        p_sum += 1.0 / total
+        p_sum[e] += (math.exp(3.0) - 1.0) / total
+    f = counts / tokens
+    want = experts * (f * p_sum / tokens).sum()
+    assert abs(float(r.balance_loss) - want) <= 226 * U * want
+    got, = torch.autograd.grad(r.balance_loss, z, torch.full((), float(tokens), device="cuda"))
+    for row, e in ((3, None), (tokens - 2, None), (5, 5), (tokens - 1, chosen[-1])):
+        p = np.full(experts, 1.0 / experts)
+        if e is not None:
+            p = np.full(experts, 1.0 / total)
+            p[e] = math.exp(3.0) / total
+        c = experts * f
+        grad, size = p * (c - (p * c).sum()), p * (c + (p * c).sum())
+        off = np.abs(got[row].double().cpu().numpy() - grad)
+        assert (off <= size * 4 * (3 + 32) * U + np.abs(grad) * 2.0 ** -8 * 1.01 + TINY).all(), row
 
 
 @pytest.mark.gpu
