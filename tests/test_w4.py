@@ -429,6 +429,94 @@ def test_experts(torch_cuda, tokens, experts, top_k, n, k, group, drop, zeros):
     _check_moe(y, slots.view(tokens * top_k, k), q, s, z, ids.view(-1, 1))
 
 
+# Cases of every form of the experts' kernel: rows an item, waves that split K; the experts' slots (with items of up to 4, 16
+# and 32 rows and of more than one item), slots without an expert, N.
+FORM_CASES = [
+    ((32, 1), [1, 4, 5, 16, 17, 32, 33, 70, 0, 2, 3, 9, 1, 0, 31, 6], 5, 1100),
+    ((32, 1), [3, 0, 20, 64, 16], 0, 3300),
+    ((32, 1), [2, 1, 40, 0, 8, 1, 1, 19, 1, 4, 1, 1, 1, 1, 1, 17], 40, 8011),  # more items than workgroups
+    ((32, 1), [1] * 200 + [7] * 56, 3, 81),
+    ((16, 1), [1, 0, 2] * 99 + [5, 16, 17, 40], 9, 100),
+    ((16, 1), [0] * 700 + [3, 33, 4] * 100, 0, 33),
+    ((16, 2), [1, 4, 5, 16, 17, 32, 33, 70, 0, 2, 3, 9, 1, 0, 31, 6], 5, 600),
+    ((16, 2), [30, 60, 16, 47], 2, 3999),  # more items than workgroups
+    ((16, 2), [2, 1, 0] * 100 + [20], 0, 40),
+    ((16, 4), [1, 4, 5, 16, 17, 33, 0, 2], 4, 500)]
+
+
+def _form(n, slots, experts):
+    """The kernel's form, by the launch's rule."""
+    waves = (n + 15) // 16 * min(slots, experts)
+    if waves >= 1024 and experts <= 256:
+        return 32, 1
+    return (16, 1) if waves >= 1024 else (16, 2) if waves >= 512 else (16, 4)
+
+
+def _slots_of(takes, without, seed):
+    """Each slot's expert in a random order, counts and order."""
+    flat = torch.cat([torch.full((c,), e) for e, c in enumerate(takes)] + [torch.full((without,), -1)])
+    flat = flat[torch.randperm(len(flat), generator=torch.Generator().manual_seed(seed))]
+    order = torch.where(flat < 0, len(takes), flat).sort(stable=True).indices.int().cuda()
+    return flat.cuda(), torch.tensor(takes, dtype=torch.int32, device="cuda"), order
+
+
+def _check_slots(y, x, q, s, z, flat, row_weights=None):
+    """y[o] against x[o] by flat[o]'s matrix, the experts one after the other; rows without one are zeros."""
+    assert (y[flat < 0] == 0).all()
+    for e in flat[flat >= 0].unique().tolist():
+        rows = (flat == e).nonzero()[:, 0]
+        check(y[rows], x[rows].double(), values(q[e], s[e], None if z is None else z[e]),
+              None if row_weights is None else row_weights[rows].double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group,k", [(128, 128), (128, 128 * 5), (256, 256 * 5), (32, 32 * 33), (64, 64 * 17), (96, 96 * 7)])
+@pytest.mark.parametrize("form,takes,without,n", FORM_CASES)
+def test_each_form_of_the_experts(torch_cuda, form, takes, without, n, group, k, zeros):
+    flat, counts, order = _slots_of(takes, without, n + k)
+    slots = len(flat)
+    assert _form(n, slots, len(takes)) == form
+    q, s, z = _weights((len(takes),), n, k, group, zeros, n)
+    x = _x(slots, k, slots)
+    first = torch_ops.moe_w4_matmul(x, q, s, counts, order, z)
+    _check_slots(first, x, q, s, z, flat)
+    rw = torch.randn(slots, generator=torch.Generator().manual_seed(5)).cuda()
+    y = torch_ops.moe_w4_matmul(x, q, s, counts, order, z, row_weights=rw, out_dtype=torch.float16)
+    _check_slots(y, x, q, s, z, flat, rw)
+    assert torch.equal(torch_ops.moe_w4_matmul(x, q, s, counts, order, z), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,k", [(128, 1408), (64, 1408), (96, 96 * 15)])
+@pytest.mark.parametrize("form,takes,without,n", FORM_CASES)
+def test_each_form_of_the_experts_is_exact(torch_cuda, form, takes, without, n, group, k):
+    """Whole numbers, as in test_sums_of_integers_are_exact."""
+    flat, counts, order = _slots_of(takes, without, n + k)
+    q, s, _ = _weights((len(takes),), n, k, group, False, n)
+    s.fill_(1.0)
+    x = torch.randint(-1, 2, (len(flat), k), generator=torch.Generator().manual_seed(20)).half().cuda()
+    x[:, 7::512] = 2048.0
+    y = torch_ops.moe_w4_matmul(x, q, s, counts, order)
+    assert (y[flat < 0] == 0).all()
+    for e in flat[flat >= 0].unique().tolist():
+        rows = (flat == e).nonzero()[:, 0]
+        assert torch.equal(y[rows].double(), x[rows].double() @ values(q[e], s[e]).t()), e
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts,n,form", [(8, 2048, (32, 1)), (300, 300, (16, 1)), (8, 1300, (16, 2))])
+def test_tokens_of_several_slots_in_each_form(torch_cuda, experts, n, form):
+    """x one row a token, three slots each."""
+    tokens, top_k, k = 70, 3, 640
+    assert _form(n, tokens * top_k, experts) == form
+    q, s, z = _weights((experts,), n, k, 64, True, n)
+    ids, counts, order = _routing(tokens, experts, top_k, n, 0.2)
+    x = _x(tokens, k, n)
+    y = torch_ops.moe_w4_matmul(x, q, s, counts, order, z)
+    _check_slots(y, x.repeat_interleave(top_k, 0), q, s, z, ids.flatten())
+
+
 @pytest.mark.gpu
 def test_one_expert_takes_all(torch_cuda):
     q, s, _ = _weights((12,), 100, 256, 128, False, 1)
