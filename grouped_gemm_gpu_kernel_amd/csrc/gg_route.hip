@@ -237,9 +237,13 @@ Plan plan_blocks(int tokens, int experts) {
   return {blocks, rows, (long long)blocks * experts > kMaxOwnSums, false, 0};
 }
 
-// So many tokens are routed by one workgroup, 64 at a time: 4.5 us for the first, 2.4 for each further 64, where two
-// launches take 10.  Its counts per wave have to fit 64 KB of LDS.
-bool is_small(int tokens, int experts) { return tokens <= 128 && experts <= 768; }
+// So many tokens are routed by one workgroup.  Up to 256 experts it takes 64 at a time, at 16 lanes each: with 64 experts
+// 4.8 us for one token and 6.7 for 128, where two launches take 7.2 for 129 (256 experts: 8.3 and 17, two launches 11: the
+// second round of 64 loses there).  Above, a wave a token, it takes 16 at a
+// time: with 512 experts and 8 slots 8.7 us for 16, 12.9 for 32, 21.5 for 64 and 38.7 for 128, where two launches take 18.
+// (More than 16 slots also take a wave each, 20 of 64 experts 12.4, 20.8, 38.1 and 72, two launches 29; but the workspace's
+// size does not know the slots.)  The counts per wave have to fit 64 KB of LDS.
+bool is_small(int tokens, int experts) { return tokens <= (experts <= 256 ? 128 : 32) && experts <= 768; }
 
 size_t workspace_ints(int experts, int blocks) {
   return (size_t)count_pitch(experts) * blocks + (size_t)experts * blocks + (size_t)blocks;

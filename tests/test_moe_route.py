@@ -158,6 +158,14 @@ def test_route_gradient_arguments_are_checked_on_the_host():
     assert status(type=-1) == 1 and status(ld=3) == 1 and status(experts=0) == 1 and status(slots=65) == 1
 
 
+def test_few_tokens_take_no_workspace():
+    """One workgroup routes 128 tokens of up to 256 experts, and 32 above, where each takes a wave."""
+    size = _lib.lib().ggk_route_workspace
+    for experts, most in ((1, 128), (64, 128), (256, 128), (257, 32), (512, 32), (768, 32), (769, 0), (1024, 0)):
+        assert size(most, experts) == 0 or most == 0
+        assert size(most + 1, experts) > 0
+
+
 def test_refusals_of_the_torch_call():
     from torch._subclasses.fake_tensor import FakeTensorMode
 
@@ -289,6 +297,17 @@ def test_shapes_and_types(torch_cuda, tokens, experts, top_k, dtype):
     dw = torch.randn(tokens, top_k, generator=torch.Generator().manual_seed(1)).cuda()
     for normalize, scale in ((True, 1.0), (False, 2.5)):
         _check(z, top_k, normalize=normalize, scale=scale, d_weights=dw, d_loss=0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [32, 33, 100, 128, 129])
+@pytest.mark.parametrize("experts,top_k", [(256, 8), (257, 8), (700, 20)])
+def test_few_tokens_of_many_experts(torch_cuda, tokens, experts, top_k):
+    """Both sides of what one workgroup routes."""
+    z = _logits(tokens, experts, "bf16", tokens + experts)
+    dw = torch.randn(tokens, top_k, generator=torch.Generator().manual_seed(1)).cuda()
+    mask = (torch.rand(tokens, generator=torch.Generator().manual_seed(2)) < 0.8).cuda()
+    _check(z, top_k, mask=mask, d_weights=dw, d_loss=0.4)
 
 
 @pytest.mark.gpu
