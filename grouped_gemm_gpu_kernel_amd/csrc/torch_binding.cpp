@@ -14,7 +14,6 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
@@ -172,18 +171,17 @@ bool is_capturing(c10::Device device) {
          status != hipStreamCaptureStatusNone;
 }
 
-// Does the backward pass go on from `node` to a leaf whose gradient belongs to the default stream?
-bool reaches_default_stream(const torch::autograd::Node* node) {
-  std::vector<const torch::autograd::Node*> left{node};
-  std::unordered_set<const torch::autograd::Node*> seen;
+// Does the graph go on from `node` to one that belongs to the default stream: a leaf that an eager graph made there holds,
+// or an operator of such a graph itself?
+bool reaches_default_stream(torch::autograd::Node* node) {
+  std::vector<torch::autograd::Node*> left{node};
+  std::unordered_set<torch::autograd::Node*> seen;
   while (!left.empty()) {
-    const torch::autograd::Node* at = left.back();
+    torch::autograd::Node* at = left.back();
     left.pop_back();
     if (at == nullptr || !seen.insert(at).second) continue;
-    if (auto* leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(at)) {
-      const auto stream = const_cast<torch::autograd::AccumulateGrad*>(leaf)->stream();
-      if (stream && stream->id() == 0) return true;
-    }
+    const auto stream = at->stream();
+    if (stream && stream->id() == 0) return true;
     for (const auto& edge : at->next_edges()) left.push_back(edge.function.get());
   }
   return false;
@@ -217,10 +215,10 @@ struct Route : torch::autograd::Function<Route> {
     const Tensor d_weights = incoming(0), d_loss = incoming(4);
     TORCH_CHECK(!has_tangent(d_weights) && !has_tangent(d_loss),
                 "moe_route's gradient has no forward-mode derivative: it was given a dual tensor");
-    // The engine would join the leaf's stream to the capture, which for the default stream ends the process.
+    // The engine would join the next node's stream to the capture, which for the default stream ends the process.
     TORCH_CHECK(!is_capturing(z.device()) || !reaches_default_stream(torch::autograd::get_current_node().get()),
                 "moe_route: a backward pass is being captured while an eager graph of the same leaves, made on the default "
-                "stream, is alive: free it first, or make it on a side stream");
+                "stream, is alive (the logits' own, or another): free it first, or make it on a side stream");
     Tensor d = at::empty({z.size(0), z.size(1)}, z.options().requires_grad(false));
     if (z.size(0) > 0) {
       ggk_route_gradient_args a{};

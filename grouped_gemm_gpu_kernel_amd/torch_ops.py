@@ -426,8 +426,8 @@ def moe_route(logits: torch.Tensor, top_k: Optional[int] = None, *, ids: Optiona
     weights and balance_loss carry gradients to logits (f_e counts as a constant; no second derivative, and no
     forward-mode one: dual tensors are refused).  Everything runs on the
     current stream of the logits' device without waiting for it, and can be captured in a graph (its
-    backward pass too, unless an eager graph of the same leaves made on the default stream is alive, which is
-    refused); the same call gives the same bits.  E at most 1024, k at most 64."""
+    backward pass with it, unless that leads into an eager graph made on the default stream, the logits' own or
+    another of the same leaves that is alive, which is refused); the same call gives the same bits.  E at most 1024, k at most 64."""
     try:
         out = _binding().route(logits, top_k, ids, token_mask, normalize, scale, balance)
     except TypeError:  # an argument of another kind

@@ -673,6 +673,53 @@ def test_capture_with_an_eager_graph_alive_is_refused(torch_cuda, leaf):
 
 
 @pytest.mark.gpu
+def test_capture_that_reaches_an_eager_operator_is_refused(torch_cuda):
+    """The leaf's gradient belongs to a side stream, but the logits were made by an operator on the default stream."""
+    w = _logits(300, 16, "f32", 0).requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = w * 1.0
+    torch.cuda.current_stream().wait_stream(side)
+    z = w * 2.0
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(torch_ops.moe_route(z, 2, balance=True).balance_loss, z)
+    torch.cuda.synchronize()
+    del alive, graph
+    # eager calls go on as before
+    got, = torch.autograd.grad(torch_ops.moe_route(z, 2, balance=True).balance_loss, w)
+    leaf = z.detach().requires_grad_(True)
+    assert torch.equal(got, 2.0 * torch.autograd.grad(torch_ops.moe_route(leaf, 2, balance=True).balance_loss, leaf)[0])
+
+
+@pytest.mark.gpu
+def test_captured_with_an_eager_graph_of_a_side_stream_alive(torch_cuda):
+    static = _logits(300, 16, "f32", 0).requires_grad_(True)
+
+    def step(z):
+        return torch.autograd.grad(torch_ops.moe_route(z, 2, balance=True).balance_loss, z)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = torch_ops.moe_route(static, 2, balance=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for seed in range(1, 4):
+        fresh = _logits(300, 16, "f32", seed)
+        with torch.no_grad():
+            static.copy_(fresh)
+        graph.replay()
+        assert torch.equal(out, step(fresh.requires_grad_(True)))
+        torch.cuda.synchronize()
+    del alive
+
+
+@pytest.mark.gpu
 def test_captured_and_replayed(torch_cuda):
     """Forward and backward in a graph, replayed with new logits between the program's own calls."""
     static = _logits(700, 48, "f32", 0).requires_grad_(True)
