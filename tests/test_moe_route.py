@@ -11,6 +11,7 @@ the sum of the magnitudes that it is a difference of, and half a step of its typ
 import ctypes
 import math
 import subprocess
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -644,6 +645,48 @@ def test_streams_and_two_calls_at_once(torch_cuda):
     for a, b in zip(got, want):
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_calls_and_gradients_from_several_threads(torch_cuda):
+    out = [None] * 6
+
+    def work(i):
+        z = _logits(3000, 64, "f32", i).requires_grad_(True)
+        for _ in range(10):
+            r = torch_ops.moe_route(z, 4, balance=True)
+            out[i], = torch.autograd.grad(r.weights.square().sum() + r.balance_loss, z)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    together = list(out)
+    for i in range(6):
+        work(i)
+    assert all(torch.equal(a, b) for a, b in zip(together, out))
+
+
+@pytest.mark.gpu
+def test_saved_on_the_host_and_computed_again(torch_cuda):
+    """Saved logits that come back in other strides (padded rows, dense again from the host), and a checkpointed call."""
+    from torch.utils.checkpoint import checkpoint
+
+    z = _logits(300, 40, "bf16", 1)[:, 3:36].detach().requires_grad_(True)
+
+    def value(z):
+        r = torch_ops.moe_route(z, 4, balance=True)
+        return r.weights.square().sum() + r.balance_loss
+
+    want, = torch.autograd.grad(value(z), z)
+    with torch.autograd.graph.save_on_cpu():
+        assert torch.equal(torch.autograd.grad(value(z), z)[0], want)
+    assert torch.equal(torch.autograd.grad(checkpoint(value, z, use_reentrant=False), z)[0], want)
+    loss = value(z)
+    for _ in range(2):  # the same graph twice
+        assert torch.equal(torch.autograd.grad(loss, z, retain_graph=True)[0], want)
 
 
 @pytest.mark.gpu

@@ -586,6 +586,28 @@ def test_long_rows_past_32_bits(torch_cuda):
 
 
 @pytest.mark.gpu
+def test_more_row_tiles_than_a_grid_has(torch_cuda):
+    """Over 65535 tiles of 32 rows of one matrix, and as many slots that a workgroup of the experts' kernel makes hundreds of
+    items; whole numbers, exact."""
+    rows = 65536 * 32 + 77
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randint(-3, 4, (rows, 32), generator=g, device="cuda").half()
+    q, s, _ = _weights((6,), 9, 32, 32, False, 2)
+    s.fill_(1.0)
+    assert torch.equal(torch_ops.w4_matmul(x, q[0], s[0]).double(), x.double() @ values(q[0], s[0]).t())
+    x = x[:300000].contiguous()
+    ids = torch.randint(-1, 6, (300000, 2), generator=g, device="cuda")
+    flat = ids.flatten()
+    slot = torch.where(flat < 0, 6, flat)
+    counts, order = torch.bincount(slot, minlength=7)[:6].int(), slot.sort(stable=True).indices.int()
+    y = torch_ops.moe_w4_matmul(x, q, s, counts, order)
+    assert (y[flat < 0] == 0).all()
+    for e in range(6):
+        at = (flat == e).nonzero()[:, 0]
+        assert torch.equal(y[at].double(), x[at // 2].double() @ values(q[e], s[e]).t())
+
+
+@pytest.mark.gpu
 def test_streams_and_graphs(torch_cuda):
     q, s, z = _weights((6,), 70, 256, 64, True, 11)
     xs = [_x(24, 256, i) for i in range(5)]
