@@ -221,9 +221,12 @@ struct Workspace {
 
 __host__ __device__ inline int count_pitch(int experts) { return (experts + 4) / 4 * 4; }
 
-// At most this many entries of `count` are summed by every block of the order kernel itself: with 64 experts and
-// 16384 tokens, two launches of 256 blocks, 10.2 us, instead of three of 512, 11.6.  With 128 experts and 8192 tokens
-// (32 K entries) it took 15.0 us, against 12.9 with the columns kernel.
+// At most this many entries of `count` are summed by every block of the order kernel itself, and with 41 to 80 experts
+// there are fewer blocks so that they stay below it: two launches instead of three.  us of 16384 tokens without and with
+// the loss, so and with 512 blocks: 41 experts 10.4, 13.3 and 11.2, 15.5; 64 experts 9.8, 12.5 and 11.2, 15.4; 80 experts
+// 10.9, 17.0 and 12.0, 16.8.  65536 tokens have more to do than fewer blocks do well: 64 experts 17.7, 22.9 and 15.4, 19.4.
+// With 128 experts and 8192 tokens (32 K entries) the order kernel's own sums took 15.0, the columns kernel 12.9; limits of
+// 10, 20, 40, 80 and 160 K: 65521 tokens of 256 experts with the loss 49.5, 50.5, 49.8, 69.7 and 65.1.
 constexpr int kMaxOwnSums = 20 * 1024;
 constexpr int kMaxBlocks = 512;
 
@@ -238,10 +241,10 @@ Plan plan_blocks(int tokens, int experts) {
 }
 
 // So many tokens are routed by one workgroup.  Up to 256 experts it takes 64 at a time, at 16 lanes each: with 64 experts
-// 4.8 us for one token and 6.7 for 128, where two launches take 7.2 for 129 (256 experts: 8.3 and 17, two launches 11: the
-// second round of 64 loses there).  Above, a wave a token, it takes 16 at a
-// time: with 512 experts and 8 slots 8.7 us for 16, 12.9 for 32, 21.5 for 64 and 38.7 for 128, where two launches take 18.
-// (More than 16 slots also take a wave each, 20 of 64 experts 12.4, 20.8, 38.1 and 72, two launches 29; but the workspace's
+// 4.5 us for one token and 6.4 for 128, where two launches take 6.7 for 129 (256 experts: 8.1 and 16.5, two launches 10.8:
+// the second round of 64 loses there).  Above, a wave a token, it takes 16 at a
+// time: with 512 experts and 8 slots 8.3 us for 16, 12.6 for 32, 21.5 for 64 and 38.7 for 128, where two launches take 18.
+// (More than 16 slots also take a wave each, 20 of 64 experts 12, 21, 38 and 72, two launches 28; but the workspace's
 // size does not know the slots.)  The counts per wave have to fit 64 KB of LDS.
 bool is_small(int tokens, int experts) { return tokens <= (experts <= 256 ? 128 : 32) && experts <= 768; }
 

@@ -415,12 +415,16 @@ __device__ __forceinline__ void run_item(const Launch& l, const RowTile& t, int 
   }
 }
 
-// R: rows of an item, at most.  Measured, among others: one row of 4096 by 14336 columns, 30 MB, 9.4 us, of which the
-// workgroups' start is 3.2 and the rest runs at 4.9 TB/s, from the cache at 5.7; 64 experts' matrices of that size,
-// 256 slots on 46 of them, 1.4 GB, 312 us (4.5 TB/s, where a sum over 4 GB reads 4.0); 64 rows of 8192 by 8192 with
-// groups of 64, 24 us; by 8 waves it took 27, and 22 without the loads of x, 25 without unpacking, 26 without reading x
-// from LDS, 3.6 in the matrix instructions alone: the parts overlap badly with a barrier every 512 values of K, and
-// sharing x among more columns took off most.
+// R: rows of an item, at most.  Measured, in calls one behind the other (a dispatch in a trace takes up to 3 us more): one row of 4096 by 14336 columns, 30 MB, 8.8 us, of which the workgroups'
+// start is 3.2 and the rest runs at the cache's rate; 64 experts' matrices of that size, 256 slots on 46 of them, 1.4 GB, 312 to
+// 343 us from card to card (4.1 to 4.5 TB/s, where a sum over 4 GB reads 4.0).  64 rows of 8192 by 8192 with groups of 64
+// take 24 us, of which 13 are the issue of vector instructions alone: 7.9 M, 120 a wave and step, of them 44 to unpack, some
+// 36 for a scale every 32 values, the rest addresses and fetches of scales; each weight is unpacked for both row tiles.  By
+// 8 waves it took 27, and 22 without the loads of x, 25 without unpacking, 26 without reading x from LDS.
+// Groups that are not whole steps cost the experts' rows the same: 64 experts of that size, all with slots, with zero points
+// 423 us in groups of 128, 652 of 64, 739 of 32 (555 of 64 without zero points).  The registers are at their bound there:
+// experts' items of 32 rows in such groups spill 12 of them (4 without zero points), and of 16 rows with one wave along K
+// and zero points 7, none of it inside the loops over K.
 template <int WAVES, int R, int WK, bool EXPERTS, bool FINE, bool ZEROS>
 __global__ __launch_bounds__(WAVES * kWave, 4) void w4_kernel(Launch l) {
   const ggk_w4_args& a = l.a;
@@ -543,7 +547,12 @@ extern "C" hipError_t ggk_w4_multiply(const ggk_w4_args* args, hipStream_t strea
   const ggk_w4_args& a = *args;
   const long long columns = (a.n + 15) / 16;
   if (a.experts > 0) {
-    // Waves that split K, where there are few without.
+    // Waves that split K, where there are few without.  us of the forms (rows, waves along K) (32, 1), (16, 1), (16, 2) and
+    // (16, 4), groups of 128, two slots a token: 64 experts of 4096 by 14336, 128 tokens 410, 398, 430, 503; 8 tokens 94, 91,
+    // 98, 109; one 15.7, 15.8, 15.9, 17.9; of 14336 by 4096, 8 tokens 95, 93, 88, 93, one 39, 39, 23, 15; 16 experts of 1024 by
+    // 2048, 512 slots 13.6, 14.4, 16.9, 21.5, by 512 9.5, 7.8, 8.1, 8.4; 8 experts of 4096 by 2048, one token 14.0, 14.1, 9.0,
+    // 6.7, by 8192 14.8, 14.8, 10.0, 9.6; 300 experts of 1024 by 1024, 1024 slots -, 42, 47, 70.  The rule is right for many
+    // slots; it does not look at K, which costs one token up to 1.5 times the best form.
     const long long waves = columns * min(a.rows, a.experts);
     if (waves >= 1024 && a.experts <= kTable<32>) return launch<32, 1, true>(a, stream);
     if (waves >= 512) return waves >= 1024 ? launch<16, 1, true>(a, stream) : launch<16, 2, true>(a, stream);
