@@ -173,7 +173,8 @@ def build_host_sanitized(out_path: Path) -> Path:
 
 def torch_binding_lacks() -> str | None:
     """What the C++ part of torch_ops cannot be built without and is not there; None if all of it is."""
-    if importlib.util.find_spec("torch") is None:
+    torch = importlib.util.find_spec("torch")
+    if torch is None or torch.origin is None:  # not there, or a folder that only has its name
         return "torch is not installed"
     headers = Path(sysconfig.get_paths()["include"])
     return None if (headers / "Python.h").exists() else f"{headers} has no Python.h"

@@ -1,5 +1,6 @@
 """The build recipe where torch, or the Python headers, are missing: everything but the PyTorch binding is
 built, as C, C++ and ctypes users need it.  A binding that was built for another torch is refused."""
+import importlib.machinery
 import importlib.util
 import sysconfig
 
@@ -21,11 +22,12 @@ def made(monkeypatch):
     return steps
 
 
-@pytest.fixture(params=["torch", "headers"])
+@pytest.fixture(params=["torch", "folder", "headers"])
 def missing(request, monkeypatch, tmp_path):
-    if request.param == "torch":
+    if request.param != "headers":
         found = importlib.util.find_spec
-        monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else found(name, *a))
+        torch = None if request.param == "torch" else importlib.machinery.ModuleSpec("torch", None, is_package=True)
+        monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: torch if name == "torch" else found(name, *a))
     else:
         paths = {**sysconfig.get_paths(), "include": str(tmp_path)}
         monkeypatch.setattr(sysconfig, "get_paths", lambda *a, **k: paths)
@@ -40,7 +42,7 @@ def test_everything_else_is_built(made, missing, capsys):
     assert made == OTHERS
     out = capsys.readouterr().out
     assert out.count("gg_torch.so is not built") == 2
-    assert ("torch is not installed" if missing == "torch" else "no Python.h") in out
+    assert ("no Python.h" if missing == "headers" else "torch is not installed") in out
 
 
 def test_no_torch_asks_for_nothing(made, missing, capsys):
