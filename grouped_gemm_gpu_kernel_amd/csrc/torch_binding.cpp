@@ -212,9 +212,9 @@ struct Route : torch::autograd::Function<Route> {
                                                                                    : grads[i].resolve_neg().contiguous();
     };
     if (!grads[0].defined() && (grads.size() < 5 || !grads[4].defined())) return {Tensor(), Tensor()};
-    const Tensor d_weights = incoming(0), d_loss = incoming(4);
-    TORCH_CHECK(!has_tangent(d_weights) && !has_tangent(d_loss),
+    TORCH_CHECK(!has_tangent(grads[0]) && (grads.size() < 5 || !has_tangent(grads[4])),
                 "moe_route's gradient has no forward-mode derivative: it was given a dual tensor");
+    const Tensor d_weights = incoming(0), d_loss = incoming(4);
     // The engine would join the next node's stream to the capture, which for the default stream ends the process.
     TORCH_CHECK(!is_capturing(z.device()) || !reaches_default_stream(torch::autograd::get_current_node().get()),
                 "moe_route: a backward pass is being captured while an eager graph of the same leaves, made on the default "
