@@ -573,6 +573,36 @@ def test_loss_over_many_tokens(torch_cuda, tokens, experts, top_k, step):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,slots,dtype", [(2 ** 21 + 11, 8, 2, "f32"), (1200007, 256, 4, "bf16"),
+                                                        (1100003, 100, 3, "f16"), (400009, 520, 2, "f32")])
+def test_loss_of_many_padded_tokens_and_given_experts(torch_cuda, tokens, experts, slots, dtype):
+    """Random logits with sums of p in runs, padding, closed experts and experts given; against float64 of the same logits.
+
+    The sums' chains as in test_loss_over_many_tokens (226 u in all), p off by (d + 32) u as for the weights."""
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    z = (torch.randn(tokens, experts, generator=g, device="cuda") * 2).to(TYPES[dtype])
+    z[:, 3].masked_fill_(torch.rand(tokens, generator=g, device="cuda") < 0.3, -math.inf)
+    mask = torch.rand(tokens, generator=g, device="cuda") < 0.9
+    for ids in (None, torch.randint(-1, experts, (tokens, slots), generator=g, device="cuda", dtype=torch.int32)):
+        r = torch_ops.moe_route(z, slots if ids is None else None, ids=ids, token_mask=mask, balance=True)
+        routed = (r.ids >= 0).any(1)
+        if ids is None:
+            assert torch.equal(routed, mask)
+        p, spread = torch.zeros(experts, dtype=torch.float64, device="cuda"), 0.0
+        for part, on in zip(z.split(1 << 17), routed.split(1 << 17)):
+            part = part[on].double()
+            p += torch.softmax(part, 1).sum(0)
+            spread = max(spread, float(part.amax() - part.masked_fill(part == -math.inf, math.inf).amin()))
+        chosen = r.ids[r.ids >= 0].long()
+        counts = torch.bincount(chosen, minlength=experts)
+        assert torch.equal(r.counts.long(), counts)
+        want = experts * float((counts / len(chosen) * p).sum() / routed.sum())
+        assert abs(float(r.balance_loss) - want) <= (226 + spread + 32) * U * want
+        flat = torch.where(r.ids < 0, experts, r.ids).flatten()
+        assert torch.equal(r.order.long(), flat.sort(stable=True).indices)
+
+
+@pytest.mark.gpu
 def test_rows_past_32_bits(torch_cuda):
     """Logits whose last rows lie past 2^31 elements: 9 GB of bfloat16, of which a few rows are looked at."""
     experts, tokens = 1024, 2 ** 31 // 1024 + 1000
