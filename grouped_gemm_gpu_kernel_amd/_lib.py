@@ -51,6 +51,12 @@ GGK_TYPE_F32, GGK_TYPE_F16, GGK_TYPE_BF16 = 0, 1, 2
 GGK_ROUTE_MAX_SLOTS = 64
 GGK_ROUTE_MAX_TOTAL_SLOTS = 1 << 30
 GGK_W4_MAX_EXTENT = 1 << 28
+GGK_FP8_BLOCK = 128
+GGK_NORM_MAX_COLUMNS = 32768
+GGK_GATE_NONE, GGK_GATE_SILU, GGK_GATE_GELU = 0, 1, 2
+GGK_FP8_MAX_N = 1 << 28
+GGK_FP8_MAX_K = 1 << 22
+GGK_FP8_MAX_LD = 1 << 22
 
 c_int_p = ctypes.POINTER(ctypes.c_int)
 c_ll_p = ctypes.POINTER(ctypes.c_longlong)
@@ -175,6 +181,33 @@ class GGKW4Args(ctypes.Structure):
     ]
 
 
+class GGKNormFp8Args(ctypes.Structure):
+    """ggk_norm_fp8_args (grouped_gemm_amd_kernels.h)"""
+    _fields_ = [
+        ("rows", ctypes.c_int), ("columns", ctypes.c_int), ("type", ctypes.c_int), ("weight_type", ctypes.c_int),
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_longlong),
+        ("weight", ctypes.c_void_p), ("eps", ctypes.c_float),
+        ("q", ctypes.c_void_p), ("ldq", ctypes.c_longlong), ("scales", ctypes.c_void_p), ("lds", ctypes.c_longlong),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong), ("sum", ctypes.c_void_p), ("ldsum", ctypes.c_longlong),
+    ]
+
+
+class GGKFp8Args(ctypes.Structure):
+    """ggk_fp8_args (grouped_gemm_amd_kernels.h)"""
+    _fields_ = [
+        ("rows", ctypes.c_int), ("x_rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int),
+        ("experts", ctypes.c_int), ("gate", ctypes.c_int),
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong), ("x_scales", ctypes.c_void_p), ("ldxs", ctypes.c_longlong),
+        ("w", ctypes.c_void_p), ("ldw", ctypes.c_longlong), ("stride_w", ctypes.c_longlong),
+        ("w_scales", ctypes.c_void_p), ("ldws", ctypes.c_longlong), ("stride_ws", ctypes.c_longlong),
+        ("up", ctypes.c_void_p), ("ldu", ctypes.c_longlong), ("stride_u", ctypes.c_longlong),
+        ("up_scales", ctypes.c_void_p), ("ldus", ctypes.c_longlong), ("stride_us", ctypes.c_longlong),
+        ("counts", ctypes.c_void_p), ("order", ctypes.c_void_p), ("row_weights", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong), ("y_type", ctypes.c_int),
+        ("y_scales", ctypes.c_void_p), ("ldys", ctypes.c_longlong),
+    ]
+
+
 _P = ctypes.POINTER
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -245,6 +278,10 @@ SIGNATURES = {
     "ggk_route_gradient": (_i, [_P(GGKRouteGradientArgs), _vp]),
     "ggk_w4_check": (_i, [_P(GGKW4Args)]),
     "ggk_w4_multiply": (_i, [_P(GGKW4Args), _vp]),
+    "ggk_norm_fp8_check": (_i, [_P(GGKNormFp8Args)]),
+    "ggk_norm_fp8": (_i, [_P(GGKNormFp8Args), _vp]),
+    "ggk_fp8_check": (_i, [_P(GGKFp8Args)]),
+    "ggk_fp8_multiply": (_i, [_P(GGKFp8Args), _vp]),
     "ggk_launch_grouped_device": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp]),
     "ggk_launch_grouped_device_done": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, c_int_p, _vp]),
     "ggk_kernel_resources_get": (_i, [_i, _i, _i, _P(GGKKernelResources)]),

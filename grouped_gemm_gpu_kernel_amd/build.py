@@ -31,7 +31,7 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC_DIR = PKG / "csrc"
 BUILD = PKG / "_build"
-DEVICE_SOURCES = ["gg_moe.hip", "gg_route.hip", "gg_w4.hip"]  # beside gg_kernels.hip, whose resources are reported
+DEVICE_SOURCES = ["gg_moe.hip", "gg_route.hip", "gg_w4.hip", "gg_norm.hip", "gg_fp8.hip"]  # beside gg_kernels.hip, whose resources are reported
 LIB_DIR = PKG / "lib"
 LIB_NAME = "libgrouped_gemm_amd.so"
 FORMS_NAME = "gg_kernel_forms.json"  # resources of every compiled kernel form, beside the objects
@@ -186,7 +186,7 @@ def build_torch_binding() -> Path | None:
     are missing: the C, C++ and ctypes sides do without."""
     lacks = torch_binding_lacks()
     if lacks is not None:
-        print(f"gg_torch.so is not built: {lacks} (the PyTorch routing and 4-bit products need it)")
+        print(f"gg_torch.so is not built: {lacks} (the PyTorch routing, 4-bit and 8-bit products need it)")
         return None
     torch = Path(importlib.util.find_spec("torch").origin).parent
     out = LIB_DIR / "gg_torch.so"

@@ -1,0 +1,148 @@
+// gg_fp8.h -- what the kernels of the 8-bit products share: loads straight into
+// LDS by address, fragments, the matrix instructions, the end of a product.
+//
+// A step of K is 128 values, one block of scales: 128 bytes of a row of x or w.  In LDS a row's eight 16-byte pieces
+// stand at piece ^ ((row >> 1) & 7), so that the 16 rows that a fragment read touches at once hit every bank once (64
+// banks hold two rows).  The matrix instructions take a lane's 32 values of a row in any order as long as it is the
+// same for both operands: lane group g (of 16 lanes) takes pieces g and g + 4, whose addresses differ in bit 6.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gg_common.h"
+#include "gg_fp8_rows.h"
+#include "grouped_gemm_amd_kernels.h"
+
+namespace gg {
+namespace fp8 {
+
+typedef int int8v __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+
+constexpr int kStep = GGK_FP8_BLOCK;
+constexpr uint32_t kOutOfRange = 0x80000000u;  // an offset past every resource's records: reads 0
+
+// What stands in for values of x at k >= K.
+static __device__ const uint4v kZeros = {0, 0, 0, 0};
+
+// 16 (4) bytes a lane from its own 64-bit address to 1 KB (256 bytes) of LDS in lane order; see load_to_lds16 for the wait
+// states.
+__device__ __forceinline__ void load_to_lds16_at(const void* p, uint32_t lds) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, off" : : "{m0}"(m0), "v"(p) : "memory");
+}
+__device__ __forceinline__ void load_to_lds4_at(const void* p, uint32_t lds) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %1, off" : : "{m0}"(m0), "v"(p) : "memory");
+}
+
+// The 32 numbers of a lane: a row's 128 bytes at `at` (LDS byte address, its swizzled piece g).
+__device__ __forceinline__ int8v read_fragment(uint32_t at) {
+  const uint4v lo = *(const GG_LDS uint4v*)(uintptr_t)at;
+  const uint4v hi = *(const GG_LDS uint4v*)(uintptr_t)(at ^ 64u);
+  return int8v{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
+
+// The same numbers in binary16, exactly (e4m3 has 4 significant bits and exponents from -9 to 8).
+struct Halves {
+  half8v v[4];
+};
+__device__ __forceinline__ Halves to_halves(const int8v& q) {
+  Halves h;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const half2v lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q[i], 1.0f, false);
+    const half2v hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q[i], 1.0f, true);
+    h.v[i / 2][4 * (i % 2) + 0] = lo[0];
+    h.v[i / 2][4 * (i % 2) + 1] = lo[1];
+    h.v[i / 2][4 * (i % 2) + 2] = hi[0];
+    h.v[i / 2][4 * (i % 2) + 3] = hi[1];
+  }
+  return h;
+}
+
+// Products of a step, 16 rows of w by 16 of x: lane (g, j) gets rows 4 g .. 4 g + 3 of w by row j of x.  The 8-bit
+// instruction aligns its products eight at a time to the largest one's power of two and drops what lies 13 bits and more
+// below (measured: 1.5e-5 of the sum's norm on normal values); sums of those groups are float.  In binary16 the products
+// and sums are float's: 1e-7.
+__device__ __forceinline__ float4v multiply(const int8v& w, const int8v& x) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ float4v multiply(const Halves& w, const Halves& x) {
+  float4v p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], x.v[i], p, 0, 0, 0);
+  return p;
+}
+
+// act(p) * u.
+__device__ __forceinline__ float gated(int gate, float p, float u) {
+  float z = p;
+  if (gate == GGK_GATE_GELU) {  // (1 + tanh(t)) / 2 = 1 / (1 + exp(-2 t))
+    z = 1.5957691216057308f * p * fmaf(0.044715f * p, p, 1.0f);
+  }
+  return p / (1.0f + expf(-z)) * u;
+}
+
+__device__ __forceinline__ void store_value(void* y, int type, long long at, float v) {
+  if (type == GGK_TYPE_BF16) {
+    static_cast<__bf16*>(y)[at] = (__bf16)v;
+  } else if (type == GGK_TYPE_F16) {
+    static_cast<_Float16*>(y)[at] = (_Float16)v;
+  } else {
+    static_cast<float*>(y)[at] = v;
+  }
+}
+
+// Columns j .. j + 3 of a row at offset `at` (in values); vec: they all exist and start on a multiple of 4 values.
+__device__ __forceinline__ void store4(void* y, int type, long long at, int count, bool vec, const float4v& v) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i < count) store_value(y, type, at + i, v[i]);
+    }
+  } else if (type == GGK_TYPE_F32) {
+    *reinterpret_cast<float4v*>(static_cast<float*>(y) + at) = v;
+  } else {
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = type == GGK_TYPE_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+    }
+    *reinterpret_cast<uint2v*>(static_cast<uint16_t*>(y) + at) =
+        uint2v{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
+  }
+}
+
+// Eight neighbouring columns j .. j + 7 of a block of an 8-bit row, by 16 neighbouring lanes for the block's 128; columns
+// past n count as 0.
+__device__ __forceinline__ void store_numbers(const ggk_fp8_args& a, long long row, int j, float (&v)[8], bool write) {
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (j + i >= a.n) v[i] = 0.0f;
+    largest = max(largest, magnitude_bits(v[i]));
+  }
+  const float scale = fp8_scale(row_max16(largest));
+  const Fp8Divisor by(scale);
+  const uint2v numbers = {fp8_numbers(v[0], v[1], v[2], v[3], by), fp8_numbers(v[4], v[5], v[6], v[7], by)};
+  if (!write || j >= a.n) return;
+  unsigned char* y = static_cast<unsigned char*>(a.y) + row * a.ldy + j;
+  if (j + 8 <= a.n && reinterpret_cast<uintptr_t>(y) % 8 == 0) {
+    *reinterpret_cast<uint2v*>(y) = numbers;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (j + i < a.n) y[i] = (unsigned char)(numbers[i / 4] >> (8 * (i % 4)));
+    }
+  }
+  if (j % kFp8Block == 0) a.y_scales[row * a.ldys + j / kFp8Block] = scale;
+}
+
+}  // namespace fp8
+}  // namespace gg

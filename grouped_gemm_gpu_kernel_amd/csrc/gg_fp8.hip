@@ -1,0 +1,328 @@
+// gg_fp8.hip -- products of few rows with matrices of 8-bit numbers, one matrix
+// or one an expert, plain or gated:
+//
+//   p[i][j] = sum over blocks b of x_scales[i][b] w_scales[j / 128][b] * sum over k in b of x[i][k] w[j][k]
+//
+// With few rows the weights' bytes are what counts.  Every wave streams its own columns through a ring of steps of its
+// own in LDS, loaded there directly, several steps ahead, with x's rows and the scales of the same step beside them: no
+// wave waits for another until its sums are whole.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gg_experts.h"
+#include "gg_fp8.h"
+
+namespace {
+
+using namespace gg::fp8;
+using gg::Experts;
+using gg::RowTile;
+using gg::kWave;
+
+constexpr int kCus = 256;
+
+struct Launch {
+  ggk_fp8_args a;
+  int blocks;  // of columns
+};
+
+// R rows of x (8, 16, 32, 64) by WN waves of NT tiles of 16 columns (with a gate: half of them gate, half up), WK waves
+// along K, DEPTH steps in a wave's ring.
+template <int R_, int NT_, int WN_, int WK_, int DEPTH_, bool GATED_, bool EXACT_>
+struct Form {
+  static constexpr int R = R_, NT = NT_, WN = WN_, WK = WK_, DEPTH = DEPTH_;
+  static constexpr bool GATED = GATED_, EXACT = EXACT_;
+  static constexpr int MT = (R + 15) / 16, WAVES = WN * WK, THREADS = WAVES * kWave;
+  static constexpr int WL = 2 * NT, XL = R / 8, SL = R == 64 ? 2 : 1;  // load instructions of a step
+  static constexpr int LOADS = WL + XL + SL;
+  static constexpr int X = 1024 * WL, S = X + 1024 * XL, STEP = S + 256 * SL;  // offsets in a step, and its bytes
+  static constexpr int WS = R == 64 ? 64 : 32;                                 // place of the weights' scales among the step's
+  static constexpr int COLUMNS = WN * 16 * NT / (GATED ? 2 : 1);               // of y a workgroup computes
+  static constexpr int SUM_LD = WN * 16 * NT + 4;
+  static constexpr int RING = WAVES * DEPTH * STEP, SUMS = 4 * WK * MT * 16 * SUM_LD;
+  static constexpr int BYTES = RING > SUMS ? RING : SUMS;
+  static_assert(LOADS * (DEPTH - 1) < 64, "outstanding loads are counted in 6 bits");
+  static_assert(!GATED || COLUMNS == 128, "a block of an 8-bit row");
+};
+
+// The wave's sums over its steps of K of one tile of rows by its columns.
+template <class F>
+__device__ __forceinline__ void multiply_item(const ggk_fp8_args& a, const RowTile& t, const int* x_row, int column0,
+                                              unsigned char* ring, float4v (&sum)[F::MT][F::NT]) {
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wk = wave % F::WK;
+  const int steps = (a.k + kStep - 1) / kStep, mine = (steps - wk + F::WK - 1) / F::WK;
+  const uint32_t ring_at = gg::lds_address(ring);
+  constexpr int kTilesOfW = F::GATED ? F::NT / 2 : F::NT;
+
+  // The lane's part of a load of 8 rows: row lane / 8, piece by the row's swizzle, which the instruction's parity flips.
+  const int part = lane / 8, piece = (lane & 7) ^ (lane >> 4);
+  uint32_t w_off[F::WL];
+  const int base_column = min(column0, a.n - 1);
+#pragma unroll
+  for (int q = 0; q < F::WL; ++q) {
+    const int tile = q / 2 % kTilesOfW, column = min(column0 + 16 * tile + 8 * (q & 1) + part, a.n - 1);
+    const long long ld = F::GATED && q / 2 >= kTilesOfW ? a.ldu : a.ldw;
+    w_off[q] = (uint32_t)((column - base_column) * ld) + 16 * (piece ^ (4 * (q & 1)));
+  }
+  const unsigned char* w0 = a.w + t.expert * a.stride_w + base_column * a.ldw;
+  const unsigned char* u0 = F::GATED ? a.up + t.expert * a.stride_u + base_column * a.ldu : nullptr;
+  const unsigned char* xp[F::XL];
+#pragma unroll
+  for (int q = 0; q < F::XL; ++q) {
+    const int r = min(8 * q + part, t.rows - 1);
+    xp[q] = a.x + (x_row != nullptr ? x_row[r] : t.first + r) * a.ldx + 16 * (piece ^ (4 * (q & 1)));
+  }
+  const int scale_row = min(F::R == 64 ? lane : lane % 32, t.rows - 1);
+  const float* xs = a.x_scales + (x_row != nullptr ? x_row[scale_row] : t.first + scale_row) * a.ldxs;
+  const float* ws = a.w_scales + t.expert * a.stride_ws + base_column / kStep * a.ldws;
+  if (F::GATED && lane % 32 == 1) ws = a.up_scales + t.expert * a.stride_us + base_column / kStep * a.ldus;
+  if (F::SL == 1 && lane >= 32) xs = ws;
+
+  auto issue = [&](int i) {  // the wave's step i into its place of the ring
+    const int step = i * F::WK + wk, k0 = step * kStep;
+    const uint32_t at = ring_at + (i % F::DEPTH) * F::STEP;
+    const bool whole = k0 + kStep <= a.k;
+#pragma unroll
+    for (int q = 0; q < F::WL; ++q) {
+      const bool in = whole || k0 + 16 * (piece ^ (4 * (q & 1))) < a.k;
+      gg::load_to_lds16((F::GATED && q / 2 >= kTilesOfW ? u0 : w0) + k0, kOutOfRange, at + 1024 * q, in ? w_off[q] : kOutOfRange, 0);
+    }
+#pragma unroll
+    for (int q = 0; q < F::XL; ++q) {
+      const bool in = whole || k0 + 16 * (piece ^ (4 * (q & 1))) < a.k;
+      load_to_lds16_at(in ? (const void*)(xp[q] + k0) : (const void*)&kZeros, at + F::X + 1024 * q);
+    }
+    load_to_lds4_at(xs + step, at + F::S);
+    if constexpr (F::SL == 2) load_to_lds4_at(ws + step, at + F::S + 256);
+  };
+
+#pragma unroll
+  for (int m = 0; m < F::MT; ++m) {
+#pragma unroll
+    for (int n = 0; n < F::NT; ++n) sum[m][n] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+#pragma unroll
+  for (int i = 0; i < F::DEPTH - 1; ++i) {
+    if (i < mine) issue(i);
+  }
+  const int j = lane % 16, g = lane / 16, x_j = F::R < 16 ? j % 8 : j;
+  const uint32_t w_at = j * 128 + ((g ^ (j >> 1)) & 7) * 16, x_at = F::X + x_j * 128 + ((g ^ (x_j >> 1)) & 7) * 16;
+#pragma unroll 1
+  for (int i = 0; i < mine; ++i) {
+    // Step i has landed when at most the loads of the DEPTH - 2 steps after it are on their way.
+    if (i + F::DEPTH - 1 <= mine) {
+      gg::wait_vmcnt<F::LOADS * (F::DEPTH - 2)>();
+    } else {
+      gg::wait_vmcnt<0>();
+    }
+    asm volatile("" ::: "memory");
+    const uint32_t at = ring_at + (i % F::DEPTH) * F::STEP;
+    using Operand = std::conditional_t<F::EXACT, Halves, int8v>;
+    auto read = [&](uint32_t from) {
+      if constexpr (F::EXACT) {
+        return to_halves(read_fragment(from));
+      } else {
+        return read_fragment(from);
+      }
+    };
+    Operand w[F::NT];
+#pragma unroll
+    for (int n = 0; n < F::NT; ++n) w[n] = read(at + w_at + 2048 * n);
+    const float w_scale = *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * F::WS);
+    const float u_scale = F::GATED ? *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * F::WS + 4) : 0.0f;
+    // The place of step i - 1 is free: every read of it has returned before its products were made.
+    if (i + F::DEPTH - 1 < mine) issue(i + F::DEPTH - 1);
+#pragma unroll
+    for (int m = 0; m < F::MT; ++m) {
+      const Operand x = read(at + x_at + 2048 * m);
+      const float x_scale = *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * (16 * m + x_j));
+      const float scale = x_scale * w_scale, scale_u = F::GATED ? x_scale * u_scale : 0.0f;
+#pragma unroll
+      for (int n = 0; n < F::NT; ++n) {
+        const float4v part_sum = multiply(w[n], x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[m][n][e] = fmaf(n < kTilesOfW ? scale : scale_u, part_sum[e], sum[m][n][e]);
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
+}
+
+// One tile of rows by the workgroup's columns from block0 on: sums, their join over the waves along K, y.
+template <class F, bool EXPERTS>
+__device__ __forceinline__ void run_item(const ggk_fp8_args& a, const RowTile& t, const int* slots, const int* x_row,
+                                         int block0, unsigned char* s_bytes) {
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int j = lane % 16, g = lane / 16, wn = wave / F::WK, wk = wave % F::WK;
+  float4v sum[F::MT][F::NT];
+  multiply_item<F>(a, t, x_row, block0 + wn * (F::COLUMNS / F::WN), s_bytes + wave * F::DEPTH * F::STEP, sum);
+  const bool vec = a.n % 4 == 0 && (a.ldy % 4 == 0 || a.rows <= 1) && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
+  float* s_sum = reinterpret_cast<float*>(s_bytes);  // [WK][16 MT][SUM_LD]
+  gg::stage_barrier();
+#pragma unroll
+  for (int m = 0; m < F::MT; ++m) {
+#pragma unroll
+    for (int n = 0; n < F::NT; ++n) {
+      *reinterpret_cast<float4v*>(&s_sum[(wk * 16 * F::MT + 16 * m + j) * F::SUM_LD + (wn * F::NT + n) * 16 + 4 * g]) = sum[m][n];
+    }
+  }
+  gg::stage_barrier();
+  auto total = [&](int r, int c) {
+    float4v v = *reinterpret_cast<const float4v*>(&s_sum[r * F::SUM_LD + c]);
+#pragma unroll
+    for (int w = 1; w < F::WK; ++w) v += *reinterpret_cast<const float4v*>(&s_sum[(w * 16 * F::MT + r) * F::SUM_LD + c]);
+    return v;
+  };
+  if constexpr (!F::GATED) {
+    constexpr int kFours = F::COLUMNS / 4;
+    for (int i = tid; i < t.rows * kFours; i += F::THREADS) {
+      const int r = i / kFours, c = i % kFours * 4, column = block0 + c, slot = EXPERTS ? slots[r] : t.first + r;
+      if (column < a.n && slot >= 0) {
+        float4v v = total(r, c);
+        if (a.row_weights != nullptr) v *= a.row_weights[slot];
+        store4(a.y, a.y_type, slot * a.ldy + column, a.n - column, vec, v);
+      }
+    }
+  } else {
+    // Sums stand as [wave][gate or up][columns]; 16 lanes take the block of a row, 8 columns each.
+    constexpr int kHalf = F::NT / 2 * 16;
+    for (int i = tid; i < (t.rows * 16 + F::THREADS - 1) / F::THREADS * F::THREADS; i += F::THREADS) {
+      const int r = min(i / 16, t.rows - 1), c = i % 16 * 8, at = c / kHalf * 2 * kHalf + c % kHalf;
+      float v[8];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float4v p = total(r, at + 4 * half), u = total(r, at + 4 * half + kHalf);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * half + e] = gated(a.gate, p[e], u[e]);
+      }
+      const int slot = EXPERTS ? slots[r] : t.first + r;
+      store_numbers(a, slot, block0 + c, v, i / 16 < t.rows && slot >= 0);
+    }
+  }
+}
+
+// Rows without an expert.
+template <class F>
+__device__ __forceinline__ void clear_item(const ggk_fp8_args& a, const RowTile& t, const int* slots, int block0) {
+  for (int i = threadIdx.x; i < t.rows * F::COLUMNS; i += F::THREADS) {
+    const int slot = slots[i / F::COLUMNS], column = block0 + i % F::COLUMNS;
+    if (column >= a.n || slot < 0) continue;
+    if constexpr (F::GATED) {
+      static_cast<unsigned char*>(a.y)[slot * a.ldy + column] = 0;
+      if (column % kStep == 0) a.y_scales[slot * a.ldys + column / kStep] = gg::kFp8SmallestScale;
+    } else {
+      store_value(a.y, a.y_type, slot * a.ldy + column, 0.0f);
+    }
+  }
+}
+
+template <class F, bool EXPERTS>
+__global__ __launch_bounds__(F::THREADS, 2) void fp8_stream_kernel(Launch l) {
+  const ggk_fp8_args& a = l.a;
+  __shared__ alignas(128) unsigned char s_bytes[F::BYTES];
+  if constexpr (!EXPERTS) {
+    const int tiles = (a.rows + F::R - 1) / F::R;
+    for (int tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
+      const RowTile t{0, tile * F::R, min(F::R, a.rows - tile * F::R)};
+      run_item<F, false>(a, t, nullptr, nullptr, blockIdx.x * F::COLUMNS, s_bytes);
+      gg::stage_barrier();
+    }
+  } else {
+    __shared__ int s_slot[F::R], s_x_row[F::R];
+    __shared__ Experts<GGK_MOE_MAX_EXPERTS> s_experts;
+    const int fan = a.rows / a.x_rows;
+    gg::list_experts<F::THREADS, F::R>(a, s_experts);
+    const long long items = (long long)s_experts.tile[a.experts + 1] * l.blocks;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+      const int tile = (int)(item / l.blocks), block = (int)(item % l.blocks);
+      const RowTile t = gg::expert_tile<F::R>(a, s_experts, tile);
+      for (int i = threadIdx.x; i < t.rows; i += F::THREADS) {
+        int slot = a.order[t.first + i];
+        if (slot >= a.rows) slot = -1;
+        s_slot[i] = slot;
+        s_x_row[i] = max(slot, 0) / fan;  // where a slot names no row, row 0: its sums are not used
+      }
+      gg::stage_barrier();
+      if (t.expert == a.experts) {
+        clear_item<F>(a, t, s_slot, block * F::COLUMNS);
+      } else {
+        run_item<F, true>(a, t, s_slot, s_x_row, block * F::COLUMNS, s_bytes);
+      }
+      gg::stage_barrier();
+    }
+  }
+}
+
+template <class F, bool EXPERTS>
+hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
+  Launch l{a, (a.n + F::COLUMNS - 1) / F::COLUMNS};
+  const long long tiles = (a.rows + F::R - 1) / F::R + (EXPERTS ? (a.rows < a.experts + 1 ? a.rows : a.experts + 1) : 0);
+  dim3 grid(l.blocks, (unsigned)(tiles < 65535 ? tiles : 65535));
+  if (EXPERTS) {
+    const long long items = tiles * l.blocks, most = kCus * (F::BYTES > 64 * 1024 ? 1 : 2);
+    grid = dim3((unsigned)(items < most ? items : most));
+  }
+  hipLaunchKernelGGL((fp8_stream_kernel<F, EXPERTS>), grid, dim3(F::THREADS), 0, stream, l);
+  return hipGetLastError();
+}
+
+template <bool EXPERTS>
+hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
+  const int rows = EXPERTS ? (a.rows + a.experts - 1) / a.experts : a.rows;
+  if (a.gate != GGK_GATE_NONE) {
+    if (rows <= 8) return launch<Form<8, 2, 8, 1, 3, true, true>, EXPERTS>(a, stream);
+    return launch<Form<16, 2, 8, 1, 2, true, true>, EXPERTS>(a, stream);
+  }
+  if (rows <= 8) return launch<Form<8, 1, 2, 4, 4, false, true>, EXPERTS>(a, stream);
+  if (rows <= 16) return launch<Form<16, 1, 2, 4, 4, false, true>, EXPERTS>(a, stream);
+  return launch<Form<32, 2, 2, 4, 2, false, true>, EXPERTS>(a, stream);
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+
+extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
+  if (args == nullptr) return hipErrorInvalidValue;
+  const ggk_fp8_args& a = *args;
+  const bool gate = a.gate != GGK_GATE_NONE;
+  if (a.rows < 0 || a.rows > GGK_ROUTE_MAX_TOTAL_SLOTS || a.x_rows < 0 || a.n < 0 || a.n > GGK_FP8_MAX_N || a.k < 16 ||
+      a.k > GGK_FP8_MAX_K || a.k % 16 != 0 || a.experts < 0 || a.experts > GGK_MOE_MAX_EXPERTS ||
+      a.gate < GGK_GATE_NONE || a.gate > GGK_GATE_GELU ||
+      (!gate && a.y_type != GGK_TYPE_F32 && a.y_type != GGK_TYPE_F16 && a.y_type != GGK_TYPE_BF16) ||
+      (gate && a.row_weights != nullptr)) {
+    return hipErrorInvalidValue;
+  }
+  if (a.experts == 0 ? a.rows != a.x_rows : (a.rows > 0 && (a.x_rows < 1 || a.rows % a.x_rows != 0))) {
+    return hipErrorInvalidValue;
+  }
+  const long long blocks_k = (a.k + kStep - 1) / kStep, blocks_n = (a.n + kStep - 1) / kStep;
+  const auto matrix = [&](const void* w, long long ld, long long stride, long long lds, long long stride_s) {
+    if (a.n > 1 && (ld < a.k || ld > GGK_FP8_MAX_LD || ld % 16 != 0)) return false;
+    if (blocks_n > 1 && lds < blocks_k) return false;
+    return aligned16(w) && stride >= 0 && stride_s >= 0 && (a.experts <= 1 || stride % 16 == 0);
+  };
+  if (!matrix(a.w, a.ldw, a.stride_w, a.ldws, a.stride_ws) ||
+      (gate && !matrix(a.up, a.ldu, a.stride_u, a.ldus, a.stride_us))) {
+    return hipErrorInvalidValue;
+  }
+  if (!aligned16(a.x) || (a.x_rows > 1 && (a.ldx < a.k || a.ldx % 16 != 0 || a.ldxs < blocks_k)) ||
+      (a.rows > 1 && (a.ldy < a.n || (gate && a.ldys < blocks_n)))) {
+    return hipErrorInvalidValue;
+  }
+  if (a.rows > 0 && a.n > 0) {
+    if (a.x == nullptr || a.x_scales == nullptr || a.w == nullptr || a.w_scales == nullptr || a.y == nullptr ||
+        (gate && (a.up == nullptr || a.up_scales == nullptr || a.y_scales == nullptr)) ||
+        (a.experts > 0 && (a.counts == nullptr || a.order == nullptr))) {
+      return hipErrorInvalidDevicePointer;
+    }
+  }
+  return hipSuccess;
+}
+
+extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t stream) {
+  const hipError_t st = ggk_fp8_check(args);
+  if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
+  return args->experts > 0 ? multiply_few<true>(*args, stream) : multiply_few<false>(*args, stream);
+}

@@ -1,0 +1,221 @@
+// gg_norm.hip -- the root-mean-square norm of rows with the residual's addition,
+// written as 8-bit rows:
+//
+//   h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight
+//   scale of 128 columns = max(max |y| / 448, 2^-126), q = y / scale
+//
+// Bound by the bytes of x, the residual and the outputs: a row is read once and held in registers, 8 neighbouring
+// columns a lane and chunk, so that a block of 128 columns is one DPP row of 16 lanes and its largest value is found
+// without LDS.  A row takes a wave up to 2048 columns, else a workgroup of 4 waves (16 above 16384), with at most 64
+// values a lane.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gg_common.h"
+#include "gg_fp8_rows.h"
+#include "grouped_gemm_amd_kernels.h"
+
+namespace {
+
+using gg::kWave;
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
+template <int TYPE>
+struct Type;
+template <>
+struct Type<GGK_TYPE_F32> {
+  using T = float;
+};
+template <>
+struct Type<GGK_TYPE_F16> {
+  using T = _Float16;
+};
+template <>
+struct Type<GGK_TYPE_BF16> {
+  using T = __bf16;
+};
+
+// `count` (0 to 8) values from p on; the rest is 0.  VEC: all 8 or none are there, on a multiple of 16 bytes.
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
+  if constexpr (VEC) {
+    uint4v raw[sizeof(T) / 2] = {};
+    if (count > 0) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4v*>(p)[i];
+    }
+    const T* t = reinterpret_cast<const T*>(raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < count ? (float)p[i] : 0.0f;
+  }
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void store8(T* p, int count, const float (&v)[8]) {
+  if constexpr (VEC) {
+    uint4v raw[sizeof(T) / 2];
+    T* t = reinterpret_cast<T*>(raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
+    if (count > 0) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4v*>(p)[i] = raw[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < count) p[i] = (T)v[i];
+    }
+  }
+}
+
+template <int TYPE, int WTYPE, int LANES, int CHUNKS, bool VEC>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_norm_fp8_args a) {
+  using T = typename Type<TYPE>::T;
+  using W = typename Type<WTYPE>::T;
+  constexpr int kThreads = LANES < 256 ? 256 : LANES, kRows = kThreads / LANES, kWaves = LANES / kWave;
+  const int lane = threadIdx.x % LANES;
+  const long long row = (long long)blockIdx.x * kRows + threadIdx.x / LANES;
+  if (kRows > 1 && row >= a.rows) return;
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* residual = a.residual != nullptr ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
+  float h[CHUNKS][8];
+  float squares = 0.0f;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int at = 8 * (c * LANES + lane), count = min(max(a.columns - at, 0), 8);
+    load8<T, VEC>(x + at, count, h[c]);
+  }
+  if (residual != nullptr) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int at = 8 * (c * LANES + lane), count = min(max(a.columns - at, 0), 8);
+      float r[8];
+      load8<T, VEC>(residual + at, count, r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[c][i] += r[i];
+    }
+  }
+  T* sum = a.sum != nullptr ? static_cast<T*>(a.sum) + row * a.ldsum : nullptr;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int at = 8 * (c * LANES + lane), count = min(max(a.columns - at, 0), 8);
+    float part = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part = fmaf(h[c][i], h[c][i], part);
+    squares += part;
+    if (sum != nullptr) store8<T, VEC>(sum + at, count, h[c]);
+  }
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d /= 2) squares += __shfl_xor(squares, d, kWave);
+  if constexpr (kWaves > 1) {
+    __shared__ float s_squares[kWaves];
+    if (lane % kWave == 0) s_squares[lane / kWave] = squares;
+    __syncthreads();
+    squares = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) squares += s_squares[w];
+  }
+  const float factor = 1.0f / sqrtf(squares / (float)a.columns + a.eps);
+  const W* weight = static_cast<const W*>(a.weight);
+  T* y = a.y != nullptr ? static_cast<T*>(a.y) + row * a.ldy : nullptr;
+  unsigned char* q = a.q + row * a.ldq;
+  float* scales = a.scales + row * a.lds;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int at = 8 * (c * LANES + lane), count = min(max(a.columns - at, 0), 8);
+    float w[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+    if (weight != nullptr) load8<W, VEC>(weight + at, count, w);
+    uint32_t largest = 0;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = VEC || i < count ? h[c][i] * factor * w[i] : 0.0f;  // past the end 0 * factor may be NaN
+      if (!VEC || count > 0) largest = max(largest, gg::magnitude_bits(v[i]));
+    }
+    if (y != nullptr) store8<T, VEC>(y + at, count, v);
+    const float scale = gg::fp8_scale(gg::row_max16(largest));
+    const gg::Fp8Divisor by(scale);
+    const uint2v numbers = {gg::fp8_numbers(v[0], v[1], v[2], v[3], by),
+                            gg::fp8_numbers(v[4], v[5], v[6], v[7], by)};
+    if constexpr (VEC) {
+      if (count > 0) *reinterpret_cast<uint2v*>(q + at) = numbers;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < count) q[at + i] = (unsigned char)(numbers[i / 4] >> (8 * (i % 4)));
+      }
+    }
+    if (lane % 16 == 0 && count > 0) scales[at / gg::kFp8Block] = scale;
+  }
+}
+
+bool aligned(const void* p, long long ld_bytes, int rows, int to) {
+  return reinterpret_cast<uintptr_t>(p) % to == 0 && (rows <= 1 || ld_bytes % to == 0);
+}
+
+template <int TYPE, int WTYPE, bool VEC>
+hipError_t launch(const ggk_norm_fp8_args& a, hipStream_t stream) {
+  const auto go = [&](auto kernel, int rows, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((a.rows + rows - 1) / rows), dim3(threads), 0, stream, a);
+    return hipGetLastError();
+  };
+  const int chunks = (a.columns + 7) / 8;
+  if (chunks <= 64) return go(norm_kernel<TYPE, WTYPE, 64, 1, VEC>, 4, 256);
+  if (chunks <= 256) return go(norm_kernel<TYPE, WTYPE, 64, 4, VEC>, 4, 256);
+  if (chunks <= 512) return go(norm_kernel<TYPE, WTYPE, 256, 2, VEC>, 1, 256);
+  if (chunks <= 1024) return go(norm_kernel<TYPE, WTYPE, 256, 4, VEC>, 1, 256);
+  if (chunks <= 2048) return go(norm_kernel<TYPE, WTYPE, 256, 8, VEC>, 1, 256);
+  return go(norm_kernel<TYPE, WTYPE, 1024, 4, VEC>, 1, 1024);
+}
+
+template <int TYPE, int WTYPE>
+hipError_t launch_aligned(const ggk_norm_fp8_args& a, hipStream_t stream) {
+  const int size = TYPE == GGK_TYPE_F32 ? 4 : 2;
+  const bool vec = a.columns % 8 == 0 && aligned(a.x, a.ldx * size, a.rows, 16) &&
+                   aligned(a.residual, a.ldr * size, a.rows, 16) && aligned(a.weight, 0, 1, 16) &&
+                   aligned(a.q, a.ldq, a.rows, 8) && aligned(a.y, a.ldy * size, a.rows, 16) &&
+                   aligned(a.sum, a.ldsum * size, a.rows, 16);
+  return vec ? launch<TYPE, WTYPE, true>(a, stream) : launch<TYPE, WTYPE, false>(a, stream);
+}
+
+bool is_type(int type) { return type == GGK_TYPE_F32 || type == GGK_TYPE_F16 || type == GGK_TYPE_BF16; }
+
+}  // namespace
+
+extern "C" hipError_t ggk_norm_fp8_check(const ggk_norm_fp8_args* args) {
+  if (args == nullptr) return hipErrorInvalidValue;
+  const ggk_norm_fp8_args& a = *args;
+  if (a.rows < 0 || a.rows > GGK_ROUTE_MAX_TOTAL_SLOTS || a.columns < 1 || a.columns > GGK_NORM_MAX_COLUMNS ||
+      !is_type(a.type) || (a.weight != nullptr && !is_type(a.weight_type)) ||
+      (a.weight != nullptr && a.weight_type != a.type && a.weight_type != GGK_TYPE_F32)) {
+    return hipErrorInvalidValue;
+  }
+  const int blocks = (a.columns + gg::kFp8Block - 1) / gg::kFp8Block;
+  if (a.rows > 1 && (a.ldx < a.columns || a.ldq < a.columns || a.lds < blocks ||
+                     (a.residual != nullptr && a.ldr < a.columns) || (a.y != nullptr && a.ldy < a.columns) ||
+                     (a.sum != nullptr && a.ldsum < a.columns))) {
+    return hipErrorInvalidValue;
+  }
+  if (a.rows > 0 && (a.x == nullptr || a.q == nullptr || a.scales == nullptr)) return hipErrorInvalidDevicePointer;
+  return hipSuccess;
+}
+
+extern "C" hipError_t ggk_norm_fp8(const ggk_norm_fp8_args* args, hipStream_t stream) {
+  const hipError_t st = ggk_norm_fp8_check(args);
+  if (st != hipSuccess || args->rows == 0) return st;
+  const ggk_norm_fp8_args& a = *args;
+  const bool same = a.weight == nullptr || a.weight_type == a.type;
+  switch (a.type) {
+    case GGK_TYPE_F32: return launch_aligned<GGK_TYPE_F32, GGK_TYPE_F32>(a, stream);
+    case GGK_TYPE_F16:
+      return same ? launch_aligned<GGK_TYPE_F16, GGK_TYPE_F16>(a, stream) : launch_aligned<GGK_TYPE_F16, GGK_TYPE_F32>(a, stream);
+    default:
+      return same ? launch_aligned<GGK_TYPE_BF16, GGK_TYPE_BF16>(a, stream)
+                  : launch_aligned<GGK_TYPE_BF16, GGK_TYPE_F32>(a, stream);
+  }
+}

@@ -1,5 +1,5 @@
-// torch_binding.cpp -- the PyTorch side of the routing and of the products with
-// 4-bit weights: argument checks, outputs, the current stream and the autograd
+// torch_binding.cpp -- the PyTorch side of the routing, of the products with
+// 4-bit weights and of the 8-bit norm and products: argument checks, outputs, the current stream and the autograd
 // node, ahead of the C entry points of include/grouped_gemm_amd_kernels.h.
 //
 // In C++ because these calls last a few microseconds on the GPU: made from
@@ -73,6 +73,7 @@ const void* data(const Tensor& t) {
     case at::kFloat: return t.const_data_ptr<float>();
     case at::kHalf: return t.const_data_ptr<at::Half>();
     case at::kBFloat16: return t.const_data_ptr<at::BFloat16>();
+    case at::kFloat8_e4m3fn: return t.const_data_ptr<at::Float8_e4m3fn>();
     case at::kInt: return t.const_data_ptr<int>();
     case at::kBool: return t.const_data_ptr<bool>();
     default: return t.const_data_ptr<uint8_t>();
@@ -353,10 +354,179 @@ py::object w4_call(const Tensor& x, const Tensor& q, const Tensor& scales, const
   return status == 0 ? py::cast(y) : py::object(py::int_(status));
 }
 
+// ---------------------------------------------------------------- 8-bit rows
+
+constexpr int64_t blocks_of(int64_t n) { return (n + GGK_FP8_BLOCK - 1) / GGK_FP8_BLOCK; }
+
+bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors) {
+    if (t != nullptr && t->requires_grad()) return true;
+  }
+  return false;
+}
+
+const Tensor* given(const MaybeTensor& t) { return t ? &*t : nullptr; }
+
+py::object norm_fp8_call(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& residual, double eps, bool plain) {
+  if (!x.is_cuda() || type_of(x.scalar_type()) < 0 || !matrix_in_order(x) || has_tangent(x)) return py::none();
+  const c10::Device device = x.device();
+  const int64_t rows = x.size(0), columns = x.size(1);
+  if (columns < 1 || columns > GGK_NORM_MAX_COLUMNS || rows > GGK_ROUTE_MAX_TOTAL_SLOTS) return py::none();
+  if (weight) {
+    if ((weight->scalar_type() != x.scalar_type() && weight->scalar_type() != at::kFloat) || weight->dim() != 1 ||
+        !vector_in_order(*weight, weight->scalar_type(), columns, device) || has_tangent(*weight)) {
+      return py::none();
+    }
+  }
+  if (residual && (residual->scalar_type() != x.scalar_type() || residual->device() != device ||
+                   !matrix_in_order(*residual) || residual->sizes() != x.sizes() || has_tangent(*residual))) {
+    return py::none();
+  }
+  if (wants_gradient({&x, given(weight), given(residual)})) return py::none();
+  const auto like_x = x.options().requires_grad(false);
+  Tensor q = at::empty({rows, columns}, like_x.dtype(at::kFloat8_e4m3fn));
+  Tensor scales = at::empty({rows, blocks_of(columns)}, like_x.dtype(at::kFloat));
+  MaybeTensor y, sum;
+  if (plain) y = at::empty({rows, columns}, like_x);
+  if (residual) sum = at::empty({rows, columns}, like_x);
+  if (rows > 0) {
+    ggk_norm_fp8_args a{};
+    a.rows = static_cast<int>(rows);
+    a.columns = static_cast<int>(columns);
+    a.type = type_of(x.scalar_type());
+    a.x = data(x);
+    a.ldx = row_stride(x);
+    if (weight) {
+      a.weight = data(*weight);
+      a.weight_type = type_of(weight->scalar_type());
+    }
+    a.eps = static_cast<float>(eps);
+    a.q = static_cast<unsigned char*>(q.mutable_data_ptr());
+    a.ldq = columns;
+    a.scales = scales.mutable_data_ptr<float>();
+    a.lds = scales.size(1);
+    if (residual) {
+      a.residual = data(*residual);
+      a.ldr = row_stride(*residual);
+      a.sum = sum->mutable_data_ptr();
+      a.ldsum = columns;
+    }
+    if (plain) {
+      a.y = y->mutable_data_ptr();
+      a.ldy = columns;
+    }
+    const int status = launch(ggk_norm_fp8, a, device);
+    if (status != 0) return py::int_(status);
+  }
+  const auto or_none = [](const MaybeTensor& t) { return t ? py::cast(*t) : py::object(py::none()); };
+  return py::make_tuple(q, scales, or_none(y), or_none(sum));
+}
+
+// A weight matrix (or one an expert) of 8-bit numbers, rows on multiples of 16 bytes, with its blocks' scales.
+bool fp8_matrix_in_order(const Tensor& w, const Tensor& scales, int64_t dim, c10::Device device) {
+  if (w.scalar_type() != at::kFloat8_e4m3fn || w.device() != device || w.dim() != dim || !is_stored(w) ||
+      scales.scalar_type() != at::kFloat || scales.device() != device || scales.dim() != dim || !is_stored(scales)) {
+    return false;
+  }
+  const int64_t n = w.size(dim - 2), k = w.size(dim - 1), rows = scales.size(dim - 2), columns = scales.size(dim - 1);
+  if (rows != blocks_of(n) || columns != blocks_of(k) || (dim == 3 && scales.size(0) != w.size(0))) return false;
+  if (k > 1 && w.stride(dim - 1) != 1) return false;
+  if (n > 1 && (w.stride(dim - 2) < k || w.stride(dim - 2) > GGK_FP8_MAX_LD || w.stride(dim - 2) % 16 != 0)) return false;
+  if (columns > 1 && scales.stride(dim - 1) != 1) return false;
+  if (rows > 1 && scales.stride(dim - 2) < columns) return false;
+  return (dim == 2 || w.size(0) <= 1 || w.stride(0) % 16 == 0) && reinterpret_cast<uintptr_t>(w.const_data_ptr()) % 16 == 0;
+}
+
+py::object fp8_call(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Tensor& w_scales, const MaybeTensor& up,
+                    const MaybeTensor& up_scales, int gate, const MaybeTensor& counts, const MaybeTensor& order,
+                    const MaybeTensor& row_weights, at::ScalarType out_type) {
+  const int64_t dim = counts ? 3 : 2;
+  const bool gated = gate != GGK_GATE_NONE;
+  if (!x.is_cuda() || x.scalar_type() != at::kFloat8_e4m3fn || !matrix_in_order(x) || w.dim() != dim ||
+      gated != up.has_value() || gated != up_scales.has_value() || gate < GGK_GATE_NONE || gate > GGK_GATE_GELU ||
+      type_of(out_type) < 0) {
+    return py::none();
+  }
+  const c10::Device device = x.device();
+  const int64_t n = w.size(dim - 2), k = w.size(dim - 1), x_rows = x.size(0), experts = counts ? w.size(0) : 0;
+  if (x.size(1) != k || k < 16 || k % 16 != 0 || k > GGK_FP8_MAX_K || n > GGK_FP8_MAX_N ||
+      (x_rows > 1 && x.stride(0) % 16 != 0) || reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 != 0 ||
+      x_scales.scalar_type() != at::kFloat || x_scales.device() != device || !matrix_in_order(x_scales) ||
+      x_scales.size(0) != x_rows || x_scales.size(1) != blocks_of(k) ||
+      !fp8_matrix_in_order(w, w_scales, dim, device) ||
+      (gated && (up->sizes() != w.sizes() || !fp8_matrix_in_order(*up, *up_scales, dim, device)))) {
+    return py::none();
+  }
+  int64_t rows = x_rows;
+  if (counts) {
+    if (!order || experts < 1 || experts > GGK_MOE_MAX_EXPERTS || !vector_in_order(*counts, at::kInt, experts, device)) {
+      return py::none();
+    }
+    rows = order->numel();
+    if (!vector_in_order(*order, at::kInt, rows, device) || (rows > 0 && (x_rows == 0 || rows % x_rows != 0)) ||
+        (row_weights && !vector_in_order(*row_weights, at::kFloat, rows, device))) {
+      return py::none();
+    }
+  }
+  if (rows > GGK_ROUTE_MAX_TOTAL_SLOTS) return py::none();
+  for (const Tensor* t : {&x, &x_scales, &w, &w_scales, given(up), given(up_scales), given(row_weights)}) {
+    if (t != nullptr && has_tangent(*t)) return py::none();
+  }
+  if (wants_gradient({&x, &x_scales, &w, &w_scales, given(up), given(up_scales), given(row_weights)})) return py::none();
+  const auto like_x = x.options().requires_grad(false);
+  Tensor y = at::empty({rows, n}, gated ? like_x : like_x.dtype(out_type)), y_scales;
+  if (gated) y_scales = at::empty({rows, blocks_of(n)}, like_x.dtype(at::kFloat));
+  if (rows > 0 && n > 0) {
+    const auto ld = [&](const Tensor& t) { return t.size(dim - 2) > 1 ? t.stride(dim - 2) : t.size(dim - 1); };
+    const auto matrix = [&](const Tensor& t) { return experts > 1 ? t.stride(0) : 0; };
+    ggk_fp8_args a{};
+    a.rows = static_cast<int>(rows);
+    a.x_rows = static_cast<int>(x_rows);
+    a.n = static_cast<int>(n);
+    a.k = static_cast<int>(k);
+    a.experts = static_cast<int>(experts);
+    a.gate = gate;
+    a.x = static_cast<const unsigned char*>(data(x));
+    a.ldx = row_stride(x);
+    a.x_scales = x_scales.const_data_ptr<float>();
+    a.ldxs = row_stride(x_scales);
+    a.w = static_cast<const unsigned char*>(data(w));
+    a.ldw = ld(w);
+    a.stride_w = matrix(w);
+    a.w_scales = w_scales.const_data_ptr<float>();
+    a.ldws = ld(w_scales);
+    a.stride_ws = matrix(w_scales);
+    if (gated) {
+      a.up = static_cast<const unsigned char*>(data(*up));
+      a.ldu = ld(*up);
+      a.stride_u = matrix(*up);
+      a.up_scales = up_scales->const_data_ptr<float>();
+      a.ldus = ld(*up_scales);
+      a.stride_us = matrix(*up_scales);
+      a.y_scales = y_scales.mutable_data_ptr<float>();
+      a.ldys = y_scales.size(1);
+    }
+    if (counts) {
+      a.counts = counts->const_data_ptr<int>();
+      a.order = order->const_data_ptr<int>();
+      a.row_weights = row_weights ? row_weights->const_data_ptr<float>() : nullptr;
+    }
+    a.y = y.mutable_data_ptr();
+    a.ldy = n;
+    a.y_type = type_of(out_type);
+    const int status = launch(ggk_fp8_multiply, a, device);
+    if (status != 0) return py::int_(status);
+  }
+  return gated ? py::object(py::make_tuple(y, y_scales)) : py::cast(y);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(gg_torch, m) {
   m.attr("torch_version") = GG_TORCH_VERSION;  // whose classes this was compiled with; the loader compares
   m.def("route", &route_call);
   m.def("w4", &w4_call);
+  m.def("norm_fp8", &norm_fp8_call);
+  m.def("fp8", &fp8_call);
 }
