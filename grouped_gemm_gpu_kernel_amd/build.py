@@ -31,7 +31,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC_DIR = PKG / "csrc"
 BUILD = PKG / "_build"
-DEVICE_SOURCES = ["gg_moe.hip", "gg_route.hip", "gg_w4.hip", "gg_norm.hip", "gg_fp8.hip"]  # beside gg_kernels.hip, whose resources are reported
+DEVICE_SOURCES = ["gg_moe.hip", "gg_route.hip", "gg_w4.hip", "gg_norm.hip", "gg_fp8.hip",
+                  "gg_fp8_tiles.hip"]  # beside gg_kernels.hip, whose resources are reported
 LIB_DIR = PKG / "lib"
 LIB_NAME = "libgrouped_gemm_amd.so"
 FORMS_NAME = "gg_kernel_forms.json"  # resources of every compiled kernel form, beside the objects

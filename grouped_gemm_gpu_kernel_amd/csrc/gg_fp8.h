@@ -80,12 +80,11 @@ __device__ __forceinline__ float4v multiply(const Halves& w, const Halves& x) {
   return p;
 }
 
-// act(p) * u.
-__device__ __forceinline__ float gated(int gate, float p, float u) {
-  float z = p;
-  if (gate == GGK_GATE_GELU) {  // (1 + tanh(t)) / 2 = 1 / (1 + exp(-2 t))
-    z = 1.5957691216057308f * p * fmaf(0.044715f * p, p, 1.0f);
-  }
+// act(p) * u; gelu: (1 + tanh(t)) / 2 = 1 / (1 + exp(-2 t)).  GELU is uniform and known ahead, so that no branch stands
+// between the values of a tile.
+template <bool GELU>
+__device__ __forceinline__ float gated(float p, float u) {
+  const float z = GELU ? 1.5957691216057308f * p * fmaf(0.044715f * p, p, 1.0f) : p;
   return p / (1.0f + expf(-z)) * u;
 }
 
@@ -143,6 +142,10 @@ __device__ __forceinline__ void store_numbers(const ggk_fp8_args& a, long long r
   }
   if (j % kFp8Block == 0) a.y_scales[row * a.ldys + j / kFp8Block] = scale;
 }
+
+// The kernel for many rows (gg_fp8_tiles.hip): does it take a call's strides, and the call (16-bit or 8-bit y).
+bool tiles_take(const ggk_fp8_args& a);
+hipError_t multiply_tiles(const ggk_fp8_args& a, hipStream_t stream);
 
 }  // namespace fp8
 }  // namespace gg

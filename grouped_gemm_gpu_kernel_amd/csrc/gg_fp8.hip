@@ -194,7 +194,9 @@ __device__ __forceinline__ void run_item(const ggk_fp8_args& a, const RowTile& t
       for (int half = 0; half < 2; ++half) {
         const float4v p = total(r, at + 4 * half), u = total(r, at + 4 * half + kHalf);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * half + e] = gated(a.gate, p[e], u[e]);
+        for (int e = 0; e < 4; ++e) {
+          v[4 * half + e] = a.gate == GGK_GATE_GELU ? gated<true>(p[e], u[e]) : gated<false>(p[e], u[e]);
+        }
       }
       const int slot = EXPERTS ? slots[r] : t.first + r;
       store_numbers(a, slot, block0 + c, v, i / 16 < t.rows && slot >= 0);
@@ -324,5 +326,8 @@ extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
 extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t stream) {
   const hipError_t st = ggk_fp8_check(args);
   if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
+  const ggk_fp8_args& a = *args;
+  const long long rows = a.experts > 0 ? a.rows / a.experts : a.rows;
+  if (rows > 100 && (a.gate != GGK_GATE_NONE || a.y_type != GGK_TYPE_F32) && tiles_take(a)) return multiply_tiles(a, stream);
   return args->experts > 0 ? multiply_few<true>(*args, stream) : multiply_few<false>(*args, stream);
 }
