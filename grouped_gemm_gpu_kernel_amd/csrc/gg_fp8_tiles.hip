@@ -15,6 +15,7 @@
 // its end for this wave's loads of unit f + 3 and its reads of the phases before; one barrier tells every wave both.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <stdlib.h>
 
 #include <type_traits>
 
@@ -32,7 +33,7 @@ using gg::kWave;
 constexpr int kCus = 256, kXcds = 8;
 constexpr int kRows = 256, kWaves = 8, kThreads = kWaves * kWave;
 constexpr int kUnit = 128 * kStep;  // bytes
-constexpr int kB0 = 0, kA0 = kUnit, kB1 = 2 * kUnit, kA1 = 3 * kUnit, kParity = 4 * kUnit;
+constexpr int kB0 = 0, kA0 = kUnit, kB1 = 2 * kUnit, kA1 = 3 * kUnit, kParity = 4 * kUnit, kPlaces = 8;
 constexpr int kLoads = 2;           // load instructions of a unit and wave
 constexpr int kScaleSteps = 4;      // stages of scales loaded at once, 16 bytes a row
 constexpr int kScales = 6 * 1024;   // bytes of those: 256 rows, and a row of each unit's weights in 1 KB each
@@ -44,6 +45,7 @@ constexpr int kColumns = GATED ? 128 : 256;
 struct Launch {
   ggk_fp8_args a;
   int blocks;            // of columns
+  int height;            // rows of a tile (one matrix)
   uint32_t scale_bytes;  // of all of x's scales (experts)
 };
 
@@ -54,7 +56,8 @@ struct Shared {
 };
 
 // Sums of one tile: [rows half][16 rows][unit of columns][16 columns].
-typedef float4v Sums[2][4][2][2];
+template <int HALVES>
+using Sums = float4v[HALVES][4][2][2];
 
 template <bool EXPERTS, bool GATED>
 struct Loader {
@@ -131,9 +134,10 @@ struct Loader {
   }
 };
 
-// The sums of the tile at rows t, columns n0 on.
-template <bool EXPERTS, bool GATED>
-__device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave, Sums& acc) {
+// The sums of the tile at rows t (at most 128 HALVES), columns n0 on.
+template <bool EXPERTS, bool GATED, int HALVES>
+__device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
+                                              Sums<HALVES>& acc) {
   const ggk_fp8_args& p = l.a;
   const int nk = (p.k + kStep - 1) / kStep;
   const Loader<EXPERTS, GATED> loader(l, t, s.x_row, n0, wave);
@@ -146,12 +150,12 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   const uint32_t w_scale_lane = scales_at + 4096 + (GATED ? 0 : (wn >> 1) * 1024);
 
   int8v a[4], b[2][2];
-  float x_scale[4], w_scale[2];
+  float x_scale[2][4], w_scale[2], w_next[2];  // x's by half of the rows; of the next stage while this one's are used
   float4v part[8];      // results of this phase's instructions, three of them alive
   float4v left[2];      // of the phase before, its last two
   float left_scale;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -166,16 +170,21 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
 
   auto read_a = [&](uint32_t unit, int i) { a[i] = read_fragment(a_lane + unit + 2048u * i); };
   auto read_b = [&](uint32_t unit, int which, int n) { b[which][n] = read_fragment(b_lane + unit + 2048u * n); };
-  // Scales of stage kt: rows of A half `half`, and the units' weights.
-  auto read_x_scales = [&](int kt, int half) {
+  // Scales of stage kt: rows of A half `half` (into set `set`), and the units' weights.  Read two phases ahead, so that their
+  // wait is none for the fragments read since.
+  auto read_x_scales = [&](int kt, int half, int set) {
     const uint32_t at = x_scale_lane + ((kt >> 2) & 1) * kScales + (kt & 3) * 4 + half * 2048;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x_scale[i] = *(const GG_LDS float*)(uintptr_t)(at + 256u * i);
+    for (int i = 0; i < 4; ++i) x_scale[set][i] = *(const GG_LDS float*)(uintptr_t)(at + 256u * i);
   };
   auto read_w_scales = [&](int kt) {
     const uint32_t at = w_scale_lane + ((kt >> 2) & 1) * kScales + (kt & 3) * 4;
-    w_scale[0] = *(const GG_LDS float*)(uintptr_t)at;
-    if constexpr (GATED) w_scale[1] = *(const GG_LDS float*)(uintptr_t)(at + 1024u);
+    w_next[0] = *(const GG_LDS float*)(uintptr_t)at;
+    if constexpr (GATED) w_next[1] = *(const GG_LDS float*)(uintptr_t)(at + 1024u);
+  };
+  auto next_w_scales = [&]() {
+    w_scale[0] = w_next[0];
+    if constexpr (GATED) w_scale[1] = w_next[1];
   };
   auto add = [&](float4v& sum, const float4v& v, float scale) {
 #pragma unroll
@@ -186,7 +195,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   auto phase = [&](int half, int unit, int last_half, int last_unit, auto&& issue, auto&& read) {
     float scale[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) scale[i] = x_scale[i] * w_scale[GATED ? unit : 0];
+    for (int i = 0; i < 4; ++i) scale[i] = x_scale[half][i] * w_scale[GATED ? unit : 0];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const int i = r >> 1, n = (i & 1) != 0 ? 1 - (r & 1) : r & 1;
@@ -199,8 +208,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
         add(acc[half][qi][unit][qn], part[q], scale[qi]);
       }
       read(r);
-      if (r == 4) issue(0);
-      if (r == 6) issue(1);
+      issue(r);
       __builtin_amdgcn_sched_barrier(0);
     }
     left[0] = part[6];
@@ -209,120 +217,193 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   };
 
   loader.issue_scales(0, scales_at);
+  if constexpr (HALVES == 1) {
+    // Unit u (stage u / 3; B0, A0, B1) lies in place u % 8.  Phase 0 of stage t issues the loads of unit 3 t + 7, phase 1
+    // those of 3 t + 8 and 3 t + 9: the units eight before them have been read and used, and a barrier stands between.
+    // Loads of stages past K read zeros without touching memory.
+    auto place_of = [&](int u) { return (uint32_t)(u % kPlaces) * kUnit; };
+    auto issue_unit = [&](int u, int kt, int which, int i) {
+      if (which == 1) {
+        loader.issue_a(kt, 0, lds + place_of(u), i);
+      } else {
+        loader.issue_b(kt, which / 2, lds + place_of(u), i);
+      }
+    };
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt) {
-    const uint32_t st = lds + kt * kParity;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) loader.issue_b(kt, 0, st + kB0, i);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) loader.issue_a(kt, 0, st + kA0, i);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) loader.issue_b(kt, 1, st + kB1, i);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) loader.issue_a(kt, 1, st + kA1, i);
-  }
-  gg::wait_vmcnt<6 * kLoads>();
-  gg::phase_barrier();
-#pragma unroll
-  for (int n = 0; n < 2; ++n) read_b(kB0, 0, n);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) read_a(kA0, i);
-  read_x_scales(0, 0);
-  read_w_scales(0);
-  gg::wait_vmcnt<5 * kLoads>();
-  gg::wait_lgkmcnt<0>();
-  gg::phase_barrier();
-
-  // One stage.  ISSUE: the loads of stage kt + 2 are issued; else everything has been and the waits count down.  LAST:
-  // nothing more is read.
-  auto stage = [&](int kt, auto issue_tag, auto last_tag) {
-    constexpr bool ISSUE = decltype(issue_tag)::value, LAST = decltype(last_tag)::value;
-    constexpr int N = kLoads;
-    const uint32_t here = (uint32_t)(kt & 1) * kParity, next = kParity - here;
-    const uint32_t st = lds + here;
-    // Scales of the next four stages, behind the last use of the set before theirs.
-    if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
-    phase(0, 0, 1, 1, [&](int i) { if constexpr (ISSUE) loader.issue_b(kt + 2, 0, st + kB0, i); },
-          [&](int r) { if (r == 1 || r == 3) read_b(here + kB1, 1, r / 2); });
-    gg::wait_lgkmcnt<0>();
-    gg::wait_vmcnt<ISSUE ? 5 * N : LAST ? 0 : 4 * N>();
+    for (int u = 0; u < 7; ++u) {
+      issue_unit(u, u / 3, u % 3, 0);
+      issue_unit(u, u / 3, u % 3, 1);
+    }
+    gg::wait_vmcnt<5 * kLoads>();
     gg::phase_barrier();
-    phase(0, 1, 0, 0, [&](int i) { if constexpr (ISSUE) loader.issue_a(kt + 2, 0, st + kA0, i); },
-          [&](int r) { if (r & 1) read_a(here + kA1, r / 2); });
-    read_x_scales(kt, 1);
-    if constexpr (!LAST) {
-      gg::wait_vmcnt<ISSUE ? 5 * N : 3 * N>();
-      gg::phase_barrier();
-    }
-    phase(1, 0, 0, 1, [&](int i) { if constexpr (ISSUE) loader.issue_b(kt + 2, 1, st + kB1, i); },
-          [&](int r) { if constexpr (!LAST) { if (r >= 6) read_b(next + kB0, 0, 7 - r); } });
-    if constexpr (!LAST) {
-      gg::wait_vmcnt<ISSUE ? 5 * N : 2 * N>();
-      gg::phase_barrier();
-    }
-    phase(1, 1, 1, 0, [&](int i) { if constexpr (ISSUE) loader.issue_a(kt + 2, 1, st + kA1, i); },
-          [&](int r) { if constexpr (!LAST) { if (r & 1) read_a(next + kA0, r / 2); } });
-    if constexpr (!LAST) {
-      gg::wait_lgkmcnt<8>();  // phase 2's reads, which nothing has used yet; this phase's eight may be on their way
-      read_x_scales(kt + 1, 0);
-      read_w_scales(kt + 1);
-      gg::wait_vmcnt<ISSUE ? 5 * N : N>();
-      gg::phase_barrier();
-    }
-  };
-  int kt = 0;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) read_b(place_of(0), 0, n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) read_a(place_of(1), i);
+    read_x_scales(0, 0, 0);
+    read_w_scales(0);
+    next_w_scales();
+    gg::wait_vmcnt<4 * kLoads>();
+    gg::phase_barrier();
 #pragma unroll 1
-  for (; kt < nk - 2; ++kt) stage(kt, std::true_type{}, std::false_type{});
-  if (nk >= 2) stage(kt++, std::false_type{}, std::false_type{});
-  stage(kt, std::false_type{}, std::true_type{});  // a single stage also waits for the (empty) loads past K
-  add(acc[1][3][1][1], left[0], left_scale);
-  add(acc[1][3][1][0], left[1], left_scale);
-  gg::wait_vmcnt<0>();
+    for (int kt = 0; kt < nk; ++kt) {
+      const int u = 3 * kt;
+      if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
+      const uint32_t b1 = place_of(u + 2), b0 = place_of(u + 3), a0 = place_of(u + 4);
+      phase(0, 0, 0, 1, [&](int r) { if (r == 4 || r == 6) issue_unit(u + 7, kt + 2, 1, r / 2 - 2); },
+            [&](int r) {
+              if (r == 1 || r == 3) read_b(b1, 1, r / 2);
+              if (r == 5) {
+                read_x_scales(kt + 1, 0, 1);
+                read_w_scales(kt + 1);
+              }
+            });
+      gg::wait_vmcnt<3 * kLoads>();
+      gg::phase_barrier();
+      phase(0, 1, 0, 0, [&](int r) { if (r >= 4) issue_unit(u + 8 + (r - 4) / 2, kt + 2 + (r - 4) / 2, r < 6 ? 2 : 0, r & 1); },
+            [&](int r) { if (r & 1) read_a(a0, r / 2); else if (r < 4) read_b(b0, 0, r / 2); });
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x_scale[0][i] = x_scale[1][i];
+      next_w_scales();
+      gg::wait_vmcnt<4 * kLoads>();
+      gg::phase_barrier();
+    }
+    add(acc[0][3][1][1], left[0], left_scale);
+    add(acc[0][3][1][0], left[1], left_scale);
+    gg::wait_vmcnt<0>();
+    return;
+  } else {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const uint32_t st = lds + kt * kParity;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) loader.issue_b(kt, 0, st + kB0, i);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) loader.issue_a(kt, 0, st + kA0, i);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) loader.issue_b(kt, 1, st + kB1, i);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) loader.issue_a(kt, 1, st + kA1, i);
+    }
+    gg::wait_vmcnt<6 * kLoads>();
+    gg::phase_barrier();
+#pragma unroll
+    for (int n = 0; n < 2; ++n) read_b(kB0, 0, n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) read_a(kA0, i);
+    read_x_scales(0, 0, 0);
+    read_w_scales(0);
+    next_w_scales();
+    gg::wait_vmcnt<5 * kLoads>();
+    gg::wait_lgkmcnt<0>();
+    gg::phase_barrier();
+
+    // One stage.  ISSUE: the loads of stage kt + 2 are issued; else everything has been and the waits count down.  LAST:
+    // nothing more is read.
+    auto stage = [&](int kt, auto issue_tag, auto last_tag) {
+      constexpr bool ISSUE = decltype(issue_tag)::value, LAST = decltype(last_tag)::value;
+      constexpr int N = kLoads;
+      const uint32_t here = (uint32_t)(kt & 1) * kParity, next = kParity - here;
+      const uint32_t st = lds + here;
+      // Scales of the next four stages, behind the last use of the set before theirs.
+      if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
+      phase(0, 0, 1, 1, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_b(kt + 2, 0, st + kB0, r / 2 - 2); },
+            [&](int r) {
+              if (r == 1 || r == 3) read_b(here + kB1, 1, r / 2);
+              if (r == 5) read_x_scales(kt, 1, 1);
+            });
+      gg::wait_vmcnt<ISSUE ? 5 * N : LAST ? 0 : 4 * N>();
+      gg::phase_barrier();
+      phase(0, 1, 0, 0, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_a(kt + 2, 0, st + kA0, r / 2 - 2); },
+            [&](int r) { if (r & 1) read_a(here + kA1, r / 2); });
+      if constexpr (!LAST) {
+        gg::wait_vmcnt<ISSUE ? 5 * N : 3 * N>();
+        gg::phase_barrier();
+      }
+      phase(1, 0, 0, 1, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_b(kt + 2, 1, st + kB1, r / 2 - 2); },
+            [&](int r) {
+              if constexpr (!LAST) {
+                if (r == 1) {
+                  read_x_scales(kt + 1, 0, 0);
+                  read_w_scales(kt + 1);
+                }
+                if (r >= 6) read_b(next + kB0, 0, 7 - r);
+              }
+            });
+      if constexpr (!LAST) {
+        gg::wait_vmcnt<ISSUE ? 5 * N : 2 * N>();
+        gg::phase_barrier();
+      }
+      phase(1, 1, 1, 0, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_a(kt + 2, 1, st + kA1, r / 2 - 2); },
+            [&](int r) { if constexpr (!LAST) { if (r & 1) read_a(next + kA0, r / 2); } });
+      if constexpr (!LAST) {
+        gg::wait_lgkmcnt<8>();  // phase 2's reads, which nothing has used yet; this phase's eight may be on their way
+        next_w_scales();
+        gg::wait_vmcnt<ISSUE ? 5 * N : N>();
+        gg::phase_barrier();
+      }
+    };
+    int kt = 0;
+#pragma unroll 1
+    for (; kt < nk - 2; ++kt) stage(kt, std::true_type{}, std::false_type{});
+    if (nk >= 2) stage(kt++, std::false_type{}, std::false_type{});
+    stage(kt, std::false_type{}, std::true_type{});  // a single stage also waits for the (empty) loads past K
+    add(acc[1][3][1][1], left[0], left_scale);
+    add(acc[1][3][1][0], left[1], left_scale);
+    gg::wait_vmcnt<0>();
+  }
 }
 
-// y of a tile, in a 16-bit type.
-template <bool EXPERTS, class T>
+// y of a tile, in a 16-bit type: four columns a lane and store; rows that do not start on multiples of four values by way
+// of LDS, value by value.
+template <bool EXPERTS, class T, int HALVES>
 __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile& t, const Shared& s, int n0, int wm, int wn,
-                                           const Sums& acc) {
+                                           const Sums<HALVES>& acc) {
+  constexpr int kLd = 2 * 256 + 16;  // bytes of a row in LDS
   const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
   const bool vec = a.n % 4 == 0 && a.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % 8 == 0;
+  if (!vec) gg::stage_barrier();
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < HALVES; ++half) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 128 * half + 64 * wm + 16 * i + j;
       const int slot = r < t.rows ? (EXPERTS ? s.slot[r] : t.first + r) : -1;
       const float weight = EXPERTS && a.row_weights != nullptr && slot >= 0 ? a.row_weights[slot] : 1.0f;
-      T* y = static_cast<T*>(a.y) + slot * a.ldy;
+      T* y = static_cast<T*>(a.y) + slot * a.ldy + n0;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const int column = n0 + 64 * wn + 32 * u + 16 * n + 4 * g;
+          const int column = 64 * wn + 32 * u + 16 * n + 4 * g;
           uint16_t h[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) h[e] = __builtin_bit_cast(uint16_t, (T)(acc[half][i][u][n][e] * weight));
-          if (slot < 0) continue;
-          if (vec) {
-            if (column < a.n) {
-              *reinterpret_cast<uint2v*>(y + column) = uint2v{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (column + e < a.n) reinterpret_cast<uint16_t*>(y)[column + e] = h[e];
-            }
+          const uint2v four = {h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
+          if (!vec) {
+            *reinterpret_cast<uint2v*>(s.stages + r * kLd + 2 * column) = four;
+          } else if (slot >= 0 && n0 + column < a.n) {
+            *reinterpret_cast<uint2v*>(y + column) = four;
           }
         }
+      }
+    }
+  }
+  if (!vec) {
+    gg::stage_barrier();
+    for (int i = threadIdx.x; i < t.rows * 256; i += kThreads) {
+      const int r = i / 256, c = i % 256, slot = EXPERTS ? s.slot[r] : t.first + r;
+      if (slot >= 0 && n0 + c < a.n) {
+        static_cast<uint16_t*>(a.y)[slot * a.ldy + n0 + c] = *reinterpret_cast<const uint16_t*>(s.stages + r * kLd + 2 * c);
       }
     }
   }
 }
 
 // The 8-bit rows of a gated tile.
-template <bool EXPERTS, bool GELU>
+template <bool EXPERTS, bool GELU, int HALVES>
 __device__ __forceinline__ void store_rows(const ggk_fp8_args& a, const RowTile& t, const Shared& s, int n0, int wm, int wn,
-                                           Sums& acc) {
+                                           Sums<HALVES>& acc) {
   const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
       // Values stay in the registers of gate's sums; a row's 128 columns lie in 4 lanes of 4 waves.
       constexpr int kLd = 128 + 16;
@@ -384,25 +465,34 @@ __device__ __forceinline__ void store_rows(const ggk_fp8_args& a, const RowTile&
       }
 }
 
-template <bool EXPERTS, bool GATED>
+template <bool EXPERTS, bool GATED, int HALVES>
 __device__ __forceinline__ void run_tile(const Launch& l, const RowTile& t, const Shared& s, int n0) {
   const ggk_fp8_args& a = l.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave >> 2, wn = wave & 3;
-  Sums acc;
-  multiply_tile<EXPERTS, GATED>(l, t, s, n0, wave, acc);
+  Sums<HALVES> acc;
+  multiply_tile<EXPERTS, GATED, HALVES>(l, t, s, n0, wave, acc);
   if constexpr (!GATED) {
     if (a.y_type == GGK_TYPE_BF16) {
-      store_tile<EXPERTS, __bf16>(a, t, s, n0, wm, wn, acc);
+      store_tile<EXPERTS, __bf16, HALVES>(a, t, s, n0, wm, wn, acc);
     } else {
-      store_tile<EXPERTS, _Float16>(a, t, s, n0, wm, wn, acc);
+      store_tile<EXPERTS, _Float16, HALVES>(a, t, s, n0, wm, wn, acc);
     }
   } else {
     if (a.gate == GGK_GATE_GELU) {
-      store_rows<EXPERTS, true>(a, t, s, n0, wm, wn, acc);
+      store_rows<EXPERTS, true, HALVES>(a, t, s, n0, wm, wn, acc);
     } else {
-      store_rows<EXPERTS, false>(a, t, s, n0, wm, wn, acc);
+      store_rows<EXPERTS, false, HALVES>(a, t, s, n0, wm, wn, acc);
     }
+  }
+}
+
+template <bool EXPERTS, bool GATED>
+__device__ __forceinline__ void run_either(const Launch& l, const RowTile& t, const Shared& s, int n0) {
+  if (t.rows <= kRows / 2) {
+    run_tile<EXPERTS, GATED, 1>(l, t, s, n0);
+  } else {
+    run_tile<EXPERTS, GATED, 2>(l, t, s, n0);
   }
 }
 
@@ -421,7 +511,7 @@ __device__ __forceinline__ void clear_tile(const ggk_fp8_args& a, const RowTile&
   }
 }
 
-// Tile and column block of place p in an order that goes along the columns kGroup row tiles at a time.
+// Row tile and column block of place p in an order that goes along the columns kGroup row tiles at a time.
 __device__ __forceinline__ void place(long long p, int tiles, int blocks, int* tile, int* block) {
   const long long group = p / ((long long)kGroup * blocks);
   const int in = (int)(p - group * kGroup * blocks), height = min(kGroup, tiles - (int)group * kGroup);
@@ -429,31 +519,94 @@ __device__ __forceinline__ void place(long long p, int tiles, int blocks, int* t
   *block = in / height;
 }
 
+// What a tile costs, by its height: on a full chip a stage of 128 rows takes this much of one of 256.
+constexpr int kWhole = 20, kHalf = 11;
+
+// Experts' tiles and their cost: cost[e] of the tiles of the experts before e, for one column block.
+template <int MOST>
+struct Costs {
+  int cost[MOST + 2];
+};
+
+// Tiles of more than 128 rows that an expert's rows make; one of the rest may follow.
+__device__ __forceinline__ int whole_tiles(int rows) { return (rows + kRows / 2 - 1) / kRows; }
+
+template <class Table, class Costs>
+__device__ __forceinline__ void list_costs(const ggk_fp8_args& a, Table& s, Costs& c) {
+  int before = 0;
+  for (int e0 = 0; e0 <= a.experts; e0 += kThreads) {
+    const int e = e0 + threadIdx.x;
+    const int rows = e <= a.experts ? s.first[e + 1] - s.first[e] : 0, tiles = (rows + kRows - 1) / kRows;
+    // Rows without an expert are cleared, which costs next to nothing.
+    const int mine = e < a.experts ? kWhole * whole_tiles(rows) + kHalf * (tiles - whole_tiles(rows)) : tiles;
+    int all;
+    const int at = gg::block_before<kThreads>(mine, 0x3fffffff, s.waves, &all) + before;
+    if (e <= a.experts) c.cost[e] = at;
+    before += all;
+  }
+  if (threadIdx.x == 0) c.cost[a.experts + 1] = before;
+  __syncthreads();
+}
+
+// Last of the a.experts + 1 entries of a rising table (times `by`) that is at most v; the first is 0.
+__device__ __forceinline__ int find_expert(const ggk_fp8_args& a, const int* table, long long by, long long v) {
+  const int lane = threadIdx.x % kWave;
+  int before = 0;
+  for (int e0 = 0; e0 <= a.experts; e0 += kWave) {
+    before += __popcll(__ballot(e0 + lane <= a.experts && table[min(e0 + lane, a.experts)] * by <= v));
+  }
+  return before - 1;
+}
+
+// First item that begins at cost `at` or after it.  An expert's items are its whole tiles by column blocks, then its rest.
+template <class Table, class Costs>
+__device__ __forceinline__ long long item_at(const ggk_fp8_args& a, const Table& s, const Costs& c, int blocks, long long at) {
+  const int e = find_expert(a, c.cost, blocks, at);
+  const long long left = at - (long long)c.cost[e] * blocks;
+  const long long whole = e < a.experts ? (long long)whole_tiles(s.first[e + 1] - s.first[e]) * blocks : 0;
+  const int rest = e < a.experts ? kHalf : 1;
+  const long long in = left <= whole * kWhole ? (left + kWhole - 1) / kWhole : whole + (left - whole * kWhole + rest - 1) / rest;
+  return (long long)s.tile[e] * blocks + in;
+}
+
 template <bool EXPERTS, bool GATED>
 __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
   const ggk_fp8_args& a = l.a;
+  constexpr int kMost = EXPERTS ? GGK_MOE_MAX_EXPERTS : 1;
   __shared__ alignas(128) unsigned char s_stages[2 * kParity + 2 * kScales];
   __shared__ int s_slot[EXPERTS ? kRows : 1], s_x_row[EXPERTS ? kRows : 1];
-  __shared__ Experts<EXPERTS ? GGK_MOE_MAX_EXPERTS : 1> s_experts;
+  __shared__ Experts<kMost> s_experts;
   const Shared s{s_stages, s_slot, s_x_row};
-  int tiles = (a.rows + kRows - 1) / kRows;
-  if constexpr (EXPERTS) {
+  // Neighbouring workgroups go to different XCDs, each with an L2 of its own: an XCD takes a run of the order, of an eighth
+  // of the cost.
+  const int xcd = blockIdx.x % kXcds;
+  if constexpr (!EXPERTS) {
+    const int tiles = (a.rows + l.height - 1) / l.height;
+    const long long items = (long long)tiles * l.blocks, share = (items + kXcds - 1) / kXcds;
+    const long long end = min((xcd + 1) * share, items);
+    for (long long item = xcd * share + blockIdx.x / kXcds; item < end; item += gridDim.x / kXcds) {
+      int tile, block;
+      place(item, tiles, l.blocks, &tile, &block);
+      const RowTile t{0, tile * l.height, min(l.height, a.rows - tile * l.height)};
+      run_either<false, GATED>(l, t, s, block * kColumns<GATED>);
+      gg::stage_barrier();
+    }
+  } else {
+    __shared__ Costs<kMost> s_costs;
     gg::list_experts<kThreads, kRows>(a, s_experts);
-    tiles = s_experts.tile[a.experts + 1];
-  }
-  // Neighbouring workgroups go to different XCDs, each with an L2 of its own: an XCD takes a run of the order.
-  const long long items = (long long)tiles * l.blocks, share = (items + kXcds - 1) / kXcds;
-  const long long first = blockIdx.x % kXcds * share, end = min(first + share, items);
-  const int fan = EXPERTS ? a.rows / a.x_rows : 1;
-  for (long long item = first + blockIdx.x / kXcds; item < end; item += gridDim.x / kXcds) {
-    int tile, block;
-    place(item, tiles, l.blocks, &tile, &block);
-    const int n0 = block * kColumns<GATED>;
-    if constexpr (!EXPERTS) {
-      const RowTile t{0, tile * kRows, min(kRows, a.rows - tile * kRows)};
-      run_tile<false, GATED>(l, t, s, n0);
-    } else {
-      const RowTile t = gg::expert_tile<kRows>(a, s_experts, tile);
+    list_costs(a, s_experts, s_costs);
+    const long long cost = (long long)s_costs.cost[a.experts + 1] * l.blocks;
+    const long long end = xcd + 1 < kXcds ? item_at(a, s_experts, s_costs, l.blocks, cost * (xcd + 1) / kXcds)
+                                          : (long long)s_experts.tile[a.experts + 1] * l.blocks;
+    const int fan = a.rows / a.x_rows;
+    for (long long item = item_at(a, s_experts, s_costs, l.blocks, cost * xcd / kXcds) + blockIdx.x / kXcds; item < end;
+         item += gridDim.x / kXcds) {
+      const int e = find_expert(a, s_experts.tile, l.blocks, item);
+      const int rows = s_experts.first[e + 1] - s_experts.first[e], whole = whole_tiles(rows);
+      const long long in = item - (long long)s_experts.tile[e] * l.blocks;
+      int tile = (int)(in / l.blocks), block = (int)(in % l.blocks);
+      if (tile < whole) place(in, whole, l.blocks, &tile, &block);
+      const RowTile t{e, s_experts.first[e] + tile * kRows, min(kRows, rows - tile * kRows)};
       for (int i = threadIdx.x; i < t.rows; i += kThreads) {
         int slot = a.order[t.first + i];
         if (slot >= a.rows) slot = -1;
@@ -461,19 +614,25 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
         s_x_row[i] = max(slot, 0) / fan;  // where a slot names no row, row 0: its sums are not used
       }
       gg::stage_barrier();
-      if (t.expert == a.experts) {
-        clear_tile<GATED>(a, t, s_slot, n0);
+      if (e == a.experts) {
+        clear_tile<GATED>(a, t, s_slot, block * kColumns<GATED>);
       } else {
-        run_tile<true, GATED>(l, t, s, n0);
+        run_either<true, GATED>(l, t, s, block * kColumns<GATED>);
       }
+      gg::stage_barrier();
     }
-    gg::stage_barrier();
   }
 }
 
 template <bool EXPERTS, bool GATED>
 hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
-  Launch l{a, (a.n + kColumns<GATED> - 1) / kColumns<GATED>, 0};
+  Launch l{a, (a.n + kColumns<GATED> - 1) / kColumns<GATED>, kRows, 0};
+  if (!EXPERTS) {
+    // What the busiest CU gets: tiles of 256 rows, or of 128 at 0.6 of their time.
+    auto rounds = [&](long long height) { return ((a.rows + height - 1) / height * l.blocks + kCus - 1) / kCus; };
+    const char* e = getenv("GG_H");
+    if (e ? atoi(e) == 128 : 10 * rounds(256) > 6 * rounds(128)) l.height = 128;
+  }
   if (EXPERTS) l.scale_bytes = (uint32_t)(((a.x_rows - 1) * a.ldxs + (a.k + kStep - 1) / kStep) * 4);
   hipLaunchKernelGGL((fp8_tile_kernel<EXPERTS, GATED>), dim3(kCus), dim3(kThreads), 0, stream, l);
   return hipGetLastError();
