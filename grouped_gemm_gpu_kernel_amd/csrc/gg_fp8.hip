@@ -8,6 +8,7 @@
 // wave waits for another until its sums are whole.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <stdlib.h>
 
 #include "gg_experts.h"
 #include "gg_fp8.h"
@@ -328,6 +329,7 @@ extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t str
   if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
   const ggk_fp8_args& a = *args;
   const long long rows = a.experts > 0 ? a.rows / a.experts : a.rows;
-  if (rows > 100 && (a.gate != GGK_GATE_NONE || a.y_type != GGK_TYPE_F32) && tiles_take(a)) return multiply_tiles(a, stream);
+  const char* env = getenv("GG_MIN");
+  if (rows > (env ? atoi(env) : 100) && (a.gate != GGK_GATE_NONE || a.y_type != GGK_TYPE_F32) && tiles_take(a)) return multiply_tiles(a, stream);
   return args->experts > 0 ? multiply_few<true>(*args, stream) : multiply_few<false>(*args, stream);
 }

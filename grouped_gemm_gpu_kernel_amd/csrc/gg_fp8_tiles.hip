@@ -26,7 +26,6 @@
 namespace {
 
 using namespace gg::fp8;
-using gg::Experts;
 using gg::RowTile;
 using gg::kWave;
 
@@ -45,7 +44,7 @@ constexpr int kColumns = GATED ? 128 : 256;
 struct Launch {
   ggk_fp8_args a;
   int blocks;            // of columns
-  int height;            // rows of a tile (one matrix)
+  int height;            // rows of a tile, 256 or 128
   uint32_t scale_bytes;  // of all of x's scales (experts)
 };
 
@@ -80,8 +79,9 @@ struct Loader {
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = min(128 * half + 64 * i + row, t.rows - 1);
-        a_off[half][i] = (uint32_t)((EXPERTS ? x_row[r] : r) * a.ldx) + piece16;
+        // Rows past the tile's are zeros: nothing is read for them, and their products take less power.
+        const int r = 128 * half + 64 * i + row;
+        a_off[half][i] = r < t.rows ? (uint32_t)((EXPERTS ? x_row[r] : r) * a.ldx) + piece16 : 0xffffffffu;
       }
     }
     const int column = GATED ? row : 64 * (row / 32) + row % 32;
@@ -496,12 +496,10 @@ __device__ __forceinline__ void run_either(const Launch& l, const RowTile& t, co
   }
 }
 
-// Rows without an expert.
 template <bool GATED>
-__device__ __forceinline__ void clear_tile(const ggk_fp8_args& a, const RowTile& t, const int* slots, int n0) {
-  for (int i = threadIdx.x; i < t.rows * kColumns<GATED>; i += kThreads) {
-    const int slot = slots[i / kColumns<GATED>], column = n0 + i % kColumns<GATED>;
-    if (column >= a.n || slot < 0) continue;
+__device__ __forceinline__ void clear_row(const ggk_fp8_args& a, int slot) {
+  if (slot < 0 || slot >= a.rows) return;
+  for (int column = threadIdx.x; column < a.n; column += kThreads) {
     if constexpr (GATED) {
       static_cast<unsigned char*>(a.y)[slot * a.ldy + column] = 0;
       if (column % kStep == 0) a.y_scales[slot * a.ldys + column / kStep] = gg::kFp8SmallestScale;
@@ -511,80 +509,101 @@ __device__ __forceinline__ void clear_tile(const ggk_fp8_args& a, const RowTile&
   }
 }
 
-// Row tile and column block of place p in an order that goes along the columns kGroup row tiles at a time.
+// Row tile and column block of place p in an order that goes along the columns kGroup row tiles at a time, so that the
+// workgroups of an XCD share both; each column block begins with another of them, so that a workgroup meets all.
 __device__ __forceinline__ void place(long long p, int tiles, int blocks, int* tile, int* block) {
   const long long group = p / ((long long)kGroup * blocks);
   const int in = (int)(p - group * kGroup * blocks), height = min(kGroup, tiles - (int)group * kGroup);
-  *tile = (int)group * kGroup + in % height;
   *block = in / height;
+  *tile = (int)group * kGroup + (in % height + *block) % height;
 }
 
-// What a tile costs, by its height: on a full chip a stage of 128 rows takes this much of one of 256.
-constexpr int kWhole = 20, kHalf = 11;
+// Experts' rows as tiles: whole ones of more than 128 rows, and a rest of at most 128 where there is one.
+constexpr int kWhole = 20, kRest = 11;  // what a tile costs: a stage of each, measured on a full chip
 
-// Experts' tiles and their cost: cost[e] of the tiles of the experts before e, for one column block.
 template <int MOST>
-struct Costs {
-  int cost[MOST + 2];
+struct Tiles {
+  int first[MOST + 2];  // places in the order, as in Experts; rows without an expert last
+  int tile[MOST + 1];   // tiles of the experts before, and of all
+  int cost[MOST + 1];   // and what they cost
+  int waves[32];
 };
 
-// Tiles of more than 128 rows that an expert's rows make; one of the rest may follow.
-__device__ __forceinline__ int whole_tiles(int rows) { return (rows + kRows / 2 - 1) / kRows; }
+__device__ __forceinline__ int whole_tiles(const Launch& l, int rows) {
+  return l.height == kRows ? (rows + kRows / 2 - 1) / kRows : 0;
+}
+__device__ __forceinline__ int tiles_of(const Launch& l, int rows) { return (rows + l.height - 1) / l.height; }
 
-template <class Table, class Costs>
-__device__ __forceinline__ void list_costs(const ggk_fp8_args& a, Table& s, Costs& c) {
-  int before = 0;
-  for (int e0 = 0; e0 <= a.experts; e0 += kThreads) {
+template <class Table>
+__device__ __forceinline__ void list_tiles(const Launch& l, Table& s) {
+  const ggk_fp8_args& a = l.a;
+  int placed = 0, tiles = 0, cost = 0;
+  for (int e0 = 0; e0 < a.experts; e0 += kThreads) {
     const int e = e0 + threadIdx.x;
-    const int rows = e <= a.experts ? s.first[e + 1] - s.first[e] : 0, tiles = (rows + kRows - 1) / kRows;
-    // Rows without an expert are cleared, which costs next to nothing.
-    const int mine = e < a.experts ? kWhole * whole_tiles(rows) + kHalf * (tiles - whole_tiles(rows)) : tiles;
-    int all;
-    const int at = gg::block_before<kThreads>(mine, 0x3fffffff, s.waves, &all) + before;
-    if (e <= a.experts) c.cost[e] = at;
-    before += all;
+    const int count = e < a.experts ? min(max(a.counts[e], 0), a.rows) : 0;
+    int all, all_tiles, all_cost;
+    const int first = gg::add_up_to(gg::block_before<kThreads>(count, a.rows, s.waves, &all), placed, a.rows);
+    const int rows = min(count, a.rows - first), mine = tiles_of(l, rows), whole = whole_tiles(l, rows);
+    const int at_tile = gg::block_before<kThreads>(mine, 0x3fffffff, s.waves, &all_tiles) + tiles;
+    const int at_cost = gg::block_before<kThreads>(kWhole * whole + kRest * (mine - whole), 0x3fffffff, s.waves, &all_cost) + cost;
+    if (e < a.experts) {
+      s.first[e] = first;
+      s.tile[e] = at_tile;
+      s.cost[e] = at_cost;
+    }
+    placed = gg::add_up_to(placed, all, a.rows);
+    tiles += all_tiles;
+    cost += all_cost;
   }
-  if (threadIdx.x == 0) c.cost[a.experts + 1] = before;
+  if (threadIdx.x == 0) {
+    s.first[a.experts] = placed;
+    s.first[a.experts + 1] = a.rows;
+    s.tile[a.experts] = tiles;
+    s.cost[a.experts] = cost;
+  }
   __syncthreads();
 }
 
-// Last of the a.experts + 1 entries of a rising table (times `by`) that is at most v; the first is 0.
+// Last of a rising table's a.experts entries (times `by`) that is at most v; the first is 0.
 __device__ __forceinline__ int find_expert(const ggk_fp8_args& a, const int* table, long long by, long long v) {
   const int lane = threadIdx.x % kWave;
   int before = 0;
-  for (int e0 = 0; e0 <= a.experts; e0 += kWave) {
-    before += __popcll(__ballot(e0 + lane <= a.experts && table[min(e0 + lane, a.experts)] * by <= v));
+  for (int e0 = 0; e0 < a.experts; e0 += kWave) {
+    before += __popcll(__ballot(e0 + lane < a.experts && table[min(e0 + lane, a.experts)] * by <= v));
   }
   return before - 1;
 }
 
-// First item that begins at cost `at` or after it.  An expert's items are its whole tiles by column blocks, then its rest.
-template <class Table, class Costs>
-__device__ __forceinline__ long long item_at(const ggk_fp8_args& a, const Table& s, const Costs& c, int blocks, long long at) {
-  const int e = find_expert(a, c.cost, blocks, at);
-  const long long left = at - (long long)c.cost[e] * blocks;
-  const long long whole = e < a.experts ? (long long)whole_tiles(s.first[e + 1] - s.first[e]) * blocks : 0;
-  const int rest = e < a.experts ? kHalf : 1;
-  const long long in = left <= whole * kWhole ? (left + kWhole - 1) / kWhole : whole + (left - whole * kWhole + rest - 1) / rest;
-  return (long long)s.tile[e] * blocks + in;
+// First item, of those that begin a column block of a group, at cost `at` of all or after it.
+template <class Table>
+__device__ __forceinline__ long long item_at(const Launch& l, const Table& s, long long at) {
+  const ggk_fp8_args& a = l.a;
+  const int blocks = l.blocks;
+  const int e = find_expert(a, s.cost, blocks, at), rows = s.first[e + 1] - s.first[e];
+  const int each = l.height == kRows ? kWhole : kRest;  // of the tiles of every group but the last
+  const int tiles = tiles_of(l, rows), groups = (tiles + kGroup - 1) / kGroup;
+  long long left = at - (long long)s.cost[e] * blocks, item = (long long)s.tile[e] * blocks;
+  const int group = (int)min(left / (kGroup * each * (long long)blocks), (long long)groups - 1);
+  left -= (long long)group * kGroup * each * blocks;
+  item += (long long)group * kGroup * blocks;
+  const int cost = group < groups - 1 ? kGroup * each : s.cost[e + 1] - s.cost[e] - group * kGroup * each;
+  return item + (left + cost - 1) / cost * min(kGroup, tiles - group * kGroup);
 }
 
 template <bool EXPERTS, bool GATED>
 __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
   const ggk_fp8_args& a = l.a;
-  constexpr int kMost = EXPERTS ? GGK_MOE_MAX_EXPERTS : 1;
   __shared__ alignas(128) unsigned char s_stages[2 * kParity + 2 * kScales];
   __shared__ int s_slot[EXPERTS ? kRows : 1], s_x_row[EXPERTS ? kRows : 1];
-  __shared__ Experts<kMost> s_experts;
   const Shared s{s_stages, s_slot, s_x_row};
-  // Neighbouring workgroups go to different XCDs, each with an L2 of its own: an XCD takes a run of the order, of an eighth
-  // of the cost.
-  const int xcd = blockIdx.x % kXcds;
+  // Neighbouring workgroups go to different XCDs, each with an L2 of its own: an XCD takes a run of the order, an eighth of
+  // the items or of what they cost.
+  const int xcd = blockIdx.x % kXcds, in_xcd = blockIdx.x / kXcds;
   if constexpr (!EXPERTS) {
     const int tiles = (a.rows + l.height - 1) / l.height;
     const long long items = (long long)tiles * l.blocks, share = (items + kXcds - 1) / kXcds;
     const long long end = min((xcd + 1) * share, items);
-    for (long long item = xcd * share + blockIdx.x / kXcds; item < end; item += gridDim.x / kXcds) {
+    for (long long item = xcd * share + in_xcd; item < end; item += kCus / kXcds) {
       int tile, block;
       place(item, tiles, l.blocks, &tile, &block);
       const RowTile t{0, tile * l.height, min(l.height, a.rows - tile * l.height)};
@@ -592,47 +611,42 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
       gg::stage_barrier();
     }
   } else {
-    __shared__ Costs<kMost> s_costs;
-    gg::list_experts<kThreads, kRows>(a, s_experts);
-    list_costs(a, s_experts, s_costs);
-    const long long cost = (long long)s_costs.cost[a.experts + 1] * l.blocks;
-    const long long end = xcd + 1 < kXcds ? item_at(a, s_experts, s_costs, l.blocks, cost * (xcd + 1) / kXcds)
-                                          : (long long)s_experts.tile[a.experts + 1] * l.blocks;
+    __shared__ Tiles<GGK_MOE_MAX_EXPERTS> s_tiles;
+    list_tiles(l, s_tiles);
+    const long long cost = (long long)s_tiles.cost[a.experts] * l.blocks, items = (long long)s_tiles.tile[a.experts] * l.blocks;
+    const long long end = xcd + 1 < kXcds && cost > 0 ? item_at(l, s_tiles, cost * (xcd + 1) / kXcds) : items;
+    const long long begin = xcd > 0 && cost > 0 ? item_at(l, s_tiles, cost * xcd / kXcds) : 0;
     const int fan = a.rows / a.x_rows;
-    for (long long item = item_at(a, s_experts, s_costs, l.blocks, cost * xcd / kXcds) + blockIdx.x / kXcds; item < end;
-         item += gridDim.x / kXcds) {
-      const int e = find_expert(a, s_experts.tile, l.blocks, item);
-      const int rows = s_experts.first[e + 1] - s_experts.first[e], whole = whole_tiles(rows);
-      const long long in = item - (long long)s_experts.tile[e] * l.blocks;
-      int tile = (int)(in / l.blocks), block = (int)(in % l.blocks);
-      if (tile < whole) place(in, whole, l.blocks, &tile, &block);
-      const RowTile t{e, s_experts.first[e] + tile * kRows, min(kRows, rows - tile * kRows)};
-      for (int i = threadIdx.x; i < t.rows; i += kThreads) {
-        int slot = a.order[t.first + i];
+    for (long long item = begin + in_xcd; item < end; item += kCus / kXcds) {
+      const int e = find_expert(a, s_tiles.tile, l.blocks, item), rows = s_tiles.first[e + 1] - s_tiles.first[e];
+      int tile, block;
+      place(item - (long long)s_tiles.tile[e] * l.blocks, tiles_of(l, rows), l.blocks, &tile, &block);
+      const RowTile t{e, s_tiles.first[e] + tile * l.height, min(l.height, rows - tile * l.height)};
+      for (int r = threadIdx.x; r < t.rows; r += kThreads) {
+        int slot = a.order[t.first + r];
         if (slot >= a.rows) slot = -1;
-        s_slot[i] = slot;
-        s_x_row[i] = max(slot, 0) / fan;  // where a slot names no row, row 0: its sums are not used
+        s_slot[r] = slot;
+        s_x_row[r] = max(slot, 0) / fan;  // where a slot names no row, row 0: its sums are not used
       }
       gg::stage_barrier();
-      if (e == a.experts) {
-        clear_tile<GATED>(a, t, s_slot, block * kColumns<GATED>);
-      } else {
-        run_either<true, GATED>(l, t, s, block * kColumns<GATED>);
-      }
+      run_either<true, GATED>(l, t, s, block * kColumns<GATED>);
       gg::stage_barrier();
     }
+    // Rows without an expert.
+    for (int at = s_tiles.first[a.experts] + blockIdx.x; at < a.rows; at += kCus) clear_row<GATED>(a, a.order[at]);
   }
 }
 
 template <bool EXPERTS, bool GATED>
 hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
   Launch l{a, (a.n + kColumns<GATED> - 1) / kColumns<GATED>, kRows, 0};
-  if (!EXPERTS) {
-    // What the busiest CU gets: tiles of 256 rows, or of 128 at 0.6 of their time.
-    auto rounds = [&](long long height) { return ((a.rows + height - 1) / height * l.blocks + kCus - 1) / kCus; };
-    const char* e = getenv("GG_H");
-    if (e ? atoi(e) == 128 : 10 * rounds(256) > 6 * rounds(128)) l.height = 128;
-  }
+  // What the busiest CU gets: tiles of 256 rows, or of 128 at 0.6 of their time; of an expert's rows half a tile more.
+  auto rounds = [&](long long height) {
+    const long long tiles = EXPERTS ? a.rows / height + a.experts / 2 : (a.rows + height - 1) / height;
+    return (tiles * l.blocks + kCus - 1) / kCus;
+  };
+  const char* e = getenv("GG_H");
+  if (e ? atoi(e) == 128 : 10 * rounds(256) > 6 * rounds(128)) l.height = 128;
   if (EXPERTS) l.scale_bytes = (uint32_t)(((a.x_rows - 1) * a.ldxs + (a.k + kStep - 1) / kStep) * 4);
   hipLaunchKernelGGL((fp8_tile_kernel<EXPERTS, GATED>), dim3(kCus), dim3(kThreads), 0, stream, l);
   return hipGetLastError();
