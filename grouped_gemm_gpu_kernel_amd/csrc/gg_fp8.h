@@ -41,11 +41,11 @@ __device__ __forceinline__ void load_to_lds4_at(const void* p, uint32_t lds) {
   asm volatile("s_nop 4\n\tglobal_load_lds_dword %1, off" : : "{m0}"(m0), "v"(p) : "memory");
 }
 
-// The 32 numbers of a lane: a row's 128 bytes at `at` (LDS byte address, its swizzled piece g).
-__device__ __forceinline__ int8v read_fragment(uint32_t at) {
-  const uint4v lo = *(const GG_LDS uint4v*)(uintptr_t)at;
-  const uint4v hi = *(const GG_LDS uint4v*)(uintptr_t)(at ^ 64u);
-  return int8v{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+// The 32 numbers of a lane: its swizzled pieces g and g + 4 of a row's 128 bytes, at lo and hi = lo ^ 64 (LDS byte addresses)
+// of some row and `offset` (whole rows) on, which the instruction adds.
+__device__ __forceinline__ int8v read_fragment(uint32_t lo, uint32_t hi, uint32_t offset) {
+  const uint4v a = *(const GG_LDS uint4v*)(uintptr_t)(lo + offset), b = *(const GG_LDS uint4v*)(uintptr_t)(hi + offset);
+  return int8v{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
 
 // The same numbers in binary16, exactly (e4m3 has 4 significant bits and exponents from -9 to 8).

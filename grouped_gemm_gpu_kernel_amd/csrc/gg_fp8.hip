@@ -12,6 +12,7 @@
 
 #include "gg_experts.h"
 #include "gg_fp8.h"
+#include "gg_phased.h"  // wait_lgkmcnt
 
 namespace {
 
@@ -20,11 +21,12 @@ using gg::Experts;
 using gg::RowTile;
 using gg::kWave;
 
-constexpr int kCus = 256;
+constexpr int kCus = 256, kXcds = 8;
 
 struct Launch {
   ggk_fp8_args a;
   int blocks;  // of columns
+  int tiles;   // of rows that the grid has (one matrix)
 };
 
 // R rows of x (8, 16, 32, 64) by WN waves of NT tiles of 16 columns (with a gate: half of them gate, half up), WK waves
@@ -42,13 +44,26 @@ struct Form {
   static constexpr int SUM_LD = WN * 16 * NT + 4;
   static constexpr int RING = WAVES * DEPTH * STEP, SUMS = 4 * WK * MT * 16 * SUM_LD;
   static constexpr int BYTES = RING > SUMS ? RING : SUMS;
-  static_assert(LOADS * (DEPTH - 1) < 64, "outstanding loads are counted in 6 bits");
+  static_assert(DEPTH >= 2 && LOADS * DEPTH < 64, "outstanding loads are counted in 6 bits");
   static_assert(!GATED || COLUMNS == 128, "a block of an 8-bit row");
 };
 
+// A step's products of 16 rows of x, times their scales.
+template <class F, class Operand>
+__device__ __forceinline__ void add_step(const Operand (&w)[F::NT], const Operand& x, float x_scale, float w_scale, float u_scale,
+                                         float4v (&sum)[F::NT]) {
+  const float scale = x_scale * w_scale, scale_u = x_scale * u_scale;
+#pragma unroll
+  for (int n = 0; n < F::NT; ++n) {
+    const float4v part = multiply(w[n], x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[n][e] = fmaf(F::GATED && n >= F::NT / 2 ? scale_u : scale, part[e], sum[n][e]);
+  }
+}
+
 // The wave's sums over its steps of K of one tile of rows by its columns.
 template <class F>
-__device__ __forceinline__ void multiply_item(const ggk_fp8_args& a, const RowTile& t, const int* x_row, int column0,
+__device__ __forceinline__ void multiply_item(const ggk_fp8_args& a, const RowTile& t, const int* x_row, int column0, int turn,
                                               unsigned char* ring, float4v (&sum)[F::MT][F::NT]) {
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wk = wave % F::WK;
@@ -80,8 +95,11 @@ __device__ __forceinline__ void multiply_item(const ggk_fp8_args& a, const RowTi
   if (F::GATED && lane % 32 == 1) ws = a.up_scales + t.expert * a.stride_us + base_column / kStep * a.ldus;
   if (F::SL == 1 && lane >= 32) xs = ws;
 
+  // In step, the waves would all read the same columns at a time, and rows a power of two apart lie in a few channels of
+  // the L2: every wave begins with another of its steps and goes on around the end.
+  const int first = (turn + wave / F::WK * max(mine / F::WN, 1)) % max(mine, 1);
   auto issue = [&](int i) {  // the wave's step i into its place of the ring
-    const int step = i * F::WK + wk, k0 = step * kStep;
+    const int turned = i + first < mine ? i + first : i + first - mine, step = turned * F::WK + wk, k0 = step * kStep;
     const uint32_t at = ring_at + (i % F::DEPTH) * F::STEP;
     const bool whole = k0 + kStep <= a.k;
 #pragma unroll
@@ -104,60 +122,58 @@ __device__ __forceinline__ void multiply_item(const ggk_fp8_args& a, const RowTi
     for (int n = 0; n < F::NT; ++n) sum[m][n] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
   }
 #pragma unroll
-  for (int i = 0; i < F::DEPTH - 1; ++i) {
+  for (int i = 0; i < F::DEPTH; ++i) {
     if (i < mine) issue(i);
   }
   const int j = lane % 16, g = lane / 16, x_j = F::R < 16 ? j % 8 : j;
-  const uint32_t w_at = j * 128 + ((g ^ (j >> 1)) & 7) * 16, x_at = F::X + x_j * 128 + ((g ^ (x_j >> 1)) & 7) * 16;
+  const uint32_t w_at = j * 128 + ((g ^ (j >> 1)) & 7) * 16, x_at = x_j * 128 + ((g ^ (x_j >> 1)) & 7) * 16;
 #pragma unroll 1
   for (int i = 0; i < mine; ++i) {
-    // Step i has landed when at most the loads of the DEPTH - 2 steps after it are on their way.
-    if (i + F::DEPTH - 1 <= mine) {
-      gg::wait_vmcnt<F::LOADS * (F::DEPTH - 2)>();
+    // Step i has landed when at most the loads of the DEPTH - 1 steps after it are on their way.
+    if (i + F::DEPTH <= mine) {
+      gg::wait_vmcnt<F::LOADS * (F::DEPTH - 1)>();
     } else {
       gg::wait_vmcnt<0>();
     }
     asm volatile("" ::: "memory");
     const uint32_t at = ring_at + (i % F::DEPTH) * F::STEP;
-    using Operand = std::conditional_t<F::EXACT, Halves, int8v>;
-    auto read = [&](uint32_t from) {
-      if constexpr (F::EXACT) {
-        return to_halves(read_fragment(from));
-      } else {
-        return read_fragment(from);
-      }
-    };
-    Operand w[F::NT];
+    int8v w[F::NT], x[F::MT];
+    float x_scale[F::MT];
 #pragma unroll
-    for (int n = 0; n < F::NT; ++n) w[n] = read(at + w_at + 2048 * n);
-    const float w_scale = *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * F::WS);
-    const float u_scale = F::GATED ? *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * F::WS + 4) : 0.0f;
-    // The place of step i - 1 is free: every read of it has returned before its products were made.
-    if (i + F::DEPTH - 1 < mine) issue(i + F::DEPTH - 1);
+    for (int n = 0; n < F::NT; ++n) w[n] = read_fragment(at + w_at, at + (w_at ^ 64), 2048 * n);
 #pragma unroll
     for (int m = 0; m < F::MT; ++m) {
-      const Operand x = read(at + x_at + 2048 * m);
-      const float x_scale = *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * (16 * m + x_j));
-      const float scale = x_scale * w_scale, scale_u = F::GATED ? x_scale * u_scale : 0.0f;
-#pragma unroll
-      for (int n = 0; n < F::NT; ++n) {
-        const float4v part_sum = multiply(w[n], x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[m][n][e] = fmaf(n < kTilesOfW ? scale : scale_u, part_sum[e], sum[m][n][e]);
-      }
+      x[m] = read_fragment(at + x_at, at + (x_at ^ 64), F::X + 2048 * m);
+      x_scale[m] = *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * (16 * m + x_j));
     }
+    const float w_scale = *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * F::WS);
+    const float u_scale = F::GATED ? *(const GG_LDS float*)(uintptr_t)(at + F::S + 4 * F::WS + 4) : 0.0f;
+    // All of the step is in registers: its place takes another.
     asm volatile("" ::: "memory");
+    gg::wait_lgkmcnt<0>();
+    if (i + F::DEPTH < mine) issue(i + F::DEPTH);
+    if constexpr (F::EXACT) {
+      Halves h[F::NT];
+#pragma unroll
+      for (int n = 0; n < F::NT; ++n) h[n] = to_halves(w[n]);
+#pragma unroll
+      for (int m = 0; m < F::MT; ++m) add_step<F>(h, to_halves(x[m]), x_scale[m], w_scale, u_scale, sum[m]);
+    } else {
+#pragma unroll
+      for (int m = 0; m < F::MT; ++m) add_step<F>(w, x[m], x_scale[m], w_scale, u_scale, sum[m]);
+    }
   }
 }
 
 // One tile of rows by the workgroup's columns from block0 on: sums, their join over the waves along K, y.
 template <class F, bool EXPERTS>
 __device__ __forceinline__ void run_item(const ggk_fp8_args& a, const RowTile& t, const int* slots, const int* x_row,
-                                         int block0, unsigned char* s_bytes) {
+                                         int block, unsigned char* s_bytes) {
+  const int block0 = block * F::COLUMNS;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int j = lane % 16, g = lane / 16, wn = wave / F::WK, wk = wave % F::WK;
   float4v sum[F::MT][F::NT];
-  multiply_item<F>(a, t, x_row, block0 + wn * (F::COLUMNS / F::WN), s_bytes + wave * F::DEPTH * F::STEP, sum);
+  multiply_item<F>(a, t, x_row, block0 + wn * (F::COLUMNS / F::WN), block / kXcds, s_bytes + wave * F::DEPTH * F::STEP, sum);
   const bool vec = a.n % 4 == 0 && (a.ldy % 4 == 0 || a.rows <= 1) && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
   float* s_sum = reinterpret_cast<float*>(s_bytes);  // [WK][16 MT][SUM_LD]
   gg::stage_barrier();
@@ -221,14 +237,18 @@ __device__ __forceinline__ void clear_item(const ggk_fp8_args& a, const RowTile&
 }
 
 template <class F, bool EXPERTS>
-__global__ __launch_bounds__(F::THREADS, 2) void fp8_stream_kernel(Launch l) {
+__global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::BYTES <= 80 * 1024 ? F::WAVES / 2 : F::WAVES / 4) void fp8_stream_kernel(Launch l) {
   const ggk_fp8_args& a = l.a;
   __shared__ alignas(128) unsigned char s_bytes[F::BYTES];
   if constexpr (!EXPERTS) {
-    const int tiles = (a.rows + F::R - 1) / F::R;
-    for (int tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
+    // Neighbouring workgroups go to different XCDs: a column block's row tiles follow each other on one, so that its L2 has
+    // the weights for all of them.
+    const int tiles = (a.rows + F::R - 1) / F::R, in_xcd = blockIdx.x / kXcds;
+    const int block = in_xcd / l.tiles * kXcds + blockIdx.x % kXcds;
+    if (block >= l.blocks) return;
+    for (int tile = in_xcd % l.tiles; tile < tiles; tile += l.tiles) {
       const RowTile t{0, tile * F::R, min(F::R, a.rows - tile * F::R)};
-      run_item<F, false>(a, t, nullptr, nullptr, blockIdx.x * F::COLUMNS, s_bytes);
+      run_item<F, false>(a, t, nullptr, nullptr, block, s_bytes);
       gg::stage_barrier();
     }
   } else {
@@ -250,7 +270,7 @@ __global__ __launch_bounds__(F::THREADS, 2) void fp8_stream_kernel(Launch l) {
       if (t.expert == a.experts) {
         clear_item<F>(a, t, s_slot, block * F::COLUMNS);
       } else {
-        run_item<F, true>(a, t, s_slot, s_x_row, block * F::COLUMNS, s_bytes);
+        run_item<F, true>(a, t, s_slot, s_x_row, block, s_bytes);
       }
       gg::stage_barrier();
     }
@@ -259,29 +279,57 @@ __global__ __launch_bounds__(F::THREADS, 2) void fp8_stream_kernel(Launch l) {
 
 template <class F, bool EXPERTS>
 hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
-  Launch l{a, (a.n + F::COLUMNS - 1) / F::COLUMNS};
+  Launch l{a, (a.n + F::COLUMNS - 1) / F::COLUMNS, 0};
   const long long tiles = (a.rows + F::R - 1) / F::R + (EXPERTS ? (a.rows < a.experts + 1 ? a.rows : a.experts + 1) : 0);
-  dim3 grid(l.blocks, (unsigned)(tiles < 65535 ? tiles : 65535));
+  long long grid;
   if (EXPERTS) {
     const long long items = tiles * l.blocks, most = kCus * (F::BYTES > 64 * 1024 ? 1 : 2);
-    grid = dim3((unsigned)(items < most ? items : most));
+    grid = items < most ? items : most;
+  } else {
+    const long long columns = (l.blocks + kXcds - 1) / kXcds * kXcds, most = (1 << 30) / columns;
+    l.tiles = (int)(tiles < most ? tiles : most);
+    grid = columns * l.tiles;
   }
-  hipLaunchKernelGGL((fp8_stream_kernel<F, EXPERTS>), grid, dim3(F::THREADS), 0, stream, l);
+  hipLaunchKernelGGL((fp8_stream_kernel<F, EXPERTS>), dim3((unsigned)grid), dim3(F::THREADS), 0, stream, l);
   return hipGetLastError();
 }
 
+#ifdef GG_FORMS
 template <bool EXPERTS>
 hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
-  const int rows = EXPERTS ? (a.rows + a.experts - 1) / a.experts : a.rows;
-  if (a.gate != GGK_GATE_NONE) {
-    if (rows <= 8) return launch<Form<8, 2, 8, 1, 3, true, true>, EXPERTS>(a, stream);
-    return launch<Form<16, 2, 8, 1, 2, true, true>, EXPERTS>(a, stream);
+  const char* f = getenv("GG_F");
+  const int i = f ? atoi(f) : 0;
+  switch (i) {
+    GG_FORMS
   }
-  if (rows <= 8) return launch<Form<8, 1, 2, 4, 4, false, true>, EXPERTS>(a, stream);
-  if (rows <= 16) return launch<Form<16, 1, 2, 4, 4, false, true>, EXPERTS>(a, stream);
-  return launch<Form<32, 2, 2, 4, 2, false, true>, EXPERTS>(a, stream);
+  return hipErrorInvalidValue;
+}
+#else
+template <bool EXPERTS>
+hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
+  const bool exact = a.y_type == GGK_TYPE_F32;
+  if constexpr (EXPERTS) {
+    if (a.gate != GGK_GATE_NONE) return launch<Form<32, 2, 8, 1, 2, true, false>, true>(a, stream);
+    if (a.rows <= 32) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream);
+    if (a.rows <= 12ll * a.experts) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream);
+    if (exact) return launch<Form<32, 2, 4, 2, 2, false, true>, true>(a, stream);
+    return launch<Form<32, 2, 4, 2, 2, false, false>, true>(a, stream);
+  } else if (a.gate != GGK_GATE_NONE) {
+    if (a.rows <= 8) return launch<Form<8, 4, 4, 1, 4, true, true>, false>(a, stream);
+    if (a.rows <= 16) return launch<Form<16, 2, 8, 1, 3, true, true>, false>(a, stream);
+    return launch<Form<32, 2, 8, 1, 2, true, false>, false>(a, stream);
+  } else {
+    if (a.rows <= 8) return launch<Form<8, 1, 1, 8, 2, false, true>, false>(a, stream);
+    if (a.rows <= 16) {
+      return a.n >= 8192 ? launch<Form<16, 1, 2, 4, 2, false, true>, false>(a, stream)
+                         : launch<Form<16, 1, 1, 8, 2, false, true>, false>(a, stream);
+    }
+    if (exact) return launch<Form<32, 2, 1, 4, 2, false, true>, false>(a, stream);
+    return launch<Form<32, 2, 1, 4, 2, false, false>, false>(a, stream);
+  }
 }
 
+#endif
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace

@@ -145,7 +145,9 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
   const int wm = wave >> 2, wn = wave & 3;
   const uint32_t lane_at = (uint32_t)(j * 128 + ((g ^ (j >> 1)) & 7) * 16);
-  const uint32_t a_lane = lds + lane_at + wm * 64 * 128, b_lane = lds + lane_at + wn * 32 * 128;
+  // Of the lane's fragments in unit 0 of the ring; the parity of the stage is added once a phase.
+  const uint32_t a_lo = lds + lane_at + wm * 64 * 128, a_hi = lds + (lane_at ^ 64) + wm * 64 * 128;
+  const uint32_t b_lo = lds + lane_at + wn * 32 * 128, b_hi = lds + (lane_at ^ 64) + wn * 32 * 128;
   const uint32_t x_scale_lane = scales_at + (wm * 64 + j) * 16;
   const uint32_t w_scale_lane = scales_at + 4096 + (GATED ? 0 : (wn >> 1) * 1024);
 
@@ -168,8 +170,22 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   left[0] = left[1] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
   left_scale = 0.0f;
 
-  auto read_a = [&](uint32_t unit, int i) { a[i] = read_fragment(a_lane + unit + 2048u * i); };
-  auto read_b = [&](uint32_t unit, int which, int n) { b[which][n] = read_fragment(b_lane + unit + 2048u * n); };
+  // Reads of a phase begin with `from`: two additions, held in registers (the empty asm), and the rest are the instructions'
+  // own offsets; with an addition for every read the vector unit was short of slots beside the matrix instructions.
+  uint32_t lo, hi;
+  auto from = [&](uint32_t lane_lo, uint32_t lane_hi, uint32_t base) {
+    lo = lane_lo + base;
+    hi = lane_hi + base;
+    asm volatile("" : "+v"(lo), "+v"(hi));
+  };
+  auto read_a = [&](uint32_t base, uint32_t unit, int i) {
+    if (i == 0) from(a_lo, a_hi, base);
+    a[i] = read_fragment(lo, hi, unit + 2048u * i);
+  };
+  auto read_b = [&](uint32_t base, uint32_t unit, int which, int n, bool begin) {
+    if (begin) from(b_lo, b_hi, base);
+    b[which][n] = read_fragment(lo, hi, unit + 2048u * n);
+  };
   // Scales of stage kt: rows of A half `half` (into set `set`), and the units' weights.  Read two phases ahead, so that their
   // wait is none for the fragments read since.
   auto read_x_scales = [&](int kt, int half, int set) {
@@ -237,9 +253,9 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
     gg::wait_vmcnt<5 * kLoads>();
     gg::phase_barrier();
 #pragma unroll
-    for (int n = 0; n < 2; ++n) read_b(place_of(0), 0, n);
+    for (int n = 0; n < 2; ++n) read_b(0, 0, 0, n, n == 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) read_a(place_of(1), i);
+    for (int i = 0; i < 4; ++i) read_a(0, kUnit, i);
     read_x_scales(0, 0, 0);
     read_w_scales(0);
     next_w_scales();
@@ -252,7 +268,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
       const uint32_t b1 = place_of(u + 2), b0 = place_of(u + 3), a0 = place_of(u + 4);
       phase(0, 0, 0, 1, [&](int r) { if (r == 4 || r == 6) issue_unit(u + 7, kt + 2, 1, r / 2 - 2); },
             [&](int r) {
-              if (r == 1 || r == 3) read_b(b1, 1, r / 2);
+              if (r == 1 || r == 3) read_b(b1, 0, 1, r / 2, r == 1);
               if (r == 5) {
                 read_x_scales(kt + 1, 0, 1);
                 read_w_scales(kt + 1);
@@ -261,7 +277,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
       gg::wait_vmcnt<3 * kLoads>();
       gg::phase_barrier();
       phase(0, 1, 0, 0, [&](int r) { if (r >= 4) issue_unit(u + 8 + (r - 4) / 2, kt + 2 + (r - 4) / 2, r < 6 ? 2 : 0, r & 1); },
-            [&](int r) { if (r & 1) read_a(a0, r / 2); else if (r < 4) read_b(b0, 0, r / 2); });
+            [&](int r) { if (r == 0) { read_b(b0, 0, 0, 0, true); read_b(b0, 0, 0, 1, false); } if (r & 1) read_a(a0, 0, r / 2); });
 #pragma unroll
       for (int i = 0; i < 4; ++i) x_scale[0][i] = x_scale[1][i];
       next_w_scales();
@@ -288,9 +304,9 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
     gg::wait_vmcnt<6 * kLoads>();
     gg::phase_barrier();
 #pragma unroll
-    for (int n = 0; n < 2; ++n) read_b(kB0, 0, n);
+    for (int n = 0; n < 2; ++n) read_b(0, kB0, 0, n, n == 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) read_a(kA0, i);
+    for (int i = 0; i < 4; ++i) read_a(0, kA0, i);
     read_x_scales(0, 0, 0);
     read_w_scales(0);
     next_w_scales();
@@ -309,13 +325,13 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
       if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
       phase(0, 0, 1, 1, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_b(kt + 2, 0, st + kB0, r / 2 - 2); },
             [&](int r) {
-              if (r == 1 || r == 3) read_b(here + kB1, 1, r / 2);
+              if (r == 1 || r == 3) read_b(here, kB1, 1, r / 2, r == 1);
               if (r == 5) read_x_scales(kt, 1, 1);
             });
       gg::wait_vmcnt<ISSUE ? 5 * N : LAST ? 0 : 4 * N>();
       gg::phase_barrier();
       phase(0, 1, 0, 0, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_a(kt + 2, 0, st + kA0, r / 2 - 2); },
-            [&](int r) { if (r & 1) read_a(here + kA1, r / 2); });
+            [&](int r) { if (r & 1) read_a(here, kA1, r / 2); });
       if constexpr (!LAST) {
         gg::wait_vmcnt<ISSUE ? 5 * N : 3 * N>();
         gg::phase_barrier();
@@ -327,7 +343,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
                   read_x_scales(kt + 1, 0, 0);
                   read_w_scales(kt + 1);
                 }
-                if (r >= 6) read_b(next + kB0, 0, 7 - r);
+                if (r >= 6) read_b(next, kB0, 0, 7 - r, r == 6);
               }
             });
       if constexpr (!LAST) {
@@ -335,7 +351,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
         gg::phase_barrier();
       }
       phase(1, 1, 1, 0, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_a(kt + 2, 1, st + kA1, r / 2 - 2); },
-            [&](int r) { if constexpr (!LAST) { if (r & 1) read_a(next + kA0, r / 2); } });
+            [&](int r) { if constexpr (!LAST) { if (r & 1) read_a(next, kA0, r / 2); } });
       if constexpr (!LAST) {
         gg::wait_lgkmcnt<8>();  // phase 2's reads, which nothing has used yet; this phase's eight may be on their way
         next_w_scales();
