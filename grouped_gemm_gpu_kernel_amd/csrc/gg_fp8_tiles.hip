@@ -32,10 +32,11 @@ using gg::kWave;
 constexpr int kCus = 256, kXcds = 8;
 constexpr int kRows = 256, kWaves = 8, kThreads = kWaves * kWave;
 constexpr int kUnit = 128 * kStep;  // bytes
-constexpr int kB0 = 0, kA0 = kUnit, kB1 = 2 * kUnit, kA1 = 3 * kUnit, kParity = 4 * kUnit, kPlaces = 8;
+constexpr int kB0 = 0, kA0 = kUnit, kB1 = 2 * kUnit, kA1 = 3 * kUnit, kParity = 4 * kUnit, kPlaces = 9;
 constexpr int kLoads = 2;           // load instructions of a unit and wave
 constexpr int kScaleSteps = 4;      // stages of scales loaded at once, 16 bytes a row
-constexpr int kScales = 6 * 1024;   // bytes of those: 256 rows, and a row of each unit's weights in 1 KB each
+constexpr int kScales = 4096 + 128; // bytes of those: 256 rows, and a row of each unit's weights
+constexpr int kMost = 512;          // experts that the table has room for
 constexpr int kGroup = 4;           // row tiles that go along the columns together
 
 template <bool GATED>
@@ -45,13 +46,13 @@ struct Launch {
   ggk_fp8_args a;
   int blocks;            // of columns
   int height;            // rows of a tile, 256 or 128
+  int fan;               // slots of a row of x
   uint32_t scale_bytes;  // of all of x's scales (experts)
 };
 
 struct Shared {
-  unsigned char* stages;  // two stages, then two sets of scales
+  unsigned char* stages;  // places of units, then two sets of scales
   int* slot;              // of the tile's rows, -1 for none
-  int* x_row;
 };
 
 // Sums of one tile: [rows half][16 rows][unit of columns][16 columns].
@@ -69,19 +70,21 @@ struct Loader {
   const float* s0;
   int piece16, wave;
 
-  __device__ __forceinline__ Loader(const Launch& l, const RowTile& t, const int* x_row, int n0, int wave_)
+  __device__ __forceinline__ Loader(const Launch& l, const RowTile& t, const int* slot, int n0, int wave_)
       : a(l.a), wave(wave_) {
     const int tid = gg::opaque_tid(wave), row = tid / 8;
     const int piece = (tid & 7) ^ (row >> 1 & 7);
     piece16 = 16 * piece;
     x0 = EXPERTS ? a.x : a.x + t.first * a.ldx;
+    // Where a slot names no row, row 0: its sums are not used.
+    auto x_row = [&](int r) { return (unsigned)max(slot[r], 0) / (unsigned)l.fan; };
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         // Rows past the tile's are zeros: nothing is read for them, and their products take less power.
         const int r = 128 * half + 64 * i + row;
-        a_off[half][i] = r < t.rows ? (uint32_t)((EXPERTS ? x_row[r] : r) * a.ldx) + piece16 : 0xffffffffu;
+        a_off[half][i] = r < t.rows ? (uint32_t)((EXPERTS ? x_row(r) : r) * a.ldx) + piece16 : 0xffffffffu;
       }
     }
     const int column = GATED ? row : 64 * (row / 32) + row % 32;
@@ -97,12 +100,11 @@ struct Loader {
       b_step[unit] = (uint32_t)((GATED ? 64 : 128) * ld);
     }
     // Scales of four stages, 16 bytes a row: waves 0 to 3 x's, 4 and 5 the units' of the weights.
-    const int lane = tid % kWave;
     const int blocks_k = (a.k + kStep - 1) / kStep;
     if (wave < 4) {
       const int r = min(tid, t.rows - 1);
       s0 = EXPERTS ? a.x_scales : a.x_scales + t.first * a.ldxs;
-      s_off = (uint32_t)((EXPERTS ? x_row[r] : r) * a.ldxs * 4);
+      s_off = (uint32_t)((EXPERTS ? x_row(r) : r) * a.ldxs * 4);
       s_records = EXPERTS ? l.scale_bytes : (uint32_t)(((t.rows - 1) * a.ldxs + blocks_k) * 4);
     } else {
       const int block = n0 / kStep, unit = wave & 1;
@@ -112,7 +114,7 @@ struct Loader {
         const int at = min(block + (GATED ? 0 : unit), (a.n - 1) / kStep);
         s0 = a.w_scales + t.expert * a.stride_ws + at * a.ldws;
       }
-      s_off = lane == 0 ? 0 : kOutOfRange;
+      s_off = 0;
       s_records = (uint32_t)(blocks_k * 4);
     }
   }
@@ -128,34 +130,51 @@ struct Loader {
                       i * b_step[which] + (GATED ? 0 : which * (b_step[which] / 4)));
   }
   __device__ __forceinline__ void issue_scales(int chunk, uint32_t scales) const {
-    if (wave >= 6) return;
     const uint32_t skip = 4 * kScaleSteps * chunk;
-    gg::load_to_lds16(s0 + kScaleSteps * chunk, s_records - skip, scales + 1024u * (uint32_t)wave, s_off, 0);
+    if (wave < 4) {
+      gg::load_to_lds16(s0 + kScaleSteps * chunk, s_records - skip, scales + 1024u * (uint32_t)wave, s_off, 0);
+    } else if (wave < 6 && gg::opaque_lane() == 0) {  // the other lanes' places are not theirs
+      gg::load_to_lds16(s0 + kScaleSteps * chunk, s_records - skip, scales + 4096u + 16u * (uint32_t)(wave - 4), s_off, 0);
+    }
   }
 };
 
-// The sums of the tile at rows t (at most 128 HALVES), columns n0 on.
-template <bool EXPERTS, bool GATED, int HALVES>
-__device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
-                                              Sums<HALVES>& acc) {
-  const ggk_fp8_args& p = l.a;
-  const int nk = (p.k + kStep - 1) / kStep;
-  const Loader<EXPERTS, GATED> loader(l, t, s.x_row, n0, wave);
-  const uint32_t lds = gg::lds_address(s.stages), scales_at = lds + 2 * kParity;
-  const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
-  const int wm = wave >> 2, wn = wave & 3;
-  const uint32_t lane_at = (uint32_t)(j * 128 + ((g ^ (j >> 1)) & 7) * 16);
-  // Of the lane's fragments in unit 0 of the ring; the parity of the stage is added once a phase.
-  const uint32_t a_lo = lds + lane_at + wm * 64 * 128, a_hi = lds + (lane_at ^ 64) + wm * 64 * 128;
-  const uint32_t b_lo = lds + lane_at + wn * 32 * 128, b_hi = lds + (lane_at ^ 64) + wn * 32 * 128;
-  const uint32_t x_scale_lane = scales_at + (wm * 64 + j) * 16;
-  const uint32_t w_scale_lane = scales_at + 4096 + (GATED ? 0 : (wn >> 1) * 1024);
+// Of a lane in the operands of the instructions: LDS byte addresses of its fragments in the first unit, in the two pieces that
+// a fragment is read as, and of its scales.
+template <bool GATED>
+struct Lane {
+  uint32_t a_lo, a_hi, b_lo, b_hi, x_scale, w_scale;
+  __device__ __forceinline__ Lane(uint32_t lds, int wave) {
+    const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
+    const int wm = wave >> 2, wn = wave & 3;
+    const uint32_t at = (uint32_t)(j * 128 + ((g ^ (j >> 1)) & 7) * 16);
+    a_lo = lds + at + wm * 64 * 128;
+    a_hi = lds + (at ^ 64) + wm * 64 * 128;
+    b_lo = lds + at + wn * 32 * 128;
+    b_hi = lds + (at ^ 64) + wn * 32 * 128;
+    x_scale = lds + kPlaces * kUnit + (wm * 64 + j) * 16;
+    w_scale = lds + kPlaces * kUnit + 4096 + (GATED ? 0 : (wn >> 1) * 16);
+  }
+};
 
-  int8v a[4], b[2][2];
-  float x_scale[2][4], w_scale[2], w_next[2];  // x's by half of the rows; of the next stage while this one's are used
-  float4v part[8];      // results of this phase's instructions, three of them alive
-  float4v left[2];      // of the phase before, its last two
-  float left_scale;
+// A lane's address in a fragment's unit, held in a register (the empty asm): reads add the rest as the instructions' own
+// offsets.  With an addition for every read the vector unit was short of slots beside the matrix instructions (8192^3: 460 us
+// instead of 444).
+__device__ __forceinline__ uint32_t held(uint32_t at) {
+  asm volatile("" : "+v"(at));
+  return at;
+}
+
+__device__ __forceinline__ void add_scaled(float4v& sum, const float4v& v, float scale) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum[e] = fmaf(scale, v[e], sum[e]);
+}
+
+// Scales of stage kt lie in set (kt / 4) % 2.
+__device__ __forceinline__ uint32_t scales_of(int kt) { return ((kt >> 2) & 1) * kScales + (kt & 3) * 4; }
+
+template <int HALVES>
+__device__ __forceinline__ void clear(Sums<HALVES>& acc) {
 #pragma unroll
   for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
@@ -167,44 +186,171 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
       }
     }
   }
+}
+
+// The sums of the tile of at most 128 rows at rows t, columns n0 on.
+template <bool EXPERTS, bool GATED>
+__device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
+                                              Sums<1>& acc) {
+  const ggk_fp8_args& p = l.a;
+  const int nk = (p.k + kStep - 1) / kStep;
+  const Loader<EXPERTS, GATED> loader(l, t, s.slot, n0, wave);
+  const uint32_t lds = gg::lds_address(s.stages), scales_at = lds + kPlaces * kUnit;
+  const Lane<GATED> lane(lds, wave);
+
+  // Two sets of operands: one is multiplied while the next stage's is read into the other.
+  int8v a[2][4], b[2][4];  // [set][16 rows], [set][2 unit + 16 columns]
+  float x_scale[2][4], w_scale[2][2];
+  float4v part[16];  // results of this stage's instructions, three of them alive
+  float4v left[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};  // of the stage before, its last two
+  float left_scale = 0.0f;
+  clear<1>(acc);
+
+  uint32_t lo, hi;
+  auto read = [&](uint32_t place, int set, int f) {  // fragment f (0..7): the stage's columns, then its rows
+    if (f == 0) {
+      lo = held(lane.b_lo + place);
+      hi = held(lane.b_hi + place);
+    }
+    if (f == 4) {
+      lo = held(lane.a_lo + place);
+      hi = held(lane.a_hi + place);
+    }
+    if (f < 4) {
+      b[set][f] = read_fragment(lo, hi, (f / 2) * 2 * kUnit + (f % 2) * 2048u);
+    } else {
+      a[set][f - 4] = read_fragment(lo, hi, kUnit + (f - 4) * 2048u);
+    }
+  };
+  auto read_scales = [&](int kt, int set) {
+    const uint32_t at = scales_of(kt);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x_scale[set][i] = *(const GG_LDS float*)(uintptr_t)(lane.x_scale + at + 256u * i);
+    w_scale[set][0] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at);
+    if constexpr (GATED) w_scale[set][1] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at + 16u);
+  };
+  auto issue = [&](int kt, uint32_t place, int i) {  // load i (0..5) of a stage; past K zeros, and memory is not touched
+    if (i / 2 == 1) {
+      loader.issue_a(kt, 0, lds + place + kUnit, i % 2);
+    } else {
+      loader.issue_b(kt, i / 4, lds + place + i / 2 * kUnit, i % 2);
+    }
+  };
+
+  loader.issue_scales(0, scales_at);
+#pragma unroll
+  for (int kt = 0; kt < 3; ++kt) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) issue(kt, kt * 3 * kUnit, i);
+  }
+  gg::wait_vmcnt<12>();
+  gg::phase_barrier();
+#pragma unroll
+  for (int f = 0; f < 8; ++f) read(0, 0, f);
+  read_scales(0, 0);
+  gg::wait_vmcnt<6>();
+  gg::wait_lgkmcnt<0>();
+  gg::phase_barrier();
+
+  // Stage kt, whose operands are in set `set` and whose three places, at `here`, are free.
+  uint32_t here = 0;
+  auto stage = [&](int kt, auto set_tag) {
+    constexpr int set = decltype(set_tag)::value, other = 1 - set;
+    const uint32_t next = here == 6 * kUnit ? 0 : here + 3 * kUnit;
+    if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
+    float scale[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      scale[0][i] = x_scale[set][i] * w_scale[set][0];
+      scale[1][i] = GATED ? x_scale[set][i] * w_scale[set][1] : scale[0][i];
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int i = r / 4, n = (i & 1) != 0 ? 3 - r % 4 : r % 4;
+      part[r] = multiply(b[set][n], a[set][i]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (r < 2) {
+        add_scaled(acc[0][3][0][1 - r], left[r], left_scale);
+      } else {
+        const int q = r - 2, qi = q / 4, qn = (qi & 1) != 0 ? 3 - q % 4 : q % 4;
+        add_scaled(acc[0][qi][qn / 2][qn % 2], part[q], scale[qn / 2][qi]);
+      }
+      if (r < 12 && r % 3 != 2) read(next, other, r / 3 * 2 + r % 3);
+      if (r == 12) read_scales(kt + 1, other);
+      if (r % 3 == 2) issue(kt + 3, here, r / 3);
+      if (r == 15) issue(kt + 3, here, 5);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    left[0] = part[14];
+    left[1] = part[15];
+    left_scale = scale[0][3];
+    // The next stage's operands are in every wave's registers, and the one after it has landed.
+    gg::wait_lgkmcnt<0>();
+    gg::wait_vmcnt<6>();
+    gg::phase_barrier();
+    here = next;
+  };
+  int kt = 0;
+#pragma unroll 1
+  for (; kt + 1 < nk; kt += 2) {
+    stage(kt, std::integral_constant<int, 0>{});
+    stage(kt + 1, std::integral_constant<int, 1>{});
+  }
+  if (kt < nk) stage(kt, std::integral_constant<int, 0>{});
+  add_scaled(acc[0][3][0][1], left[0], left_scale);
+  add_scaled(acc[0][3][0][0], left[1], left_scale);
+  gg::wait_vmcnt<0>();
+}
+
+// The sums of the tile of more rows at rows t, columns n0 on.
+template <bool EXPERTS, bool GATED>
+__device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
+                                              Sums<2>& acc) {
+  const ggk_fp8_args& p = l.a;
+  const int nk = (p.k + kStep - 1) / kStep;
+  const Loader<EXPERTS, GATED> loader(l, t, s.slot, n0, wave);
+  const uint32_t lds = gg::lds_address(s.stages), scales_at = lds + kPlaces * kUnit;
+  const Lane<GATED> lane(lds, wave);
+
+  int8v a[4], b[2][2];
+  float x_scale[2][4], w_scale[2], w_next[2];  // x's by half of the rows; of the next stage while this one's are used
+  float4v part[8];      // results of this phase's instructions, three of them alive
+  float4v left[2];      // of the phase before, its last two
+  float left_scale;
+  clear<2>(acc);
   left[0] = left[1] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
   left_scale = 0.0f;
 
-  // Reads of a phase begin with `from`: two additions, held in registers (the empty asm), and the rest are the instructions'
-  // own offsets; with an addition for every read the vector unit was short of slots beside the matrix instructions.
   uint32_t lo, hi;
-  auto from = [&](uint32_t lane_lo, uint32_t lane_hi, uint32_t base) {
-    lo = lane_lo + base;
-    hi = lane_hi + base;
-    asm volatile("" : "+v"(lo), "+v"(hi));
-  };
-  auto read_a = [&](uint32_t base, uint32_t unit, int i) {
-    if (i == 0) from(a_lo, a_hi, base);
+  auto read_a = [&](uint32_t parity, uint32_t unit, int i) {
+    if (i == 0) {
+      lo = held(lane.a_lo + parity);
+      hi = held(lane.a_hi + parity);
+    }
     a[i] = read_fragment(lo, hi, unit + 2048u * i);
   };
-  auto read_b = [&](uint32_t base, uint32_t unit, int which, int n, bool begin) {
-    if (begin) from(b_lo, b_hi, base);
+  auto read_b = [&](uint32_t parity, uint32_t unit, int which, int n, bool begin) {
+    if (begin) {
+      lo = held(lane.b_lo + parity);
+      hi = held(lane.b_hi + parity);
+    }
     b[which][n] = read_fragment(lo, hi, unit + 2048u * n);
   };
   // Scales of stage kt: rows of A half `half` (into set `set`), and the units' weights.  Read two phases ahead, so that their
   // wait is none for the fragments read since.
   auto read_x_scales = [&](int kt, int half, int set) {
-    const uint32_t at = x_scale_lane + ((kt >> 2) & 1) * kScales + (kt & 3) * 4 + half * 2048;
+    const uint32_t at = lane.x_scale + scales_of(kt) + half * 2048;
 #pragma unroll
     for (int i = 0; i < 4; ++i) x_scale[set][i] = *(const GG_LDS float*)(uintptr_t)(at + 256u * i);
   };
   auto read_w_scales = [&](int kt) {
-    const uint32_t at = w_scale_lane + ((kt >> 2) & 1) * kScales + (kt & 3) * 4;
+    const uint32_t at = lane.w_scale + scales_of(kt);
     w_next[0] = *(const GG_LDS float*)(uintptr_t)at;
-    if constexpr (GATED) w_next[1] = *(const GG_LDS float*)(uintptr_t)(at + 1024u);
+    if constexpr (GATED) w_next[1] = *(const GG_LDS float*)(uintptr_t)(at + 16u);
   };
   auto next_w_scales = [&]() {
     w_scale[0] = w_next[0];
     if constexpr (GATED) w_scale[1] = w_next[1];
-  };
-  auto add = [&](float4v& sum, const float4v& v, float scale) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] = fmaf(scale, v[e], sum[e]);
   };
   // The 8 instructions of (A half, B unit), rows first, columns back and forth; the sums of the two before last are brought
   // in behind each.  last_half, last_unit: of the phase before.
@@ -218,10 +364,10 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
       part[r] = multiply(b[unit][n], a[i]);
       __builtin_amdgcn_sched_barrier(0);
       if (r < 2) {
-        add(acc[last_half][3][last_unit][1 - r], left[r], left_scale);
+        add_scaled(acc[last_half][3][last_unit][1 - r], left[r], left_scale);
       } else {
         const int q = r - 2, qi = q >> 1, qn = (qi & 1) != 0 ? 1 - (q & 1) : q & 1;
-        add(acc[half][qi][unit][qn], part[q], scale[qi]);
+        add_scaled(acc[half][qi][unit][qn], part[q], scale[qi]);
       }
       read(r);
       issue(r);
@@ -233,141 +379,84 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   };
 
   loader.issue_scales(0, scales_at);
-  if constexpr (HALVES == 1) {
-    // Unit u (stage u / 3; B0, A0, B1) lies in place u % 8.  Phase 0 of stage t issues the loads of unit 3 t + 7, phase 1
-    // those of 3 t + 8 and 3 t + 9: the units eight before them have been read and used, and a barrier stands between.
-    // Loads of stages past K read zeros without touching memory.
-    auto place_of = [&](int u) { return (uint32_t)(u % kPlaces) * kUnit; };
-    auto issue_unit = [&](int u, int kt, int which, int i) {
-      if (which == 1) {
-        loader.issue_a(kt, 0, lds + place_of(u), i);
-      } else {
-        loader.issue_b(kt, which / 2, lds + place_of(u), i);
-      }
-    };
 #pragma unroll
-    for (int u = 0; u < 7; ++u) {
-      issue_unit(u, u / 3, u % 3, 0);
-      issue_unit(u, u / 3, u % 3, 1);
+  for (int kt = 0; kt < 2; ++kt) {
+    const uint32_t st = lds + kt * kParity;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) loader.issue_b(kt, 0, st + kB0, i);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) loader.issue_a(kt, 0, st + kA0, i);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) loader.issue_b(kt, 1, st + kB1, i);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) loader.issue_a(kt, 1, st + kA1, i);
+  }
+  gg::wait_vmcnt<6 * kLoads>();
+  gg::phase_barrier();
+#pragma unroll
+  for (int n = 0; n < 2; ++n) read_b(0, kB0, 0, n, n == 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read_a(0, kA0, i);
+  read_x_scales(0, 0, 0);
+  read_w_scales(0);
+  next_w_scales();
+  gg::wait_vmcnt<5 * kLoads>();
+  gg::wait_lgkmcnt<0>();
+  gg::phase_barrier();
+
+  // One stage.  ISSUE: the loads of stage kt + 2 are issued; else everything has been and the waits count down.  LAST:
+  // nothing more is read.
+  auto stage = [&](int kt, auto issue_tag, auto last_tag) {
+    constexpr bool ISSUE = decltype(issue_tag)::value, LAST = decltype(last_tag)::value;
+    constexpr int N = kLoads;
+    const uint32_t here = (uint32_t)(kt & 1) * kParity, next = kParity - here;
+    const uint32_t st = lds + here;
+    // Scales of the next four stages, behind the last use of the set before theirs.
+    if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
+    phase(0, 0, 1, 1, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_b(kt + 2, 0, st + kB0, r / 2 - 2); },
+          [&](int r) {
+            if (r == 1 || r == 3) read_b(here, kB1, 1, r / 2, r == 1);
+            if (r == 5) read_x_scales(kt, 1, 1);
+          });
+    gg::wait_vmcnt<ISSUE ? 5 * N : LAST ? 0 : 4 * N>();
+    gg::phase_barrier();
+    phase(0, 1, 0, 0, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_a(kt + 2, 0, st + kA0, r / 2 - 2); },
+          [&](int r) { if (r & 1) read_a(here, kA1, r / 2); });
+    if constexpr (!LAST) {
+      gg::wait_vmcnt<ISSUE ? 5 * N : 3 * N>();
+      gg::phase_barrier();
     }
-    gg::wait_vmcnt<5 * kLoads>();
-    gg::phase_barrier();
-#pragma unroll
-    for (int n = 0; n < 2; ++n) read_b(0, 0, 0, n, n == 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) read_a(0, kUnit, i);
-    read_x_scales(0, 0, 0);
-    read_w_scales(0);
-    next_w_scales();
-    gg::wait_vmcnt<4 * kLoads>();
-    gg::phase_barrier();
-#pragma unroll 1
-    for (int kt = 0; kt < nk; ++kt) {
-      const int u = 3 * kt;
-      if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
-      const uint32_t b1 = place_of(u + 2), b0 = place_of(u + 3), a0 = place_of(u + 4);
-      phase(0, 0, 0, 1, [&](int r) { if (r == 4 || r == 6) issue_unit(u + 7, kt + 2, 1, r / 2 - 2); },
-            [&](int r) {
-              if (r == 1 || r == 3) read_b(b1, 0, 1, r / 2, r == 1);
-              if (r == 5) {
-                read_x_scales(kt + 1, 0, 1);
+    phase(1, 0, 0, 1, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_b(kt + 2, 1, st + kB1, r / 2 - 2); },
+          [&](int r) {
+            if constexpr (!LAST) {
+              if (r == 1) {
+                read_x_scales(kt + 1, 0, 0);
                 read_w_scales(kt + 1);
               }
-            });
-      gg::wait_vmcnt<3 * kLoads>();
+              if (r >= 6) read_b(next, kB0, 0, 7 - r, r == 6);
+            }
+          });
+    if constexpr (!LAST) {
+      gg::wait_vmcnt<ISSUE ? 5 * N : 2 * N>();
       gg::phase_barrier();
-      phase(0, 1, 0, 0, [&](int r) { if (r >= 4) issue_unit(u + 8 + (r - 4) / 2, kt + 2 + (r - 4) / 2, r < 6 ? 2 : 0, r & 1); },
-            [&](int r) { if (r == 0) { read_b(b0, 0, 0, 0, true); read_b(b0, 0, 0, 1, false); } if (r & 1) read_a(a0, 0, r / 2); });
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x_scale[0][i] = x_scale[1][i];
+    }
+    phase(1, 1, 1, 0, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_a(kt + 2, 1, st + kA1, r / 2 - 2); },
+          [&](int r) { if constexpr (!LAST) { if (r & 1) read_a(next, kA0, r / 2); } });
+    if constexpr (!LAST) {
+      gg::wait_lgkmcnt<8>();  // phase 2's reads, which nothing has used yet; this phase's eight may be on their way
       next_w_scales();
-      gg::wait_vmcnt<4 * kLoads>();
+      gg::wait_vmcnt<ISSUE ? 5 * N : N>();
       gg::phase_barrier();
     }
-    add(acc[0][3][1][1], left[0], left_scale);
-    add(acc[0][3][1][0], left[1], left_scale);
-    gg::wait_vmcnt<0>();
-    return;
-  } else {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const uint32_t st = lds + kt * kParity;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) loader.issue_b(kt, 0, st + kB0, i);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) loader.issue_a(kt, 0, st + kA0, i);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) loader.issue_b(kt, 1, st + kB1, i);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) loader.issue_a(kt, 1, st + kA1, i);
-    }
-    gg::wait_vmcnt<6 * kLoads>();
-    gg::phase_barrier();
-#pragma unroll
-    for (int n = 0; n < 2; ++n) read_b(0, kB0, 0, n, n == 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) read_a(0, kA0, i);
-    read_x_scales(0, 0, 0);
-    read_w_scales(0);
-    next_w_scales();
-    gg::wait_vmcnt<5 * kLoads>();
-    gg::wait_lgkmcnt<0>();
-    gg::phase_barrier();
-
-    // One stage.  ISSUE: the loads of stage kt + 2 are issued; else everything has been and the waits count down.  LAST:
-    // nothing more is read.
-    auto stage = [&](int kt, auto issue_tag, auto last_tag) {
-      constexpr bool ISSUE = decltype(issue_tag)::value, LAST = decltype(last_tag)::value;
-      constexpr int N = kLoads;
-      const uint32_t here = (uint32_t)(kt & 1) * kParity, next = kParity - here;
-      const uint32_t st = lds + here;
-      // Scales of the next four stages, behind the last use of the set before theirs.
-      if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
-      phase(0, 0, 1, 1, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_b(kt + 2, 0, st + kB0, r / 2 - 2); },
-            [&](int r) {
-              if (r == 1 || r == 3) read_b(here, kB1, 1, r / 2, r == 1);
-              if (r == 5) read_x_scales(kt, 1, 1);
-            });
-      gg::wait_vmcnt<ISSUE ? 5 * N : LAST ? 0 : 4 * N>();
-      gg::phase_barrier();
-      phase(0, 1, 0, 0, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_a(kt + 2, 0, st + kA0, r / 2 - 2); },
-            [&](int r) { if (r & 1) read_a(here, kA1, r / 2); });
-      if constexpr (!LAST) {
-        gg::wait_vmcnt<ISSUE ? 5 * N : 3 * N>();
-        gg::phase_barrier();
-      }
-      phase(1, 0, 0, 1, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_b(kt + 2, 1, st + kB1, r / 2 - 2); },
-            [&](int r) {
-              if constexpr (!LAST) {
-                if (r == 1) {
-                  read_x_scales(kt + 1, 0, 0);
-                  read_w_scales(kt + 1);
-                }
-                if (r >= 6) read_b(next, kB0, 0, 7 - r, r == 6);
-              }
-            });
-      if constexpr (!LAST) {
-        gg::wait_vmcnt<ISSUE ? 5 * N : 2 * N>();
-        gg::phase_barrier();
-      }
-      phase(1, 1, 1, 0, [&](int r) { if (ISSUE && (r == 4 || r == 6)) loader.issue_a(kt + 2, 1, st + kA1, r / 2 - 2); },
-            [&](int r) { if constexpr (!LAST) { if (r & 1) read_a(next, kA0, r / 2); } });
-      if constexpr (!LAST) {
-        gg::wait_lgkmcnt<8>();  // phase 2's reads, which nothing has used yet; this phase's eight may be on their way
-        next_w_scales();
-        gg::wait_vmcnt<ISSUE ? 5 * N : N>();
-        gg::phase_barrier();
-      }
-    };
-    int kt = 0;
+  };
+  int kt = 0;
 #pragma unroll 1
-    for (; kt < nk - 2; ++kt) stage(kt, std::true_type{}, std::false_type{});
-    if (nk >= 2) stage(kt++, std::false_type{}, std::false_type{});
-    stage(kt, std::false_type{}, std::true_type{});  // a single stage also waits for the (empty) loads past K
-    add(acc[1][3][1][1], left[0], left_scale);
-    add(acc[1][3][1][0], left[1], left_scale);
-    gg::wait_vmcnt<0>();
-  }
+  for (; kt < nk - 2; ++kt) stage(kt, std::true_type{}, std::false_type{});
+  if (nk >= 2) stage(kt++, std::false_type{}, std::false_type{});
+  stage(kt, std::false_type{}, std::true_type{});  // a single stage also waits for the (empty) loads past K
+  add_scaled(acc[1][3][1][1], left[0], left_scale);
+  add_scaled(acc[1][3][1][0], left[1], left_scale);
+  gg::wait_vmcnt<0>();
 }
 
 // y of a tile, in a 16-bit type: four columns a lane and store; rows that do not start on multiples of four values by way
@@ -487,7 +576,7 @@ __device__ __forceinline__ void run_tile(const Launch& l, const RowTile& t, cons
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave >> 2, wn = wave & 3;
   Sums<HALVES> acc;
-  multiply_tile<EXPERTS, GATED, HALVES>(l, t, s, n0, wave, acc);
+  multiply_tile<EXPERTS, GATED>(l, t, s, n0, wave, acc);
   if constexpr (!GATED) {
     if (a.y_type == GGK_TYPE_BF16) {
       store_tile<EXPERTS, __bf16, HALVES>(a, t, s, n0, wm, wn, acc);
@@ -609,9 +698,9 @@ __device__ __forceinline__ long long item_at(const Launch& l, const Table& s, lo
 template <bool EXPERTS, bool GATED>
 __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
   const ggk_fp8_args& a = l.a;
-  __shared__ alignas(128) unsigned char s_stages[2 * kParity + 2 * kScales];
-  __shared__ int s_slot[EXPERTS ? kRows : 1], s_x_row[EXPERTS ? kRows : 1];
-  const Shared s{s_stages, s_slot, s_x_row};
+  __shared__ alignas(128) unsigned char s_stages[kPlaces * kUnit + 2 * kScales];
+  __shared__ int s_slot[EXPERTS ? kRows : 1];
+  const Shared s{s_stages, s_slot};
   // Neighbouring workgroups go to different XCDs, each with an L2 of its own: an XCD takes a run of the order, an eighth of
   // the items or of what they cost.
   const int xcd = blockIdx.x % kXcds, in_xcd = blockIdx.x / kXcds;
@@ -627,22 +716,19 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
       gg::stage_barrier();
     }
   } else {
-    __shared__ Tiles<GGK_MOE_MAX_EXPERTS> s_tiles;
+    __shared__ Tiles<kMost> s_tiles;
     list_tiles(l, s_tiles);
     const long long cost = (long long)s_tiles.cost[a.experts] * l.blocks, items = (long long)s_tiles.tile[a.experts] * l.blocks;
     const long long end = xcd + 1 < kXcds && cost > 0 ? item_at(l, s_tiles, cost * (xcd + 1) / kXcds) : items;
     const long long begin = xcd > 0 && cost > 0 ? item_at(l, s_tiles, cost * xcd / kXcds) : 0;
-    const int fan = a.rows / a.x_rows;
     for (long long item = begin + in_xcd; item < end; item += kCus / kXcds) {
       const int e = find_expert(a, s_tiles.tile, l.blocks, item), rows = s_tiles.first[e + 1] - s_tiles.first[e];
       int tile, block;
       place(item - (long long)s_tiles.tile[e] * l.blocks, tiles_of(l, rows), l.blocks, &tile, &block);
       const RowTile t{e, s_tiles.first[e] + tile * l.height, min(l.height, rows - tile * l.height)};
       for (int r = threadIdx.x; r < t.rows; r += kThreads) {
-        int slot = a.order[t.first + r];
-        if (slot >= a.rows) slot = -1;
-        s_slot[r] = slot;
-        s_x_row[r] = max(slot, 0) / fan;  // where a slot names no row, row 0: its sums are not used
+        const int slot = a.order[t.first + r];
+        s_slot[r] = slot < a.rows ? slot : -1;
       }
       gg::stage_barrier();
       run_either<true, GATED>(l, t, s, block * kColumns<GATED>);
@@ -655,7 +741,7 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
 
 template <bool EXPERTS, bool GATED>
 hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
-  Launch l{a, (a.n + kColumns<GATED> - 1) / kColumns<GATED>, kRows, 0};
+  Launch l{a, (a.n + kColumns<GATED> - 1) / kColumns<GATED>, kRows, a.rows / a.x_rows, 0};
   // What the busiest CU gets: tiles of 256 rows, or of 128 at 0.6 of their time; of an expert's rows half a tile more.
   auto rounds = [&](long long height) {
     const long long tiles = EXPERTS ? a.rows / height + a.experts / 2 : (a.rows + height - 1) / height;
@@ -676,7 +762,7 @@ namespace fp8 {
 bool tiles_take(const ggk_fp8_args& a) {
   // Offsets from the tile's first row (experts: from x) are 32 bits.
   const long long rows = a.experts > 0 ? a.x_rows : kRows;
-  return rows * a.ldx < 0xfffffff0ll - kStep && rows * a.ldxs * 4 < 0x7fffffffll;
+  return a.experts <= kMost && rows * a.ldx < 0xfffffff0ll - kStep && rows * a.ldxs * 4 < 0x7fffffffll;
 }
 
 hipError_t multiply_tiles(const ggk_fp8_args& a, hipStream_t stream) {
