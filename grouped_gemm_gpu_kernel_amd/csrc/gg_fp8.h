@@ -143,8 +143,17 @@ __device__ __forceinline__ void store_numbers(const ggk_fp8_args& a, long long r
   if (j % kFp8Block == 0) a.y_scales[row * a.ldys + j / kFp8Block] = scale;
 }
 
-// The kernel for many rows (gg_fp8_tiles.hip): does it take a call's strides, and the call (16-bit or 8-bit y).
+// Row tiles of a call, about: the counts of experts are on the device, and each one's rows end somewhere in a tile.
+inline double row_tiles(const ggk_fp8_args& a, int height) {
+  if (a.experts == 0) return (a.rows + height - 1) / height;
+  const double with_rows = a.rows < a.experts ? a.rows : a.experts, tiles = a.rows / (double)height + 0.6 * with_rows;
+  return tiles > with_rows ? tiles : with_rows;
+}
+
+// The kernel for many rows (gg_fp8_tiles.hip): does it take a call's strides, how long it takes in us, and the call (16-bit
+// or 8-bit y).
 bool tiles_take(const ggk_fp8_args& a);
+double estimate_tiles(const ggk_fp8_args& a);
 hipError_t multiply_tiles(const ggk_fp8_args& a, hipStream_t stream);
 
 }  // namespace fp8

@@ -8,7 +8,8 @@
 // wave waits for another until its sums are whole.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
-#include <stdlib.h>
+
+#include <cmath>
 
 #include "gg_experts.h"
 #include "gg_fp8.h"
@@ -294,22 +295,20 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-#ifdef GG_FORMS
-template <bool EXPERTS>
-hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
-  const char* f = getenv("GG_F");
-  const int i = f ? atoi(f) : 0;
-  switch (i) {
-    GG_FORMS
-  }
-  return hipErrorInvalidValue;
+// What a call takes in the form for more than 16 rows, in us: what the busiest CU gets, workgroups of 32 rows by 32 columns,
+// two on a CU, or by 128, one.
+double estimate_few(const ggk_fp8_args& a) {
+  const double tiles = row_tiles(a, 32), steps = a.k / 128.0;
+  if (a.gate != GGK_GATE_NONE) return 5 + ceil(tiles * ceil(a.n / 128.0) / kCus) * (1 + 0.85 * steps);
+  if (a.experts > 0) return 5 + ceil(tiles * ceil(a.n / 128.0) / kCus) * 0.6 * steps;
+  return 4 + ceil(tiles * ceil(a.n / 32.0) / (2 * kCus)) * (1.3 + 0.15 * steps);
 }
-#else
+
 template <bool EXPERTS>
 hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
   const bool exact = a.y_type == GGK_TYPE_F32;
   if constexpr (EXPERTS) {
-    if (a.gate != GGK_GATE_NONE) return launch<Form<32, 2, 8, 1, 2, true, false>, true>(a, stream);
+    if (a.gate != GGK_GATE_NONE) return launch<Form<32, 2, 8, 1, 2, true, true>, true>(a, stream);
     if (a.rows <= 32) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream);
     if (a.rows <= 12ll * a.experts) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream);
     if (exact) return launch<Form<32, 2, 4, 2, 2, false, true>, true>(a, stream);
@@ -317,19 +316,23 @@ hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
   } else if (a.gate != GGK_GATE_NONE) {
     if (a.rows <= 8) return launch<Form<8, 4, 4, 1, 4, true, true>, false>(a, stream);
     if (a.rows <= 16) return launch<Form<16, 2, 8, 1, 3, true, true>, false>(a, stream);
-    return launch<Form<32, 2, 8, 1, 2, true, false>, false>(a, stream);
+    return launch<Form<32, 2, 8, 1, 2, true, true>, false>(a, stream);
   } else {
     if (a.rows <= 8) return launch<Form<8, 1, 1, 8, 2, false, true>, false>(a, stream);
     if (a.rows <= 16) {
       return a.n >= 8192 ? launch<Form<16, 1, 2, 4, 2, false, true>, false>(a, stream)
                          : launch<Form<16, 1, 1, 8, 2, false, true>, false>(a, stream);
     }
+    // 64 rows at once where enough columns remain for it: us, 61 rows of 4096 by 14335 20.3, 18.4, 64 of 8192 by 8192 18.9, 27.
+    if (a.rows > 32 && a.rows <= 64 && a.n >= 3 * 64 * kCus / 4) {
+      return exact ? launch<Form<64, 4, 1, 4, 2, false, true>, false>(a, stream)
+                   : launch<Form<64, 4, 1, 4, 2, false, false>, false>(a, stream);
+    }
     if (exact) return launch<Form<32, 2, 1, 4, 2, false, true>, false>(a, stream);
     return launch<Form<32, 2, 1, 4, 2, false, false>, false>(a, stream);
   }
 }
 
-#endif
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
@@ -376,8 +379,11 @@ extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t str
   const hipError_t st = ggk_fp8_check(args);
   if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
   const ggk_fp8_args& a = *args;
-  const long long rows = a.experts > 0 ? a.rows / a.experts : a.rows;
-  const char* env = getenv("GG_MIN");
-  if (rows > (env ? atoi(env) : 100) && (a.gate != GGK_GATE_NONE || a.y_type != GGK_TYPE_F32) && tiles_take(a)) return multiply_tiles(a, stream);
+  // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 512 rows of 2048 by 2048 10, 20,
+  // 2048 rows 35, 21; 128 of 8192 by 8192 29, 52, 512 103, 56; 16 experts of 1024 by 2048, 512 slots 15, 19, 2048 slots 29,
+  // 21, gated 22, 37 and 46, 36; 64 experts of 4096 by 14336, 256 slots 480, 474, 2048 slots 972, 751.
+  if (tiles_take(a) && estimate_tiles(a) < estimate_few(a)) {
+    return multiply_tiles(a, stream);
+  }
   return args->experts > 0 ? multiply_few<true>(*args, stream) : multiply_few<false>(*args, stream);
 }

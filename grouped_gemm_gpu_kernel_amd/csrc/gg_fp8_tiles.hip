@@ -15,8 +15,8 @@
 // its end for this wave's loads of unit f + 3 and its reads of the phases before; one barrier tells every wave both.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
-#include <stdlib.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "gg_experts.h"
@@ -302,6 +302,110 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   gg::wait_vmcnt<0>();
 }
 
+// The same in binary16, which holds the numbers exactly, for float32 and 8-bit y (a row's scale is as exact as its largest
+// value).  A fragment is turned into binary16 once a stage, which takes the vector unit about as long as the matrix unit
+// needs for the products; each frees its registers for the next stage's.
+template <bool EXPERTS, bool GATED>
+__device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
+                                                    Sums<1>& acc) {
+  const ggk_fp8_args& p = l.a;
+  const int nk = (p.k + kStep - 1) / kStep;
+  const Loader<EXPERTS, GATED> loader(l, t, s.slot, n0, wave);
+  const uint32_t lds = gg::lds_address(s.stages), scales_at = lds + kPlaces * kUnit;
+  const Lane<GATED> lane(lds, wave);
+  int8v a[4], b[4];
+  float x_scale[4], w_scale[2], x_next[4], w_next[2];
+  clear<1>(acc);
+  // Of the wave's four times 16 rows, those that the tile has: the matrix unit bounds this loop.
+  const int live = min(max(t.rows - 64 * (wave >> 2) + 15, 0) / 16, 4);
+
+  auto read_a = [&](uint32_t place, int i) { a[i] = read_fragment(lane.a_lo + place, lane.a_hi + place, kUnit + i * 2048u); };
+  auto read_b = [&](uint32_t place, int f) {
+    b[f] = read_fragment(lane.b_lo + place, lane.b_hi + place, (f / 2) * 2 * kUnit + (f % 2) * 2048u);
+  };
+  auto read_scales = [&](int kt) {
+    const uint32_t at = scales_of(kt);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x_next[i] = *(const GG_LDS float*)(uintptr_t)(lane.x_scale + at + 256u * i);
+    w_next[0] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at);
+    if constexpr (GATED) w_next[1] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at + 16u);
+  };
+  auto issue = [&](int kt, uint32_t place, int i) {  // load i (0..5) of a stage; past K zeros, and memory is not touched
+    if (i / 2 == 1) {
+      loader.issue_a(kt, 0, lds + place + kUnit, i % 2);
+    } else {
+      loader.issue_b(kt, i / 4, lds + place + i / 2 * kUnit, i % 2);
+    }
+  };
+
+  loader.issue_scales(0, scales_at);
+#pragma unroll
+  for (int kt = 0; kt < 3; ++kt) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) issue(kt, kt * 3 * kUnit, i);
+  }
+  gg::wait_vmcnt<12>();
+  gg::phase_barrier();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read_b(0, i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read_a(0, i);
+  read_scales(0);
+  gg::wait_vmcnt<6>();
+  gg::wait_lgkmcnt<0>();
+  gg::phase_barrier();
+
+  // Stage kt, whose operands are in registers and whose three places, at `here`, are free.
+  uint32_t here = 0;
+#pragma unroll 1
+  for (int kt = 0; kt < nk; ++kt) {
+    const uint32_t next = here == 6 * kUnit ? 0 : here + 3 * kUnit;
+    if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x_scale[i] = x_next[i];
+    w_scale[0] = w_next[0];
+    if constexpr (GATED) w_scale[1] = w_next[1];
+    Halves w[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      w[n] = to_halves(b[n]);
+      read_b(next, n);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // The loads of stage kt + 3.
+      if (i < 2) issue(kt + 3, here, i);
+      if (i >= 2) issue(kt + 3, here, 2 * i - 2);
+      if (i >= 2) issue(kt + 3, here, 2 * i - 1);
+      if (i < live) {
+        const Halves x = to_halves(a[i]);
+        read_a(next, i);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // two chains of products at a time
+          float4v part[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              part[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[2 * u + n].v[q], x.v[q], part[n], 0, 0, 0);
+            }
+          }
+          const float scale = x_scale[i] * w_scale[GATED ? u : 0];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) add_scaled(acc[0][i][u][n], part[n], scale);
+        }
+      }
+    }
+    read_scales(kt + 1);
+    // The next stage's operands are in every wave's registers, and the one after it has landed.
+    gg::wait_lgkmcnt<0>();
+    gg::wait_vmcnt<6>();
+    gg::phase_barrier();
+    here = next;
+  }
+  gg::wait_vmcnt<0>();
+}
+
 // The sums of the tile of more rows at rows t, columns n0 on.
 template <bool EXPERTS, bool GATED>
 __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
@@ -459,14 +563,16 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   gg::wait_vmcnt<0>();
 }
 
-// y of a tile, in a 16-bit type: four columns a lane and store; rows that do not start on multiples of four values by way
-// of LDS, value by value.
+// y of a tile: four columns a lane and store; rows that do not start on multiples of four values by way of LDS, value by
+// value.
 template <bool EXPERTS, class T, int HALVES>
 __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile& t, const Shared& s, int n0, int wm, int wn,
                                            const Sums<HALVES>& acc) {
-  constexpr int kLd = 2 * 256 + 16;  // bytes of a row in LDS
+  typedef T Four __attribute__((ext_vector_type(4)));
+  constexpr int kLd = sizeof(T) * 256 + 16;  // bytes of a row in LDS
+  static_assert(128 * HALVES * kLd <= kPlaces * kUnit, "the tile fits LDS");
   const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
-  const bool vec = a.n % 4 == 0 && a.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % 8 == 0;
+  const bool vec = a.n % 4 == 0 && a.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % sizeof(Four) == 0;
   if (!vec) gg::stage_barrier();
 #pragma unroll
   for (int half = 0; half < HALVES; ++half) {
@@ -481,14 +587,13 @@ __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile&
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int column = 64 * wn + 32 * u + 16 * n + 4 * g;
-          uint16_t h[4];
+          Four four;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) h[e] = __builtin_bit_cast(uint16_t, (T)(acc[half][i][u][n][e] * weight));
-          const uint2v four = {h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
+          for (int e = 0; e < 4; ++e) four[e] = (T)(acc[half][i][u][n][e] * weight);
           if (!vec) {
-            *reinterpret_cast<uint2v*>(s.stages + r * kLd + 2 * column) = four;
+            *reinterpret_cast<Four*>(s.stages + r * kLd + sizeof(T) * column) = four;
           } else if (slot >= 0 && n0 + column < a.n) {
-            *reinterpret_cast<uint2v*>(y + column) = four;
+            *reinterpret_cast<Four*>(y + column) = four;
           }
         }
       }
@@ -499,7 +604,7 @@ __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile&
     for (int i = threadIdx.x; i < t.rows * 256; i += kThreads) {
       const int r = i / 256, c = i % 256, slot = EXPERTS ? s.slot[r] : t.first + r;
       if (slot >= 0 && n0 + c < a.n) {
-        static_cast<uint16_t*>(a.y)[slot * a.ldy + n0 + c] = *reinterpret_cast<const uint16_t*>(s.stages + r * kLd + 2 * c);
+        static_cast<T*>(a.y)[slot * a.ldy + n0 + c] = *reinterpret_cast<const T*>(s.stages + r * kLd + sizeof(T) * c);
       }
     }
   }
@@ -510,97 +615,104 @@ template <bool EXPERTS, bool GELU, int HALVES>
 __device__ __forceinline__ void store_rows(const ggk_fp8_args& a, const RowTile& t, const Shared& s, int n0, int wm, int wn,
                                            Sums<HALVES>& acc) {
   const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
-      // Values stay in the registers of gate's sums; a row's 128 columns lie in 4 lanes of 4 waves.
-      constexpr int kLd = 128 + 16;
-      uint32_t* s_most = reinterpret_cast<uint32_t*>(s.stages + kRows * kLd);  // [256][4]
-      gg::stage_barrier();
-  #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-  #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t most = 0;
-  #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-  #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v = gated<GELU>(acc[half][i][0][n][e], acc[half][i][1][n][e]);
-              if (n0 + 32 * wn + 16 * n + 4 * g + e >= a.n) v = 0.0f;
-              acc[half][i][0][n][e] = v;
-              most = max(most, gg::magnitude_bits(v));
-            }
-          }
-          most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
-          most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
-          if (g == 0) s_most[(128 * half + 64 * wm + 16 * i + j) * 4 + wn] = most;
+  // Values stay in the registers of gate's sums; a row's 128 columns lie in 4 lanes of 4 waves.
+  constexpr int kLd = 128 + 16;
+  uint32_t* s_most = reinterpret_cast<uint32_t*>(s.stages + kRows * kLd);  // [256][4]
+  gg::stage_barrier();
+#pragma unroll
+  for (int half = 0; half < HALVES; ++half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = gated<GELU>(acc[half][i][0][n][e], acc[half][i][1][n][e]);
+          if (n0 + 32 * wn + 16 * n + 4 * g + e >= a.n) v = 0.0f;
+          acc[half][i][0][n][e] = v;
+          most = max(most, gg::magnitude_bits(v));
         }
       }
-      gg::stage_barrier();
-  #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-  #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 128 * half + 64 * wm + 16 * i + j;
-          const uint4v most = *reinterpret_cast<const uint4v*>(&s_most[r * 4]);
-          const float scale = gg::fp8_scale(max(max(most.x, most.y), max(most.z, most.w)));
-          const gg::Fp8Divisor by(scale);
-  #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const float4v v = acc[half][i][0][n];
-            *reinterpret_cast<uint32_t*>(s.stages + r * kLd + 32 * wn + 16 * n + 4 * g) =
-                gg::fp8_numbers(v[0], v[1], v[2], v[3], by);
-          }
-          if (wn == 0 && g == 0 && r < t.rows) {
-            const int slot = EXPERTS ? s.slot[r] : t.first + r;
-            if (slot >= 0) a.y_scales[slot * a.ldys + n0 / kStep] = scale;
-          }
-        }
+      most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
+      most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+      if (g == 0) s_most[(128 * half + 64 * wm + 16 * i + j) * 4 + wn] = most;
+    }
+  }
+  gg::stage_barrier();
+#pragma unroll
+  for (int half = 0; half < HALVES; ++half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 128 * half + 64 * wm + 16 * i + j;
+      const uint4v most = *reinterpret_cast<const uint4v*>(&s_most[r * 4]);
+      const float scale = gg::fp8_scale(max(max(most.x, most.y), max(most.z, most.w)));
+      const gg::Fp8Divisor by(scale);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float4v v = acc[half][i][0][n];
+        *reinterpret_cast<uint32_t*>(s.stages + r * kLd + 32 * wn + 16 * n + 4 * g) =
+            gg::fp8_numbers(v[0], v[1], v[2], v[3], by);
       }
-      gg::stage_barrier();
-      const int tid = threadIdx.x;
-      for (int i = tid; i < t.rows * 8; i += kThreads) {
-        const int r = i / 8, column = n0 + i % 8 * 16, slot = EXPERTS ? s.slot[r] : t.first + r;
-        if (slot < 0 || column >= a.n) continue;
-        const unsigned char* from = s.stages + r * kLd + i % 8 * 16;
-        unsigned char* y = static_cast<unsigned char*>(a.y) + slot * a.ldy + column;
-        if (column + 16 <= a.n && reinterpret_cast<uintptr_t>(y) % 16 == 0) {
-          *reinterpret_cast<uint4v*>(y) = *reinterpret_cast<const uint4v*>(from);
-        } else {
-          for (int c = 0; c < 16 && column + c < a.n; ++c) y[c] = from[c];
-        }
+      if (wn == 0 && g == 0 && r < t.rows) {
+        const int slot = EXPERTS ? s.slot[r] : t.first + r;
+        if (slot >= 0) a.y_scales[slot * a.ldys + n0 / kStep] = scale;
       }
+    }
+  }
+  gg::stage_barrier();
+  const int tid = threadIdx.x;
+  for (int i = tid; i < t.rows * 8; i += kThreads) {
+    const int r = i / 8, column = n0 + i % 8 * 16, slot = EXPERTS ? s.slot[r] : t.first + r;
+    if (slot < 0 || column >= a.n) continue;
+    const unsigned char* from = s.stages + r * kLd + i % 8 * 16;
+    unsigned char* y = static_cast<unsigned char*>(a.y) + slot * a.ldy + column;
+    if (column + 16 <= a.n && reinterpret_cast<uintptr_t>(y) % 16 == 0) {
+      *reinterpret_cast<uint4v*>(y) = *reinterpret_cast<const uint4v*>(from);
+    } else {
+      for (int c = 0; c < 16 && column + c < a.n; ++c) y[c] = from[c];
+    }
+  }
 }
 
-template <bool EXPERTS, bool GATED, int HALVES>
+template <bool EXPERTS, bool GATED, bool EXACT, int HALVES>
 __device__ __forceinline__ void run_tile(const Launch& l, const RowTile& t, const Shared& s, int n0) {
   const ggk_fp8_args& a = l.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave >> 2, wn = wave & 3;
   Sums<HALVES> acc;
-  multiply_tile<EXPERTS, GATED>(l, t, s, n0, wave, acc);
-  if constexpr (!GATED) {
-    if (a.y_type == GGK_TYPE_BF16) {
-      store_tile<EXPERTS, __bf16, HALVES>(a, t, s, n0, wm, wn, acc);
-    } else {
-      store_tile<EXPERTS, _Float16, HALVES>(a, t, s, n0, wm, wn, acc);
-    }
+  if constexpr (EXACT) {
+    multiply_tile_exact<EXPERTS, GATED>(l, t, s, n0, wave, acc);
   } else {
+    multiply_tile<EXPERTS, GATED>(l, t, s, n0, wave, acc);
+  }
+  if constexpr (GATED) {
     if (a.gate == GGK_GATE_GELU) {
       store_rows<EXPERTS, true, HALVES>(a, t, s, n0, wm, wn, acc);
     } else {
       store_rows<EXPERTS, false, HALVES>(a, t, s, n0, wm, wn, acc);
     }
-  }
-}
-
-template <bool EXPERTS, bool GATED>
-__device__ __forceinline__ void run_either(const Launch& l, const RowTile& t, const Shared& s, int n0) {
-  if (t.rows <= kRows / 2) {
-    run_tile<EXPERTS, GATED, 1>(l, t, s, n0);
+  } else if constexpr (EXACT) {
+    store_tile<EXPERTS, float, HALVES>(a, t, s, n0, wm, wn, acc);
+  } else if (a.y_type == GGK_TYPE_BF16) {
+    store_tile<EXPERTS, __bf16, HALVES>(a, t, s, n0, wm, wn, acc);
   } else {
-    run_tile<EXPERTS, GATED, 2>(l, t, s, n0);
+    store_tile<EXPERTS, _Float16, HALVES>(a, t, s, n0, wm, wn, acc);
   }
 }
 
+template <bool EXPERTS, bool GATED, bool EXACT>
+__device__ __forceinline__ void run_either(const Launch& l, const RowTile& t, const Shared& s, int n0) {
+  if constexpr (EXACT) {
+    run_tile<EXPERTS, GATED, true, 1>(l, t, s, n0);
+  } else if (t.rows <= kRows / 2) {
+    run_tile<EXPERTS, GATED, false, 1>(l, t, s, n0);
+  } else {
+    run_tile<EXPERTS, GATED, false, 2>(l, t, s, n0);
+  }
+}
+
+// Rows without an expert.
 template <bool GATED>
 __device__ __forceinline__ void clear_row(const ggk_fp8_args& a, int slot) {
   if (slot < 0 || slot >= a.rows) return;
@@ -695,7 +807,7 @@ __device__ __forceinline__ long long item_at(const Launch& l, const Table& s, lo
   return item + (left + cost - 1) / cost * min(kGroup, tiles - group * kGroup);
 }
 
-template <bool EXPERTS, bool GATED>
+template <bool EXPERTS, bool GATED, bool EXACT>
 __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
   const ggk_fp8_args& a = l.a;
   __shared__ alignas(128) unsigned char s_stages[kPlaces * kUnit + 2 * kScales];
@@ -712,7 +824,7 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
       int tile, block;
       place(item, tiles, l.blocks, &tile, &block);
       const RowTile t{0, tile * l.height, min(l.height, a.rows - tile * l.height)};
-      run_either<false, GATED>(l, t, s, block * kColumns<GATED>);
+      run_either<false, GATED, EXACT>(l, t, s, block * kColumns<GATED>);
       gg::stage_barrier();
     }
   } else {
@@ -731,7 +843,7 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
         s_slot[r] = slot < a.rows ? slot : -1;
       }
       gg::stage_barrier();
-      run_either<true, GATED>(l, t, s, block * kColumns<GATED>);
+      run_either<true, GATED, EXACT>(l, t, s, block * kColumns<GATED>);
       gg::stage_barrier();
     }
     // Rows without an expert.
@@ -739,19 +851,36 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_tile_kernel(Launch l) {
   }
 }
 
-template <bool EXPERTS, bool GATED>
-hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
-  Launch l{a, (a.n + kColumns<GATED> - 1) / kColumns<GATED>, kRows, a.rows / a.x_rows, 0};
-  // What the busiest CU gets: tiles of 256 rows, or of 128 at 0.6 of their time; of an expert's rows half a tile more.
-  auto rounds = [&](long long height) {
-    const long long tiles = EXPERTS ? a.rows / height + a.experts / 2 : (a.rows + height - 1) / height;
-    return (tiles * l.blocks + kCus - 1) / kCus;
-  };
-  const char* e = getenv("GG_H");
-  if (e ? atoi(e) == 128 : 10 * rounds(256) > 6 * rounds(128)) l.height = 128;
+template <bool EXPERTS, bool GATED, bool EXACT>
+hipError_t launch(const ggk_fp8_args& a, int height, hipStream_t stream) {
+  Launch l{a, (a.n + kColumns<GATED> - 1) / kColumns<GATED>, height, a.rows / a.x_rows, 0};
   if (EXPERTS) l.scale_bytes = (uint32_t)(((a.x_rows - 1) * a.ldxs + (a.k + kStep - 1) / kStep) * 4);
-  hipLaunchKernelGGL((fp8_tile_kernel<EXPERTS, GATED>), dim3(kCus), dim3(kThreads), 0, stream, l);
+  hipLaunchKernelGGL((fp8_tile_kernel<EXPERTS, GATED, EXACT>), dim3(kCus), dim3(kThreads), 0, stream, l);
   return hipGetLastError();
+}
+
+template <bool EXPERTS>
+hipError_t launch(const ggk_fp8_args& a, int height, hipStream_t stream) {
+  if (a.gate != GGK_GATE_NONE) return launch<EXPERTS, true, true>(a, height, stream);
+  return a.y_type == GGK_TYPE_F32 ? launch<EXPERTS, false, true>(a, height, stream) : launch<EXPERTS, false, false>(a, height, stream);
+}
+
+bool is_exact(const ggk_fp8_args& a) { return a.gate != GGK_GATE_NONE || a.y_type == GGK_TYPE_F32; }
+
+// What a call takes on tiles of `height` rows, in us: what the busiest CU gets.  Where all CUs work a stage takes 1.85 us for a
+// tile of 256 rows, 0.8 for one of 128, in binary16 1.4.
+double estimate(const ggk_fp8_args& a, int height) {
+  const bool gate = a.gate != GGK_GATE_NONE;
+  const double columns = gate ? 128 : 256, stages = (a.k + kStep - 1) / kStep;
+  const double rounds = ceil(row_tiles(a, height) * ceil(a.n / columns) / kCus);
+  const double stage = is_exact(a) ? 1.4 : height == kRows ? 1.85 : 0.8;
+  return (a.experts > 0 ? 10 : 8) + rounds * (stage * stages + (gate ? 4 : 2));
+}
+
+// Tiles of 256 rows or of 128.  us of the two: 777 rows of 8192 by 8192 100, 60; 1500 of 4096 by 4096 56, 36; 2048 of 8192 by
+// 8192 118, 131.  In binary16 the registers hold 128.
+int height_of(const ggk_fp8_args& a) {
+  return !is_exact(a) && estimate(a, kRows) <= estimate(a, kRows / 2) ? kRows : kRows / 2;
 }
 
 }  // namespace
@@ -765,9 +894,10 @@ bool tiles_take(const ggk_fp8_args& a) {
   return a.experts <= kMost && rows * a.ldx < 0xfffffff0ll - kStep && rows * a.ldxs * 4 < 0x7fffffffll;
 }
 
+double estimate_tiles(const ggk_fp8_args& a) { return estimate(a, height_of(a)); }
+
 hipError_t multiply_tiles(const ggk_fp8_args& a, hipStream_t stream) {
-  if (a.experts > 0) return a.gate != GGK_GATE_NONE ? launch<true, true>(a, stream) : launch<true, false>(a, stream);
-  return a.gate != GGK_GATE_NONE ? launch<false, true>(a, stream) : launch<false, false>(a, stream);
+  return a.experts > 0 ? launch<true>(a, height_of(a), stream) : launch<false>(a, height_of(a), stream);
 }
 
 }  // namespace fp8
