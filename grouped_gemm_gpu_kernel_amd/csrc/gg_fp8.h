@@ -52,17 +52,20 @@ __device__ __forceinline__ int8v read_fragment(uint32_t lo, uint32_t hi, uint32_
 struct Halves {
   half8v v[4];
 };
+__device__ __forceinline__ void to_halves(const int8v& q, int i, Halves& h) {  // a quarter
+  uint4v v;
+#pragma unroll
+  for (int pair = 0; pair < 4; ++pair) {
+    const int four = q[2 * i + pair / 2];
+    v[pair] = __builtin_bit_cast(uint32_t, pair % 2 == 0 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(four, 1.0f, false)
+                                                         : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(four, 1.0f, true));
+  }
+  h.v[i] = __builtin_bit_cast(half8v, v);
+}
 __device__ __forceinline__ Halves to_halves(const int8v& q) {
   Halves h;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const half2v lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q[i], 1.0f, false);
-    const half2v hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q[i], 1.0f, true);
-    h.v[i / 2][4 * (i % 2) + 0] = lo[0];
-    h.v[i / 2][4 * (i % 2) + 1] = lo[1];
-    h.v[i / 2][4 * (i % 2) + 2] = hi[0];
-    h.v[i / 2][4 * (i % 2) + 3] = hi[1];
-  }
+  for (int i = 0; i < 4; ++i) to_halves(q, i, h);
   return h;
 }
 

@@ -299,7 +299,7 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
 // two on a CU, or by 128, one.
 double estimate_few(const ggk_fp8_args& a) {
   const double tiles = row_tiles(a, 32), steps = a.k / 128.0;
-  if (a.gate != GGK_GATE_NONE) return 5 + ceil(tiles * ceil(a.n / 128.0) / kCus) * (1 + 0.85 * steps);
+  if (a.gate != GGK_GATE_NONE) return 5 + ceil(tiles * ceil(a.n / 128.0) / kCus) * (1 + 1.1 * steps);
   if (a.experts > 0) return 5 + ceil(tiles * ceil(a.n / 128.0) / kCus) * 0.6 * steps;
   return 4 + ceil(tiles * ceil(a.n / 32.0) / (2 * kCus)) * (1.3 + 0.15 * steps);
 }
@@ -323,8 +323,9 @@ hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
       return a.n >= 8192 ? launch<Form<16, 1, 2, 4, 2, false, true>, false>(a, stream)
                          : launch<Form<16, 1, 1, 8, 2, false, true>, false>(a, stream);
     }
-    // 64 rows at once where enough columns remain for it: us, 61 rows of 4096 by 14335 20.3, 18.4, 64 of 8192 by 8192 18.9, 27.
-    if (a.rows > 32 && a.rows <= 64 && a.n >= 3 * 64 * kCus / 4) {
+    // 64 rows at once where their blocks of 64 columns fill the CUs, else 32 twice.  us of the two: 64 rows of 8192 by 28672
+    // 59.5, 72.7, of 4096 by 16384 16.4, 16.8, in float 17.6, 19.3; of 4096 by 12288 15.6, 13.5, of 8192 by 8192 24, 17.
+    if (a.rows > 32 && a.rows <= 64 && a.n > 64 * (kCus - kCus / 8)) {
       return exact ? launch<Form<64, 4, 1, 4, 2, false, true>, false>(a, stream)
                    : launch<Form<64, 4, 1, 4, 2, false, false>, false>(a, stream);
     }
@@ -380,10 +381,8 @@ extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t str
   if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
   const ggk_fp8_args& a = *args;
   // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 512 rows of 2048 by 2048 10, 20,
-  // 2048 rows 35, 21; 128 of 8192 by 8192 29, 52, 512 103, 56; 16 experts of 1024 by 2048, 512 slots 15, 19, 2048 slots 29,
-  // 21, gated 22, 37 and 46, 36; 64 experts of 4096 by 14336, 256 slots 480, 474, 2048 slots 972, 751.
-  if (tiles_take(a) && estimate_tiles(a) < estimate_few(a)) {
-    return multiply_tiles(a, stream);
-  }
+  // 2048 rows 35, 21; 128 of 8192 by 8192 29, 49, 512 103, 56; 16 experts of 1024 by 2048, 512 slots 15, 18, 2048 slots 29,
+  // 20, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 256 slots 479, 463, 2048 slots 972, 751.
+  if (tiles_take(a) && estimate_tiles(a) < estimate_few(a)) return multiply_tiles(a, stream);
   return args->experts > 0 ? multiply_few<true>(*args, stream) : multiply_few<false>(*args, stream);
 }

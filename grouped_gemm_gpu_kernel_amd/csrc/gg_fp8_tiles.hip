@@ -303,8 +303,10 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
 }
 
 // The same in binary16, which holds the numbers exactly, for float32 and 8-bit y (a row's scale is as exact as its largest
-// value).  A fragment is turned into binary16 once a stage, which takes the vector unit about as long as the matrix unit
-// needs for the products; each frees its registers for the next stage's.
+// value).  A wave turns its fragments into binary16 once a stage, 128 instructions beside 64 products that take the matrix
+// unit four times as long each: while a quarter of x's or w's is multiplied for the last time, the next one takes its
+// registers.  Turned into binary16 in front of the stage's products, 8192^3 in float took 1026 us, so 970; leaving out products
+// of rows past the tile's, in tiles of 64 or 32 rows or by a branch around them, gained nothing: zeros take little power.
 template <bool EXPERTS, bool GATED>
 __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
                                                     Sums<1>& acc) {
@@ -316,12 +318,12 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
   int8v a[4], b[4];
   float x_scale[4], w_scale[2], x_next[4], w_next[2];
   clear<1>(acc);
-  // Of the wave's four times 16 rows, those that the tile has: the matrix unit bounds this loop.
-  const int live = min(max(t.rows - 64 * (wave >> 2) + 15, 0) / 16, 4);
 
   auto read_a = [&](uint32_t place, int i) { a[i] = read_fragment(lane.a_lo + place, lane.a_hi + place, kUnit + i * 2048u); };
-  auto read_b = [&](uint32_t place, int f) {
-    b[f] = read_fragment(lane.b_lo + place, lane.b_hi + place, (f / 2) * 2 * kUnit + (f % 2) * 2048u);
+  auto read_b = [&](uint32_t place, int f, int half) {
+    const int8v v = read_fragment(lane.b_lo + place, lane.b_hi + place, (f / 2) * 2 * kUnit + (f % 2) * 2048u);
+#pragma unroll
+    for (int e = 4 * half; e < 4 * half + 4; ++e) b[f][e] = v[e];
   };
   auto read_scales = [&](int kt) {
     const uint32_t at = scales_of(kt);
@@ -347,7 +349,10 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
   gg::wait_vmcnt<12>();
   gg::phase_barrier();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) read_b(0, i);
+  for (int i = 0; i < 4; ++i) {
+    read_b(0, i, 0);
+    read_b(0, i, 1);
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) read_a(0, i);
   read_scales(0);
@@ -355,7 +360,12 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
   gg::wait_lgkmcnt<0>();
   gg::phase_barrier();
 
-  // Stage kt, whose operands are in registers and whose three places, at `here`, are free.
+  Halves w[4], x = to_halves(a[0]);
+#pragma unroll
+  for (int n = 0; n < 4; ++n) w[n] = to_halves(b[n]);
+
+  // Stage kt, whose operands are in registers and whose three places, at `here`, are free.  As the last products with a
+  // quarter of x or w are on their way, the next ones' numbers take its registers.
   uint32_t here = 0;
 #pragma unroll 1
   for (int kt = 0; kt < nk; ++kt) {
@@ -365,36 +375,33 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
     for (int i = 0; i < 4; ++i) x_scale[i] = x_next[i];
     w_scale[0] = w_next[0];
     if constexpr (GATED) w_scale[1] = w_next[1];
-    Halves w[4];
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      w[n] = to_halves(b[n]);
-      read_b(next, n);
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       // The loads of stage kt + 3.
-      if (i < 2) issue(kt + 3, here, i);
-      if (i >= 2) issue(kt + 3, here, 2 * i - 2);
-      if (i >= 2) issue(kt + 3, here, 2 * i - 1);
-      if (i < live) {
-        const Halves x = to_halves(a[i]);
-        read_a(next, i);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {  // two chains of products at a time
-          float4v part[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+      for (int load = 6 * i / 4; load < 6 * (i + 1) / 4; ++load) issue(kt + 3, here, load);
+      read_a(next, i);
+      float4v part[4] = {};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 4; ++q) {
+        if (i == 3 && q % 2 == 0) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              part[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[2 * u + n].v[q], x.v[q], part[n], 0, 0, 0);
-            }
-          }
-          const float scale = x_scale[i] * w_scale[GATED ? u : 0];
-#pragma unroll
-          for (int n = 0; n < 2; ++n) add_scaled(acc[0][i][u][n], part[n], scale);
+          for (int n = 0; n < 4; ++n) read_b(next, n, q / 2);
         }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) part[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[n].v[q], x.v[q], part[n], 0, 0, 0);
+        to_halves(a[(i + 1) % 4], q, x);
+        if (i == 3 && q % 2 == 1) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            to_halves(b[n], q - 1, w[n]);
+            to_halves(b[n], q, w[n]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) add_scaled(acc[0][i][n / 2][n % 2], part[n], x_scale[i] * w_scale[GATED ? n / 2 : 0]);
     }
     read_scales(kt + 1);
     // The next stage's operands are in every wave's registers, and the one after it has landed.
@@ -867,13 +874,14 @@ hipError_t launch(const ggk_fp8_args& a, int height, hipStream_t stream) {
 
 bool is_exact(const ggk_fp8_args& a) { return a.gate != GGK_GATE_NONE || a.y_type == GGK_TYPE_F32; }
 
-// What a call takes on tiles of `height` rows, in us: what the busiest CU gets.  Where all CUs work a stage takes 1.85 us for a
-// tile of 256 rows, 0.8 for one of 128, in binary16 1.4.
+// What a call takes on tiles of `height` rows, in us: what the busiest CU gets; of experts' tiles, whose counts the host does
+// not know, a tenth more.  Where all CUs work a stage takes 1.85 us for a tile of 256 rows, 0.8 for one of 128, in binary16
+// 1.75.
 double estimate(const ggk_fp8_args& a, int height) {
   const bool gate = a.gate != GGK_GATE_NONE;
   const double columns = gate ? 128 : 256, stages = (a.k + kStep - 1) / kStep;
-  const double rounds = ceil(row_tiles(a, height) * ceil(a.n / columns) / kCus);
-  const double stage = is_exact(a) ? 1.4 : height == kRows ? 1.85 : 0.8;
+  const double rounds = ceil(row_tiles(a, height) * ceil(a.n / columns) * (a.experts > 0 ? 1.1 : 1) / kCus);
+  const double stage = is_exact(a) ? 1.75 : height == kRows ? 1.85 : 0.8;
   return (a.experts > 0 ? 10 : 8) + rounds * (stage * stages + (gate ? 4 : 2));
 }
 
