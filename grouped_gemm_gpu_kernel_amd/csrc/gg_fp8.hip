@@ -308,6 +308,8 @@ template <bool EXPERTS>
 hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
   const bool exact = a.y_type == GGK_TYPE_F32;
   if constexpr (EXPERTS) {
+    // us with 32 rows at once, 16, 8: 16 experts of 1024 by 2048, 64 slots 16, 16, 18, 512 slots 25, 29, 41; 64 experts of 4096
+    // by 14336, 16 slots 223, 218, 216, 256 slots 1011, 1022, 1095.
     if (a.gate != GGK_GATE_NONE) return launch<Form<32, 2, 8, 1, 2, true, true>, true>(a, stream);
     if (a.rows <= 32) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream);
     if (a.rows <= 12ll * a.experts) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream);
@@ -315,7 +317,9 @@ hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
     return launch<Form<32, 2, 4, 2, 2, false, false>, true>(a, stream);
   } else if (a.gate != GGK_GATE_NONE) {
     if (a.rows <= 8) return launch<Form<8, 4, 4, 1, 4, true, true>, false>(a, stream);
-    if (a.rows <= 16) return launch<Form<16, 2, 8, 1, 3, true, true>, false>(a, stream);
+    // 16 rows at once where every CU can get its own tile, else 32.  us of the two: 32 rows of 4096 by 14336 36, 48, 128 of
+    // 4096 by 4096 25.5, 30; 64 rows of 4096 by 14336 62, 45, 32 of 8192 by 28672 133, 108.
+    if (row_tiles(a, 16) * ceil(a.n / 128.0) <= kCus) return launch<Form<16, 2, 8, 1, 3, true, true>, false>(a, stream);
     return launch<Form<32, 2, 8, 1, 2, true, true>, false>(a, stream);
   } else {
     if (a.rows <= 8) return launch<Form<8, 1, 1, 8, 2, false, true>, false>(a, stream);
