@@ -130,8 +130,9 @@ __device__ __forceinline__ void store_numbers(const ggk_fp8_args& a, long long r
     if (j + i >= a.n) v[i] = 0.0f;
     largest = max(largest, magnitude_bits(v[i]));
   }
-  const float scale = fp8_scale(row_max16(largest));
-  const Fp8Divisor by(scale);
+  largest = row_max16(largest);
+  const float scale = fp8_scale(largest);
+  const Fp8Divisor by(scale, __builtin_bit_cast(float, largest));
   const uint2v numbers = {fp8_numbers(v[0], v[1], v[2], v[3], by), fp8_numbers(v[4], v[5], v[6], v[7], by)};
   if (!write || j >= a.n) return;
   unsigned char* y = static_cast<unsigned char*>(a.y) + row * a.ldy + j;

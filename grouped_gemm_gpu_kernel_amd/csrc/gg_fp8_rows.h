@@ -29,16 +29,21 @@ __device__ __forceinline__ float fp8_scale(uint32_t largest_bits) {
   return s < kFp8SmallestScale ? kFp8SmallestScale : s;  // a NaN stays
 }
 
-// What a block's values are divided by: the quotient by the reciprocal and one correction, within half a unit of the last
-// place of it but for rare ties (without the correction a number in some 10^6 was the other neighbour).  An infinite
-// scale leaves 0 of finite values and NaN of infinite ones.
+// What a block's values are divided by, a 448th of the block's largest magnitude, here as the scale and what its rounding left
+// out: the quotient by an about equal reciprocal and one correction then rounds to the number of the exact quotient, but for
+// ties closer than its last place.  (Against 64 bits 1500 of the 134 million numbers of a norm of 16384 rows of 8192 were the
+// other neighbour with the rounded scale, none to two so.)  The smallest scale stands for itself; an infinite one leaves 0 of
+// finite values and NaN of infinite ones.
 struct Fp8Divisor {
-  float scale, inverse;
-  __device__ __forceinline__ explicit Fp8Divisor(float s)
-      : scale(s == __builtin_inff() ? 0.0f : s), inverse(1.0f / s) {}
+  float scale, rest, inverse;
+  __device__ __forceinline__ Fp8Divisor(float s, float largest)
+      : scale(s == __builtin_inff() ? 0.0f : s), rest(0.0f), inverse(__builtin_amdgcn_rcpf(s)) {
+    const float left = fmaf(-kFp8Largest, s, largest);
+    if (fabsf(left) <= s * (kFp8Largest * 0x1p-22f)) rest = left * (1.0f / kFp8Largest);
+  }
   __device__ __forceinline__ float operator()(float y) const {
     const float t = y * inverse;
-    return fmaf(fmaf(-t, scale, y), inverse, t);
+    return fmaf(fmaf(-t, rest, fmaf(-t, scale, y)), inverse, t);
   }
 };
 

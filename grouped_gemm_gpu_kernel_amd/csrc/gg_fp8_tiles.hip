@@ -653,8 +653,9 @@ __device__ __forceinline__ void store_rows(const ggk_fp8_args& a, const RowTile&
     for (int i = 0; i < 4; ++i) {
       const int r = 128 * half + 64 * wm + 16 * i + j;
       const uint4v most = *reinterpret_cast<const uint4v*>(&s_most[r * 4]);
-      const float scale = gg::fp8_scale(max(max(most.x, most.y), max(most.z, most.w)));
-      const gg::Fp8Divisor by(scale);
+      const uint32_t largest = max(max(most.x, most.y), max(most.z, most.w));
+      const float scale = gg::fp8_scale(largest);
+      const gg::Fp8Divisor by(scale, __builtin_bit_cast(float, largest));
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const float4v v = acc[half][i][0][n];

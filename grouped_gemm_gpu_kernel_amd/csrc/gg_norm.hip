@@ -120,7 +120,13 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_nor
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) squares += s_squares[w];
   }
+  // Numbers are quotients in which the factor cancels: values carry its power of two, which rounds nothing, and scales and y
+  // the rest of it.
   const float factor = 1.0f / sqrtf(squares / (float)a.columns + a.eps);
+  const bool splits = factor > 0.0f && factor < __builtin_inff();
+  int exponent = 0;
+  const float part_of_one = frexpf(factor, &exponent), rest = splits ? part_of_one : 1.0f;
+  const float power = splits ? ldexpf(1.0f, exponent) : factor;
   const W* weight = static_cast<const W*>(a.weight);
   T* y = a.y != nullptr ? static_cast<T*>(a.y) + row * a.ldy : nullptr;
   unsigned char* q = a.q + row * a.ldq;
@@ -134,12 +140,18 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_nor
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = VEC || i < count ? h[c][i] * factor * w[i] : 0.0f;  // past the end 0 * factor may be NaN
+      v[i] = VEC || i < count ? h[c][i] * power * w[i] : 0.0f;  // past the end 0 * power may be NaN
       if (!VEC || count > 0) largest = max(largest, gg::magnitude_bits(v[i]));
     }
-    if (y != nullptr) store8<T, VEC>(y + at, count, v);
-    const float scale = gg::fp8_scale(gg::row_max16(largest));
-    const gg::Fp8Divisor by(scale);
+    if (y != nullptr) {
+      float out[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = v[i] * rest;
+      store8<T, VEC>(y + at, count, out);
+    }
+    const float most = __builtin_bit_cast(float, gg::row_max16(largest));
+    const float scale = gg::fp8_scale(gg::magnitude_bits(most * rest));
+    const gg::Fp8Divisor by(scale == gg::kFp8SmallestScale ? scale / rest : most * (1.0f / gg::kFp8Largest), most);
     const uint2v numbers = {gg::fp8_numbers(v[0], v[1], v[2], v[3], by),
                             gg::fp8_numbers(v[4], v[5], v[6], v[7], by)};
     if constexpr (VEC) {
