@@ -570,16 +570,38 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   gg::wait_vmcnt<0>();
 }
 
-// y of a tile: four columns a lane and store; rows that do not start on multiples of four values by way of LDS, value by
-// value.
+// Of a lane's four columns of two neighbouring 16s, what 16 bytes hold of one: lanes 16 apart trade (a row of y then gets 64
+// bytes of an instruction, not 32).
+template <class T>
+struct Sixteen {
+  typedef T Four __attribute__((ext_vector_type(4)));
+  static constexpr bool kTrade = sizeof(T) == 2;
+  uint4v v[kTrade ? 1 : 2];
+  __device__ __forceinline__ Sixteen(const Four& a, const Four& b) {
+    if constexpr (kTrade) {
+      const uint2v p = __builtin_bit_cast(uint2v, a), q = __builtin_bit_cast(uint2v, b);
+      const auto lo = __builtin_amdgcn_permlane16_swap(p.x, q.x, false, false);
+      const auto hi = __builtin_amdgcn_permlane16_swap(p.y, q.y, false, false);
+      v[0] = uint4v{lo[0], hi[0], lo[1], hi[1]};
+    } else {
+      v[0] = __builtin_bit_cast(uint4v, a);
+      v[1] = __builtin_bit_cast(uint4v, b);
+    }
+  }
+  // First column of v[i] for lanes g of a row.
+  static __device__ __forceinline__ int column(int g, int i) { return kTrade ? 16 * (g & 1) + 8 * (g >> 1) : 16 * i + 4 * g; }
+};
+
+// y of a tile: 16 bytes a lane and store; rows that do not start on multiples of 16 bytes by way of LDS, value by value.
 template <bool EXPERTS, class T, int HALVES>
 __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile& t, const Shared& s, int n0, int wm, int wn,
                                            const Sums<HALVES>& acc) {
-  typedef T Four __attribute__((ext_vector_type(4)));
+  using Four = typename Sixteen<T>::Four;
   constexpr int kLd = sizeof(T) * 256 + 16;  // bytes of a row in LDS
+  constexpr int kEach = 16 / sizeof(T);
   static_assert(128 * HALVES * kLd <= kPlaces * kUnit, "the tile fits LDS");
   const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
-  const bool vec = a.n % 4 == 0 && a.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % sizeof(Four) == 0;
+  const bool vec = a.n % kEach == 0 && a.ldy % kEach == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
   if (!vec) gg::stage_barrier();
 #pragma unroll
   for (int half = 0; half < HALVES; ++half) {
@@ -591,16 +613,20 @@ __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile&
       T* y = static_cast<T*>(a.y) + slot * a.ldy + n0;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
+        Four four[2];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const int column = 64 * wn + 32 * u + 16 * n + 4 * g;
-          Four four;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) four[e] = (T)(acc[half][i][u][n][e] * weight);
+          for (int e = 0; e < 4; ++e) four[n][e] = (T)(acc[half][i][u][n][e] * weight);
+        }
+        const Sixteen<T> part(four[0], four[1]);
+#pragma unroll
+        for (int n = 0; n < (int)(sizeof(part.v) / 16); ++n) {
+          const int column = 64 * wn + 32 * u + Sixteen<T>::column(g, n);
           if (!vec) {
-            *reinterpret_cast<Four*>(s.stages + r * kLd + sizeof(T) * column) = four;
+            *reinterpret_cast<uint4v*>(s.stages + r * kLd + sizeof(T) * column) = part.v[n];
           } else if (slot >= 0 && n0 + column < a.n) {
-            *reinterpret_cast<Four*>(y + column) = four;
+            *reinterpret_cast<uint4v*>(y + column) = part.v[n];
           }
         }
       }
