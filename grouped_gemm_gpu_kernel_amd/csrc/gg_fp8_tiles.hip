@@ -902,20 +902,24 @@ hipError_t launch(const ggk_fp8_args& a, int height, hipStream_t stream) {
 bool is_exact(const ggk_fp8_args& a) { return a.gate != GGK_GATE_NONE || a.y_type == GGK_TYPE_F32; }
 
 // What a call takes on tiles of `height` rows, in us: what the busiest CU gets; of experts' tiles, whose counts the host does
-// not know, a tenth more.  Where all CUs work a stage takes 1.85 us for a tile of 256 rows, 0.8 for one of 128, in binary16
-// 1.75.
+// not know, a tenth more.  A stage of a tile of 256 rows takes 1.2 us where half of the CUs work and 1.7 where all do, one of 128
+// rows 0.65 and 0.95, in binary16 1.75.
 double estimate(const ggk_fp8_args& a, int height) {
   const bool gate = a.gate != GGK_GATE_NONE;
   const double columns = gate ? 128 : 256, stages = (a.k + kStep - 1) / kStep;
-  const double rounds = ceil(row_tiles(a, height) * ceil(a.n / columns) * (a.experts > 0 ? 1.1 : 1) / kCus);
-  const double stage = is_exact(a) ? 1.75 : height == kRows ? 1.85 : 0.8;
+  const double of_a_cu = row_tiles(a, height) * ceil(a.n / columns) * (a.experts > 0 ? 1.1 : 1) / kCus, rounds = ceil(of_a_cu);
+  const double at_work = of_a_cu / rounds;
+  const double stage = is_exact(a) ? 1.75 : height == kRows ? 0.9 + 0.8 * at_work : 0.45 + 0.5 * at_work;
   return (a.experts > 0 ? 10 : 8) + rounds * (stage * stages + (gate ? 4 : 2));
 }
 
-// Tiles of 256 rows or of 128.  us of the two: 777 rows of 8192 by 8192 100, 60; 1500 of 4096 by 4096 56, 36; 2048 of 8192 by
-// 8192 118, 131.  In binary16 the registers hold 128.
+// Tiles of 256 rows or of 128.  us of the two: 1024 rows of 8192 by 8192 86, 65, 1280 90, 107, 8192 453, 522; 1500 of 4096 by
+// 4096 46, 30.  Experts' tiles of 256 rows, with a rest of 128 and less each, where those of 128 would not fit the CUs at once:
+// 64 experts of 4096 by 14336, 16384 slots 1338, 1438, 16 of 1024 by 2048, 2048 slots 20, 18.  In binary16 the registers hold 128.
 int height_of(const ggk_fp8_args& a) {
-  return !is_exact(a) && estimate(a, kRows) <= estimate(a, kRows / 2) ? kRows : kRows / 2;
+  if (is_exact(a)) return kRows / 2;
+  const bool small = a.experts > 0 ? row_tiles(a, kRows / 2) * ceil(a.n / 256.0) <= kCus : estimate(a, kRows / 2) < estimate(a, kRows);
+  return small ? kRows / 2 : kRows;
 }
 
 }  // namespace
@@ -929,7 +933,7 @@ bool tiles_take(const ggk_fp8_args& a) {
   return a.experts <= kMost && rows * a.ldx < 0xfffffff0ll - kStep && rows * a.ldxs * 4 < 0x7fffffffll;
 }
 
-double estimate_tiles(const ggk_fp8_args& a) { return estimate(a, height_of(a)); }
+double estimate_tiles(const ggk_fp8_args& a) { return estimate(a, a.experts > 0 ? kRows / 2 : height_of(a)); }
 
 hipError_t multiply_tiles(const ggk_fp8_args& a, hipStream_t stream) {
   return a.experts > 0 ? launch<true>(a, height_of(a), stream) : launch<false>(a, height_of(a), stream);
