@@ -697,9 +697,9 @@ def test_long_matrix_past_32_bits(torch_cuda):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tokens,n", [(90, 140), (9000, 400)])
-def test_streams_graphs_and_threads(torch_cuda, tokens, n):
-    experts, k = 6, 272
+@pytest.mark.parametrize("tokens,n,k", [(90, 140, 272), (9000, 520, 1040)])
+def test_streams_graphs_and_threads(torch_cuda, tokens, n, k):
+    experts = 6
     w, up = matrix_of((experts,), n, k, 1), matrix_of((experts,), n, k, 2)
     inputs = [torch.randn(tokens, k, generator=_gen(i), device="cuda").bfloat16() for i in range(5)]
     routes = [routing(tokens, experts, 2, i, 0.1)[1:] for i in range(5)]
