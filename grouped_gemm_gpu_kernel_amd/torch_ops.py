@@ -695,9 +695,9 @@ def fp8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
 
     K is a multiple of 16; x and w start on multiples of 16 bytes, and so do their rows, which may be padded; rows
     of scales may be padded too.  Sums are float32.  y is float32, float16 or bfloat16, rounded once.  For
-    float32 the products are made in binary16, which holds 8-bit numbers exactly; for the 16-bit types and more than a
-    few rows by the 8-bit matrix instructions, twice as fast, which leave an error of about 1.5e-5 of a sum's terms
-    (8 products at a time are aligned to the largest, to 13 bits below it).
+    float32 the products are made in binary16, which holds 8-bit numbers exactly; for the 16-bit types and more than 16
+    rows (with experts, 12 slots each) by the 8-bit matrix instructions, twice as fast, which leave an error of about
+    1.5e-5 of a sum's terms (8 products at a time are aligned to the largest, to 13 bits below it).
 
     Runs on the current stream of x's device, without waiting; no gradient (inputs that require one are
     refused, and dual tensors of forward mode)."""
@@ -709,7 +709,7 @@ def fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_
     """act(x @ gate.T) * (x @ up.T) as 8-bit rows, both projections of a gated feed-forward block, the activation and
     their product in one kernel; operands as fp8_matmul's, gate and up [N, K] (the halves of one matrix of both can be given
     as views).  activation: "silu", or "gelu" (the form with tanh).  Rows are made of float32 as rms_norm_fp8 makes
-    them; for more than a few rows the sums are those of the 8-bit matrix instructions (see fp8_matmul)."""
+    them, of products in binary16 as fp8_matmul's for float32."""
     return _fp8(x, x_scales, gate, gate_scales, up, up_scales, activation, None, None, None, None)
 
 
