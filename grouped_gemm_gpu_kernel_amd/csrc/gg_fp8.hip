@@ -329,7 +329,7 @@ hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
     }
     // 64 rows at once where their blocks of 64 columns fill the CUs, else 32 twice.  us of the two: 64 rows of 8192 by 28672
     // 59.5, 72.7, of 4096 by 16384 16.4, 16.8, in float 17.6, 19.3; of 4096 by 12288 15.6, 13.5, of 8192 by 8192 24, 17.
-    if (a.rows > 32 && a.rows <= 64 && a.n > 64 * (kCus - kCus / 8)) {
+    if (a.rows > 32 && a.rows <= 64 && (a.n + 63) / 64 >= kCus / 8 * 7) {
       return exact ? launch<Form<64, 4, 1, 4, 2, false, true>, false>(a, stream)
                    : launch<Form<64, 4, 1, 4, 2, false, false>, false>(a, stream);
     }
