@@ -41,10 +41,14 @@ __device__ __forceinline__ void load_to_lds4_at(const void* p, uint32_t lds) {
   asm volatile("s_nop 4\n\tglobal_load_lds_dword %1, off" : : "{m0}"(m0), "v"(p) : "memory");
 }
 
+__device__ __forceinline__ uint4v read_piece(uint32_t at, uint32_t offset) {
+  return *(const GG_LDS uint4v*)(uintptr_t)(at + offset);
+}
+
 // The 32 numbers of a lane: its swizzled pieces g and g + 4 of a row's 128 bytes, at lo and hi = lo ^ 64 (LDS byte addresses)
 // of some row and `offset` (whole rows) on, which the instruction adds.
 __device__ __forceinline__ int8v read_fragment(uint32_t lo, uint32_t hi, uint32_t offset) {
-  const uint4v a = *(const GG_LDS uint4v*)(uintptr_t)(lo + offset), b = *(const GG_LDS uint4v*)(uintptr_t)(hi + offset);
+  const uint4v a = read_piece(lo, offset), b = read_piece(hi, offset);
   return int8v{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
 
@@ -52,20 +56,18 @@ __device__ __forceinline__ int8v read_fragment(uint32_t lo, uint32_t hi, uint32_
 struct Halves {
   half8v v[4];
 };
-__device__ __forceinline__ void to_halves(const int8v& q, int i, Halves& h) {  // a quarter
+__device__ __forceinline__ half8v to_halves(uint32_t lo, uint32_t hi) {
   uint4v v;
-#pragma unroll
-  for (int pair = 0; pair < 4; ++pair) {
-    const int four = q[2 * i + pair / 2];
-    v[pair] = __builtin_bit_cast(uint32_t, pair % 2 == 0 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(four, 1.0f, false)
-                                                         : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(four, 1.0f, true));
-  }
-  h.v[i] = __builtin_bit_cast(half8v, v);
+  v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+  v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+  v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+  v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+  return __builtin_bit_cast(half8v, v);
 }
 __device__ __forceinline__ Halves to_halves(const int8v& q) {
   Halves h;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) to_halves(q, i, h);
+  for (int i = 0; i < 4; ++i) h.v[i] = to_halves(q[2 * i], q[2 * i + 1]);
   return h;
 }
 

@@ -315,22 +315,27 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
   const Loader<EXPERTS, GATED> loader(l, t, s.slot, n0, wave);
   const uint32_t lds = gg::lds_address(s.stages), scales_at = lds + kPlaces * kUnit;
   const Lane<GATED> lane(lds, wave);
-  int8v a[4], b[4];
-  float x_scale[4], w_scale[2], x_next[4], w_next[2];
+  uint4v a[4][2], b[2][4];  // pieces of 16 numbers
+  float x_scale[4], w_scale[2];
   clear<1>(acc);
 
-  auto read_a = [&](uint32_t place, int i) { a[i] = read_fragment(lane.a_lo + place, lane.a_hi + place, kUnit + i * 2048u); };
-  auto read_b = [&](uint32_t place, int f, int half) {
-    const int8v v = read_fragment(lane.b_lo + place, lane.b_hi + place, (f / 2) * 2 * kUnit + (f % 2) * 2048u);
-#pragma unroll
-    for (int e = 4 * half; e < 4 * half + 4; ++e) b[f][e] = v[e];
+  auto read_a = [&](uint32_t place, int i) {
+    a[i][0] = read_piece(lane.a_lo + place, kUnit + i * 2048u);
+    a[i][1] = read_piece(lane.a_hi + place, kUnit + i * 2048u);
   };
+  auto read_b = [&](uint32_t place, int half) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      b[half][n] = read_piece((half == 0 ? lane.b_lo : lane.b_hi) + place, (n / 2) * 2 * kUnit + (n % 2) * 2048u);
+    }
+  };
+  auto quarter = [](const uint4v& piece, int q) { return q % 2 == 0 ? to_halves(piece.x, piece.y) : to_halves(piece.z, piece.w); };
   auto read_scales = [&](int kt) {
     const uint32_t at = scales_of(kt);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x_next[i] = *(const GG_LDS float*)(uintptr_t)(lane.x_scale + at + 256u * i);
-    w_next[0] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at);
-    if constexpr (GATED) w_next[1] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at + 16u);
+    for (int i = 0; i < 4; ++i) x_scale[i] = *(const GG_LDS float*)(uintptr_t)(lane.x_scale + at + 256u * i);
+    w_scale[0] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at);
+    if constexpr (GATED) w_scale[1] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at + 16u);
   };
   auto issue = [&](int kt, uint32_t place, int i) {  // load i (0..5) of a stage; past K zeros, and memory is not touched
     if (i / 2 == 1) {
@@ -348,21 +353,21 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
   }
   gg::wait_vmcnt<12>();
   gg::phase_barrier();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    read_b(0, i, 0);
-    read_b(0, i, 1);
-  }
+  read_b(0, 0);
+  read_b(0, 1);
 #pragma unroll
   for (int i = 0; i < 4; ++i) read_a(0, i);
-  read_scales(0);
   gg::wait_vmcnt<6>();
   gg::wait_lgkmcnt<0>();
   gg::phase_barrier();
 
-  Halves w[4], x = to_halves(a[0]);
+  half8v w[4][4], x[4];  // [16 columns][quarter], [quarter]
 #pragma unroll
-  for (int n = 0; n < 4; ++n) w[n] = to_halves(b[n]);
+  for (int q = 0; q < 4; ++q) {
+    x[q] = quarter(a[0][q / 2], q);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) w[n][q] = quarter(b[q / 2][n], q);
+  }
 
   // Stage kt, whose operands are in registers and whose three places, at `here`, are free.  As the last products with a
   // quarter of x or w are on their way, the next ones' numbers take its registers.
@@ -371,10 +376,7 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
   for (int kt = 0; kt < nk; ++kt) {
     const uint32_t next = here == 6 * kUnit ? 0 : here + 3 * kUnit;
     if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x_scale[i] = x_next[i];
-    w_scale[0] = w_next[0];
-    if constexpr (GATED) w_scale[1] = w_next[1];
+    read_scales(kt);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       // The loads of stage kt + 3.
@@ -384,18 +386,15 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
       float4v part[4] = {};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        if (i == 3 && q % 2 == 0) {
+        if (i == 3 && q % 2 == 0) read_b(next, q / 2);
 #pragma unroll
-          for (int n = 0; n < 4; ++n) read_b(next, n, q / 2);
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) part[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[n].v[q], x.v[q], part[n], 0, 0, 0);
-        to_halves(a[(i + 1) % 4], q, x);
+        for (int n = 0; n < 4; ++n) part[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[n][q], x[q], part[n], 0, 0, 0);
+        x[q] = quarter(a[(i + 1) % 4][q / 2], q);
         if (i == 3 && q % 2 == 1) {
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            to_halves(b[n], q - 1, w[n]);
-            to_halves(b[n], q, w[n]);
+            w[n][q - 1] = quarter(b[q / 2][n], q - 1);
+            w[n][q] = quarter(b[q / 2][n], q);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -403,7 +402,6 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
 #pragma unroll
       for (int n = 0; n < 4; ++n) add_scaled(acc[0][i][n / 2][n % 2], part[n], x_scale[i] * w_scale[GATED ? n / 2 : 0]);
     }
-    read_scales(kt + 1);
     // The next stage's operands are in every wave's registers, and the one after it has landed.
     gg::wait_lgkmcnt<0>();
     gg::wait_vmcnt<6>();
