@@ -189,18 +189,18 @@ __device__ __forceinline__ void clear(Sums<HALVES>& acc) {
 }
 
 // The sums of the tile of at most 128 rows at rows t, columns n0 on.
-template <bool EXPERTS, bool GATED>
+template <bool EXPERTS>
 __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
                                               Sums<1>& acc) {
   const ggk_fp8_args& p = l.a;
   const int nk = (p.k + kStep - 1) / kStep;
-  const Loader<EXPERTS, GATED> loader(l, t, s.slot, n0, wave);
+  const Loader<EXPERTS, false> loader(l, t, s.slot, n0, wave);
   const uint32_t lds = gg::lds_address(s.stages), scales_at = lds + kPlaces * kUnit;
-  const Lane<GATED> lane(lds, wave);
+  const Lane<false> lane(lds, wave);
 
   // Two sets of operands: one is multiplied while the next stage's is read into the other.
   int8v a[2][4], b[2][4];  // [set][16 rows], [set][2 unit + 16 columns]
-  float x_scale[2][4], w_scale[2][2];
+  float x_scale[2][4], w_scale[2];
   float4v part[16];  // results of this stage's instructions, three of them alive
   float4v left[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};  // of the stage before, its last two
   float left_scale = 0.0f;
@@ -226,8 +226,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
     const uint32_t at = scales_of(kt);
 #pragma unroll
     for (int i = 0; i < 4; ++i) x_scale[set][i] = *(const GG_LDS float*)(uintptr_t)(lane.x_scale + at + 256u * i);
-    w_scale[set][0] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at);
-    if constexpr (GATED) w_scale[set][1] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at + 16u);
+    w_scale[set] = *(const GG_LDS float*)(uintptr_t)(lane.w_scale + at);
   };
   auto issue = [&](int kt, uint32_t place, int i) {  // load i (0..5) of a stage; past K zeros, and memory is not touched
     if (i / 2 == 1) {
@@ -258,12 +257,9 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
     constexpr int set = decltype(set_tag)::value, other = 1 - set;
     const uint32_t next = here == 6 * kUnit ? 0 : here + 3 * kUnit;
     if ((kt & 3) == 0 && kt + kScaleSteps < nk) loader.issue_scales(kt / 4 + 1, scales_at + ((kt / 4 + 1) & 1) * kScales);
-    float scale[2][4];
+    float scale[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      scale[0][i] = x_scale[set][i] * w_scale[set][0];
-      scale[1][i] = GATED ? x_scale[set][i] * w_scale[set][1] : scale[0][i];
-    }
+    for (int i = 0; i < 4; ++i) scale[i] = x_scale[set][i] * w_scale[set];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int i = r / 4, n = (i & 1) != 0 ? 3 - r % 4 : r % 4;
@@ -273,7 +269,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
         add_scaled(acc[0][3][0][1 - r], left[r], left_scale);
       } else {
         const int q = r - 2, qi = q / 4, qn = (qi & 1) != 0 ? 3 - q % 4 : q % 4;
-        add_scaled(acc[0][qi][qn / 2][qn % 2], part[q], scale[qn / 2][qi]);
+        add_scaled(acc[0][qi][qn / 2][qn % 2], part[q], scale[qi]);
       }
       if (r < 12 && r % 3 != 2) read(next, other, r / 3 * 2 + r % 3);
       if (r == 12) read_scales(kt + 1, other);
@@ -283,7 +279,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
     }
     left[0] = part[14];
     left[1] = part[15];
-    left_scale = scale[0][3];
+    left_scale = scale[3];
     // The next stage's operands are in every wave's registers, and the one after it has landed.
     gg::wait_lgkmcnt<0>();
     gg::wait_vmcnt<6>();
@@ -412,17 +408,17 @@ __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTi
 }
 
 // The sums of the tile of more rows at rows t, columns n0 on.
-template <bool EXPERTS, bool GATED>
+template <bool EXPERTS>
 __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
                                               Sums<2>& acc) {
   const ggk_fp8_args& p = l.a;
   const int nk = (p.k + kStep - 1) / kStep;
-  const Loader<EXPERTS, GATED> loader(l, t, s.slot, n0, wave);
+  const Loader<EXPERTS, false> loader(l, t, s.slot, n0, wave);
   const uint32_t lds = gg::lds_address(s.stages), scales_at = lds + kPlaces * kUnit;
-  const Lane<GATED> lane(lds, wave);
+  const Lane<false> lane(lds, wave);
 
   int8v a[4], b[2][2];
-  float x_scale[2][4], w_scale[2], w_next[2];  // x's by half of the rows; of the next stage while this one's are used
+  float x_scale[2][4], w_scale, w_next;  // x's by half of the rows; of the next stage while this one's are used
   float4v part[8];      // results of this phase's instructions, three of them alive
   float4v left[2];      // of the phase before, its last two
   float left_scale;
@@ -454,19 +450,17 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   };
   auto read_w_scales = [&](int kt) {
     const uint32_t at = lane.w_scale + scales_of(kt);
-    w_next[0] = *(const GG_LDS float*)(uintptr_t)at;
-    if constexpr (GATED) w_next[1] = *(const GG_LDS float*)(uintptr_t)(at + 16u);
+    w_next = *(const GG_LDS float*)(uintptr_t)at;
   };
   auto next_w_scales = [&]() {
-    w_scale[0] = w_next[0];
-    if constexpr (GATED) w_scale[1] = w_next[1];
+    w_scale = w_next;
   };
   // The 8 instructions of (A half, B unit), rows first, columns back and forth; the sums of the two before last are brought
   // in behind each.  last_half, last_unit: of the phase before.
   auto phase = [&](int half, int unit, int last_half, int last_unit, auto&& issue, auto&& read) {
     float scale[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) scale[i] = x_scale[half][i] * w_scale[GATED ? unit : 0];
+    for (int i = 0; i < 4; ++i) scale[i] = x_scale[half][i] * w_scale;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const int i = r >> 1, n = (i & 1) != 0 ? 1 - (r & 1) : r & 1;
@@ -641,55 +635,49 @@ __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile&
   }
 }
 
-// The 8-bit rows of a gated tile.
-template <bool EXPERTS, bool GELU, int HALVES>
+// The 8-bit rows of a gated tile, of 128 rows.
+template <bool EXPERTS, bool GELU>
 __device__ __forceinline__ void store_rows(const ggk_fp8_args& a, const RowTile& t, const Shared& s, int n0, int wm, int wn,
-                                           Sums<HALVES>& acc) {
+                                           Sums<1>& acc) {
   const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
   // Values stay in the registers of gate's sums; a row's 128 columns lie in 4 lanes of 4 waves.
   constexpr int kLd = 128 + 16;
-  uint32_t* s_most = reinterpret_cast<uint32_t*>(s.stages + kRows * kLd);  // [256][4]
+  uint32_t* s_most = reinterpret_cast<uint32_t*>(s.stages + 128 * kLd);  // [128][4]
   gg::stage_barrier();
 #pragma unroll
-  for (int half = 0; half < HALVES; ++half) {
+  for (int i = 0; i < 4; ++i) {
+    uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t most = 0;
+    for (int n = 0; n < 2; ++n) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = gated<GELU>(acc[half][i][0][n][e], acc[half][i][1][n][e]);
-          if (n0 + 32 * wn + 16 * n + 4 * g + e >= a.n) v = 0.0f;
-          acc[half][i][0][n][e] = v;
-          most = max(most, gg::magnitude_bits(v));
-        }
+      for (int e = 0; e < 4; ++e) {
+        float v = gated<GELU>(acc[0][i][0][n][e], acc[0][i][1][n][e]);
+        if (n0 + 32 * wn + 16 * n + 4 * g + e >= a.n) v = 0.0f;
+        acc[0][i][0][n][e] = v;
+        most = max(most, gg::magnitude_bits(v));
       }
-      most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
-      most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
-      if (g == 0) s_most[(128 * half + 64 * wm + 16 * i + j) * 4 + wn] = most;
     }
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+    if (g == 0) s_most[(64 * wm + 16 * i + j) * 4 + wn] = most;
   }
   gg::stage_barrier();
 #pragma unroll
-  for (int half = 0; half < HALVES; ++half) {
+  for (int i = 0; i < 4; ++i) {
+    const int r = 64 * wm + 16 * i + j;
+    const uint4v most = *reinterpret_cast<const uint4v*>(&s_most[r * 4]);
+    const uint32_t largest = max(max(most.x, most.y), max(most.z, most.w));
+    const float scale = gg::fp8_scale(largest);
+    const gg::Fp8Divisor by(scale, __builtin_bit_cast(float, largest));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 128 * half + 64 * wm + 16 * i + j;
-      const uint4v most = *reinterpret_cast<const uint4v*>(&s_most[r * 4]);
-      const uint32_t largest = max(max(most.x, most.y), max(most.z, most.w));
-      const float scale = gg::fp8_scale(largest);
-      const gg::Fp8Divisor by(scale, __builtin_bit_cast(float, largest));
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float4v v = acc[half][i][0][n];
-        *reinterpret_cast<uint32_t*>(s.stages + r * kLd + 32 * wn + 16 * n + 4 * g) =
-            gg::fp8_numbers(v[0], v[1], v[2], v[3], by);
-      }
-      if (wn == 0 && g == 0 && r < t.rows) {
-        const int slot = EXPERTS ? s.slot[r] : t.first + r;
-        if (slot >= 0) a.y_scales[slot * a.ldys + n0 / kStep] = scale;
-      }
+    for (int n = 0; n < 2; ++n) {
+      const float4v v = acc[0][i][0][n];
+      *reinterpret_cast<uint32_t*>(s.stages + r * kLd + 32 * wn + 16 * n + 4 * g) =
+          gg::fp8_numbers(v[0], v[1], v[2], v[3], by);
+    }
+    if (wn == 0 && g == 0 && r < t.rows) {
+      const int slot = EXPERTS ? s.slot[r] : t.first + r;
+      if (slot >= 0) a.y_scales[slot * a.ldys + n0 / kStep] = scale;
     }
   }
   gg::stage_barrier();
@@ -716,13 +704,13 @@ __device__ __forceinline__ void run_tile(const Launch& l, const RowTile& t, cons
   if constexpr (EXACT) {
     multiply_tile_exact<EXPERTS, GATED>(l, t, s, n0, wave, acc);
   } else {
-    multiply_tile<EXPERTS, GATED>(l, t, s, n0, wave, acc);
+    multiply_tile<EXPERTS>(l, t, s, n0, wave, acc);
   }
   if constexpr (GATED) {
     if (a.gate == GGK_GATE_GELU) {
-      store_rows<EXPERTS, true, HALVES>(a, t, s, n0, wm, wn, acc);
+      store_rows<EXPERTS, true>(a, t, s, n0, wm, wn, acc);
     } else {
-      store_rows<EXPERTS, false, HALVES>(a, t, s, n0, wm, wn, acc);
+      store_rows<EXPERTS, false>(a, t, s, n0, wm, wn, acc);
     }
   } else if constexpr (EXACT) {
     store_tile<EXPERTS, float, HALVES>(a, t, s, n0, wm, wn, acc);
