@@ -103,23 +103,22 @@ __device__ __forceinline__ void store_value(void* y, int type, long long at, flo
   }
 }
 
-// Columns j .. j + 3 of a row at offset `at` (in values); vec: they all exist and start on a multiple of 4 values.
-__device__ __forceinline__ void store4(void* y, int type, long long at, int count, bool vec, const float4v& v) {
-  if (!vec) {
+// Four columns of a row at offset `at` (in values), `count` (1 or more) of them there.
+__device__ __forceinline__ void store4(void* y, int type, long long at, int count, const float4v& v) {
+  if (count < 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 3; ++i) {
       if (i < count) store_value(y, type, at + i, v[i]);
     }
   } else if (type == GGK_TYPE_F32) {
-    *reinterpret_cast<float4v*>(static_cast<float*>(y) + at) = v;
+    *reinterpret_cast<Any16*>(static_cast<float*>(y) + at) = __builtin_bit_cast(uint4v, v);
   } else {
     uint16_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h[i] = type == GGK_TYPE_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
     }
-    *reinterpret_cast<uint2v*>(static_cast<uint16_t*>(y) + at) =
-        uint2v{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
+    *reinterpret_cast<Any8*>(static_cast<uint16_t*>(y) + at) = uint2v{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
   }
 }
 
@@ -138,11 +137,11 @@ __device__ __forceinline__ void store_numbers(const ggk_fp8_args& a, long long r
   const uint2v numbers = {fp8_numbers(v[0], v[1], v[2], v[3], by), fp8_numbers(v[4], v[5], v[6], v[7], by)};
   if (!write || j >= a.n) return;
   unsigned char* y = static_cast<unsigned char*>(a.y) + row * a.ldy + j;
-  if (j + 8 <= a.n && reinterpret_cast<uintptr_t>(y) % 8 == 0) {
-    *reinterpret_cast<uint2v*>(y) = numbers;
+  if (j + 8 <= a.n) {
+    *reinterpret_cast<Any8*>(y) = numbers;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 7; ++i) {
       if (j + i < a.n) y[i] = (unsigned char)(numbers[i / 4] >> (8 * (i % 4)));
     }
   }

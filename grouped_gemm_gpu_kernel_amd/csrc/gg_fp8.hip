@@ -175,7 +175,6 @@ __device__ __forceinline__ void run_item(const ggk_fp8_args& a, const RowTile& t
   const int j = lane % 16, g = lane / 16, wn = wave / F::WK, wk = wave % F::WK;
   float4v sum[F::MT][F::NT];
   multiply_item<F>(a, t, x_row, block0 + wn * (F::COLUMNS / F::WN), block / kXcds, s_bytes + wave * F::DEPTH * F::STEP, sum);
-  const bool vec = a.n % 4 == 0 && (a.ldy % 4 == 0 || a.rows <= 1) && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
   float* s_sum = reinterpret_cast<float*>(s_bytes);  // [WK][16 MT][SUM_LD]
   gg::stage_barrier();
 #pragma unroll
@@ -199,7 +198,7 @@ __device__ __forceinline__ void run_item(const ggk_fp8_args& a, const RowTile& t
       if (column < a.n && slot >= 0) {
         float4v v = total(r, c);
         if (a.row_weights != nullptr) v *= a.row_weights[slot];
-        store4(a.y, a.y_type, slot * a.ldy + column, a.n - column, vec, v);
+        store4(a.y, a.y_type, slot * a.ldy + column, a.n - column, v);
       }
     }
   } else {

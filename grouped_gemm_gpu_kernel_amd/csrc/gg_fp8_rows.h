@@ -7,6 +7,10 @@
 
 namespace gg {
 
+// 16 and 8 bytes that stand anywhere: the memory's instructions take any address, at the price of the lines that they touch.
+typedef uint32_t Any16 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t Any8 __attribute__((ext_vector_type(2), aligned(1)));
+
 constexpr int kFp8Block = 128;
 constexpr float kFp8Largest = 448.0f;
 constexpr float kFp8SmallestScale = 1.17549435e-38f;  // 2^-126: above it 1 / scale is finite

@@ -584,17 +584,17 @@ struct Sixteen {
   static __device__ __forceinline__ int column(int g, int i) { return kTrade ? 16 * (g & 1) + 8 * (g >> 1) : 16 * i + 4 * g; }
 };
 
-// y of a tile: 16 bytes a lane and store; rows that do not start on multiples of 16 bytes by way of LDS, value by value.
+// y of a tile: 16 bytes a lane and store, wherever rows begin; the 16 bytes of a row that n cuts by way of LDS, value by value.
+// (With all of a tile's rows by way of LDS where they do not begin on multiples of 16 bytes, 5076 slots of 16 experts of 288 by
+// 2082 took 56 us, so 28.)
 template <bool EXPERTS, class T, int HALVES>
 __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile& t, const Shared& s, int n0, int wm, int wn,
                                            const Sums<HALVES>& acc) {
   using Four = typename Sixteen<T>::Four;
-  constexpr int kLd = sizeof(T) * 256 + 16;  // bytes of a row in LDS
   constexpr int kEach = 16 / sizeof(T);
-  static_assert(128 * HALVES * kLd <= kPlaces * kUnit, "the tile fits LDS");
   const int lane = gg::opaque_lane(), g = lane >> 4, j = lane & 15;
-  const bool vec = a.n % kEach == 0 && a.ldy % kEach == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
-  if (!vec) gg::stage_barrier();
+  const int columns = min(a.n - n0, 256), whole = columns / kEach * kEach;
+  if (whole < columns) gg::stage_barrier();
 #pragma unroll
   for (int half = 0; half < HALVES; ++half) {
 #pragma unroll
@@ -615,21 +615,18 @@ __device__ __forceinline__ void store_tile(const ggk_fp8_args& a, const RowTile&
 #pragma unroll
         for (int n = 0; n < (int)(sizeof(part.v) / 16); ++n) {
           const int column = 64 * wn + 32 * u + Sixteen<T>::column(g, n);
-          if (!vec) {
-            *reinterpret_cast<uint4v*>(s.stages + r * kLd + sizeof(T) * column) = part.v[n];
-          } else if (slot >= 0 && n0 + column < a.n) {
-            *reinterpret_cast<uint4v*>(y + column) = part.v[n];
-          }
+          if (slot >= 0 && column < whole) *reinterpret_cast<gg::Any16*>(y + column) = part.v[n];
+          if (whole < columns && column == whole) *reinterpret_cast<uint4v*>(s.stages + 16 * r) = part.v[n];
         }
       }
     }
   }
-  if (!vec) {
+  if (whole < columns) {
     gg::stage_barrier();
-    for (int i = threadIdx.x; i < t.rows * 256; i += kThreads) {
-      const int r = i / 256, c = i % 256, slot = EXPERTS ? s.slot[r] : t.first + r;
-      if (slot >= 0 && n0 + c < a.n) {
-        static_cast<T*>(a.y)[slot * a.ldy + n0 + c] = *reinterpret_cast<const T*>(s.stages + r * kLd + sizeof(T) * c);
+    for (int i = threadIdx.x; i < t.rows * kEach; i += kThreads) {
+      const int r = i / kEach, c = whole + i % kEach, slot = EXPERTS ? s.slot[r] : t.first + r;
+      if (slot >= 0 && c < columns) {
+        static_cast<T*>(a.y)[slot * a.ldy + n0 + c] = *reinterpret_cast<const T*>(s.stages + sizeof(T) * i);
       }
     }
   }
@@ -687,8 +684,8 @@ __device__ __forceinline__ void store_rows(const ggk_fp8_args& a, const RowTile&
     if (slot < 0 || column >= a.n) continue;
     const unsigned char* from = s.stages + r * kLd + i % 8 * 16;
     unsigned char* y = static_cast<unsigned char*>(a.y) + slot * a.ldy + column;
-    if (column + 16 <= a.n && reinterpret_cast<uintptr_t>(y) % 16 == 0) {
-      *reinterpret_cast<uint4v*>(y) = *reinterpret_cast<const uint4v*>(from);
+    if (column + 16 <= a.n) {
+      *reinterpret_cast<gg::Any16*>(y) = *reinterpret_cast<const uint4v*>(from);
     } else {
       for (int c = 0; c < 16 && column + c < a.n; ++c) y[c] = from[c];
     }

@@ -36,44 +36,49 @@ struct Type<GGK_TYPE_BF16> {
   using T = __bf16;
 };
 
-// `count` (0 to 8) values from p on; the rest is 0.  VEC: all 8 or none are there, on a multiple of 16 bytes.
-template <class T, bool VEC>
+// `count` (0 to 8) values from p on; the rest is 0.  Rows may begin anywhere: 8 values are moved by instructions of 16 bytes at
+// their type's alignment.  WHOLE: all 8 or none are there (columns in multiples of 8; 8192 rows of 5120 float take 101 us so, 115
+// with the other loop).
+template <class T, bool WHOLE>
 __device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
-  if constexpr (VEC) {
-    uint4v raw[sizeof(T) / 2] = {};
-    if (count > 0) {
+  T t[8] = {};
+  if (WHOLE ? count > 0 : count == 8) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4v*>(p)[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint4v part = reinterpret_cast<const gg::Any16*>(p)[i];
+      __builtin_memcpy(t + i * (16 / sizeof(T)), &part, 16);
     }
-    const T* t = reinterpret_cast<const T*>(raw);
+  } else if (!WHOLE && count > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? (float)p[i] : 0.0f;
+    for (int i = 0; i < 7; ++i) {
+      if (i < count) t[i] = p[i];
+    }
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
 }
 
-template <class T, bool VEC>
+template <class T, bool WHOLE>
 __device__ __forceinline__ void store8(T* p, int count, const float (&v)[8]) {
-  if constexpr (VEC) {
-    uint4v raw[sizeof(T) / 2];
-    T* t = reinterpret_cast<T*>(raw);
+  T t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
-    if (count > 0) {
+  for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
+  if (WHOLE ? count > 0 : count == 8) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4v*>(p)[i] = raw[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      uint4v part;
+      __builtin_memcpy(&part, t + i * (16 / sizeof(T)), 16);
+      reinterpret_cast<gg::Any16*>(p)[i] = part;
     }
-  } else {
+  } else if (!WHOLE && count > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i < count) p[i] = (T)v[i];
+    for (int i = 0; i < 7; ++i) {
+      if (i < count) p[i] = t[i];
     }
   }
 }
 
-template <int TYPE, int WTYPE, int LANES, int CHUNKS, bool VEC>
+template <int TYPE, int WTYPE, int LANES, int CHUNKS, bool WHOLE>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_norm_fp8_args a) {
   using T = typename Type<TYPE>::T;
   using W = typename Type<WTYPE>::T;
@@ -88,14 +93,14 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_nor
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int at = 8 * (c * LANES + lane), count = min(max(a.columns - at, 0), 8);
-    load8<T, VEC>(x + at, count, h[c]);
+    load8<T, WHOLE>(x + at, count, h[c]);
   }
   if (residual != nullptr) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int at = 8 * (c * LANES + lane), count = min(max(a.columns - at, 0), 8);
       float r[8];
-      load8<T, VEC>(residual + at, count, r);
+      load8<T, WHOLE>(residual + at, count, r);
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[c][i] += r[i];
     }
@@ -108,7 +113,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_nor
 #pragma unroll
     for (int i = 0; i < 8; ++i) part = fmaf(h[c][i], h[c][i], part);
     squares += part;
-    if (sum != nullptr) store8<T, VEC>(sum + at, count, h[c]);
+    if (sum != nullptr) store8<T, WHOLE>(sum + at, count, h[c]);
   }
 #pragma unroll
   for (int d = kWave / 2; d > 0; d /= 2) squares += __shfl_xor(squares, d, kWave);
@@ -135,30 +140,30 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_nor
   for (int c = 0; c < CHUNKS; ++c) {
     const int at = 8 * (c * LANES + lane), count = min(max(a.columns - at, 0), 8);
     float w[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
-    if (weight != nullptr) load8<W, VEC>(weight + at, count, w);
+    if (weight != nullptr) load8<W, WHOLE>(weight + at, count, w);
     uint32_t largest = 0;
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = VEC || i < count ? h[c][i] * power * w[i] : 0.0f;  // past the end 0 * power may be NaN
-      if (!VEC || count > 0) largest = max(largest, gg::magnitude_bits(v[i]));
+      v[i] = (WHOLE ? count > 0 : i < count) ? h[c][i] * power * w[i] : 0.0f;  // past the end 0 * power may be NaN
+      largest = max(largest, gg::magnitude_bits(v[i]));
     }
     if (y != nullptr) {
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = v[i] * rest;
-      store8<T, VEC>(y + at, count, out);
+      store8<T, WHOLE>(y + at, count, out);
     }
     const float most = __builtin_bit_cast(float, gg::row_max16(largest));
     const float scale = gg::fp8_scale(gg::magnitude_bits(most * rest));
     const gg::Fp8Divisor by(scale == gg::kFp8SmallestScale ? scale / rest : most * (1.0f / gg::kFp8Largest), most);
     const uint2v numbers = {gg::fp8_numbers(v[0], v[1], v[2], v[3], by),
                             gg::fp8_numbers(v[4], v[5], v[6], v[7], by)};
-    if constexpr (VEC) {
-      if (count > 0) *reinterpret_cast<uint2v*>(q + at) = numbers;
-    } else {
+    if (WHOLE ? count > 0 : count == 8) {
+      *reinterpret_cast<gg::Any8*>(q + at) = numbers;
+    } else if (!WHOLE && count > 0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 7; ++i) {
         if (i < count) q[at + i] = (unsigned char)(numbers[i / 4] >> (8 * (i % 4)));
       }
     }
@@ -166,33 +171,24 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_nor
   }
 }
 
-bool aligned(const void* p, long long ld_bytes, int rows, int to) {
-  return reinterpret_cast<uintptr_t>(p) % to == 0 && (rows <= 1 || ld_bytes % to == 0);
-}
-
-template <int TYPE, int WTYPE, bool VEC>
-hipError_t launch(const ggk_norm_fp8_args& a, hipStream_t stream) {
+template <int TYPE, int WTYPE, bool WHOLE>
+hipError_t launch_rows(const ggk_norm_fp8_args& a, hipStream_t stream) {
   const auto go = [&](auto kernel, int rows, int threads) {
     hipLaunchKernelGGL(kernel, dim3((a.rows + rows - 1) / rows), dim3(threads), 0, stream, a);
     return hipGetLastError();
   };
   const int chunks = (a.columns + 7) / 8;
-  if (chunks <= 64) return go(norm_kernel<TYPE, WTYPE, 64, 1, VEC>, 4, 256);
-  if (chunks <= 256) return go(norm_kernel<TYPE, WTYPE, 64, 4, VEC>, 4, 256);
-  if (chunks <= 512) return go(norm_kernel<TYPE, WTYPE, 256, 2, VEC>, 1, 256);
-  if (chunks <= 1024) return go(norm_kernel<TYPE, WTYPE, 256, 4, VEC>, 1, 256);
-  if (chunks <= 2048) return go(norm_kernel<TYPE, WTYPE, 256, 8, VEC>, 1, 256);
-  return go(norm_kernel<TYPE, WTYPE, 1024, 4, VEC>, 1, 1024);
+  if (chunks <= 64) return go(norm_kernel<TYPE, WTYPE, 64, 1, WHOLE>, 4, 256);
+  if (chunks <= 256) return go(norm_kernel<TYPE, WTYPE, 64, 4, WHOLE>, 4, 256);
+  if (chunks <= 512) return go(norm_kernel<TYPE, WTYPE, 256, 2, WHOLE>, 1, 256);
+  if (chunks <= 1024) return go(norm_kernel<TYPE, WTYPE, 256, 4, WHOLE>, 1, 256);
+  if (chunks <= 2048) return go(norm_kernel<TYPE, WTYPE, 256, 8, WHOLE>, 1, 256);
+  return go(norm_kernel<TYPE, WTYPE, 1024, 4, WHOLE>, 1, 1024);
 }
 
 template <int TYPE, int WTYPE>
-hipError_t launch_aligned(const ggk_norm_fp8_args& a, hipStream_t stream) {
-  const int size = TYPE == GGK_TYPE_F32 ? 4 : 2;
-  const bool vec = a.columns % 8 == 0 && aligned(a.x, a.ldx * size, a.rows, 16) &&
-                   aligned(a.residual, a.ldr * size, a.rows, 16) && aligned(a.weight, 0, 1, 16) &&
-                   aligned(a.q, a.ldq, a.rows, 8) && aligned(a.y, a.ldy * size, a.rows, 16) &&
-                   aligned(a.sum, a.ldsum * size, a.rows, 16);
-  return vec ? launch<TYPE, WTYPE, true>(a, stream) : launch<TYPE, WTYPE, false>(a, stream);
+hipError_t launch(const ggk_norm_fp8_args& a, hipStream_t stream) {
+  return a.columns % 8 == 0 ? launch_rows<TYPE, WTYPE, true>(a, stream) : launch_rows<TYPE, WTYPE, false>(a, stream);
 }
 
 bool is_type(int type) { return type == GGK_TYPE_F32 || type == GGK_TYPE_F16 || type == GGK_TYPE_BF16; }
@@ -223,11 +219,11 @@ extern "C" hipError_t ggk_norm_fp8(const ggk_norm_fp8_args* args, hipStream_t st
   const ggk_norm_fp8_args& a = *args;
   const bool same = a.weight == nullptr || a.weight_type == a.type;
   switch (a.type) {
-    case GGK_TYPE_F32: return launch_aligned<GGK_TYPE_F32, GGK_TYPE_F32>(a, stream);
+    case GGK_TYPE_F32: return launch<GGK_TYPE_F32, GGK_TYPE_F32>(a, stream);
     case GGK_TYPE_F16:
-      return same ? launch_aligned<GGK_TYPE_F16, GGK_TYPE_F16>(a, stream) : launch_aligned<GGK_TYPE_F16, GGK_TYPE_F32>(a, stream);
+      return same ? launch<GGK_TYPE_F16, GGK_TYPE_F16>(a, stream) : launch<GGK_TYPE_F16, GGK_TYPE_F32>(a, stream);
     default:
-      return same ? launch_aligned<GGK_TYPE_BF16, GGK_TYPE_BF16>(a, stream)
-                  : launch_aligned<GGK_TYPE_BF16, GGK_TYPE_F32>(a, stream);
+      return same ? launch<GGK_TYPE_BF16, GGK_TYPE_BF16>(a, stream)
+                  : launch<GGK_TYPE_BF16, GGK_TYPE_F32>(a, stream);
   }
 }
