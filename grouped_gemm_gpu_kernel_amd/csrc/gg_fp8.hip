@@ -97,7 +97,8 @@ __device__ __forceinline__ void multiply_item(const ggk_fp8_args& a, const RowTi
   if (F::SL == 1 && lane >= 32) xs = ws;
 
   // In step, the waves would all read the same columns at a time, and rows a power of two apart lie in a few channels of
-  // the L2: every wave begins with another of its steps and goes on around the end.
+  // the L2: every wave begins with another of its steps and goes on around the end, and so do neighbouring workgroups of an XCD
+  // and XCDs.
   const int first = (turn + wave / F::WK * max(mine / F::WN, 1)) % max(mine, 1);
   auto issue = [&](int i) {  // the wave's step i into its place of the ring
     const int turned = i + first < mine ? i + first : i + first - mine, step = turned * F::WK + wk, k0 = step * kStep;
@@ -174,7 +175,7 @@ __device__ __forceinline__ void run_item(const ggk_fp8_args& a, const RowTile& t
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int j = lane % 16, g = lane / 16, wn = wave / F::WK, wk = wave % F::WK;
   float4v sum[F::MT][F::NT];
-  multiply_item<F>(a, t, x_row, block0 + wn * (F::COLUMNS / F::WN), block / kXcds, s_bytes + wave * F::DEPTH * F::STEP, sum);
+  multiply_item<F>(a, t, x_row, block0 + wn * (F::COLUMNS / F::WN), block + (int)(blockIdx.x % kXcds), s_bytes + wave * F::DEPTH * F::STEP, sum);
   float* s_sum = reinterpret_cast<float*>(s_bytes);  // [WK][16 MT][SUM_LD]
   gg::stage_barrier();
 #pragma unroll
@@ -241,12 +242,12 @@ __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::B
   const ggk_fp8_args& a = l.a;
   __shared__ alignas(128) unsigned char s_bytes[F::BYTES];
   if constexpr (!EXPERTS) {
-    // Neighbouring workgroups go to different XCDs: a column block's row tiles follow each other on one, so that its L2 has
-    // the weights for all of them.
-    const int tiles = (a.rows + F::R - 1) / F::R, in_xcd = blockIdx.x / kXcds;
-    const int block = in_xcd / l.tiles * kXcds + blockIdx.x % kXcds;
-    if (block >= l.blocks) return;
-    for (int tile = in_xcd % l.tiles; tile < tiles; tile += l.tiles) {
+    // Neighbouring workgroups go to different XCDs: each takes an eighth of the items in the order of column blocks, so that the
+    // row tiles of a block follow each other and its L2 has the weights for all of them.
+    const int tiles = (a.rows + F::R - 1) / F::R, items = l.blocks * l.tiles, share = (items + kXcds - 1) / kXcds;
+    const int item = (int)(blockIdx.x % kXcds) * share + (int)(blockIdx.x / kXcds), block = item / l.tiles;
+    if (item >= items) return;
+    for (int tile = item % l.tiles; tile < tiles; tile += l.tiles) {
       const RowTile t{0, tile * F::R, min(F::R, a.rows - tile * F::R)};
       run_item<F, false>(a, t, nullptr, nullptr, block, s_bytes);
       gg::stage_barrier();
@@ -286,9 +287,9 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
     const long long items = tiles * l.blocks, most = kCus * (F::BYTES > 64 * 1024 ? 1 : 2);
     grid = items < most ? items : most;
   } else {
-    const long long columns = (l.blocks + kXcds - 1) / kXcds * kXcds, most = (1 << 30) / columns;
+    const long long most = (1 << 30) / l.blocks;
     l.tiles = (int)(tiles < most ? tiles : most);
-    grid = columns * l.tiles;
+    grid = ((long long)l.blocks * l.tiles + kXcds - 1) / kXcds * kXcds;
   }
   hipLaunchKernelGGL((fp8_stream_kernel<F, EXPERTS>), dim3((unsigned)grid), dim3(F::THREADS), 0, stream, l);
   return hipGetLastError();
