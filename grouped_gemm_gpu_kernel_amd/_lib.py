@@ -204,7 +204,7 @@ class GGKFp8Args(ctypes.Structure):
         ("up_scales", ctypes.c_void_p), ("ldus", ctypes.c_longlong), ("stride_us", ctypes.c_longlong),
         ("counts", ctypes.c_void_p), ("order", ctypes.c_void_p), ("row_weights", ctypes.c_void_p),
         ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong), ("y_type", ctypes.c_int),
-        ("y_scales", ctypes.c_void_p), ("ldys", ctypes.c_longlong),
+        ("y_scales", ctypes.c_void_p), ("ldys", ctypes.c_longlong), ("workspace", ctypes.c_void_p),
     ]
 
 
@@ -281,6 +281,7 @@ SIGNATURES = {
     "ggk_norm_fp8_check": (_i, [_P(GGKNormFp8Args)]),
     "ggk_norm_fp8": (_i, [_P(GGKNormFp8Args), _vp]),
     "ggk_fp8_check": (_i, [_P(GGKFp8Args)]),
+    "ggk_fp8_workspace": (_i, [_P(GGKFp8Args), _P(ctypes.c_longlong)]),
     "ggk_fp8_multiply": (_i, [_P(GGKFp8Args), _vp]),
     "ggk_launch_grouped_device": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp]),
     "ggk_launch_grouped_device_done": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, c_int_p, _vp]),

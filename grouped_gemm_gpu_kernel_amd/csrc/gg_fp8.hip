@@ -25,9 +25,10 @@ using gg::kWave;
 constexpr int kCus = 256, kXcds = 8;
 
 struct Launch {
-  ggk_fp8_args a;
-  int blocks;  // of columns
-  int tiles;   // of rows that the grid has (one matrix)
+  ggk_fp8_args a, second;  // a second product, of the same rows, after the first one's column blocks (one matrix, no gate)
+  int blocks;              // of columns
+  int blocks_of_a;         // of those, the first product's
+  int tiles;               // of rows that the grid has (one matrix)
 };
 
 // R rows of x (8, 16, 32, 64) by WN waves of NT tiles of 16 columns (with a gate: half of them gate, half up), WK waves
@@ -240,7 +241,7 @@ __device__ __forceinline__ void clear_item(const ggk_fp8_args& a, const RowTile&
 template <class F, bool EXPERTS>
 __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::BYTES <= 80 * 1024 ? F::WAVES / 2 : F::WAVES / 4) void fp8_stream_kernel(Launch l) {
   const ggk_fp8_args& a = l.a;
-  __shared__ alignas(128) unsigned char s_bytes[F::BYTES];
+  __shared__ alignas(128) unsigned char s_bytes[F::BYTES];  // each wave's ring, then the sums
   if constexpr (!EXPERTS) {
     // Neighbouring workgroups go to different XCDs: each takes an eighth of the items in the order of column blocks, so that the
     // row tiles of a block follow each other and its L2 has the weights for all of them.
@@ -249,7 +250,8 @@ __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::B
     if (item >= items) return;
     for (int tile = item % l.tiles; tile < tiles; tile += l.tiles) {
       const RowTile t{0, tile * F::R, min(F::R, a.rows - tile * F::R)};
-      run_item<F, false>(a, t, nullptr, nullptr, block, s_bytes);
+      const bool first = block < l.blocks_of_a;
+      run_item<F, false>(first ? l.a : l.second, t, nullptr, nullptr, first ? block : block - l.blocks_of_a, s_bytes);
       gg::stage_barrier();
     }
   } else {
@@ -278,9 +280,31 @@ __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::B
   }
 }
 
+// The 8-bit rows of gated products in a workspace, [2][rows][ld]: 16 lanes a block of a row.
+__global__ __launch_bounds__(256) void fp8_gate_kernel(ggk_fp8_args a, long long ld) {
+  const long long blocks = (a.n + kStep - 1) / kStep, all = a.rows * blocks;
+  const long long at = (long long)blockIdx.x * 16 + threadIdx.x / 16, of = at < all ? at : all - 1, row = of / blocks;
+  const int j = (int)(of % blocks) * kStep + threadIdx.x % 16 * 8;
+  const float* gate = a.workspace + row * ld + j;
+  const float* up = gate + a.rows * ld;
+  float v[8];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float4v p = {0.0f, 0.0f, 0.0f, 0.0f}, u = p;
+    if (j + 4 * half < ld) {
+      p = reinterpret_cast<const float4v*>(gate)[half];
+      u = reinterpret_cast<const float4v*>(up)[half];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[4 * half + e] = a.gate == GGK_GATE_GELU ? gated<true>(p[e], u[e]) : gated<false>(p[e], u[e]);
+  }
+  store_numbers(a, row, j, v, at < all);
+}
+
 template <class F, bool EXPERTS>
-hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
-  Launch l{a, (a.n + F::COLUMNS - 1) / F::COLUMNS, 0};
+hipError_t launch(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
+  const int blocks = (a.n + F::COLUMNS - 1) / F::COLUMNS;
+  Launch l{a, second != nullptr ? *second : a, second != nullptr ? 2 * blocks : blocks, blocks, 0};
   const long long tiles = (a.rows + F::R - 1) / F::R + (EXPERTS ? (a.rows < a.experts + 1 ? a.rows : a.experts + 1) : 0);
   long long grid;
   if (EXPERTS) {
@@ -295,13 +319,44 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// What a call takes in the form for more than 16 rows, in us: what the busiest CU gets, workgroups of 32 rows by 32 columns,
-// two on a CU, or by 128, one.
+// What a plain call with n columns takes, in us: what the busiest CU gets, workgroups of 8 or 16 rows by 16 columns, or of 32 by 32,
+// two on a CU.
+double estimate_rows(const ggk_fp8_args& a, double n) {
+  const double steps = a.k / 128.0;
+  if (a.rows <= 16) return 4 + ceil(ceil(n / 16) / (2 * kCus)) * (1 + 0.08 * steps);
+  return 4 + ceil(row_tiles(a, 32) * ceil(n / 32) / (2 * kCus)) * (1.3 + 0.15 * steps);
+}
+
+// Gated products of 16 rows at once where every CU can get its own tile, else of 32.  us of the two: 32 rows of 4096 by 14336
+// 36, 48, 128 of 4096 by 4096 25.5, 30; 64 rows of 4096 by 14336 62, 45, 32 of 8192 by 28672 133, 108.
+bool has_own_tiles(const ggk_fp8_args& a) { return row_tiles(a, 16) * ceil(a.n / 128.0) <= kCus; }
+
+// What a call takes here, in us; gated workgroups are alone on a CU.
 double estimate_few(const ggk_fp8_args& a) {
-  const double tiles = row_tiles(a, 32), steps = a.k / 128.0;
-  if (a.gate != GGK_GATE_NONE) return 5 + ceil(tiles * ceil(a.n / 128.0) / kCus) * (1 + 1.1 * steps);
-  if (a.experts > 0) return 5 + ceil(tiles * ceil(a.n / 128.0) / kCus) * 0.6 * steps;
-  return 4 + ceil(tiles * ceil(a.n / 32.0) / (2 * kCus)) * (1.3 + 0.15 * steps);
+  const double items = row_tiles(a, 32) * ceil(a.n / 128.0), rounds = ceil(items / kCus), steps = a.k / 128.0;
+  if (a.gate == GGK_GATE_NONE) return a.experts > 0 ? 5 + rounds * 0.6 * steps : estimate_rows(a, a.n);
+  if (a.experts > 0) return 5 + rounds * (1 + 1.1 * steps);
+  const double cus = has_own_tiles(a) ? 0.62 * steps : rounds * (1 + (rounds > 1 ? 1.05 : 0.85) * steps), memory = 2.0 * a.n * a.k / 4.5e6;
+  return 4.5 + (cus > memory ? cus : memory);
+}
+
+// One matrix, or two of one shape: y and second's from the same rows.
+hipError_t multiply_rows(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
+  const bool exact = a.y_type == GGK_TYPE_F32;
+  const long long n = second != nullptr ? 2ll * a.n : a.n;
+  if (a.rows <= 8) return launch<Form<8, 1, 1, 8, 2, false, true>, false>(a, stream, second);
+  if (a.rows <= 16) {
+    return n >= 8192 ? launch<Form<16, 1, 2, 4, 2, false, true>, false>(a, stream, second)
+                       : launch<Form<16, 1, 1, 8, 2, false, true>, false>(a, stream, second);
+  }
+  // 64 rows at once where their blocks of 64 columns fill the CUs, else 32 twice.  us of the two: 64 rows of 8192 by 28672
+  // 59.5, 72.7, of 4096 by 16384 16.4, 16.8, in float 17.6, 19.3; of 4096 by 12288 15.6, 13.5, of 8192 by 8192 24, 17.
+  if (a.rows > 32 && a.rows <= 64 && (n + 63) / 64 >= kCus / 8 * 7) {
+    return exact ? launch<Form<64, 4, 1, 4, 2, false, true>, false>(a, stream, second)
+                 : launch<Form<64, 4, 1, 4, 2, false, false>, false>(a, stream, second);
+  }
+  if (exact) return launch<Form<32, 2, 1, 4, 2, false, true>, false>(a, stream, second);
+  return launch<Form<32, 2, 1, 4, 2, false, false>, false>(a, stream, second);
 }
 
 template <bool EXPERTS>
@@ -317,25 +372,40 @@ hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
     return launch<Form<32, 2, 4, 2, 2, false, false>, true>(a, stream);
   } else if (a.gate != GGK_GATE_NONE) {
     if (a.rows <= 8) return launch<Form<8, 4, 4, 1, 4, true, true>, false>(a, stream);
-    // 16 rows at once where every CU can get its own tile, else 32.  us of the two: 32 rows of 4096 by 14336 36, 48, 128 of
-    // 4096 by 4096 25.5, 30; 64 rows of 4096 by 14336 62, 45, 32 of 8192 by 28672 133, 108.
-    if (row_tiles(a, 16) * ceil(a.n / 128.0) <= kCus) return launch<Form<16, 2, 8, 1, 3, true, true>, false>(a, stream);
+    if (has_own_tiles(a)) return launch<Form<16, 2, 8, 1, 3, true, true>, false>(a, stream);
     return launch<Form<32, 2, 8, 1, 2, true, true>, false>(a, stream);
   } else {
-    if (a.rows <= 8) return launch<Form<8, 1, 1, 8, 2, false, true>, false>(a, stream);
-    if (a.rows <= 16) {
-      return a.n >= 8192 ? launch<Form<16, 1, 2, 4, 2, false, true>, false>(a, stream)
-                         : launch<Form<16, 1, 1, 8, 2, false, true>, false>(a, stream);
-    }
-    // 64 rows at once where their blocks of 64 columns fill the CUs, else 32 twice.  us of the two: 64 rows of 8192 by 28672
-    // 59.5, 72.7, of 4096 by 16384 16.4, 16.8, in float 17.6, 19.3; of 4096 by 12288 15.6, 13.5, of 8192 by 8192 24, 17.
-    if (a.rows > 32 && a.rows <= 64 && (a.n + 63) / 64 >= kCus / 8 * 7) {
-      return exact ? launch<Form<64, 4, 1, 4, 2, false, true>, false>(a, stream)
-                   : launch<Form<64, 4, 1, 4, 2, false, false>, false>(a, stream);
-    }
-    if (exact) return launch<Form<32, 2, 1, 4, 2, false, true>, false>(a, stream);
-    return launch<Form<32, 2, 1, 4, 2, false, false>, false>(a, stream);
+    return multiply_rows(a, stream);
   }
+}
+
+// Gated products as both plain products, whose workgroups take 16 or 32 columns and share K, and their rows in a second launch:
+// a block of an 8-bit row needs the largest of 128 columns, and so few workgroups cannot bring in the weights as fast.  us by one
+// launch and by two: 1 row of 4096 by 14336 28.6, 25.3, by 2048 24.7, 9.3; 42 of 13280 by 1666 86, 22; 256 of 4096 by 1792 25.6,
+// 22.3; 1 of 512 by 512 6.3, 9.4; 512 of 4096 by 1792 31, 34.6; 7267 of 480 by 246 15.7, 27.
+long long pair_ld(const ggk_fp8_args& a) { return (a.n + 3) / 4 * 4; }
+bool as_pair(const ggk_fp8_args& a) {
+  if (a.gate == GGK_GATE_NONE || a.experts > 0 || a.rows == 0 || a.n == 0) return false;
+  const double cus = estimate_rows(a, 2.0 * a.n) - 4, memory = 2.0 * a.n * a.k / 5.5e6;
+  const double two = 6 + (cus > memory ? cus : memory) + 16.0 * a.rows * a.n / 4e6, pair = two > 9.5 ? two : 9.5;
+  return pair < estimate_few(a) && !(tiles_take(a) && estimate_tiles(a) <= 1.15 * pair);
+}
+hipError_t multiply_pair(const ggk_fp8_args& a, hipStream_t stream) {
+  const long long ld = pair_ld(a), blocks = (a.n + kStep - 1) / kStep;
+  ggk_fp8_args gate = a;
+  gate.gate = GGK_GATE_NONE;
+  gate.y = a.workspace;
+  gate.ldy = ld;
+  gate.y_type = GGK_TYPE_F32;
+  ggk_fp8_args up = gate;
+  up.w = a.up;
+  up.ldw = a.ldu;
+  up.w_scales = a.up_scales;
+  up.ldws = a.ldus;
+  up.y = a.workspace + a.rows * ld;
+  if (const hipError_t st = multiply_rows(gate, stream, &up); st != hipSuccess) return st;
+  hipLaunchKernelGGL(fp8_gate_kernel, dim3((unsigned)((a.rows * blocks + 15) / 16)), dim3(256), 0, stream, a, ld);
+  return hipGetLastError();
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -370,6 +440,7 @@ extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
       (a.rows > 1 && (a.ldy < a.n || (gate && a.ldys < blocks_n)))) {
     return hipErrorInvalidValue;
   }
+  if (!aligned16(a.workspace)) return hipErrorInvalidValue;
   if (a.rows > 0 && a.n > 0) {
     if (a.x == nullptr || a.x_scales == nullptr || a.w == nullptr || a.w_scales == nullptr || a.y == nullptr ||
         (gate && (a.up == nullptr || a.up_scales == nullptr || a.y_scales == nullptr)) ||
@@ -380,10 +451,17 @@ extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
   return hipSuccess;
 }
 
+extern "C" hipError_t ggk_fp8_workspace(const ggk_fp8_args* args, long long* floats) {
+  const hipError_t st = floats == nullptr ? hipErrorInvalidValue : ggk_fp8_check(args);
+  if (st == hipSuccess) *floats = as_pair(*args) ? 2 * args->rows * pair_ld(*args) : 0;
+  return st;
+}
+
 extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t stream) {
   const hipError_t st = ggk_fp8_check(args);
   if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
   const ggk_fp8_args& a = *args;
+  if (a.workspace != nullptr && as_pair(a)) return multiply_pair(a, stream);
   // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 512 rows of 2048 by 2048 10, 20,
   // 2048 rows 35, 21; 128 of 8192 by 8192 29, 49, 512 103, 56; 16 experts of 1024 by 2048, 512 slots 15, 18, 2048 slots 29,
   // 20, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 256 slots 479, 463, 2048 slots 972, 751.

@@ -515,6 +515,13 @@ py::object fp8_call(const Tensor& x, const Tensor& x_scales, const Tensor& w, co
     a.y = y.mutable_data_ptr();
     a.ldy = n;
     a.y_type = type_of(out_type);
+    Tensor workspace;  // goes back to the allocator in the stream's order
+    long long floats = 0;
+    if (const int status = ggk_fp8_workspace(&a, &floats); status != 0) return py::int_(status);
+    if (floats > 0) {
+      workspace = at::empty({floats}, like_x.dtype(at::kFloat));
+      a.workspace = workspace.mutable_data_ptr<float>();
+    }
     const int status = launch(ggk_fp8_multiply, a, device);
     if (status != 0) return py::int_(status);
   }

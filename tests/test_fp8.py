@@ -203,6 +203,20 @@ def test_product_arguments_are_checked_on_the_host(over, status):
     assert _lib.lib().ggk_fp8_check(None) == 1 and _lib.lib().ggk_fp8_multiply(None, None) == 1
 
 
+@pytest.mark.parametrize("over,floats", [
+    ({}, 0), (MOE, 0), ({**MOE, **GATE, "stride_u": 200 * 272, "stride_us": 6}, 0), ({**GATE, "up": None}, 0), (GATE, 0),
+    ({**GATE, "k": 4096, "ldx": 4096, "ldw": 4096, "ldu": 4096, "ldxs": 32, "ldws": 32, "ldus": 32}, 2 * 4 * 200),
+    ({**GATE, "n": 199, "k": 4096, "ldx": 4096, "ldw": 4096, "ldu": 4096, "ldxs": 32, "ldws": 32, "ldus": 32}, 2 * 4 * 200)])
+def test_workspace_of_gated_calls(over, floats):
+    args, got = _lib.GGKFp8Args(**{**BASE, **over}), ctypes.c_longlong(-1)
+    status = _lib.lib().ggk_fp8_check(ctypes.byref(args))
+    assert _lib.lib().ggk_fp8_workspace(ctypes.byref(args), ctypes.byref(got)) == status
+    assert got.value == (-1 if status else floats)
+    assert _lib.lib().ggk_fp8_workspace(None, ctypes.byref(got)) == 1 and _lib.lib().ggk_fp8_workspace(ctypes.byref(args), None) == 1
+    args.workspace = 0x1008
+    assert _lib.lib().ggk_fp8_check(ctypes.byref(args)) == 1
+
+
 def _fake(*shape, dtype=torch.float32, device="cuda:0"):
     return torch.empty(*shape, dtype=dtype, device=device)
 
@@ -466,6 +480,68 @@ def test_gated(torch_cuda, activation, m, k, n):
     x, gate, up = rows_of(m, k, m + n), matrix_of((), n, k, 7 * k + n), matrix_of((), n, k, 9 * k + n)
     out = torch_ops.fp8_gated(*x, *gate, *up, activation=activation)
     check_gated(out, row_values(*x), matrix_values(*gate), matrix_values(*up), activation)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 520), (7, 8192, 129), (13, 2080, 300), (50, 4096, 257), (64, 2064, 7171), (200, 2064, 389)])
+def test_gated_with_and_without_a_workspace(torch_cuda, m, k, n, activation):
+    """One launch, or both products into a workspace and their rows in a second; nothing past the workspace is written, nor to
+    one that the call does not want (64 rows of many columns)."""
+    x, gate, up = rows_of(m, k, m + n), matrix_of((), n, k, 7 * k + n), matrix_of((), n, k, 9 * k + n)
+    values = row_values(*x), matrix_values(*gate), matrix_values(*up)
+    check_gated(torch_ops.fp8_gated(*x, *gate, *up, activation=activation), *values, activation)
+    for with_it in (False, True):
+        y = torch.zeros(m, n, dtype=torch.uint8, device="cuda")
+        scales = torch.zeros(m, blocks(n), device="cuda")
+        args = _lib.GGKFp8Args(
+            rows=m, x_rows=m, n=n, k=k, gate=1 if activation == "silu" else 2, x=x[0].data_ptr(), ldx=k, x_scales=x[1].data_ptr(),
+            ldxs=blocks(k), w=gate[0].data_ptr(), ldw=k, w_scales=gate[1].data_ptr(), ldws=blocks(k), up=up[0].data_ptr(), ldu=k,
+            up_scales=up[1].data_ptr(), ldus=blocks(k), y=y.data_ptr(), ldy=n, y_scales=scales.data_ptr(), ldys=blocks(n))
+        wanted = ctypes.c_longlong(-1)
+        assert _lib.lib().ggk_fp8_workspace(ctypes.byref(args), ctypes.byref(wanted)) == 0
+        floats = wanted.value
+        assert floats == (0 if m == 64 else 2 * m * ((n + 3) // 4 * 4))
+        workspace = torch.full((floats + 64,), 77.0, device="cuda")
+        if with_it:
+            args.workspace = workspace.data_ptr()
+        assert _lib.lib().ggk_fp8_multiply(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == 0
+        check_gated(torch_ops.Fp8Rows(y.view(FP8), scales), *values, activation)
+        assert (workspace[floats if with_it else 0:] == 77).all()
+
+
+@pytest.mark.gpu
+def test_gated_on_streams_and_in_a_graph(torch_cuda):
+    """Calls that use a workspace, several at a time."""
+    m, k, n = 5, 4096, 700
+    gate, up = matrix_of((), n, k, 1), matrix_of((), n, k, 2)
+    inputs = [rows_of(m, k, 10 + i) for i in range(4)]
+
+    def call(x):
+        out = torch_ops.fp8_gated(*x, *gate, *up)
+        return out.q.view(torch.uint8), out.scales
+
+    eager = [call(x) for x in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    for _ in range(5):
+        got = []
+        for x, stream in zip(inputs, streams):
+            with torch.cuda.stream(stream):
+                got.append(call(x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for a, b in zip(got, eager) for p, q in zip(a, b))
+    x = tuple(t.clone() for t in inputs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, again = call(x), call(x)
+    for i in (2, 0, 3, 1):
+        x[0].copy_(inputs[i][0])
+        x[1].copy_(inputs[i][1])
+        graph.replay()
+        assert all(torch.equal(p, q) for p, q in zip(out, eager[i])) and all(torch.equal(p, q) for p, q in zip(again, eager[i]))
+        call(inputs[3 - i])
+        torch.cuda.synchronize()
 
 
 @pytest.mark.gpu
