@@ -5,7 +5,8 @@
 //
 // With few rows the weights' bytes are what counts.  Every wave streams its own columns through a ring of steps of its
 // own in LDS, loaded there directly, several steps ahead, with x's rows and the scales of the same step beside them: no
-// wave waits for another until its sums are whole.
+// wave waits for another until its sums are whole.  1 row of 4096 by 14336 takes 11.5 us, 5.0 TB/s with the launch; 61 rows in
+// float 17.4; 1 row gated 25.2, by two launches (below).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -383,9 +384,10 @@ hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
 // a block of an 8-bit row needs the largest of 128 columns, and so few workgroups cannot bring in the weights as fast.  us by one
 // launch and by two: 1 row of 4096 by 14336 28.6, 25.3, by 2048 24.7, 9.3; 42 of 13280 by 1666 86, 22; 256 of 4096 by 1792 25.6,
 // 22.3; 1 of 512 by 512 6.3, 9.4; 512 of 4096 by 1792 31, 34.6; 7267 of 480 by 246 15.7, 27.
+constexpr long long kMostOfPair = 1 << 24;  // values of either product: 128 MB of workspace at most
 long long pair_ld(const ggk_fp8_args& a) { return (a.n + 3) / 4 * 4; }
 bool as_pair(const ggk_fp8_args& a) {
-  if (a.gate == GGK_GATE_NONE || a.experts > 0 || a.rows == 0 || a.n == 0) return false;
+  if (a.gate == GGK_GATE_NONE || a.experts > 0 || a.rows == 0 || a.n == 0 || a.rows * pair_ld(a) > kMostOfPair) return false;
   const double cus = estimate_rows(a, 2.0 * a.n) - 4, memory = 2.0 * a.n * a.k / 5.5e6;
   const double two = 6 + (cus > memory ? cus : memory) + 16.0 * a.rows * a.n / 4e6, pair = two > 9.5 ? two : 9.5;
   return pair < estimate_few(a) && !(tiles_take(a) && estimate_tiles(a) <= 1.15 * pair);
@@ -453,7 +455,7 @@ extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
 
 extern "C" hipError_t ggk_fp8_workspace(const ggk_fp8_args* args, long long* floats) {
   const hipError_t st = floats == nullptr ? hipErrorInvalidValue : ggk_fp8_check(args);
-  if (st == hipSuccess) *floats = as_pair(*args) ? 2 * args->rows * pair_ld(*args) : 0;
+  if (st == hipSuccess) *floats = as_pair(*args) ? 2ll * args->rows * pair_ld(*args) : 0;
   return st;
 }
 

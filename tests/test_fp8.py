@@ -206,6 +206,9 @@ def test_product_arguments_are_checked_on_the_host(over, status):
 @pytest.mark.parametrize("over,floats", [
     ({}, 0), (MOE, 0), ({**MOE, **GATE, "stride_u": 200 * 272, "stride_us": 6}, 0), ({**GATE, "up": None}, 0), (GATE, 0),
     ({**GATE, "k": 4096, "ldx": 4096, "ldw": 4096, "ldu": 4096, "ldxs": 32, "ldws": 32, "ldus": 32}, 2 * 4 * 200),
+    ({**GATE, "rows": 1 << 24, "x_rows": 1 << 24, "n": 1, "k": 4096, "ldx": 4096, "ldxs": 32, "ldws": 32, "ldus": 32, "ldw": 4096,
+      "ldu": 4096}, 0), ({**GATE, "rows": 1 << 22, "x_rows": 1 << 22, "n": 1, "k": 4096, "ldx": 4096, "ldxs": 32, "ldws": 32, "ldus": 32,
+                         "ldw": 4096, "ldu": 4096}, 1 << 25),
     ({**GATE, "n": 199, "k": 4096, "ldx": 4096, "ldw": 4096, "ldu": 4096, "ldxs": 32, "ldws": 32, "ldus": 32}, 2 * 4 * 200)])
 def test_workspace_of_gated_calls(over, floats):
     args, got = _lib.GGKFp8Args(**{**BASE, **over}), ctypes.c_longlong(-1)
