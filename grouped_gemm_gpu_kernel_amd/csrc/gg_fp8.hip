@@ -321,10 +321,11 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args*
 }
 
 // What a plain call with n columns takes, in us: what the busiest CU gets, workgroups of 8 or 16 rows by 16 columns, or of 32 by 32,
-// two on a CU.
+// two on a CU; of 32 by 16 where one is enough.
 double estimate_rows(const ggk_fp8_args& a, double n) {
   const double steps = a.k / 128.0;
   if (a.rows <= 16) return 4 + ceil(ceil(n / 16) / (2 * kCus)) * (1 + 0.08 * steps);
+  if (row_tiles(a, 32) * ceil(n / 16) <= kCus) return 5 + 0.075 * steps;
   return 4 + ceil(row_tiles(a, 32) * ceil(n / 32) / (2 * kCus)) * (1.3 + 0.15 * steps);
 }
 
@@ -355,6 +356,12 @@ hipError_t multiply_rows(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp
   if (a.rows > 32 && a.rows <= 64 && (n + 63) / 64 >= kCus / 8 * 7) {
     return exact ? launch<Form<64, 4, 1, 4, 2, false, true>, false>(a, stream, second)
                  : launch<Form<64, 4, 1, 4, 2, false, false>, false>(a, stream, second);
+  }
+  // 16 columns with K shared by 8 waves where every CU can get its own, else 32 by 4.  us of the two: 128 rows of 8192 by 1024
+  // 8.9, 10, 32 rows 7.2, 9.7, in float 8.3, 12; 32 of 14336 by 4096 14.2, 15.5; 64 of 4096 by 4096 9.9, 7.0.
+  if (row_tiles(a, 32) * ceil(n / 16.0) <= kCus) {
+    return exact ? launch<Form<32, 1, 1, 8, 2, false, true>, false>(a, stream, second)
+                 : launch<Form<32, 1, 1, 8, 2, false, false>, false>(a, stream, second);
   }
   if (exact) return launch<Form<32, 2, 1, 4, 2, false, true>, false>(a, stream, second);
   return launch<Form<32, 2, 1, 4, 2, false, false>, false>(a, stream, second);
