@@ -321,12 +321,15 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args*
 }
 
 // What a plain call with n columns takes, in us: what the busiest CU gets, workgroups of 8 or 16 rows by 16 columns, or of 32 by 32,
-// two on a CU; of 32 by 16 where one is enough.
+// two on a CU; of 32 by 16 where one is enough.  Where x is larger than an XCD's L2, its rows come from beyond it for every column
+// block.
 double estimate_rows(const ggk_fp8_args& a, double n) {
   const double steps = a.k / 128.0;
   if (a.rows <= 16) return 4 + ceil(ceil(n / 16) / (2 * kCus)) * (1 + 0.08 * steps);
   if (row_tiles(a, 32) * ceil(n / 16) <= kCus) return 5 + 0.075 * steps;
-  return 4 + ceil(row_tiles(a, 32) * ceil(n / 32) / (2 * kCus)) * (1.3 + 0.15 * steps);
+  const double in_l2 = (double)a.rows * a.k / 4e6, more = in_l2 < 1 ? 1 : in_l2 > 2 ? 2 : in_l2;
+  const double step = (a.y_type == GGK_TYPE_F32 || a.gate != GGK_GATE_NONE ? 0.19 : 0.15) * more;
+  return 4 + ceil(row_tiles(a, 32) * ceil(n / 32) / (2 * kCus)) * (1.3 + step * steps);
 }
 
 // Gated products of 16 rows at once where every CU can get its own tile, else of 32.  us of the two: 32 rows of 4096 by 14336
@@ -337,8 +340,9 @@ bool has_own_tiles(const ggk_fp8_args& a) { return row_tiles(a, 16) * ceil(a.n /
 double estimate_few(const ggk_fp8_args& a) {
   const double items = row_tiles(a, 32) * ceil(a.n / 128.0), rounds = ceil(items / kCus), steps = a.k / 128.0;
   if (a.gate == GGK_GATE_NONE) return a.experts > 0 ? 5 + rounds * 0.6 * steps : estimate_rows(a, a.n);
-  if (a.experts > 0) return 5 + rounds * (1 + 1.1 * steps);
-  const double cus = has_own_tiles(a) ? 0.62 * steps : rounds * (1 + (rounds > 1 ? 1.05 : 0.85) * steps), memory = 2.0 * a.n * a.k / 4.5e6;
+  if (a.experts > 0) return 5 + rounds * (2.5 + 1.15 * steps);
+  const double cus = has_own_tiles(a) ? 0.62 * steps : rounds > 1 ? rounds * (2 + 1.05 * steps) : 1 + 0.85 * steps,
+               memory = 2.0 * a.n * a.k / 4.5e6;
   return 4.5 + (cus > memory ? cus : memory);
 }
 
@@ -397,7 +401,7 @@ bool as_pair(const ggk_fp8_args& a) {
   if (a.gate == GGK_GATE_NONE || a.experts > 0 || a.rows == 0 || a.n == 0 || a.rows * pair_ld(a) > kMostOfPair) return false;
   const double cus = estimate_rows(a, 2.0 * a.n) - 4, memory = 2.0 * a.n * a.k / 5.5e6;
   const double two = 6 + (cus > memory ? cus : memory) + 16.0 * a.rows * a.n / 4e6, pair = two > 9.5 ? two : 9.5;
-  return pair < estimate_few(a) && !(tiles_take(a) && estimate_tiles(a) <= 1.15 * pair);
+  return pair < estimate_few(a) && !(tiles_take(a) && estimate_tiles(a) <= pair);
 }
 hipError_t multiply_pair(const ggk_fp8_args& a, hipStream_t stream) {
   const long long ld = pair_ld(a), blocks = (a.n + kStep - 1) / kStep;
