@@ -701,7 +701,7 @@ def fp8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
 
     Runs on the current stream of x's device, without waiting; no gradient (inputs that require one are
     refused, and dual tensors of forward mode)."""
-    return _fp8(x, x_scales, w, w_scales, None, None, None, None, None, None, out_dtype)
+    return _fp8(x, x_scales, w, w_scales, None, None, _lib.GGK_GATE_NONE, None, None, None, out_dtype)
 
 
 def fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor,
@@ -710,7 +710,7 @@ def fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_
     their product in one kernel; operands as fp8_matmul's, gate and up [N, K] (the halves of one matrix of both can be given
     as views).  activation: "silu", or "gelu" (the form with tanh).  Rows are made of float32 as rms_norm_fp8 makes
     them, of products in binary16 as fp8_matmul's for float32."""
-    return _fp8(x, x_scales, gate, gate_scales, up, up_scales, activation, None, None, None, None)
+    return _fp8(x, x_scales, gate, gate_scales, up, up_scales, _gate(activation), None, None, None, torch.float32)
 
 
 def moe_fp8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, counts: torch.Tensor,
@@ -727,7 +727,7 @@ def moe_fp8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_s
     left unwritten, and each value of one that it names twice is one of its products'."""
     if counts is None or order is None:
         raise TypeError("counts and order must be torch.Tensors")
-    return _fp8(x, x_scales, w, w_scales, None, None, None, counts, order, row_weights, out_dtype)
+    return _fp8(x, x_scales, w, w_scales, None, None, _lib.GGK_GATE_NONE, counts, order, row_weights, out_dtype)
 
 
 def moe_fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_scales: torch.Tensor,
@@ -738,16 +738,17 @@ def moe_fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, g
     may get one product's numbers with the other's scales."""
     if counts is None or order is None:
         raise TypeError("counts and order must be torch.Tensors")
-    return _fp8(x, x_scales, gate, gate_scales, up, up_scales, activation, counts, order, None, None)
+    return _fp8(x, x_scales, gate, gate_scales, up, up_scales, _gate(activation), counts, order, None, torch.float32)
 
 
-def _fp8(x, x_scales, w, w_scales, up, up_scales, activation, counts, order, row_weights, out_dtype):
-    if activation is not None and activation not in _GATES:
+def _gate(activation) -> int:
+    if not isinstance(activation, str) or activation not in _GATES:
         raise ValueError(f"activation must be one of {sorted(_GATES)}, got {activation!r}")
-    if activation is None:
-        gate = _lib.GGK_GATE_NONE
-    else:
-        gate, out_dtype = _GATES[activation], torch.float32  # not read: the rows are 8-bit ones
+    return _GATES[activation]
+
+
+def _fp8(x, x_scales, w, w_scales, up, up_scales, gate, counts, order, row_weights, out_dtype):
+    """out_dtype is not read with a gate: the rows are 8-bit ones."""
     try:
         out = _binding().fp8(x, x_scales, w, w_scales, up, up_scales, gate, counts, order, row_weights, out_dtype)
     except TypeError:  # an argument of another kind

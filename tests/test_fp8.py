@@ -18,12 +18,15 @@ Norm: mean(h^2) of H terms, chains of at most 64 + 16 additions, (H / 512 + 80) 
 rounding of its terms' sizes, the factor, its product and the weight's 4 u."""
 import ctypes
 import math
+import re
+import subprocess
 import threading
+from pathlib import Path
 
 import pytest
 import torch
 
-from grouped_gemm_gpu_kernel_amd import _lib, torch_ops
+from grouped_gemm_gpu_kernel_amd import _lib, build, torch_ops
 from test_kernel_resources import _scratch
 from test_moe_route import _c_layout
 
@@ -298,8 +301,9 @@ def test_refusals_of_the_products():
                                     (w, None, TypeError, "up_scales must be"), (None, ws, TypeError, "up must be")]:
             with pytest.raises(error, match=text):
                 torch_ops.fp8_gated(x, xs, w, ws, up, us)
-        with pytest.raises(ValueError, match="activation"):
-            torch_ops.fp8_gated(x, xs, w, ws, w, ws, activation="tanh")
+        for activation in ("tanh", None, 1, ["silu"]):
+            with pytest.raises(ValueError, match="activation"):
+                torch_ops.fp8_gated(x, xs, w, ws, w, ws, activation=activation)
         with pytest.raises(ValueError, match="gate has shape|gate_scales has shape"):
             torch_ops.fp8_gated(x, xs, w, _fake(1, 3), w, ws)
         w3, ws3, counts, order = q(4, 200, 272), _fake(4, 2, 3), _fake(4, dtype=torch.int32), _fake(6, dtype=torch.int32)
@@ -331,6 +335,59 @@ def test_refusals_of_the_products():
 @pytest.mark.parametrize("name", ["gg_norm.o", "gg_fp8.o", "gg_fp8_tiles.o"])
 def test_kernels_spill_nothing(name, tmp_path):
     assert not {k: v for k, v in _scratch(name, tmp_path).items() if v}
+
+
+@pytest.mark.parametrize("name", ["gg_fp8.o", "gg_fp8_tiles.o"])
+def test_matrix_results_and_lds_loads_have_their_wait_states(name, tmp_path):
+    """In the built kernels no result of a matrix instruction is read by another kind, and no branch taken, before its wait states
+    (8 for 16 x 16 x 32, 12 for 16 x 16 x 128), and every load into LDS directly follows the 5 of its statement."""
+    built = build.BUILD / name
+    if not built.exists():
+        pytest.skip("no regular build in the tree (build first)")
+    llvm = Path("/opt/rocm/llvm/bin")
+    subprocess.run([str(llvm / "llvm-objcopy"), f"--dump-section=.hip_fatbin={tmp_path / 'fat'}", str(built),
+                    str(tmp_path / "copy.o")], check=True)
+    subprocess.run([str(llvm / "clang-offload-bundler"), "--unbundle", "--type=o",
+                    "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", f"--input={tmp_path / 'fat'}",
+                    f"--output={tmp_path / 'gfx950.o'}"], check=True)
+    text = subprocess.run([str(llvm / "llvm-objdump"), "-d", "--mcpu=gfx950", str(tmp_path / "gfx950.o")], check=True,
+                          capture_output=True, text=True).stdout
+    code = [line.split("//")[0].strip() for line in text.splitlines() if line.startswith("\t")]
+    needed = {"v_mfma_f32_16x16x32_f16": 8, "v_mfma_f32_16x16x128_f8f6f4": 12}
+
+    def registers(operands):
+        found = set()
+        for first, last, one in re.findall(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b", operands):
+            found |= {int(one)} if one else set(range(int(first), int(last) + 1))
+        return found
+
+    def states_of(line):
+        return int(line.split()[1], 0) + 1 if line.startswith("s_nop") else 1
+
+    bad, products, loads = [], 0, 0
+    for i, line in enumerate(code):
+        kind = line.split()[0] if line else ""
+        if kind.startswith("global_load_lds") or (kind.startswith("buffer_load") and line.endswith(" lds")):
+            loads += 1
+            if not code[i - 1].startswith("s_nop") or states_of(code[i - 1]) < 5:
+                bad.append((code[i - 1], line))
+        if not kind.startswith("v_mfma"):
+            continue
+        products += 1
+        result, states = registers(line.split(",")[0]), 0
+        for after in code[i + 1:]:
+            if states >= needed[kind]:
+                break
+            if after.startswith("v_mfma"):
+                if result & registers(",".join(after.split(",")[1:3])):
+                    bad.append((line, after, states))
+                if result & registers(after):  # the next of a chain: checked as the one before
+                    break
+            elif result & registers(after) or after.startswith(("s_cbranch", "s_branch", "s_setpc")):
+                bad.append((line, after, states))
+                break
+            states += states_of(after)
+    assert products > 100 and loads > 50 and not bad, bad[:3]
 
 
 # ---------------------------------------------------------------- the norm
