@@ -26,7 +26,7 @@ using gg::kWave;
 constexpr int kCus = 256, kXcds = 8;
 
 struct Launch {
-  ggk_fp8_args a, second;  // a second product, of the same rows, after the first one's column blocks (one matrix, no gate)
+  ggk_fp8_args a, second;  // a second product, of the same rows, after the first one's column blocks (no gate)
   int blocks;              // of columns
   int blocks_of_a;         // of those, the first product's
   int tiles;               // of rows that the grid has (one matrix)
@@ -239,7 +239,8 @@ __device__ __forceinline__ void clear_item(const ggk_fp8_args& a, const RowTile&
   }
 }
 
-template <class F, bool EXPERTS>
+// PAIR: with a second product (with the arguments chosen at run time every call of experts took 2 us longer).
+template <class F, bool EXPERTS, bool PAIR>
 __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::BYTES <= 80 * 1024 ? F::WAVES / 2 : F::WAVES / 4) void fp8_stream_kernel(Launch l) {
   const ggk_fp8_args& a = l.a;
   __shared__ alignas(128) unsigned char s_bytes[F::BYTES];  // each wave's ring, then the sums
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::B
     if (item >= items) return;
     for (int tile = item % l.tiles; tile < tiles; tile += l.tiles) {
       const RowTile t{0, tile * F::R, min(F::R, a.rows - tile * F::R)};
-      const bool first = block < l.blocks_of_a;
+      const bool first = !PAIR || block < l.blocks_of_a;
       run_item<F, false>(first ? l.a : l.second, t, nullptr, nullptr, first ? block : block - l.blocks_of_a, s_bytes);
       gg::stage_barrier();
     }
@@ -262,7 +263,10 @@ __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::B
     gg::list_experts<F::THREADS, F::R>(a, s_experts);
     const long long items = (long long)s_experts.tile[a.experts + 1] * l.blocks;
     for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-      const int tile = (int)(item / l.blocks), block = (int)(item % l.blocks);
+      const int tile = (int)(item / l.blocks), of = (int)(item % l.blocks);
+      const bool first = !PAIR || of < l.blocks_of_a;
+      const ggk_fp8_args& b = first ? l.a : l.second;
+      const int block = first ? of : of - l.blocks_of_a;
       const RowTile t = gg::expert_tile<F::R>(a, s_experts, tile);
       for (int i = threadIdx.x; i < t.rows; i += F::THREADS) {
         int slot = a.order[t.first + i];
@@ -272,20 +276,25 @@ __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::B
       }
       gg::stage_barrier();
       if (t.expert == a.experts) {
-        clear_item<F>(a, t, s_slot, block * F::COLUMNS);
+        clear_item<F>(b, t, s_slot, block * F::COLUMNS);
       } else {
-        run_item<F, true>(a, t, s_slot, s_x_row, block, s_bytes);
+        run_item<F, true>(b, t, s_slot, s_x_row, block, s_bytes);
       }
       gg::stage_barrier();
     }
   }
 }
 
-// The 8-bit rows of gated products in a workspace, [2][rows][ld]: 16 lanes a block of a row.
+// The 8-bit rows of gated products in a workspace, [2][rows][ld]: 16 lanes a block of a row.  Experts' slots in their order, so
+// that those which it does not name stay as they are.
 __global__ __launch_bounds__(256) void fp8_gate_kernel(ggk_fp8_args a, long long ld) {
   const long long blocks = (a.n + kStep - 1) / kStep, all = a.rows * blocks;
-  const long long at = (long long)blockIdx.x * 16 + threadIdx.x / 16, of = at < all ? at : all - 1, row = of / blocks;
+  const long long at = (long long)blockIdx.x * 16 + threadIdx.x / 16, of = at < all ? at : all - 1;
   const int j = (int)(of % blocks) * kStep + threadIdx.x % 16 * 8;
+  long long row = of / blocks;
+  if (a.experts > 0) row = a.order[row];
+  const bool named = at < all && row >= 0 && row < a.rows;
+  if (!named) row = 0;
   const float* gate = a.workspace + row * ld + j;
   const float* up = gate + a.rows * ld;
   float v[8];
@@ -299,7 +308,7 @@ __global__ __launch_bounds__(256) void fp8_gate_kernel(ggk_fp8_args a, long long
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[4 * half + e] = a.gate == GGK_GATE_GELU ? gated<true>(p[e], u[e]) : gated<false>(p[e], u[e]);
   }
-  store_numbers(a, row, j, v, at < all);
+  store_numbers(a, row, j, v, named);
 }
 
 template <class F, bool EXPERTS>
@@ -316,7 +325,13 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args*
     l.tiles = (int)(tiles < most ? tiles : most);
     grid = ((long long)l.blocks * l.tiles + kXcds - 1) / kXcds * kXcds;
   }
-  hipLaunchKernelGGL((fp8_stream_kernel<F, EXPERTS>), dim3((unsigned)grid), dim3(F::THREADS), 0, stream, l);
+  if constexpr (F::EXACT && !F::GATED) {
+    if (second != nullptr) {
+      hipLaunchKernelGGL((fp8_stream_kernel<F, EXPERTS, true>), dim3((unsigned)grid), dim3(F::THREADS), 0, stream, l);
+      return hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((fp8_stream_kernel<F, EXPERTS, false>), dim3((unsigned)grid), dim3(F::THREADS), 0, stream, l);
   return hipGetLastError();
 }
 
@@ -340,7 +355,7 @@ bool has_own_tiles(const ggk_fp8_args& a) { return row_tiles(a, 16) * ceil(a.n /
 double estimate_few(const ggk_fp8_args& a) {
   const double items = row_tiles(a, 32) * ceil(a.n / 128.0), rounds = ceil(items / kCus), steps = a.k / 128.0;
   if (a.gate == GGK_GATE_NONE) return a.experts > 0 ? 5 + rounds * 0.6 * steps : estimate_rows(a, a.n);
-  if (a.experts > 0) return 5 + rounds * (2.5 + 1.15 * steps);
+  if (a.experts > 0) return 5 + (rounds > 1 ? rounds * (2.5 + 1.15 * steps) : 1.5 + 0.95 * steps);
   const double cus = has_own_tiles(a) ? 0.62 * steps : rounds > 1 ? rounds * (2 + 1.05 * steps) : 1 + 0.85 * steps,
                memory = 2.0 * a.n * a.k / 4.5e6;
   return 4.5 + (cus > memory ? cus : memory);
@@ -371,17 +386,27 @@ hipError_t multiply_rows(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp
   return launch<Form<32, 2, 1, 4, 2, false, false>, false>(a, stream, second);
 }
 
+// The same for experts' slots.
+hipError_t multiply_slots(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
+  if (a.rows <= 32) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream, second);
+  if (a.rows <= 12ll * a.experts) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream, second);
+  if (a.y_type == GGK_TYPE_F32) return launch<Form<32, 2, 4, 2, 2, false, true>, true>(a, stream, second);
+  return launch<Form<32, 2, 4, 2, 2, false, false>, true>(a, stream, second);
+}
+double estimate_slots(const ggk_fp8_args& a, double n) {
+  const double steps = a.k / 128.0;
+  if (a.rows <= 32) return 5 + ceil(row_tiles(a, 8) * ceil(n / 32) / (2 * kCus)) * (1 + 0.19 * steps);
+  if (a.rows <= 12ll * a.experts) return 5 + ceil(row_tiles(a, 16) * ceil(n / 256) / kCus) * 0.8 * steps;
+  return 5 + ceil(row_tiles(a, 32) * ceil(n / 128) / kCus) * 0.6 * steps;
+}
+
 template <bool EXPERTS>
 hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
-  const bool exact = a.y_type == GGK_TYPE_F32;
   if constexpr (EXPERTS) {
     // us with 32 rows at once, 16, 8: 16 experts of 1024 by 2048, 64 slots 16, 16, 18, 512 slots 25, 29, 41; 64 experts of 4096
     // by 14336, 16 slots 223, 218, 216, 256 slots 1011, 1022, 1095.
     if (a.gate != GGK_GATE_NONE) return launch<Form<32, 2, 8, 1, 2, true, true>, true>(a, stream);
-    if (a.rows <= 32) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream);
-    if (a.rows <= 12ll * a.experts) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream);
-    if (exact) return launch<Form<32, 2, 4, 2, 2, false, true>, true>(a, stream);
-    return launch<Form<32, 2, 4, 2, 2, false, false>, true>(a, stream);
+    return multiply_slots(a, stream);
   } else if (a.gate != GGK_GATE_NONE) {
     if (a.rows <= 8) return launch<Form<8, 4, 4, 1, 4, true, true>, false>(a, stream);
     if (has_own_tiles(a)) return launch<Form<16, 2, 8, 1, 3, true, true>, false>(a, stream);
@@ -394,14 +419,17 @@ hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
 // Gated products as both plain products, whose workgroups take 16 or 32 columns and share K, and their rows in a second launch:
 // a block of an 8-bit row needs the largest of 128 columns, and so few workgroups cannot bring in the weights as fast.  us by one
 // launch and by two: 1 row of 4096 by 14336 28.6, 25.3, by 2048 24.7, 9.3; 42 of 13280 by 1666 86, 22; 256 of 4096 by 1792 25.6,
-// 22.3; 1 of 512 by 512 6.3, 9.4; 512 of 4096 by 1792 31, 34.6; 7267 of 480 by 246 15.7, 27.
+// 22.3; 1 of 512 by 512 6.3, 9.4; 512 of 4096 by 1792 31, 34.6; 7267 of 480 by 246 15.7, 27; 2 slots of 8 experts of 4096 by 1792
+// 31, 13, by 14336 45.8, 47.5; 512 slots of 16 experts of 1024 by 2048 25, 32.
 constexpr long long kMostOfPair = 1 << 24;  // values of either product: 128 MB of workspace at most
 long long pair_ld(const ggk_fp8_args& a) { return (a.n + 3) / 4 * 4; }
 bool as_pair(const ggk_fp8_args& a) {
-  if (a.gate == GGK_GATE_NONE || a.experts > 0 || a.rows == 0 || a.n == 0 || a.rows * pair_ld(a) > kMostOfPair) return false;
-  const double cus = estimate_rows(a, 2.0 * a.n) - 4, memory = 2.0 * a.n * a.k / 5.5e6;
+  if (a.gate == GGK_GATE_NONE || a.rows == 0 || a.n == 0 || a.rows * pair_ld(a) > kMostOfPair) return false;
+  const double matrices = a.experts == 0 ? 1 : a.rows < a.experts ? a.rows : a.experts;
+  const double memory = matrices * 2.0 * a.n * a.k / 5.5e6;
+  const double cus = a.experts > 0 ? estimate_slots(a, 2.0 * a.n) - 2 : estimate_rows(a, 2.0 * a.n) - 4;
   const double two = 6 + (cus > memory ? cus : memory) + 16.0 * a.rows * a.n / 4e6, pair = two > 9.5 ? two : 9.5;
-  return pair < estimate_few(a) && !(tiles_take(a) && estimate_tiles(a) <= pair);
+  return pair < (a.experts > 0 ? 0.9 : 1) * estimate_few(a) && !(tiles_take(a) && estimate_tiles(a) <= pair);
 }
 hipError_t multiply_pair(const ggk_fp8_args& a, hipStream_t stream) {
   const long long ld = pair_ld(a), blocks = (a.n + kStep - 1) / kStep;
@@ -415,8 +443,11 @@ hipError_t multiply_pair(const ggk_fp8_args& a, hipStream_t stream) {
   up.ldw = a.ldu;
   up.w_scales = a.up_scales;
   up.ldws = a.ldus;
+  up.stride_w = a.stride_u;
+  up.stride_ws = a.stride_us;
   up.y = a.workspace + a.rows * ld;
-  if (const hipError_t st = multiply_rows(gate, stream, &up); st != hipSuccess) return st;
+  const hipError_t st = a.experts > 0 ? multiply_slots(gate, stream, &up) : multiply_rows(gate, stream, &up);
+  if (st != hipSuccess) return st;
   hipLaunchKernelGGL(fp8_gate_kernel, dim3((unsigned)((a.rows * blocks + 15) / 16)), dim3(256), 0, stream, a, ld);
   return hipGetLastError();
 }

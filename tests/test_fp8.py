@@ -719,7 +719,9 @@ def test_empty(torch_cuda):
 MOE_CASES = [(1, 4, 2, 130, 144, 0.0), (7, 8, 2, 64, 272, 0.3), (40, 3, 1, 257, 128, 0.1), (200, 16, 3, 200, 400, 0.2),
              (600, 5, 2, 300, 256, 0.1), (1500, 4, 2, 140, 400, 0.05), (300, 200, 4, 96, 128, 0.0), (90, 1024, 2, 33, 16, 0.1),
              (2500, 2, 1, 520, 528, 0.0), (9000, 5, 2, 520, 1040, 0.1), (9000, 7, 2, 519, 1040, 0.0), (1500, 4, 2, 1000, 1040, 0.2),
-             (6000, 600, 1, 130, 528, 0.0)]
+             (6000, 600, 1, 130, 528, 0.0),
+             # gated by way of a workspace, with few slots and with many an expert
+             (1, 8, 2, 1792, 4096, 0.0), (3, 4, 2, 301, 4096, 0.2), (16, 2, 2, 200, 4096, 0.0), (174, 5, 4, 396, 3008, 0.1)]
 
 
 @pytest.mark.gpu
@@ -736,7 +738,7 @@ def test_experts(torch_cuda, tokens, experts, top_k, n, k, drop):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tokens,n,k", [(37, 140, 144), (700, 140, 144), (9000, 520, 1040)])
+@pytest.mark.parametrize("tokens,n,k", [(37, 140, 144), (700, 140, 144), (9000, 520, 1040), (5, 139, 4096), (60, 139, 4096)])
 def test_counts_and_order_are_not_trusted(torch_cuda, tokens, n, k):
     """Negative counts are 0, counts past the rows are cut, entries outside [0, R) are dropped, rows that the order does not
     name stay as they were; in a slot named twice each value is one of its products."""
@@ -749,7 +751,7 @@ def test_counts_and_order_are_not_trusted(torch_cuda, tokens, n, k):
     lost = sorted(set(range(rows)) - set(order.tolist()))
     counts = torch.tensor([rows // 2, -5, 1 << 30, 1 << 30], dtype=torch.int32, device="cuda")
     expert = torch.where(torch.arange(rows) < rows // 2, 0, 2)
-    for gate in (0, 1):
+    for gate, with_workspace in ((0, False), (1, False), (1, True)):
         y = torch.full((rows, n), 0x55, dtype=torch.uint8, device="cuda") if gate else torch.full((rows, n), 77.0, device="cuda")
         scales = torch.full((rows, in_n), 77.0, device="cuda")
         args = _lib.GGKFp8Args(
@@ -760,6 +762,12 @@ def test_counts_and_order_are_not_trusted(torch_cuda, tokens, n, k):
             args.up, args.ldu, args.stride_u = up[0].data_ptr(), k, n * k
             args.up_scales, args.ldus, args.stride_us = up[1].data_ptr(), in_k, in_n * in_k
             args.y_scales, args.ldys = scales.data_ptr(), in_n
+        if with_workspace:
+            wanted = ctypes.c_longlong(-1)
+            assert _lib.lib().ggk_fp8_workspace(ctypes.byref(args), ctypes.byref(wanted)) == 0
+            assert wanted.value == (2 * rows * ((n + 3) // 4 * 4) if k == 4096 else 0)
+            workspace = torch.full((wanted.value + 4,), math.nan, device="cuda")
+            args.workspace = workspace.data_ptr()
         assert _lib.lib().ggk_fp8_multiply(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == 0
         ids = torch.full((rows,), -2)
         for place, slot in enumerate(order.tolist()):
