@@ -365,10 +365,12 @@ double estimate_few(const ggk_fp8_args& a) {
 hipError_t multiply_rows(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
   const bool exact = a.y_type == GGK_TYPE_F32;
   const long long n = second != nullptr ? 2ll * a.n : a.n;
+  // us by 8 rows at once, by 16, by 16 and 32 columns: 8 rows of 4096 by 4096 5.7, 6.0, 6.7, by 14336 11.5, 12.4, 11.3; 16 rows
+  // 6.2, 5.7, 6.8 and 13.8, 12.4, 11.5, of 8192 by 8192 14.6, 12.3, 12.3.
   if (a.rows <= 8) return launch<Form<8, 1, 1, 8, 2, false, true>, false>(a, stream, second);
   if (a.rows <= 16) {
     return n >= 8192 ? launch<Form<16, 1, 2, 4, 2, false, true>, false>(a, stream, second)
-                       : launch<Form<16, 1, 1, 8, 2, false, true>, false>(a, stream, second);
+                     : launch<Form<16, 1, 1, 8, 2, false, true>, false>(a, stream, second);
   }
   // 64 rows at once where their blocks of 64 columns fill the CUs, else 32 twice.  us of the two: 64 rows of 8192 by 28672
   // 59.5, 72.7, of 4096 by 16384 16.4, 16.8, in float 17.6, 19.3; of 4096 by 12288 15.6, 13.5, of 8192 by 8192 24, 17.
@@ -386,17 +388,21 @@ hipError_t multiply_rows(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp
   return launch<Form<32, 2, 1, 4, 2, false, false>, false>(a, stream, second);
 }
 
-// The same for experts' slots.
+// The same for experts' slots.  us by 8 rows by 32 columns, 16 by 256, 32 by 128: 2 slots of 8 experts of 4096 by 14336 25, 25, 21,
+// by 3584 in float 9 by the first where the last takes 25; 256 slots of 64 experts of 2048 by 2048 51, 43, 46, 64 slots of 4096 by
+// 14336 252, 254, 246; 512 slots of 16 experts of 1024 by 2048 32, 19, 15.
+bool is_narrow(const ggk_fp8_args& a, double n) { return a.rows <= 32 && row_tiles(a, 32) * ceil(n / 128) <= kCus / 4 * 3; }
+bool is_sparse(const ggk_fp8_args& a) { return a.rows > 32 && a.rows <= 12ll * a.experts; }
 hipError_t multiply_slots(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
-  if (a.rows <= 32) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream, second);
-  if (a.rows <= 12ll * a.experts) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream, second);
+  if (is_narrow(a, second != nullptr ? 2.0 * a.n : a.n)) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream, second);
+  if (is_sparse(a)) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream, second);
   if (a.y_type == GGK_TYPE_F32) return launch<Form<32, 2, 4, 2, 2, false, true>, true>(a, stream, second);
   return launch<Form<32, 2, 4, 2, 2, false, false>, true>(a, stream, second);
 }
 double estimate_slots(const ggk_fp8_args& a, double n) {
   const double steps = a.k / 128.0;
-  if (a.rows <= 32) return 5 + ceil(row_tiles(a, 8) * ceil(n / 32) / (2 * kCus)) * (1 + 0.19 * steps);
-  if (a.rows <= 12ll * a.experts) return 5 + ceil(row_tiles(a, 16) * ceil(n / 256) / kCus) * 0.8 * steps;
+  if (is_narrow(a, n)) return 5 + ceil(row_tiles(a, 8) * ceil(n / 32) / (2 * kCus)) * (1 + 0.19 * steps);
+  if (is_sparse(a)) return 5 + ceil(row_tiles(a, 16) * ceil(n / 256) / kCus) * 0.8 * steps;
   return 5 + ceil(row_tiles(a, 32) * ceil(n / 128) / kCus) * 0.6 * steps;
 }
 

@@ -695,9 +695,9 @@ def fp8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
 
     K is a multiple of 16; x and w start on multiples of 16 bytes, and so do their rows, which may be padded; rows
     of scales may be padded too.  Sums are float32.  y is float32, float16 or bfloat16, rounded once.  For
-    float32 the products are made in binary16, which holds 8-bit numbers exactly; for the 16-bit types and more than 16
-    rows (with experts, 12 slots each) by the 8-bit matrix instructions, twice as fast, which leave an error of about
-    1.5e-5 of a sum's terms (8 products at a time are aligned to the largest, to 13 bits below it).
+    float32 the products are made in binary16, which holds 8-bit numbers exactly; for the 16-bit types and more than a
+    few rows by the 8-bit matrix instructions, twice as fast, which leave an error of about 1.5e-5 of a sum's terms
+    (8 products at a time are aligned to the largest, to 13 bits below it).
 
     Runs on the current stream of x's device, without waiting; no gradient (inputs that require one are
     refused, and dual tensors of forward mode)."""
