@@ -203,7 +203,7 @@ class GGKFp8Args(ctypes.Structure):
         ("up", ctypes.c_void_p), ("ldu", ctypes.c_longlong), ("stride_u", ctypes.c_longlong),
         ("up_scales", ctypes.c_void_p), ("ldus", ctypes.c_longlong), ("stride_us", ctypes.c_longlong),
         ("counts", ctypes.c_void_p), ("order", ctypes.c_void_p), ("row_weights", ctypes.c_void_p),
-        ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong), ("y_type", ctypes.c_int),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong), ("y_type", ctypes.c_int), ("fast", ctypes.c_int),
         ("y_scales", ctypes.c_void_p), ("ldys", ctypes.c_longlong), ("workspace", ctypes.c_void_p),
     ]
 

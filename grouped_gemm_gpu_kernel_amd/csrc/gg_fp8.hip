@@ -343,7 +343,7 @@ double estimate_rows(const ggk_fp8_args& a, double n) {
   if (a.rows <= 16) return 4 + ceil(ceil(n / 16) / (2 * kCus)) * (1 + 0.08 * steps);
   if (row_tiles(a, 32) * ceil(n / 16) <= kCus) return 5 + 0.075 * steps;
   const double in_l2 = (double)a.rows * a.k / 4e6, more = in_l2 < 1 ? 1 : in_l2 > 2 ? 2 : in_l2;
-  const double step = (a.y_type == GGK_TYPE_F32 || a.gate != GGK_GATE_NONE ? 0.19 : 0.15) * more;
+  const double step = (is_exact(a) ? 0.19 : 0.15) * more;
   return 4 + ceil(row_tiles(a, 32) * ceil(n / 32) / (2 * kCus)) * (1.3 + step * steps);
 }
 
@@ -363,7 +363,7 @@ double estimate_few(const ggk_fp8_args& a) {
 
 // One matrix, or two of one shape: y and second's from the same rows.
 hipError_t multiply_rows(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
-  const bool exact = a.y_type == GGK_TYPE_F32;
+  const bool exact = is_exact(a);
   const long long n = second != nullptr ? 2ll * a.n : a.n;
   // us by 8 rows at once, by 16, by 16 and 32 columns: 8 rows of 4096 by 4096 5.7, 6.0, 6.7, by 14336 11.5, 12.4, 11.3; 16 rows
   // 6.2, 5.7, 6.8 and 13.8, 12.4, 11.5, of 8192 by 8192 14.6, 12.3, 12.3.
@@ -396,7 +396,7 @@ bool is_sparse(const ggk_fp8_args& a) { return a.rows > 32 && a.rows <= 12ll * a
 hipError_t multiply_slots(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
   if (is_narrow(a, second != nullptr ? 2.0 * a.n : a.n)) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream, second);
   if (is_sparse(a)) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream, second);
-  if (a.y_type == GGK_TYPE_F32) return launch<Form<32, 2, 4, 2, 2, false, true>, true>(a, stream, second);
+  if (is_exact(a)) return launch<Form<32, 2, 4, 2, 2, false, true>, true>(a, stream, second);
   return launch<Form<32, 2, 4, 2, 2, false, false>, true>(a, stream, second);
 }
 double estimate_slots(const ggk_fp8_args& a, double n) {
@@ -470,7 +470,7 @@ extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
       a.k > GGK_FP8_MAX_K || a.k % 16 != 0 || a.experts < 0 || a.experts > GGK_MOE_MAX_EXPERTS ||
       a.gate < GGK_GATE_NONE || a.gate > GGK_GATE_GELU ||
       (!gate && a.y_type != GGK_TYPE_F32 && a.y_type != GGK_TYPE_F16 && a.y_type != GGK_TYPE_BF16) ||
-      (gate && a.row_weights != nullptr)) {
+      (gate && a.row_weights != nullptr) || a.fast < 0 || a.fast > 1 || (a.fast != 0 && (gate || a.y_type == GGK_TYPE_F32))) {
     return hipErrorInvalidValue;
   }
   if (a.experts == 0 ? a.rows != a.x_rows : (a.rows > 0 && (a.x_rows < 1 || a.rows % a.x_rows != 0))) {
@@ -512,9 +512,11 @@ extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t str
   if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
   const ggk_fp8_args& a = *args;
   if (a.workspace != nullptr && as_pair(a)) return multiply_pair(a, stream);
-  // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 512 rows of 2048 by 2048 10, 20,
-  // 2048 rows 35, 21; 128 of 8192 by 8192 29, 49, 512 103, 56; 16 experts of 1024 by 2048, 512 slots 15, 18, 2048 slots 29,
-  // 20, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 256 slots 479, 463, 2048 slots 972, 751.
+  // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 1024 rows of 2048 by 2048 21, 32,
+  // 2048 rows 39, 33; 256 of 8192 by 8192 58, 110, 777 202, 113; 16 experts of 1024 by 2048, 512 slots 16, 24, 2048 slots 33,
+  // 25, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 256 slots 467, 626, 2048 slots 981, 989.  With the 8-bit
+  // instructions: 512 rows of 2048 by 2048 10, 20, 2048 rows 35, 21; 128 of 8192 by 8192 29, 49, 512 103, 56; 64 experts of 4096
+  // by 14336, 256 slots 479, 463, 2048 slots 972, 751.
   if (tiles_take(a) && estimate_tiles(a) < estimate_few(a)) return multiply_tiles(a, stream);
   return args->experts > 0 ? multiply_few<true>(*args, stream) : multiply_few<false>(*args, stream);
 }

@@ -15,8 +15,8 @@
 // its end for this wave's loads of unit f + 3 and its reads of the phases before; one barrier tells every wave both.
 //
 // Tiles of 128 rows (A0 alone) hold three stages in LDS and the next stage's fragments in a second set of registers, with one
-// barrier a stage.  Float results and gated rows are made in binary16, on tiles of 128 rows; with a gate a tile has 128 columns of
-// both matrices.  8192^3 takes 431 to 508 us by card (2.2 to 2.5 PFLOP/s), at the clock that its power allows; on zeros 331.  In
+// barrier a stage.  Products are made in binary16, on tiles of 128 rows, unless the caller asks for the 8-bit instructions; with a
+// gate a tile has 128 columns of both matrices.  8192^3 takes 431 to 508 us by card (2.2 to 2.5 PFLOP/s), at the clock that its power allows; on zeros 331.  In
 // float 930 to 975.  64 experts of 4096 by 14336, 16384 slots: 1300 to 1370 us, by HBM where experts have few rows.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -303,8 +303,7 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   gg::wait_vmcnt<0>();
 }
 
-// The same in binary16, which holds the numbers exactly, for float32 and 8-bit y (a row's scale is as exact as its largest
-// value).  A wave turns its fragments into binary16 once a stage, 128 instructions beside 64 products that take the matrix
+// The same in binary16, which holds the numbers exactly.  A wave turns its fragments into binary16 once a stage, 128 instructions beside 64 products that take the matrix
 // unit four times as long each: while a quarter of x's or w's is multiplied for the last time, the next one takes its
 // registers.  Turned into binary16 in front of the stage's products, 8192^3 in float took 1026 us, so 970; leaving out products
 // of rows past the tile's, in tiles of 64 or 32 rows or by a branch around them, gained nothing: zeros take little power.
@@ -714,7 +713,7 @@ __device__ __forceinline__ void run_tile(const Launch& l, const RowTile& t, cons
     } else {
       store_rows<EXPERTS, false>(a, t, s, n0, wm, wn, acc);
     }
-  } else if constexpr (EXACT) {
+  } else if (EXACT && a.y_type == GGK_TYPE_F32) {
     store_tile<EXPERTS, float, HALVES>(a, t, s, n0, wm, wn, acc);
   } else if (a.y_type == GGK_TYPE_BF16) {
     store_tile<EXPERTS, __bf16, HALVES>(a, t, s, n0, wm, wn, acc);
@@ -884,10 +883,8 @@ hipError_t launch(const ggk_fp8_args& a, int height, hipStream_t stream) {
 template <bool EXPERTS>
 hipError_t launch(const ggk_fp8_args& a, int height, hipStream_t stream) {
   if (a.gate != GGK_GATE_NONE) return launch<EXPERTS, true, true>(a, height, stream);
-  return a.y_type == GGK_TYPE_F32 ? launch<EXPERTS, false, true>(a, height, stream) : launch<EXPERTS, false, false>(a, height, stream);
+  return is_exact(a) ? launch<EXPERTS, false, true>(a, height, stream) : launch<EXPERTS, false, false>(a, height, stream);
 }
-
-bool is_exact(const ggk_fp8_args& a) { return a.gate != GGK_GATE_NONE || a.y_type == GGK_TYPE_F32; }
 
 // What a call takes on tiles of `height` rows, in us: what the busiest CU gets; of experts' tiles, whose counts the host does
 // not know, a tenth more.  A stage of a tile of 256 rows takes 1.2 us where half of the CUs work and 1.7 where all do, one of 128

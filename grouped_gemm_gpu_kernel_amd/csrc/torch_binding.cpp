@@ -440,12 +440,12 @@ bool fp8_matrix_in_order(const Tensor& w, const Tensor& scales, int64_t dim, c10
 
 py::object fp8_call(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Tensor& w_scales, const MaybeTensor& up,
                     const MaybeTensor& up_scales, int gate, const MaybeTensor& counts, const MaybeTensor& order,
-                    const MaybeTensor& row_weights, at::ScalarType out_type) {
+                    const MaybeTensor& row_weights, at::ScalarType out_type, bool fast) {
   const int64_t dim = counts ? 3 : 2;
   const bool gated = gate != GGK_GATE_NONE;
   if (!x.is_cuda() || x.scalar_type() != at::kFloat8_e4m3fn || !matrix_in_order(x) || w.dim() != dim ||
       gated != up.has_value() || gated != up_scales.has_value() || gate < GGK_GATE_NONE || gate > GGK_GATE_GELU ||
-      type_of(out_type) < 0) {
+      type_of(out_type) < 0 || (fast && (gated || out_type == at::kFloat))) {
     return py::none();
   }
   const c10::Device device = x.device();
@@ -515,6 +515,7 @@ py::object fp8_call(const Tensor& x, const Tensor& x_scales, const Tensor& w, co
     a.y = y.mutable_data_ptr();
     a.ldy = n;
     a.y_type = type_of(out_type);
+    a.fast = fast ? 1 : 0;
     Tensor workspace;  // goes back to the allocator in the stream's order
     long long floats = 0;
     if (const int status = ggk_fp8_workspace(&a, &floats); status != 0) return py::int_(status);

@@ -538,9 +538,11 @@ hipError_t ggk_norm_fp8(const ggk_norm_fp8_args* args, hipStream_t stream);
  * row_weights (none with a gate) as for ggk_w4_multiply: slot o = order[r] reads x row o / (rows / x_rows) and
  * writes y row o; slots past the counts' sum are set to 0 (with a gate: numbers 0, scales 2^-126).  In a slot named twice
  * each value is one of its products' (with a gate, numbers of one may meet scales of the other).
- * Sums are float.  With y in float or as 8-bit rows the products are made in binary16, which holds the numbers exactly;
- * else, for more than a few rows, on the 8-bit matrix instructions: those align 8 products at a time to the largest and cut
- * what lies 2^-13 of its power of two and more below it, which is 2^-16 of a sum of terms of one size.
+ * Sums are float, of products in binary16, which holds the numbers exactly: fast == 0.  fast == 1 (16-bit y without a gate)
+ * lets a call take the 8-bit matrix instructions where that is quicker, at twice the rate for many rows: those align 8
+ * products at a time to the largest and cut what lies 2^-13 of its power of two and more below it.  Of a sum of normal terms
+ * that is 1.5e-5; a term 2^13 times the seven beside it leaves nothing of them, also where another one cancels it.
+ * A product of two scales is a float: below 2^-126 it has fewer bits, above 2^128 it is infinite.
  * rows <= GGK_ROUTE_MAX_TOTAL_SLOTS, n <= GGK_FP8_MAX_N, k <= GGK_FP8_MAX_K, ldw <= GGK_FP8_MAX_LD. */
 enum { GGK_GATE_NONE = 0, GGK_GATE_SILU = 1, GGK_GATE_GELU = 2 };
 #define GGK_FP8_MAX_N (1 << 28)
@@ -572,6 +574,7 @@ typedef struct ggk_fp8_args {
   void* y;
   long long ldy;
   int y_type;
+  int fast; /* 0 or 1 */
   float* y_scales;
   long long ldys;
   float* workspace; /* NULL: none */
