@@ -171,11 +171,32 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(ggk_nor
   }
 }
 
+// The rows from `first` on, `rows` of them.
+template <class T>
+ggk_norm_fp8_args run_of(const ggk_norm_fp8_args& a, long long first, int rows) {
+  ggk_norm_fp8_args b = a;
+  b.rows = rows;
+  b.x = static_cast<const T*>(a.x) + first * a.ldx;
+  if (a.residual != nullptr) b.residual = static_cast<const T*>(a.residual) + first * a.ldr;
+  b.q = a.q + first * a.ldq;
+  b.scales = a.scales + first * a.lds;
+  if (a.y != nullptr) b.y = static_cast<T*>(a.y) + first * a.ldy;
+  if (a.sum != nullptr) b.sum = static_cast<T*>(a.sum) + first * a.ldsum;
+  return b;
+}
+
 template <int TYPE, int WTYPE, bool WHOLE>
 hipError_t launch_rows(const ggk_norm_fp8_args& a, hipStream_t stream) {
+  // A launch has less than 2^32 threads: more rows (2^21 of the widest and up) go by several.
   const auto go = [&](auto kernel, int rows, int threads) {
-    hipLaunchKernelGGL(kernel, dim3((a.rows + rows - 1) / rows), dim3(threads), 0, stream, a);
-    return hipGetLastError();
+    const int most = (int)((1ll << 31) / threads) * rows;
+    for (int first = 0; first < a.rows; first += most) {
+      const ggk_norm_fp8_args b = run_of<typename Type<TYPE>::T>(a, first, a.rows - first < most ? a.rows - first : most);
+      hipLaunchKernelGGL(kernel, dim3((b.rows + rows - 1) / rows), dim3(threads), 0, stream, b);
+      const hipError_t st = hipGetLastError();
+      if (st != hipSuccess) return st;
+    }
+    return hipSuccess;
   };
   const int chunks = (a.columns + 7) / 8;
   if (chunks <= 64) return go(norm_kernel<TYPE, WTYPE, 64, 1, WHOLE>, 4, 256);

@@ -1,0 +1,48 @@
+"""The 8-bit path at sizes where one launch ends: threads of a launch are counted in 32 bits."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from grouped_gemm_gpu_kernel_amd import _lib, torch_ops
+from test_fp8 import (BASE, FP8, GATE, MOE, _gen, blocks, check_gated, check_norm, check_product, matrix_of, matrix_values, numbers,
+                      row_values, rows_of)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,columns", [(2 ** 26 + 2 ** 25 + 7, 16), (2 ** 24 + 5, 2049)])
+def test_norm_of_more_rows_than_a_launch_has(torch_cuda, rows, columns):
+    """Rows of a wave each (four a workgroup of 256 threads) and of a workgroup each."""
+    torch.cuda.empty_cache()
+    x = torch.zeros(rows, columns, dtype=torch.bfloat16, device="cuda")
+    marked = torch.tensor([0, 1, 2 ** 23 - 1, 2 ** 23, 2 ** 23 + 1, rows // 2, rows - 6, rows - 2, rows - 1], device="cuda")
+    if rows > 2 ** 25:
+        marked = torch.cat((marked, torch.tensor([2 ** 25 - 1, 2 ** 25, 2 ** 26 - 1, 2 ** 26, 2 ** 26 + 1], device="cuda")))
+    some = torch.randn(len(marked), columns, generator=_gen(1), device="cuda").bfloat16()
+    x[marked] = some
+    out = torch_ops.rms_norm_fp8(x)
+    del x
+    q = out.q.view(torch.uint8)
+    check_norm(torch_ops.Fp8Norm(q[marked].view(FP8), out.scales[marked], None, None), some, None, None)
+    q[marked] = 0
+    out.scales[marked] = 2.0 ** -126
+    for first in range(0, rows, 2 ** 22):  # a part at a time: reductions of many values take room
+        assert not q[first:first + 2 ** 22].any() and (out.scales[first:first + 2 ** 22] == 2.0 ** -126).all()
+    del out, q
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_norm_of_several_launches_has_every_output(torch_cuda):
+    """With residual, weight and y, rows padded."""
+    rows, columns = 2 ** 25 + 3, 8
+    torch.cuda.empty_cache()
+    wide = torch.zeros(rows, 9, dtype=torch.float16, device="cuda")
+    last = torch.randn(40, columns, generator=_gen(2), device="cuda").half()
+    wide[-40:, :columns] = last
+    x, weight = wide[:, :columns], torch.randn(columns, generator=_gen(3), device="cuda").half()
+    out = torch_ops.rms_norm_fp8(x, weight, x, plain=True)
+    tail = torch_ops.Fp8Norm(out.q.view(torch.uint8)[-40:].view(FP8), out.scales[-40:], out.y[-40:], out.residual[-40:])
+    check_norm(tail, last, weight, last)
+    assert not out.q.view(torch.uint8)[:-40].any() and not out.y[:-40].any() and not out.residual[:-40].any()
