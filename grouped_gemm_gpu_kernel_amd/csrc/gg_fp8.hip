@@ -29,7 +29,7 @@ struct Launch {
   ggk_fp8_args a, second;  // a second product, of the same rows, after the first one's column blocks (no gate)
   int blocks;              // of columns
   int blocks_of_a;         // of those, the first product's
-  int tiles;               // of rows that the grid has (one matrix)
+  int tiles;               // of rows (one matrix)
 };
 
 // R rows of x (8, 16, 32, 64) by WN waves of NT tiles of 16 columns (with a gate: half of them gate, half up), WK waves
@@ -247,10 +247,10 @@ __global__ __launch_bounds__(F::THREADS, F::BYTES <= 40 * 1024 ? F::WAVES : F::B
   if constexpr (!EXPERTS) {
     // Neighbouring workgroups go to different XCDs: each takes an eighth of the items in the order of column blocks, so that the
     // row tiles of a block follow each other and its L2 has the weights for all of them.
-    const int tiles = (a.rows + F::R - 1) / F::R, items = l.blocks * l.tiles, share = (items + kXcds - 1) / kXcds;
-    const int item = (int)(blockIdx.x % kXcds) * share + (int)(blockIdx.x / kXcds), block = item / l.tiles;
-    if (item >= items) return;
-    for (int tile = item % l.tiles; tile < tiles; tile += l.tiles) {
+    const int items = l.blocks * l.tiles, share = (items + kXcds - 1) / kXcds, first_item = (int)(blockIdx.x % kXcds) * share;
+    const int end = min(first_item + share, items);
+    for (int item = first_item + (int)(blockIdx.x / kXcds); item < end; item += (int)(gridDim.x / kXcds)) {
+      const int block = item / l.tiles, tile = item % l.tiles;
       const RowTile t{0, tile * F::R, min(F::R, a.rows - tile * F::R)};
       const bool first = !PAIR || block < l.blocks_of_a;
       run_item<F, false>(first ? l.a : l.second, t, nullptr, nullptr, first ? block : block - l.blocks_of_a, s_bytes);
@@ -321,9 +321,11 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args*
     const long long items = tiles * l.blocks, most = kCus * (F::BYTES > 64 * 1024 ? 1 : 2);
     grid = items < most ? items : most;
   } else {
-    const long long most = (1 << 30) / l.blocks;
-    l.tiles = (int)(tiles < most ? tiles : most);
-    grid = ((long long)l.blocks * l.tiles + kXcds - 1) / kXcds * kXcds;
+    // A launch has less than 2^32 threads; workgroups take further items in turn.  (2^30 items are 2^38 values of y at least.)
+    const long long items = tiles * l.blocks, most = (1ll << 31) / F::THREADS;
+    if (items > 1 << 30) return hipErrorInvalidValue;
+    l.tiles = (int)tiles;
+    grid = items < most ? (items + kXcds - 1) / kXcds * kXcds : most;
   }
   if constexpr (F::EXACT && !F::GATED) {
     if (second != nullptr) {

@@ -46,3 +46,54 @@ def test_norm_of_several_launches_has_every_output(torch_cuda):
     tail = torch_ops.Fp8Norm(out.q.view(torch.uint8)[-40:].view(FP8), out.scales[-40:], out.y[-40:], out.residual[-40:])
     check_norm(tail, last, weight, last)
     assert not out.q.view(torch.uint8)[:-40].any() and not out.y[:-40].any() and not out.residual[:-40].any()
+
+
+def marks(count, n):
+    """Places near both ends, near powers of two and in between."""
+    at = {0, 1, n - 1, n - 2, n // 2, n // 3}
+    for p in range(20, 30):
+        at |= {2 ** p - 1, 2 ** p, 2 ** p + 1}
+    return torch.tensor(sorted(a for a in at if a < n)[-count:], device="cuda")
+
+
+@pytest.mark.gpu
+def test_product_of_more_rows_than_a_launch_has(torch_cuda):
+    """Streams of 32 rows by 32 columns, 256 threads each: 2^24 of them are 2^32 threads."""
+    torch.cuda.empty_cache()
+    rows, k = 2 ** 29 + 2 ** 20 + 11, 16
+    x = torch.zeros(rows, k, dtype=torch.uint8, device="cuda")
+    at = marks(24, rows)
+    some = numbers((len(at), k), 1)
+    x[at] = some.view(torch.uint8)
+    xs = torch.ones(rows, 1, device="cuda")
+    w = matrix_of((), 1, k, 2)
+    y = torch_ops.fp8_matmul(x.view(FP8), xs, *w, out_dtype=torch.float32)
+    del x, xs
+    check_product(y[at], some.double(), matrix_values(*w), True)
+    y[at] = 0
+    for first in range(0, rows, 2 ** 26):
+        assert not y[first:first + 2 ** 26].any()
+    del y
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(1, 2 ** 27 + 2 ** 20 + 5), (12, 2 ** 28), (20, 2 ** 27 + 33)])
+def test_product_of_more_columns_than_a_launch_has(torch_cuda, rows, n):
+    """Up to 8 rows by 16 columns, up to 16 by 32, of 512 threads each: 2^23 of them are 2^32 threads; n up to its limit."""
+    torch.cuda.empty_cache()
+    k = 16
+    w = torch.zeros(n, k, dtype=torch.uint8, device="cuda")
+    at = marks(24, n)
+    some = numbers((len(at), k), 1)
+    w[at] = some.view(torch.uint8)
+    ws = torch.ones(blocks(n), 1, device="cuda")
+    x = rows_of(rows, k, 2)
+    y = torch_ops.fp8_matmul(*x, w.view(FP8), ws)
+    del w, ws
+    check_product(y[:, at], row_values(*x), some.double(), True)
+    y[:, at] = 0
+    for first in range(0, n, 2 ** 24):
+        assert not y[:, first:first + 2 ** 24].any()
+    del y
+    torch.cuda.empty_cache()
