@@ -205,6 +205,7 @@ class GGKFp8Args(ctypes.Structure):
         ("counts", ctypes.c_void_p), ("order", ctypes.c_void_p), ("row_weights", ctypes.c_void_p),
         ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong), ("y_type", ctypes.c_int), ("fast", ctypes.c_int),
         ("y_scales", ctypes.c_void_p), ("ldys", ctypes.c_longlong), ("workspace", ctypes.c_void_p),
+        ("workspace_floats", ctypes.c_longlong),
     ]
 
 

@@ -460,13 +460,14 @@ hipError_t multiply_pair(const ggk_fp8_args& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+long long pair_floats(const ggk_fp8_args& a) { return 2ll * a.rows * pair_ld(a); }
+// As two launches: where the workspace is there for it.
+bool with_workspace(const ggk_fp8_args& a) { return a.workspace != nullptr && a.workspace_floats > 0 && as_pair(a); }
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-}  // namespace
-
-extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
-  if (args == nullptr) return hipErrorInvalidValue;
-  const ggk_fp8_args& a = *args;
+// Everything but the workspace's size.
+hipError_t check(const ggk_fp8_args& a) {
   const bool gate = a.gate != GGK_GATE_NONE;
   if (a.rows < 0 || a.rows > GGK_ROUTE_MAX_TOTAL_SLOTS || a.x_rows < 0 || a.n < 0 || a.n > GGK_FP8_MAX_N || a.k < 16 ||
       a.k > GGK_FP8_MAX_K || a.k % 16 != 0 || a.experts < 0 || a.experts > GGK_MOE_MAX_EXPERTS ||
@@ -503,22 +504,39 @@ extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
   return hipSuccess;
 }
 
+// used: with_workspace(a).
+hipError_t check_workspace(const ggk_fp8_args& a, bool used) {
+  return a.workspace_floats < 0 || (used && a.workspace_floats < pair_floats(a)) ? hipErrorInvalidValue : hipSuccess;
+}
+
+}  // namespace
+
+extern "C" hipError_t ggk_fp8_check(const ggk_fp8_args* args) {
+  if (args == nullptr) return hipErrorInvalidValue;
+  const hipError_t st = check(*args);
+  return st != hipSuccess ? st : check_workspace(*args, with_workspace(*args));
+}
+
 extern "C" hipError_t ggk_fp8_workspace(const ggk_fp8_args* args, long long* floats) {
-  const hipError_t st = floats == nullptr ? hipErrorInvalidValue : ggk_fp8_check(args);
-  if (st == hipSuccess) *floats = as_pair(*args) ? 2ll * args->rows * pair_ld(*args) : 0;
+  const hipError_t st = floats == nullptr || args == nullptr ? hipErrorInvalidValue : check(*args);
+  if (st == hipSuccess) *floats = as_pair(*args) ? pair_floats(*args) : 0;
   return st;
 }
 
 extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t stream) {
-  const hipError_t st = ggk_fp8_check(args);
-  if (st != hipSuccess || args->rows == 0 || args->n == 0) return st;
+  if (args == nullptr) return hipErrorInvalidValue;
   const ggk_fp8_args& a = *args;
-  if (a.workspace != nullptr && as_pair(a)) return multiply_pair(a, stream);
+  hipError_t st = check(a);
+  if (st != hipSuccess) return st;
+  const bool pair = with_workspace(a);
+  st = check_workspace(a, pair);
+  if (st != hipSuccess || a.rows == 0 || a.n == 0) return st;
+  if (pair) return multiply_pair(a, stream);
   // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 1024 rows of 2048 by 2048 21, 32,
   // 2048 rows 39, 33; 256 of 8192 by 8192 58, 110, 777 202, 113; 16 experts of 1024 by 2048, 512 slots 16, 24, 2048 slots 33,
   // 25, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 256 slots 467, 626, 2048 slots 981, 989.  With the 8-bit
   // instructions: 512 rows of 2048 by 2048 10, 20, 2048 rows 35, 21; 128 of 8192 by 8192 29, 49, 512 103, 56; 64 experts of 4096
   // by 14336, 256 slots 479, 463, 2048 slots 972, 751.
   if (tiles_take(a) && estimate_tiles(a) < estimate_few(a)) return multiply_tiles(a, stream);
-  return args->experts > 0 ? multiply_few<true>(*args, stream) : multiply_few<false>(*args, stream);
+  return a.experts > 0 ? multiply_few<true>(a, stream) : multiply_few<false>(a, stream);
 }

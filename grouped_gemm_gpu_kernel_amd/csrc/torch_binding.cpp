@@ -522,6 +522,7 @@ py::object fp8_call(const Tensor& x, const Tensor& x_scales, const Tensor& w, co
     if (floats > 0) {
       workspace = at::empty({floats}, like_x.dtype(at::kFloat));
       a.workspace = workspace.mutable_data_ptr<float>();
+      a.workspace_floats = floats;
     }
     const int status = launch(ggk_fp8_multiply, a, device);
     if (status != 0) return py::int_(status);

@@ -578,13 +578,15 @@ typedef struct ggk_fp8_args {
   float* y_scales;
   long long ldys;
   float* workspace; /* NULL: none */
+  long long workspace_floats; /* 0: not used */
 } ggk_fp8_args;
 
 /* The host-side checks ggk_fp8_multiply makes before it launches anything. */
 hipError_t ggk_fp8_check(const ggk_fp8_args* args);
 /* *floats: of workspace (on a multiple of 16 bytes) that make a call faster: gated products of few rows or columns are then
  * two launches, both products into the workspace and rows from it.  0: none; a workspace is then not used.  Calls that run at
- * the same time need one each. */
+ * the same time need one each.  ggk_fp8_multiply refuses a workspace of fewer workspace_floats, unless they are 0: the call then
+ * does without.  (Not read here.) */
 hipError_t ggk_fp8_workspace(const ggk_fp8_args* args, long long* floats);
 hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t stream);
 
