@@ -284,6 +284,7 @@ SIGNATURES = {
     "ggk_fp8_check": (_i, [_P(GGKFp8Args)]),
     "ggk_fp8_workspace": (_i, [_P(GGKFp8Args), _P(ctypes.c_longlong)]),
     "ggk_fp8_multiply": (_i, [_P(GGKFp8Args), _vp]),
+    "ggk_fp8_form": (_i, [_P(GGKFp8Args), ctypes.c_char_p, _i]),
     "ggk_launch_grouped_device": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp]),
     "ggk_launch_grouped_device_done": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, c_int_p, _vp]),
     "ggk_kernel_resources_get": (_i, [_i, _i, _i, _P(GGKKernelResources)]),

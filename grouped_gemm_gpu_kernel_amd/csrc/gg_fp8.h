@@ -159,10 +159,11 @@ inline double row_tiles(const ggk_fp8_args& a, int height) {
   return tiles > with_rows ? tiles : with_rows;
 }
 
-// The kernel for many rows (gg_fp8_tiles.hip): does it take a call's strides, how long it takes in us, and the call (16-bit
-// or 8-bit y).
+// The kernel for many rows (gg_fp8_tiles.hip): does it take a call's strides, how long it takes in us, rows of its tiles, and the
+// call.
 bool tiles_take(const ggk_fp8_args& a);
 double estimate_tiles(const ggk_fp8_args& a);
+int tile_rows(const ggk_fp8_args& a);
 hipError_t multiply_tiles(const ggk_fp8_args& a, hipStream_t stream);
 
 }  // namespace fp8

@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include <cmath>
+#include <cstdio>
 
 #include "gg_experts.h"
 #include "gg_fp8.h"
@@ -337,6 +338,32 @@ hipError_t launch(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args*
   return hipGetLastError();
 }
 
+// What the rules below do with the form that they chose for a call: launch it, or say which it is.
+struct Launches {
+  hipStream_t stream;
+  template <class F, bool EXPERTS>
+  hipError_t take(const ggk_fp8_args& a, const ggk_fp8_args* second = nullptr) const {
+    return launch<F, EXPERTS>(a, stream, second);
+  }
+  hipError_t take_tiles(const ggk_fp8_args& a) const { return multiply_tiles(a, stream); }
+};
+struct Names {
+  char* text;
+  int size;
+  template <class F, bool EXPERTS>
+  hipError_t take(const ggk_fp8_args&, const ggk_fp8_args* second = nullptr) const {
+    snprintf(text, size, "stream rows=%d columns=%d k=%d %s %s %s", F::R, F::COLUMNS, F::WK, F::EXACT ? "float" : "8-bit",
+             F::GATED ? "gated" : second != nullptr ? "pair" : "plain", EXPERTS ? "experts" : "one");
+    return hipSuccess;
+  }
+  hipError_t take_tiles(const ggk_fp8_args& a) const {
+    const bool gate = a.gate != GGK_GATE_NONE;
+    snprintf(text, size, "tiles rows=%d columns=%d %s %s %s", tile_rows(a), gate ? 128 : 256, is_exact(a) ? "float" : "8-bit",
+             gate ? "gated" : "plain", a.experts > 0 ? "experts" : "one");
+    return hipSuccess;
+  }
+};
+
 // What a plain call with n columns takes, in us: what the busiest CU gets, workgroups of 8 or 16 rows by 16 columns, or of 32 by 32,
 // two on a CU; of 32 by 16 where one is enough.  Where x is larger than an XCD's L2, its rows come from beyond it for every column
 // block.
@@ -364,30 +391,31 @@ double estimate_few(const ggk_fp8_args& a) {
 }
 
 // One matrix, or two of one shape: y and second's from the same rows.
-hipError_t multiply_rows(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
+template <class Run>
+hipError_t multiply_rows(const ggk_fp8_args& a, const Run& run, const ggk_fp8_args* second = nullptr) {
   const bool exact = is_exact(a);
   const long long n = second != nullptr ? 2ll * a.n : a.n;
   // us by 8 rows at once, by 16, by 16 and 32 columns: 8 rows of 4096 by 4096 5.7, 6.0, 6.7, by 14336 11.5, 12.4, 11.3; 16 rows
   // 6.2, 5.7, 6.8 and 13.8, 12.4, 11.5, of 8192 by 8192 14.6, 12.3, 12.3.
-  if (a.rows <= 8) return launch<Form<8, 1, 1, 8, 2, false, true>, false>(a, stream, second);
+  if (a.rows <= 8) return run.template take<Form<8, 1, 1, 8, 2, false, true>, false>(a, second);
   if (a.rows <= 16) {
-    return n >= 8192 ? launch<Form<16, 1, 2, 4, 2, false, true>, false>(a, stream, second)
-                     : launch<Form<16, 1, 1, 8, 2, false, true>, false>(a, stream, second);
+    return n >= 8192 ? run.template take<Form<16, 1, 2, 4, 2, false, true>, false>(a, second)
+                     : run.template take<Form<16, 1, 1, 8, 2, false, true>, false>(a, second);
   }
   // 64 rows at once where their blocks of 64 columns fill the CUs, else 32 twice.  us of the two: 64 rows of 8192 by 28672
   // 59.5, 72.7, of 4096 by 16384 16.4, 16.8, in float 17.6, 19.3; of 4096 by 12288 15.6, 13.5, of 8192 by 8192 24, 17.
   if (a.rows > 32 && a.rows <= 64 && (n + 63) / 64 >= kCus / 8 * 7) {
-    return exact ? launch<Form<64, 4, 1, 4, 2, false, true>, false>(a, stream, second)
-                 : launch<Form<64, 4, 1, 4, 2, false, false>, false>(a, stream, second);
+    return exact ? run.template take<Form<64, 4, 1, 4, 2, false, true>, false>(a, second)
+                 : run.template take<Form<64, 4, 1, 4, 2, false, false>, false>(a, second);
   }
   // 16 columns with K shared by 8 waves where every CU can get its own, else 32 by 4.  us of the two: 128 rows of 8192 by 1024
   // 8.9, 10, 32 rows 7.2, 9.7, in float 8.3, 12; 32 of 14336 by 4096 14.2, 15.5; 64 of 4096 by 4096 9.9, 7.0.
   if (row_tiles(a, 32) * ceil(n / 16.0) <= kCus) {
-    return exact ? launch<Form<32, 1, 1, 8, 2, false, true>, false>(a, stream, second)
-                 : launch<Form<32, 1, 1, 8, 2, false, false>, false>(a, stream, second);
+    return exact ? run.template take<Form<32, 1, 1, 8, 2, false, true>, false>(a, second)
+                 : run.template take<Form<32, 1, 1, 8, 2, false, false>, false>(a, second);
   }
-  if (exact) return launch<Form<32, 2, 1, 4, 2, false, true>, false>(a, stream, second);
-  return launch<Form<32, 2, 1, 4, 2, false, false>, false>(a, stream, second);
+  if (exact) return run.template take<Form<32, 2, 1, 4, 2, false, true>, false>(a, second);
+  return run.template take<Form<32, 2, 1, 4, 2, false, false>, false>(a, second);
 }
 
 // The same for experts' slots.  us by 8 rows by 32 columns, 16 by 256, 32 by 128: 2 slots of 8 experts of 4096 by 14336 25, 25, 21,
@@ -395,11 +423,12 @@ hipError_t multiply_rows(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp
 // 14336 252, 254, 246; 512 slots of 16 experts of 1024 by 2048 32, 19, 15.
 bool is_narrow(const ggk_fp8_args& a, double n) { return a.rows <= 32 && row_tiles(a, 32) * ceil(n / 128) <= kCus / 4 * 3; }
 bool is_sparse(const ggk_fp8_args& a) { return a.rows > 32 && a.rows <= 12ll * a.experts; }
-hipError_t multiply_slots(const ggk_fp8_args& a, hipStream_t stream, const ggk_fp8_args* second = nullptr) {
-  if (is_narrow(a, second != nullptr ? 2.0 * a.n : a.n)) return launch<Form<8, 1, 2, 4, 2, false, true>, true>(a, stream, second);
-  if (is_sparse(a)) return launch<Form<16, 2, 8, 1, 3, false, true>, true>(a, stream, second);
-  if (is_exact(a)) return launch<Form<32, 2, 4, 2, 2, false, true>, true>(a, stream, second);
-  return launch<Form<32, 2, 4, 2, 2, false, false>, true>(a, stream, second);
+template <class Run>
+hipError_t multiply_slots(const ggk_fp8_args& a, const Run& run, const ggk_fp8_args* second = nullptr) {
+  if (is_narrow(a, second != nullptr ? 2.0 * a.n : a.n)) return run.template take<Form<8, 1, 2, 4, 2, false, true>, true>(a, second);
+  if (is_sparse(a)) return run.template take<Form<16, 2, 8, 1, 3, false, true>, true>(a, second);
+  if (is_exact(a)) return run.template take<Form<32, 2, 4, 2, 2, false, true>, true>(a, second);
+  return run.template take<Form<32, 2, 4, 2, 2, false, false>, true>(a, second);
 }
 double estimate_slots(const ggk_fp8_args& a, double n) {
   const double steps = a.k / 128.0;
@@ -408,19 +437,19 @@ double estimate_slots(const ggk_fp8_args& a, double n) {
   return 5 + ceil(row_tiles(a, 32) * ceil(n / 128) / kCus) * 0.6 * steps;
 }
 
-template <bool EXPERTS>
-hipError_t multiply_few(const ggk_fp8_args& a, hipStream_t stream) {
+template <bool EXPERTS, class Run>
+hipError_t multiply_few(const ggk_fp8_args& a, const Run& run) {
   if constexpr (EXPERTS) {
     // us with 32 rows at once, 16, 8: 16 experts of 1024 by 2048, 64 slots 16, 16, 18, 512 slots 25, 29, 41; 64 experts of 4096
     // by 14336, 16 slots 223, 218, 216, 256 slots 1011, 1022, 1095.
-    if (a.gate != GGK_GATE_NONE) return launch<Form<32, 2, 8, 1, 2, true, true>, true>(a, stream);
-    return multiply_slots(a, stream);
+    if (a.gate != GGK_GATE_NONE) return run.template take<Form<32, 2, 8, 1, 2, true, true>, true>(a);
+    return multiply_slots(a, run);
   } else if (a.gate != GGK_GATE_NONE) {
-    if (a.rows <= 8) return launch<Form<8, 4, 4, 1, 4, true, true>, false>(a, stream);
-    if (has_own_tiles(a)) return launch<Form<16, 2, 8, 1, 3, true, true>, false>(a, stream);
-    return launch<Form<32, 2, 8, 1, 2, true, true>, false>(a, stream);
+    if (a.rows <= 8) return run.template take<Form<8, 4, 4, 1, 4, true, true>, false>(a);
+    if (has_own_tiles(a)) return run.template take<Form<16, 2, 8, 1, 3, true, true>, false>(a);
+    return run.template take<Form<32, 2, 8, 1, 2, true, true>, false>(a);
   } else {
-    return multiply_rows(a, stream);
+    return multiply_rows(a, run);
   }
 }
 
@@ -439,8 +468,9 @@ bool as_pair(const ggk_fp8_args& a) {
   const double two = 6 + (cus > memory ? cus : memory) + 16.0 * a.rows * a.n / 4e6, pair = two > 9.5 ? two : 9.5;
   return pair < (a.experts > 0 ? 0.9 : 1) * estimate_few(a) && !(tiles_take(a) && estimate_tiles(a) <= pair);
 }
-hipError_t multiply_pair(const ggk_fp8_args& a, hipStream_t stream) {
-  const long long ld = pair_ld(a), blocks = (a.n + kStep - 1) / kStep;
+template <class Run>
+hipError_t multiply_both(const ggk_fp8_args& a, const Run& run) {
+  const long long ld = pair_ld(a);
   ggk_fp8_args gate = a;
   gate.gate = GGK_GATE_NONE;
   gate.y = a.workspace;
@@ -454,7 +484,11 @@ hipError_t multiply_pair(const ggk_fp8_args& a, hipStream_t stream) {
   up.stride_w = a.stride_u;
   up.stride_ws = a.stride_us;
   up.y = a.workspace + a.rows * ld;
-  const hipError_t st = a.experts > 0 ? multiply_slots(gate, stream, &up) : multiply_rows(gate, stream, &up);
+  return a.experts > 0 ? multiply_slots(gate, run, &up) : multiply_rows(gate, run, &up);
+}
+hipError_t multiply_pair(const ggk_fp8_args& a, hipStream_t stream) {
+  const long long ld = pair_ld(a), blocks = (a.n + kStep - 1) / kStep;
+  const hipError_t st = multiply_both(a, Launches{stream});
   if (st != hipSuccess) return st;
   hipLaunchKernelGGL(fp8_gate_kernel, dim3((unsigned)((a.rows * blocks + 15) / 16)), dim3(256), 0, stream, a, ld);
   return hipGetLastError();
@@ -504,6 +538,18 @@ hipError_t check(const ggk_fp8_args& a) {
   return hipSuccess;
 }
 
+// One launch.
+template <class Run>
+hipError_t multiply_one(const ggk_fp8_args& a, const Run& run) {
+  // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 1024 rows of 2048 by 2048 21, 32,
+  // 2048 rows 39, 33; 256 of 8192 by 8192 58, 110, 777 202, 113; 16 experts of 1024 by 2048, 512 slots 16, 24, 2048 slots 33,
+  // 25, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 256 slots 467, 626, 2048 slots 981, 989.  With the 8-bit
+  // instructions: 512 rows of 2048 by 2048 10, 20, 2048 rows 35, 21; 128 of 8192 by 8192 29, 49, 512 103, 56; 64 experts of 4096
+  // by 14336, 256 slots 479, 463, 2048 slots 972, 751.
+  if (tiles_take(a) && estimate_tiles(a) < estimate_few(a)) return run.take_tiles(a);
+  return a.experts > 0 ? multiply_few<true>(a, run) : multiply_few<false>(a, run);
+}
+
 // used: with_workspace(a).
 hipError_t check_workspace(const ggk_fp8_args& a, bool used) {
   return a.workspace_floats < 0 || (used && a.workspace_floats < pair_floats(a)) ? hipErrorInvalidValue : hipSuccess;
@@ -532,11 +578,14 @@ extern "C" hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t str
   st = check_workspace(a, pair);
   if (st != hipSuccess || a.rows == 0 || a.n == 0) return st;
   if (pair) return multiply_pair(a, stream);
-  // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 1024 rows of 2048 by 2048 21, 32,
-  // 2048 rows 39, 33; 256 of 8192 by 8192 58, 110, 777 202, 113; 16 experts of 1024 by 2048, 512 slots 16, 24, 2048 slots 33,
-  // 25, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 256 slots 467, 626, 2048 slots 981, 989.  With the 8-bit
-  // instructions: 512 rows of 2048 by 2048 10, 20, 2048 rows 35, 21; 128 of 8192 by 8192 29, 49, 512 103, 56; 64 experts of 4096
-  // by 14336, 256 slots 479, 463, 2048 slots 972, 751.
-  if (tiles_take(a) && estimate_tiles(a) < estimate_few(a)) return multiply_tiles(a, stream);
-  return a.experts > 0 ? multiply_few<true>(a, stream) : multiply_few<false>(a, stream);
+  return multiply_one(a, Launches{stream});
+}
+
+extern "C" hipError_t ggk_fp8_form(const ggk_fp8_args* args, char* text, int size) {
+  hipError_t st = text == nullptr || size < 1 ? hipErrorInvalidValue : ggk_fp8_check(args);
+  if (st != hipSuccess) return st;
+  text[0] = 0;
+  if (args->rows == 0 || args->n == 0) return st;
+  const Names names{text, size};
+  return with_workspace(*args) ? multiply_both(*args, names) : multiply_one(*args, names);
 }

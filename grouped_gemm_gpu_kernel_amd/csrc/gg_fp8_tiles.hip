@@ -921,6 +921,8 @@ bool tiles_take(const ggk_fp8_args& a) {
 
 double estimate_tiles(const ggk_fp8_args& a) { return estimate(a, a.experts > 0 ? kRows / 2 : height_of(a)); }
 
+int tile_rows(const ggk_fp8_args& a) { return height_of(a); }
+
 hipError_t multiply_tiles(const ggk_fp8_args& a, hipStream_t stream) {
   return a.experts > 0 ? launch<true>(a, height_of(a), stream) : launch<false>(a, height_of(a), stream);
 }

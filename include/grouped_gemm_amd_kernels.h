@@ -589,6 +589,10 @@ hipError_t ggk_fp8_check(const ggk_fp8_args* args);
  * does without.  (Not read here.) */
 hipError_t ggk_fp8_workspace(const ggk_fp8_args* args, long long* floats);
 hipError_t ggk_fp8_multiply(const ggk_fp8_args* args, hipStream_t stream);
+/* Which form of the kernels these arguments take (with a workspace, the first launch's), as text of at most size - 1 characters:
+ * "stream rows=8 columns=16 k=8 float plain one", "tiles rows=256 columns=256 8-bit plain experts"; empty where nothing is
+ * launched.  On the host alone, for checking a choice without a GPU. */
+hipError_t ggk_fp8_form(const ggk_fp8_args* args, char* text, int size);
 
 /* One problem, one workgroup per work tile, row-major work-tile order
  * (single_problem_gemm_kernel + launch_single_problem_variant,
