@@ -402,9 +402,10 @@ hipError_t multiply_rows(const ggk_fp8_args& a, const Run& run, const ggk_fp8_ar
     return n >= 8192 ? run.template take<Form<16, 1, 2, 4, 2, false, true>, false>(a, second)
                      : run.template take<Form<16, 1, 1, 8, 2, false, true>, false>(a, second);
   }
-  // 64 rows at once where their blocks of 64 columns fill the CUs, else 32 twice.  us of the two: 64 rows of 8192 by 28672
-  // 59.5, 72.7, of 4096 by 16384 16.4, 16.8, in float 17.6, 19.3; of 4096 by 12288 15.6, 13.5, of 8192 by 8192 24, 17.
-  if (a.rows > 32 && a.rows <= 64 && (n + 63) / 64 >= kCus / 8 * 7) {
+  // 32 rows twice where no CU gets a fourth of those workgroups (two are at work at once), else 64 at once.  us of the two: 64 rows of
+  // 4096 by 12288 15.4, 16.7, by 12544 18.7, 16.8, 33 rows 14.9, 16.1 and 18.0, 16.2; of 8192 by 8192 17, 24, by 12800 42, 32; by
+  // the 8-bit instructions 64 rows of 4096 by 12288 13.2, 15.4, by 12544 16.0, 15.5, 33 rows 12.5, 14.8 and 15.0, 14.8.
+  if (a.rows > 32 && a.rows <= 64 && 2 * ((n + 31) / 32) > 3 * kCus) {
     return exact ? run.template take<Form<64, 4, 1, 4, 2, false, true>, false>(a, second)
                  : run.template take<Form<64, 4, 1, 4, 2, false, false>, false>(a, second);
   }

@@ -91,6 +91,14 @@ def test_every_form_is_run_here(tmp_path):
     assert len(kernels) == len({tuple(f.split()[2:]) for f in found if f.startswith("tiles")})
 
 
+@pytest.mark.parametrize("fast", [False, True])
+def test_64_rows_at_once_where_a_cu_would_get_a_fourth_workgroup(fast):
+    for rows in (33, 64):
+        assert form(rows=rows, k=4096, n=12288, fast=fast).startswith("stream rows=32 columns=32 ")
+        assert form(rows=rows, k=4096, n=12289, fast=fast).startswith("stream rows=64 columns=64 ")
+    assert form(rows=40, k=4096, n=6145, gate=1, workspace=True) == "stream rows=64 columns=64 k=4 float pair one"
+
+
 def test_form_of_refused_and_empty_calls():
     text = ctypes.create_string_buffer(b"x" * 20, 20)
     ask = _lib.lib().ggk_fp8_form
