@@ -419,11 +419,13 @@ hipError_t multiply_rows(const ggk_fp8_args& a, const Run& run, const ggk_fp8_ar
   return run.template take<Form<32, 2, 1, 4, 2, false, false>, false>(a, second);
 }
 
-// The same for experts' slots.  us by 8 rows by 32 columns, 16 by 256, 32 by 128: 2 slots of 8 experts of 4096 by 14336 25, 25, 21,
-// by 3584 in float 9 by the first where the last takes 25; 256 slots of 64 experts of 2048 by 2048 51, 43, 46, 64 slots of 4096 by
-// 14336 252, 254, 246; 512 slots of 16 experts of 1024 by 2048 32, 19, 15.
+// The same for experts' slots: 8 rows by 32 columns, 16 by 256 or 32 by 128 (those share K by 4 waves, none and 2).  us of the three:
+// 2 slots of 8 experts of 4096 by 14336 25, 25, 22, by 3584 9 by the first, 17.5 by the last.  Of the last two, by K: 256 slots of 128
+// experts of 512 by 1408 twice 31, 34, 1200 slots of 1024 by 2048 59, 64; 64 slots of 64 experts of 2048 by 2048 21, 23.5, 700
+// slots 59, 63; 256 slots of 32 experts of 4096 by 1408 twice 78, 73, 128 slots of 7168 114, 104, of 16 of 8192 by 512 52, 36;
+// by slots an expert: 512 slots of 16 experts of 1024 by 2048 18, 16, 180 slots 11, 16.
 bool is_narrow(const ggk_fp8_args& a, double n) { return a.rows <= 32 && row_tiles(a, 32) * ceil(n / 128) <= kCus / 4 * 3; }
-bool is_sparse(const ggk_fp8_args& a) { return a.rows > 32 && a.rows <= 12ll * a.experts; }
+bool is_sparse(const ggk_fp8_args& a) { return a.rows > 32 && a.rows <= 12ll * a.experts && a.k <= 2048; }
 template <class Run>
 hipError_t multiply_slots(const ggk_fp8_args& a, const Run& run, const ggk_fp8_args* second = nullptr) {
   if (is_narrow(a, second != nullptr ? 2.0 * a.n : a.n)) return run.template take<Form<8, 1, 2, 4, 2, false, true>, true>(a, second);

@@ -99,6 +99,12 @@ def test_64_rows_at_once_where_a_cu_would_get_a_fourth_workgroup(fast):
     assert form(rows=40, k=4096, n=6145, gate=1, workspace=True) == "stream rows=64 columns=64 k=4 float pair one"
 
 
+def test_experts_of_few_slots_by_k_and_slots():
+    assert form(rows=384, k=2048, n=300, experts=64, fan=2) == "stream rows=16 columns=256 k=1 float plain experts"
+    assert form(rows=384, k=2064, n=300, experts=64, fan=2) == "stream rows=32 columns=128 k=2 float plain experts"
+    assert form(rows=385, k=2048, n=300, experts=64, fan=2) == "stream rows=32 columns=128 k=2 float plain experts"
+
+
 def test_form_of_refused_and_empty_calls():
     text = ctypes.create_string_buffer(b"x" * 20, 20)
     ask = _lib.lib().ggk_fp8_form
