@@ -366,13 +366,13 @@ struct Names {
 
 // What a plain call with n columns takes, in us: what the busiest CU gets, workgroups of 8 or 16 rows by 16 columns, or of 32 by 32,
 // two on a CU; of 32 by 16 where one is enough.  Where x is larger than an XCD's L2, its rows come from beyond it for every column
-// block.
+// block: a step of 4 MB of x takes 0.19 us in binary16 (0.15 by the 8-bit instructions), of 6 MB 0.22, of 8 MB and more 0.27.
 double estimate_rows(const ggk_fp8_args& a, double n) {
   const double steps = a.k / 128.0;
   if (a.rows <= 16) return 4 + ceil(ceil(n / 16) / (2 * kCus)) * (1 + 0.08 * steps);
   if (row_tiles(a, 32) * ceil(n / 16) <= kCus) return 5 + 0.075 * steps;
-  const double in_l2 = (double)a.rows * a.k / 4e6, more = in_l2 < 1 ? 1 : in_l2 > 2 ? 2 : in_l2;
-  const double step = (is_exact(a) ? 0.19 : 0.15) * more;
+  const double in_l2 = (double)a.rows * a.k / 4e6, memory = 0.15 * (in_l2 > 1.8 ? 1.8 : in_l2), unit = is_exact(a) ? 0.19 : 0.15;
+  const double step = memory > unit ? memory : unit;
   return 4 + ceil(row_tiles(a, 32) * ceil(n / 32) / (2 * kCus)) * (1.3 + step * steps);
 }
 
@@ -544,11 +544,11 @@ hipError_t check(const ggk_fp8_args& a) {
 // One launch.
 template <class Run>
 hipError_t multiply_one(const ggk_fp8_args& a, const Run& run) {
-  // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 1024 rows of 2048 by 2048 21, 32,
-  // 2048 rows 39, 33; 256 of 8192 by 8192 58, 110, 777 202, 113; 16 experts of 1024 by 2048, 512 slots 16, 24, 2048 slots 33,
-  // 25, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 256 slots 467, 626, 2048 slots 981, 989.  With the 8-bit
-  // instructions: 512 rows of 2048 by 2048 10, 20, 2048 rows 35, 21; 128 of 8192 by 8192 29, 49, 512 103, 56; 64 experts of 4096
-  // by 14336, 256 slots 479, 463, 2048 slots 972, 751.
+  // Few rows stream, many go on tiles, by what either is expected to take.  us of the two: 1536 rows of 2048 by 2048 30, 33, 2048
+  // 39, 33; 512 of 4096 by 4096 33, 58, 1024 64, 59; 1024 of 8192 by 2048 73, 110, 1536 114, 111; 16 experts of 1024 by 2048, 512
+  // slots 16, 24, 2048 slots 33, 25, gated 25, 46 and 53, 50; 64 experts of 4096 by 14336, 1024 slots 764, 882, 4096 slots 1366,
+  // 1099.  By the 8-bit instructions 768 rows of 2048 by 2048 14, 16, 1536 25, 17; 384 of 4096 by 4096 22, 26, 768 40, 27; 64 experts
+  // of 4096 by 14336, 512 slots 588, 574 (256 slots, 456 and 470, are missed: their counts are not known here).
   if (tiles_take(a) && estimate_tiles(a) < estimate_few(a)) return run.take_tiles(a);
   return a.experts > 0 ? multiply_few<true>(a, run) : multiply_few<false>(a, run);
 }

@@ -888,14 +888,15 @@ hipError_t launch(const ggk_fp8_args& a, int height, hipStream_t stream) {
 
 // What a call takes on tiles of `height` rows, in us: what the busiest CU gets; of experts' tiles, whose counts the host does
 // not know, a tenth more.  A stage of a tile of 256 rows takes 1.2 us where half of the CUs work and 1.7 where all do, one of 128
-// rows 0.7 and 0.95 (0.62 where few work), in binary16 1.75.
+// rows 0.7 and 0.95 (0.62 where few work), in binary16 1.6 and 1.75, gated 1.75.
 double estimate(const ggk_fp8_args& a, int height) {
   const bool gate = a.gate != GGK_GATE_NONE;
   const double columns = gate ? 128 : 256, stages = (a.k + kStep - 1) / kStep;
   const double of_a_cu = row_tiles(a, height) * ceil(a.n / columns) * (a.experts > 0 ? 1.1 : 1) / kCus, rounds = ceil(of_a_cu);
   const double at_work = of_a_cu / rounds;
   const double of_128 = at_work < 0.34 ? 0.62 : 0.45 + 0.5 * at_work;
-  const double stage = is_exact(a) ? 1.75 : height == kRows ? 0.9 + 0.8 * at_work : of_128;
+  const double of_exact = gate ? 1.75 : 1.55 + 0.2 * at_work;
+  const double stage = is_exact(a) ? of_exact : height == kRows ? 0.9 + 0.8 * at_work : of_128;
   return (a.experts > 0 ? 10 : 8) + rounds * (stage * stages + (gate ? 4 : 2));
 }
 
