@@ -97,3 +97,51 @@ def test_product_of_more_columns_than_a_launch_has(torch_cuda, rows, n):
         assert not y[:, first:first + 2 ** 24].any()
     del y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(3, 20), (40, 70), (130, 260)])
+def test_longest_rows(torch_cuda, rows, n):
+    """K and the distance of rows at their limit.  Sums of whole numbers are exact: terms of one, of which a float holds 2^24."""
+    torch.cuda.empty_cache()
+    k = _lib.GGK_FP8_MAX_K
+    x, w = (torch.randint(-1, 2, shape, generator=_gen(shape[0]), device="cuda", dtype=torch.int8).to(FP8)
+            for shape in ((rows, k), (n, k)))
+    xs, ws = torch.ones(rows, blocks(k), device="cuda"), torch.ones(blocks(n), blocks(k), device="cuda")
+    want = torch.zeros(rows, n, dtype=torch.float64, device="cuda")
+    for at in range(0, k, 2 ** 18):
+        want += x[:, at:at + 2 ** 18].double() @ w[:, at:at + 2 ** 18].double().t()
+    for fast, dtype in ((False, torch.float32), (False, torch.bfloat16), (True, torch.float16)):
+        assert torch.equal(torch_ops.fp8_matmul(x, xs, w, ws, out_dtype=dtype, fast=fast), want.to(dtype))
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(1)).int().cuda()
+    counts = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    y = torch_ops.moe_fp8_matmul(x, xs, w.expand(2, n, k), ws.expand(2, *ws.shape), counts, order, out_dtype=torch.float32)
+    assert torch.equal(y.double(), want)
+    gated = torch_ops.fp8_gated(x, xs * 2.0 ** -8, w, ws, w, ws)
+    p = want * 2.0 ** -8
+    h = p * torch.sigmoid(p) * p
+    off = (gated.q.double() * gated.scales.double().repeat_interleave(128, 1)[:, :n] - h).abs()
+    most = h.abs().amax(1, keepdim=True)  # a number is off by half a step, 2^-4 of the value or 2^-10 of the scale
+    assert (off <= torch.maximum(2.0 ** -4 * h.abs(), 2.0 ** -10 / 448 * most) * 1.001).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 40, 300])
+def test_rows_of_x_far_apart(torch_cuda, rows):
+    """Offsets of x past 32 bits inside a tile, and rows of scales that are padded."""
+    torch.cuda.empty_cache()
+    k, n, apart = 272, 150, 2 ** 25 + 16
+    far = torch.empty(rows, apart, dtype=torch.uint8, device="cuda")[:, 16:16 + k].view(FP8)
+    x, xs = rows_of(rows, k, 1)
+    far.view(torch.uint8).copy_(x.view(torch.uint8))
+    wide = torch.full((rows, 1000), math.nan, device="cuda")
+    wide[:, 7:10] = xs
+    w, up = matrix_of((), n, k, 2), matrix_of((), n, k, 3)
+    for dtype in (torch.float32, torch.bfloat16):
+        check_product(torch_ops.fp8_matmul(far, wide[:, 7:10], *w, out_dtype=dtype), row_values(x, xs), matrix_values(*w), True)
+    check_gated(torch_ops.fp8_gated(far, wide[:, 7:10], *w, *up), row_values(x, xs), matrix_values(*w), matrix_values(*up))
+    counts, order = torch.tensor([rows], dtype=torch.int32, device="cuda"), torch.arange(rows, dtype=torch.int32, device="cuda")
+    y = torch_ops.moe_fp8_matmul(far, wide[:, 7:10], w[0][None], w[1][None], counts, order, out_dtype=torch.float32)
+    check_product(y, row_values(x, xs), matrix_values(*w), True)
+    del far
+    torch.cuda.empty_cache()
