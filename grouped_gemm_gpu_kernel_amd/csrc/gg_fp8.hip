@@ -5,8 +5,9 @@
 //
 // With few rows the weights' bytes are what counts.  Every wave streams its own columns through a ring of steps of its
 // own in LDS, loaded there directly, several steps ahead, with x's rows and the scales of the same step beside them: no
-// wave waits for another until its sums are whole.  1 row of 4096 by 14336 takes 11.5 us, 5.0 TB/s with the launch; 61 rows in
-// float 17.4; 1 row gated 25.2, by two launches (below).
+// wave waits for another until its sums are whole.  1 row of 4096 by 14336 takes 11.2 us where the 59 MB of weights are still in the
+// cache behind the L2s and 12.7 where they are not (4.6 TB/s with the launch); 61 rows in float 17.2 and 19.7; 1 row gated 24.8 and
+// 25.0, by two launches (below).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -422,7 +423,7 @@ hipError_t multiply_rows(const ggk_fp8_args& a, const Run& run, const ggk_fp8_ar
 // The same for experts' slots: 8 rows by 32 columns, 16 by 256 or 32 by 128 (those share K by 4 waves, none and 2).  us of the three:
 // 2 slots of 8 experts of 4096 by 14336 25, 25, 22, by 3584 9 by the first, 17.5 by the last.  Of the last two, by K: 256 slots of 128
 // experts of 512 by 1408 twice 31, 34, 1200 slots of 1024 by 2048 59, 64; 64 slots of 64 experts of 2048 by 2048 21, 23.5, 700
-// slots 59, 63; 256 slots of 32 experts of 4096 by 1408 twice 78, 73, 128 slots of 7168 114, 104, of 16 of 8192 by 512 52, 36;
+// slots 59, 63; 256 slots of 32 experts of 4096 by 1408 twice 86, 80, 128 slots of 7168 125, 115, of 16 of 8192 by 512 51, 36;
 // by slots an expert: 512 slots of 16 experts of 1024 by 2048 18, 16, 180 slots 11, 16.
 bool is_narrow(const ggk_fp8_args& a, double n) { return a.rows <= 32 && row_tiles(a, 32) * ceil(n / 128) <= kCus / 4 * 3; }
 bool is_sparse(const ggk_fp8_args& a) { return a.rows > 32 && a.rows <= 12ll * a.experts && a.k <= 2048; }

@@ -16,8 +16,9 @@
 //
 // Tiles of 128 rows (A0 alone) hold three stages in LDS and the next stage's fragments in a second set of registers, with one
 // barrier a stage.  Products are made in binary16, on tiles of 128 rows, unless the caller asks for the 8-bit instructions; with a
-// gate a tile has 128 columns of both matrices.  8192^3 takes 431 to 508 us by card (2.2 to 2.5 PFLOP/s), at the clock that its power allows; on zeros 331.  In
-// float 930 to 975.  64 experts of 4096 by 14336, 16384 slots: 1300 to 1370 us, by HBM where experts have few rows.
+// gate a tile has 128 columns of both matrices.  8192^3 takes 915 to 975 us by card (1.1 to 1.2 PFLOP/s), by the 8-bit instructions
+// 428 to 508 (2.2 to 2.6), at the clock that its power allows; on zeros those take 331.  64 experts of 4096 by 14336, 16384 slots: 2235
+// to 2340 us, and 1265 to 1370, the latter by HBM where experts have few rows.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -303,10 +304,11 @@ __device__ __forceinline__ void multiply_tile(const Launch& l, const RowTile& t,
   gg::wait_vmcnt<0>();
 }
 
-// The same in binary16, which holds the numbers exactly.  A wave turns its fragments into binary16 once a stage, 128 instructions beside 64 products that take the matrix
-// unit four times as long each: while a quarter of x's or w's is multiplied for the last time, the next one takes its
-// registers.  Turned into binary16 in front of the stage's products, 8192^3 in float took 1026 us, so 970; leaving out products
-// of rows past the tile's, in tiles of 64 or 32 rows or by a branch around them, gained nothing: zeros take little power.
+// The same in binary16, which holds the numbers exactly.  A wave turns its fragments into binary16 once a stage, 128
+// instructions beside 64 products that take the matrix unit four times as long each: while a quarter of x's or w's is multiplied
+// for the last time, the next one takes its registers.  Turned into binary16 in front of the stage's products, 8192^3 in float
+// took 1026 us, so 970 on the same card; leaving out products of rows past the tile's, in tiles of 64 or 32 rows or by a branch
+// around them, gained nothing: zeros take little power.
 template <bool EXPERTS, bool GATED>
 __device__ __forceinline__ void multiply_tile_exact(const Launch& l, const RowTile& t, const Shared& s, int n0, int wave,
                                                     Sums<1>& acc) {
@@ -900,7 +902,7 @@ double estimate(const ggk_fp8_args& a, int height) {
   return (a.experts > 0 ? 10 : 8) + rounds * (stage * stages + (gate ? 4 : 2));
 }
 
-// Tiles of 256 rows or of 128.  us of the two: 1024 rows of 8192 by 8192 86, 65, 1280 90, 107, 8192 453, 522; 1500 of 4096 by
+// Tiles of 256 rows or of 128.  us of the two, by the 8-bit instructions: 1024 rows of 8192 by 8192 86, 65, 1280 90, 107, 8192 453, 522; 1500 of 4096 by
 // 4096 46, 30.  Experts' tiles of 256 rows, with a rest of 128 and less each, where those of 128 would not fit the CUs at once:
 // 64 experts of 4096 by 14336, 16384 slots 1338, 1438, 16 of 1024 by 2048, 2048 slots 20, 18.  In binary16 the registers hold 128.
 int height_of(const ggk_fp8_args& a) {
